@@ -75,6 +75,9 @@ enum mtk_precision {
                           parity bar (<= 1e-4 relative; ~1e-5 measured) at several times the rate of MTK_PREC_FP32 */
 };
 
+/* Element types of the row, adapter and AdamW entry points. */
+enum mtk_dtype { MTK_DT_F32 = 0, MTK_DT_BF16 = 1, MTK_DT_F16 = 2 };
+
 /* Arithmetic of the diffusion kernels (mtk_q_sample, mtk_loss_rows, mtk_p_sample_step, mtk_sample_init). */
 enum mtk_math {
     MTK_MATH_REFERENCE = 0, /* accurate expf/logf, every fp32 op rounded as the reference's eager ops, the block
@@ -485,6 +488,67 @@ int mtk_edm_loss_keep(mtk_edm* edm, int64_t B, const float* y, int64_t y_ld, con
                       double p_std, double sigma_data, float* loss, mtk_stream stream);
 int mtk_edm_backward(mtk_edm* edm, int64_t B, const float* gout, int64_t g_ld, float* const* dW, float* const* db, mtk_stream stream);
 int mtk_edm_set_weights(mtk_edm* edm, const float* const* W, const float* const* b, mtk_stream stream);
+
+/* ---- (record, model) pairs sorted by model and back.  No reference counterpart: the reference evaluates its shadow models one after
+ * the other (attacks/ensemble/rmia/shadow_model_training.py:308); here the pairs of all models run as one batch.
+ *
+ * mtk_route_rows plans n_pairs pairs by index[i] in [0, n_groups), or -1 for a pair without a model.  order: the pairs in stable
+ * ascending order of their model, those without one last (a pair whose index is out of range too, stored as ~pair); slot: each
+ * pair's place in it; offsets [n_groups + 1]: model e's pairs are order[offsets[e]] .. order[offsets[e + 1] - 1].  work: int32,
+ * mtk_route_rows_work elements (0: may be NULL).
+ *
+ * mtk_rows_dispatch: xs[s] = x[order[s] / k] for the n_rows * k pairs of n_rows records with k copies each, times w[order[s]] where w
+ * is given; pair index = record * k + copy.  x: row stride x_ld; xs: dense, n_rows * k rows.  Rows of out-of-range pairs are NaN.
+ * With y (dense, like xs) and dw: dw[order[s]] = <x[order[s] / k], y[s]> too (xs may then be NULL).
+ * mtk_rows_combine: out[n] = sum_j w[n k + j] y[slot[n k + j]], j ascending, in fp32; w NULL: ones.
+ * Each of the two is the other's gradient.  dtype: enum mtk_dtype of x / xs / y / out; w and dw are fp32. */
+#define MTK_ROUTE_MAX_GROUPS 1024
+int64_t mtk_route_rows_work(int64_t n_pairs, int n_groups);
+int mtk_route_rows(int64_t n_pairs, const int64_t* index, int n_groups, int32_t* order, int32_t* slot, int32_t* offsets, int32_t* work,
+                   int64_t work_elems, mtk_stream stream);
+int mtk_rows_dispatch(int64_t n_rows, int k, int64_t D, int dtype, const void* x, int64_t x_ld, const int32_t* order, const float* w, void* xs,
+                      const void* y, float* dw, mtk_stream stream);
+int mtk_rows_combine(int64_t n_rows, int k, int64_t D, int dtype, const void* y, int64_t y_ld, const int32_t* slot, const float* w, void* out,
+                     mtk_stream stream);
+
+/* ---- a linear layer shared by n_models models with one low-rank update per model, on rows sorted by model.  No reference counterpart:
+ * the reference fine-tunes whole copies of one base model (attacks/ensemble/clavaddpm_fine_tuning.py:45).
+ *   y = act(x W^T + bias + s_e (x down_e^T) up_e^T) for rows offsets[e] .. offsets[e + 1] - 1; rows from offsets[n_models] on (and
+ *   before offsets[0]) have the shared layer alone.
+ * x [M, din] with row stride x_ld; W [dout, din], bias [dout] or NULL, down [n_models, r, din], up [n_models, dout, r], y [M, dout]:
+ * dense; all of `dtype`.  s_e = scales[e] (fp32), or `scale` where scales is NULL.  act: enum mtk_activation.
+ * saved (mtk_adapter_saved_bytes, 256-byte aligned): holds s_e x down_e^T; mtk_adapter_backward reads it, and with keep = 0 it is
+ * scratch.  mtk_adapter_backward: dx [M, din], ddown, dup (each may be NULL) from dy [M, dout] dense, for the same arguments;
+ * y is read under an activation only.  W and bias are frozen and get no gradient.  work: mtk_adapter_work_bytes, 256-byte aligned.
+ * Sums in fp32; identical run to run. */
+#define MTK_ADAPTER_MAX_RANK 256
+#define MTK_ADAPTER_MAX_WIDTH 8192
+#define MTK_ADAPTER_MAX_ROWS 16777216
+enum mtk_activation { MTK_ACT_NONE = 0, MTK_ACT_RELU = 1 };
+int64_t mtk_adapter_saved_bytes(int64_t M, int r, int dtype);
+int64_t mtk_adapter_work_bytes(int64_t M, int din, int dout, int r, int n_models, int dtype, int act);
+int mtk_adapter_forward(int64_t M, int din, int dout, int r, int n_models, int dtype, const void* x, int64_t x_ld, const void* W, const void* bias,
+                        const void* down, const void* up, const int32_t* offsets, const float* scales, double scale, int act, int keep, void* y,
+                        void* saved, int64_t saved_bytes, mtk_stream stream);
+int mtk_adapter_backward(int64_t M, int din, int dout, int r, int n_models, int dtype, const void* x, int64_t x_ld, const void* W, const void* down,
+                         const void* up, const int32_t* offsets, const float* scales, double scale, int act, const void* y, const void* dy,
+                         const void* saved, void* dx, void* ddown, void* dup, void* work, int64_t work_bytes, mtk_stream stream);
+
+/* ---- one AdamW step over many tensors (torch.optim.AdamW's update, which the reference's loops call: models/clavaddpm/trainer.py:94,
+ * models/clavaddpm/train.py:425).  p, g: dense tensors of `dtype`; the arrays hold n_tensors HOST-side entries of DEVICE pointers and
+ * may be released when the call returns.  state_bits = 32: m, v are fp32 (v the mean square).  state_bits = 8: m and v hold e4m3 codes of the
+ * mean and of the ROOT mean square, value = code * scale, one fp32 power-of-two scale per 256 values of a tensor
+ * (mtk_adamw_scales(numel) of them); a non-finite value is NaN.  step: the count of this step, from 1.
+ * mtk_adamw_count: for a step count on the device (*step is raised by one when the call RUNS, so a captured step counts its replays);
+ * it writes what the step needs to hyper_dev (mtk_adamw_hyper_bytes), which mtk_adamw_step then reads instead of lr ... step.
+ * lr_dev: fp32 scalar read instead of lr, or NULL. */
+int64_t mtk_adamw_scales(int64_t numel);
+int64_t mtk_adamw_hyper_bytes(void);
+int mtk_adamw_count(int64_t* step, const float* lr_dev, double lr, double beta1, double beta2, double eps, double weight_decay, void* hyper_dev,
+                    mtk_stream stream);
+int mtk_adamw_step(int n_tensors, void* const* p_host, const void* const* g_host, void* const* m_host, void* const* v_host, float* const* m_scale_host,
+                   float* const* v_scale_host, const int64_t* numel_host, int dtype, int state_bits, double lr, double beta1, double beta2, double eps,
+                   double weight_decay, int64_t step, const void* hyper_dev, mtk_stream stream);
 
 #ifdef __cplusplus
 }

@@ -1,4 +1,5 @@
 """midst_toolkit_amd — MI355X-native diffusion hot path of midst-toolkit (drop-in classes)."""
+from .adapters import LowRankEnsemble, adapter_linear  # noqa: F401
 from .attack_features import AttackFeatureDriver  # noqa: F401
 from .classifier import Classifier, get_conditioning_function  # noqa: F401
 from . import tabsyn  # noqa: F401
@@ -21,6 +22,8 @@ from .model import (  # noqa: F401
     ModelType,
     timestep_frequencies,
 )
+from .optim import AdamW, adamw_step  # noqa: F401
+from .routing import RowPlan, combine_rows, dispatch_rows, route_rows  # noqa: F401
 from .schedule import SchedulerType, betas_for_alpha_bar, get_named_beta_schedule  # noqa: F401
 from .scoring import mixed_loss as tartan_federer_mixed_loss  # noqa: F401
 from .scoring import score_records  # noqa: F401

@@ -95,6 +95,19 @@ _SIGS = {
     "mtk_edm_loss_keep": (C.c_int, [_p, _i64, _p, _i64, _p, _p, C.c_double, C.c_double, C.c_double, _p, _p]),
     "mtk_edm_backward": (C.c_int, [_p, _i64, _p, _i64, _p, _p, _p]),
     "mtk_edm_set_weights": (C.c_int, [_p, _p, _p, _p]),
+    "mtk_route_rows_work": (_i64, [_i64, _i32]),
+    "mtk_route_rows": (C.c_int, [_i64, _p, _i32, _p, _p, _p, _p, _i64, _p]),
+    "mtk_rows_dispatch": (C.c_int, [_i64, _i32, _i64, _i32, _p, _i64, _p, _p, _p, _p, _p, _p]),
+    "mtk_rows_combine": (C.c_int, [_i64, _i32, _i64, _i32, _p, _i64, _p, _p, _p, _p]),
+    "mtk_adapter_saved_bytes": (_i64, [_i64, _i32, _i32]),
+    "mtk_adapter_work_bytes": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "mtk_adapter_forward": (C.c_int, [_i64, _i32, _i32, _i32, _i32, _i32, _p, _i64, _p, _p, _p, _p, _p, _p, C.c_double, _i32, _i32, _p, _p, _i64, _p]),
+    "mtk_adapter_backward": (C.c_int, [_i64, _i32, _i32, _i32, _i32, _i32, _p, _i64, _p, _p, _p, _p, _p, C.c_double, _i32, _p, _p, _p, _p, _p, _p, _p,
+                                       _i64, _p]),
+    "mtk_adamw_scales": (_i64, [_i64]),
+    "mtk_adamw_hyper_bytes": (_i64, []),
+    "mtk_adamw_count": (C.c_int, [_p, _p, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, _p, _p]),
+    "mtk_adamw_step": (C.c_int, [_i32, _p, _p, _p, _p, _p, _p, _p, _i32, _i32, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, _i64, _p, _p]),
     "mtk_train_export": (C.c_int, [_p, _i32, _p, _p, _p]),
     "mtk_train_import": (C.c_int, [_p, _i32, _p, _p, _p]),
 }

@@ -17,6 +17,10 @@ hipcc $FLAGS -c mtk_mlp_f32.hip -o _build/mtk_mlp_f32.o & pids+=($!)
 hipcc $FLAGS -c mtk_mlp_bf16.hip -o _build/mtk_mlp_bf16.o & pids+=($!)
 hipcc $FLAGS -c mtk_mlp_bf16_layered.hip -o _build/mtk_mlp_bf16_layered.o & pids+=($!)
 hipcc $FLAGS -ffp-contract=off -c mtk_transform.hip -o _build/mtk_transform.o & pids+=($!)
+hipcc $FLAGS -c mtk_rows.hip -o _build/mtk_rows.o & pids+=($!)
+hipcc $FLAGS -c mtk_adapter.hip -o _build/mtk_adapter.o & pids+=($!)
+# AdamW: each product and sum rounded by itself, so the update is the one torch's elementary operations give
+hipcc $FLAGS -ffp-contract=off -c mtk_optim.hip -o _build/mtk_optim.o & pids+=($!)
 for p in "${pids[@]}"; do wait "$p"; done
 hipcc --offload-arch=gfx950 -shared -fPIC _build/*.o -o ../libmtk_hip.so
 echo "built $(cd .. && pwd)/libmtk_hip.so"

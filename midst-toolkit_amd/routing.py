@@ -1,0 +1,155 @@
+"""(record, model) pairs sorted by model and back, on MI355X.
+
+An ensemble of shadow models (attacks/ensemble/rmia/shadow_model_training.py:308 trains 16 of one base) is evaluated by the reference
+model after model.  Here the pairs of all models run as one batch: ``route_rows`` plans it, ``dispatch_rows`` copies every record's row
+to its pairs' places, the layers work on rows sorted by model (``adapters.adapter_linear`` takes ``plan.offsets``), and
+``combine_rows`` brings the results back to the records, weighted.  Both copies carry gradients.  There is no CPU path.
+"""
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import check
+
+MAX_GROUPS = 1024  # MTK_ROUTE_MAX_GROUPS of include/mtk.h
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # enum mtk_dtype
+
+
+def dtype_code(t: Tensor, what: str) -> int:
+    code = DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what}: {t.dtype} (float32, bfloat16 or float16)")
+    return code
+
+
+def rows_of(t: Tensor) -> Tensor:
+    """``t`` [n, D] itself where its rows are contiguous (any row stride, also 0 of an expanded row), else a contiguous copy."""
+    return t if t.shape[0] == 0 or ((t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= 0) else t.contiguous()
+
+
+class RowPlan:
+    """Where the pairs go: what ``route_rows`` returns.  ``order`` [P] int32: the pair in each place (``~pair`` for one whose index was out
+    of range), ``slot`` (the shape of ``index``) int32: the place of each pair, ``offsets`` [n_groups + 1] int32: model e's pairs are in
+    places ``offsets[e]`` to ``offsets[e + 1] - 1``, pairs without a model behind them all."""
+
+    __slots__ = ("order", "slot", "offsets", "n_groups", "n_rows", "copies")
+
+    def __init__(self, order: Tensor, slot: Tensor, offsets: Tensor, n_groups: int, n_rows: int, copies: int):
+        self.order, self.slot, self.offsets = order, slot, offsets
+        self.n_groups, self.n_rows, self.copies = n_groups, n_rows, copies
+
+
+def route_rows(index: Tensor, n_groups: int) -> RowPlan:
+    """Plan for ``index`` [N] or [N, k] (whole numbers): the model of record n's copy j, in [0, n_groups), or -1 for a copy without a
+    model.  The same model twice in a record is two pairs.  Pairs keep their order within a model.  A pair whose index is out of
+    range is treated like -1 and its dispatched row is NaN."""
+    if not index.is_cuda:
+        raise RuntimeError("route_rows: midst_toolkit_amd has no CPU path; move the indices to the MI355X")
+    if index.dim() not in (1, 2) or index.dtype.is_floating_point or index.dtype.is_complex or index.dtype == torch.bool:
+        raise ValueError(f"route_rows: index is [N] or [N, k] whole numbers, got {tuple(index.shape)} {index.dtype}")
+    if not 1 <= n_groups <= MAX_GROUPS:
+        raise ValueError(f"route_rows: {n_groups} groups (1 to {MAX_GROUPS})")
+    copies = 1 if index.dim() == 1 else index.shape[1]
+    if copies < 1:
+        raise ValueError("route_rows: index has no copies")
+    dev, P = index.device, index.numel()
+    if P > 0x7FFFFFFF:
+        raise ValueError(f"route_rows: {P} pairs exceed 2^31 - 1")
+    idx = index.to(torch.int64).contiguous()
+    l = _lib.lib()
+    order = torch.empty(P, dtype=torch.int32, device=dev)
+    slot = torch.empty(index.shape, dtype=torch.int32, device=dev)
+    offsets = torch.empty(n_groups + 1, dtype=torch.int32, device=dev)
+    need = l.mtk_route_rows_work(P, n_groups)
+    work = torch.empty(need, dtype=torch.int32, device=dev) if need else None
+    with torch.cuda.device(dev):
+        check(l.mtk_route_rows(P, idx.data_ptr(), n_groups, order.data_ptr(), slot.data_ptr(), offsets.data_ptr(),
+                               work.data_ptr() if work is not None else None, need, _lib.stream_handle(dev)))
+    return RowPlan(order, slot, offsets, n_groups, index.shape[0], copies)
+
+
+def _check_rows(what: str, t: Tensor, rows: int, plan: RowPlan) -> int:
+    if not t.is_cuda:
+        raise RuntimeError(f"{what}: midst_toolkit_amd has no CPU path; move the rows to the MI355X")
+    if t.device != plan.order.device:
+        raise ValueError(f"{what}: rows on {t.device}, plan on {plan.order.device}")
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1:
+        raise ValueError(f"{what}: expected [{rows}, width] rows, got {tuple(t.shape)}")
+    return dtype_code(t, what)
+
+
+def _dispatch(x: Tensor, plan: RowPlan, w: Tensor | None, y: Tensor | None = None, want_rows: bool = True):
+    """mtk_rows_dispatch: (xs, dw)."""
+    dev, D = x.device, x.shape[1]
+    x = rows_of(x)
+    P = plan.n_rows * plan.copies
+    xs = torch.empty((P, D), dtype=x.dtype, device=dev) if want_rows else None
+    dw = torch.empty((plan.n_rows, plan.copies), dtype=torch.float32, device=dev) if y is not None else None
+    if P:
+        with torch.cuda.device(dev):
+            check(_lib.lib().mtk_rows_dispatch(plan.n_rows, plan.copies, D, DTYPES[x.dtype], x.data_ptr(), x.stride(0), plan.order.data_ptr(),
+                                               None if w is None else w.data_ptr(), None if xs is None else xs.data_ptr(),
+                                               None if y is None else y.data_ptr(), None if dw is None else dw.data_ptr(), _lib.stream_handle(dev)))
+    return xs, dw
+
+
+def _combine(y: Tensor, plan: RowPlan, w: Tensor | None) -> Tensor:
+    dev, D = y.device, y.shape[1]
+    y = rows_of(y)
+    out = torch.empty((plan.n_rows, D), dtype=y.dtype, device=dev)
+    if plan.n_rows:
+        with torch.cuda.device(dev):
+            check(_lib.lib().mtk_rows_combine(plan.n_rows, plan.copies, D, DTYPES[y.dtype], y.data_ptr(), y.stride(0), plan.slot.data_ptr(),
+                                              None if w is None else w.data_ptr(), out.data_ptr(), _lib.stream_handle(dev)))
+    return out
+
+
+class _Dispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, plan):
+        ctx.plan = plan
+        return _dispatch(x, plan, None)[0]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        return _combine(g, ctx.plan, None), None
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, plan):
+        ctx.plan = plan
+        ctx.save_for_backward(y if weights is not None and ctx.needs_input_grad[1] else None, weights)
+        return _combine(y, plan, weights)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        y, w = ctx.saved_tensors
+        want_w = w is not None and ctx.needs_input_grad[1]
+        gy, gw = _dispatch(g, ctx.plan, w, y.contiguous() if want_w else None, ctx.needs_input_grad[0])
+        return gy, gw, None
+
+
+def dispatch_rows(x: Tensor, plan: RowPlan) -> Tensor:
+    """``x`` [N, D] -> [N * k, D]: every record's row in the places of its k pairs, sorted by model.  Differentiable in ``x`` (a record's
+    gradient is the sum over its pairs, in fp32, in the order of its copies)."""
+    _check_rows("dispatch_rows", x, plan.n_rows, plan)
+    return _Dispatch.apply(x, plan)
+
+
+def combine_rows(y: Tensor, plan: RowPlan, weights: Tensor | None = None) -> Tensor:
+    """``y`` [N * k, D] in the plan's order -> [N, D]: ``sum_j weights[n, j] * y[slot[n, j]]`` (``weights`` None: ones), summed in fp32 and
+    rounded once.  ``weights``: float32 of ``index``'s shape.  Differentiable in both."""
+    _check_rows("combine_rows", y, plan.n_rows * plan.copies, plan)
+    if weights is not None:
+        if weights.device != y.device:
+            raise ValueError(f"combine_rows: weights on {weights.device}, rows on {y.device}")
+        if weights.dtype != torch.float32 or weights.numel() != plan.n_rows * plan.copies or weights.shape[0] != plan.n_rows:
+            raise ValueError(f"combine_rows: weights are float32 [{plan.n_rows}, {plan.copies}], got {weights.dtype} {tuple(weights.shape)}")
+        weights = weights.reshape(plan.n_rows, plan.copies).contiguous()
+    return _Combine.apply(y, weights, plan)

@@ -1,0 +1,797 @@
+"""GPU: rows sorted by model and back, low-rank adapted linear layers, AdamW over many tensors - each against 64 bits (tests/operator_refs.py).
+
+Tolerances count roundings.  A sum of K fp32 products is off by at most (K + 2) 2^-24 of the sum of its terms' magnitudes (each product
+and each addition rounds by half a step); TWICE is allowed for the matrix instructions, whose inner additions may be in any order and
+truncate (a whole step).  A stored 16-bit value is off by half a step of its type, eps / 2 of its magnitude; subnormal fp16 results by
+half the smallest step, 2^-25."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import midst_toolkit_amd as mtk
+from tests.operator_refs import adamw8_reference, adapter_reference, route_reference
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+U32, TWICE = 2.0**-24, 2.0
+
+
+def half(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def tiny(dt):
+    return 2.0**-25 if dt == torch.float16 else 2.0**-133 if dt == torch.bfloat16 else 2.0**-149
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def randn(g, *shape, dt=torch.float32):
+    return torch.randn(shape, generator=g).to(dt).to(DEV)
+
+
+def within(got, want, tol):
+    got = got.detach().cpu().double()
+    assert got.shape == want.shape
+    bad = ~((got - want).abs() <= tol)
+    assert not bool(bad.any()), (float(((got - want).abs() - tol).max()), bad.nonzero()[:4].tolist())
+
+
+# ------------------------------------------------------------------------------------------------------------------- rows
+def make_index(g, N, k, E, kind):
+    if kind == "one":
+        return torch.full((N, k), E - 1, dtype=torch.int64)
+    if kind == "none":
+        return torch.full((N, k), -1, dtype=torch.int64)
+    idx = torch.randint(-1, E, (N, k), generator=g)
+    if kind == "few":  # most models without a pair
+        idx = torch.where(idx < 0, idx, idx // max(1, E // 2) * max(1, E // 2))
+    if kind == "bad" and N:
+        idx[N // 2, 0], idx[N - 1, k - 1] = E, -7
+    return idx
+
+
+@pytest.mark.parametrize("N,k,E,kind", [(1, 1, 1, "any"), (1, 1, 1, "none"), (5, 3, 4, "bad"), (63, 1, 2, "any"), (64, 2, 1024, "any"), (777, 3, 31, "few"), (4096, 2, 16, "one"),
+                                        (4097, 2, 17, "any"), (9000, 1, 3, "bad"), (30011, 4, 300, "any"), (70000, 3, 1024, "few"), (300000, 4, 5, "any")])
+def test_plan_is_the_stable_sort(N, k, E, kind):
+    idx = make_index(gen(N + k + E), N, k, E, kind)
+    plan = mtk.route_rows(idx.to(DEV), E)
+    order, slot, offsets = route_reference(idx.numpy(), E)
+    assert np.array_equal(plan.order.cpu().numpy(), order)
+    assert np.array_equal(plan.slot.cpu().numpy(), slot)
+    assert np.array_equal(plan.offsets.cpu().numpy(), offsets)
+
+
+def test_plan_shapes_and_types():
+    for idx in (torch.tensor([2, 0, -1, 2]), torch.tensor([2, 0, -1, 2], dtype=torch.int32), torch.tensor([[2, 0, -1, 2]]).t(), torch.tensor([2, 0, -1, 2])[:0]):
+        plan = mtk.route_rows(idx.to(DEV), 3)
+        order, slot, offsets = route_reference(idx.numpy(), 3)
+        assert np.array_equal(plan.order.cpu().numpy(), order) and np.array_equal(plan.slot.cpu().numpy(), slot) and np.array_equal(plan.offsets.cpu().numpy(), offsets)
+    for bad in (torch.zeros(3), torch.zeros(3, dtype=torch.bool), torch.zeros(2, 2, 2, dtype=torch.int64), torch.zeros(3, 0, dtype=torch.int64)):
+        with pytest.raises(ValueError):
+            mtk.route_rows(bad.to(DEV), 3)
+    for e in (0, 1025):
+        with pytest.raises(ValueError):
+            mtk.route_rows(torch.zeros(3, dtype=torch.int64, device=DEV), e)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("N,k,E,D", [(0, 2, 3, 5), (1, 1, 1, 1), (3, 8, 2, 2), (33, 2, 5, 7), (100, 4, 9, 33), (257, 3, 16, 120), (1000, 2, 7, 257), (70, 5, 1000, 1021), (50, 2, 4, 2050)])
+def test_rows_forth_and_back(N, k, E, D, dt):
+    g = gen(N * 31 + D)
+    idx = make_index(g, N, k, E, "any").reshape(N, k)
+    x, y, w = randn(g, N, D, dt=dt), randn(g, N * k, D, dt=dt), randn(g, N, k)
+    gx, go = randn(g, N * k, D, dt=dt), randn(g, N, D, dt=dt)
+    for t in (x, y, w):
+        t.requires_grad_()
+    plan = mtk.route_rows(idx.to(DEV), E)
+    xs, out = mtk.dispatch_rows(x, plan), mtk.combine_rows(y, plan, w)
+    dx, dy, dw = torch.autograd.grad((xs, out), (x, y, w), (gx, go))
+    order, slot, _ = route_reference(idx.numpy(), E)
+    order, slot = torch.from_numpy(order), torch.from_numpy(slot)
+    c = lambda t: t.detach().cpu()  # noqa: E731
+    assert torch.equal(c(xs), c(x)[order // k])
+    terms = c(y).double()[slot.reshape(-1)].view(N, k, D) * c(w).double()[:, :, None]
+    want, mag = terms.sum(1), terms.abs().sum(1)
+    within(out, want, (k + 2) * U32 * mag + half(dt) * want.abs() * 1.001 + tiny(dt))
+    terms = c(gx).double()[slot.reshape(-1)].view(N, k, D)
+    want, mag = terms.sum(1), terms.abs().sum(1)
+    within(dx, want, (k + 2) * U32 * mag + half(dt) * want.abs() * 1.001 + tiny(dt))
+    want = c(go).double()[order // k] * c(w).double().reshape(-1)[order][:, None]
+    within(dy, want, (half(dt) + 2 * U32) * want.abs() * 1.001 + tiny(dt))
+    terms = c(y).double()[slot.reshape(-1)].view(N, k, D) * c(go).double()[:, None, :]
+    within(dw, terms.sum(2), (D + 2) * U32 * terms.abs().sum(2))
+    again = torch.autograd.grad((mtk.dispatch_rows(x, plan), mtk.combine_rows(y, plan, w)), (x, y, w), (gx, go))
+    assert all(torch.equal(a, b) for a, b in zip(again, (dx, dy, dw)))  # the same bits
+    # without weights, and with a gradient for one side only
+    want = c(y).double()[slot.reshape(-1)].view(N, k, D)
+    within(mtk.combine_rows(y.detach(), plan), want.sum(1), (k + 2) * U32 * want.abs().sum(1) + half(dt) * want.sum(1).abs() * 1.001 + tiny(dt))
+    assert torch.equal(torch.autograd.grad(mtk.combine_rows(y.detach(), plan, w), w, go)[0], dw)
+    assert torch.equal(torch.autograd.grad(mtk.combine_rows(y, plan, w.detach()), y, go)[0], dy)
+
+
+def test_rows_gradients_against_differences():
+    """<gradient, direction> against the change of the loss along it: every map is linear in each argument, so the difference is exact but
+    for rounding - the fp32 sums behind both sides, (D k + 4) 2^-24 of the sum of magnitudes, times 4 for the two losses and the product."""
+    g = gen(5)
+    N, k, E, D = 40, 3, 6, 29
+    plan = mtk.route_rows(make_index(g, N, k, E, "any").to(DEV), E)
+    x, y, w = randn(g, N, D), randn(g, N * k, D), randn(g, N, k)
+    gx, go = randn(g, N * k, D), randn(g, N, D)
+    f = {"x": (x, lambda t: (mtk.dispatch_rows(t, plan).double() * gx.double())), "y": (y, lambda t: mtk.combine_rows(t, plan, w).double() * go.double()),
+         "w": (w, lambda t: mtk.combine_rows(y, plan, t).double() * go.double())}
+    for name, (t, loss) in f.items():
+        d = randn(g, *t.shape)
+        leaf = t.clone().requires_grad_()
+        grad = torch.autograd.grad(loss(leaf).sum(), leaf)[0]
+        up, down = loss(t + d), loss(t - d)
+        tol = 4 * (D * k + 4) * U32 * float(up.abs().sum() + down.abs().sum() + (grad * d).abs().sum())
+        assert abs(float((up.sum() - down.sum()) / 2 - (grad.double() * d.double()).sum())) <= tol, name
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_rows_keep_bad_values_to_themselves(dt):
+    """An index out of range gives a NaN row and touches no other; infinities and NaN stay in their records."""
+    g = gen(2)
+    N, k, E, D = 50, 2, 4, 19
+    idx = make_index(g, N, k, E, "bad")
+    x = randn(g, N, D, dt=dt)
+    x[7], x[9, 3] = float("nan"), float("inf")
+    plan = mtk.route_rows(idx.to(DEV), E)
+    xs = mtk.dispatch_rows(x, plan).cpu()
+    order, slot, _ = route_reference(idx.numpy(), E)
+    bad = torch.from_numpy(order < 0)
+    assert int(bad.sum()) == 2 and bool(torch.isnan(xs[bad]).all())
+    src = torch.from_numpy(np.where(order < 0, ~order, order)) // k
+    assert torch.equal(torch.nan_to_num(xs[~bad].float()), torch.nan_to_num(x.cpu()[src[~bad]].float()))
+    y = randn(g, N * k, D, dt=dt)
+    clean = mtk.combine_rows(y, plan)
+    s = int(slot[11, 1])
+    y[s] = float("nan")
+    got = mtk.combine_rows(y, plan)
+    assert bool(torch.isnan(got[11]).all())
+    rest = torch.arange(N) != 11
+    assert torch.equal(got.cpu()[rest], clean.cpu()[rest])
+
+
+def test_rows_strides_and_shapes():
+    g = gen(3)
+    N, k, E, D = 40, 2, 5, 24
+    idx = make_index(g, N, k, E, "any")
+    plan = mtk.route_rows(idx.to(DEV), E)
+    wide, yw = randn(g, N, 3 * D), randn(g, N * k, D + 3)
+    for x in (wide[:, D:2 * D], wide[:, :D].t().contiguous().t(), wide[:1, :D].expand(N, D), wide[:, ::3], wide.flip(0)[:, 1:D + 1]):
+        assert torch.equal(mtk.dispatch_rows(x, plan), mtk.dispatch_rows(x.contiguous(), plan))
+    for y in (yw[:, 3:], yw[:, 1:2], yw[:, :D].t().contiguous().t(), yw[:1].expand(N * k, D + 3)):
+        assert torch.equal(mtk.combine_rows(y, plan), mtk.combine_rows(y.contiguous(), plan))
+    w = randn(g, k, N).t()
+    assert torch.equal(mtk.combine_rows(yw, plan, w), mtk.combine_rows(yw, plan, w.contiguous()))
+    x = wide.clone().requires_grad_()
+    mtk.dispatch_rows(x, plan).sum().backward()  # an expanded gradient
+    assert torch.equal(x.grad, torch.full_like(x, float(k)))
+    for bad in (wide[:N - 1], wide.double(), wide[:, :0], wide[0]):
+        with pytest.raises(ValueError):
+            mtk.dispatch_rows(bad, plan)
+    for bad in (w.double(), w[:, :1], w.reshape(-1), w.half()):
+        with pytest.raises(ValueError):
+            mtk.combine_rows(yw, plan, bad)
+
+
+# ---------------------------------------------------------------------------------------------------------------- adapters
+def make_offsets(g, M, E, kind):
+    if kind == "base":  # no row has a model
+        return torch.zeros(E + 1, dtype=torch.int32)
+    if kind == "last":  # the last model owns everything
+        return torch.tensor([0] * E + [M], dtype=torch.int32)
+    idx = torch.randint(0, E + 1, (M,), generator=g)
+    if kind == "few":
+        idx = torch.where(idx == E, idx, idx // max(1, E // 3) * max(1, E // 3))
+    return torch.searchsorted(idx.sort().values, torch.arange(E + 1)).to(torch.int32)
+
+
+def adapter_inputs(g, M, din, dout, r, E, dt, kind="any"):
+    return dict(x=randn(g, M, din, dt=dt), weight=(randn(g, dout, din) / math.sqrt(din)).to(dt), bias=randn(g, dout, dt=dt), down=(randn(g, E, r, din) / math.sqrt(din)).to(dt),
+                up=(randn(g, E, dout, r) / math.sqrt(r)).to(dt), offsets=make_offsets(g, M, E, kind).to(DEV), scale=(torch.rand(E, generator=g) + 0.5).to(DEV))
+
+
+def call(a, **kw):
+    a = {**a, **kw}
+    return mtk.adapter_linear(a["x"], a["weight"], a["bias"], a["down"], a["up"], a["offsets"], a["scale"], kw.get("activation", "none"))
+
+
+def tol(terms, low, K, r, want, dt):
+    """Sums of K products over `terms`; the low-rank part sums K, then r, and its inner value is rounded to the type once (and to fp32's
+    denormals: nothing).  The stored value rounds once more."""
+    inner = 0.0 if dt == torch.float32 else half(dt) * 1.01
+    return TWICE * (K + 2) * U32 * terms + (TWICE * (K + r + 8) * U32 + inner) * low + half(dt) * want.abs() * 1.01 + tiny(dt) * 4
+
+
+SHAPES = [(1, 1, 1, 1, 1, "any"), (1, 64, 64, 8, 4, "any"), (2, 7, 5, 3, 2, "any"), (31, 130, 67, 12, 5, "any"), (33, 64, 128, 16, 3, "last"), (64, 33, 130, 17, 64, "any"),
+          (127, 257, 129, 33, 7, "few"), (130, 96, 200, 64, 4, "any"), (300, 70, 66, 100, 2, "any"), (129, 40, 24, 256, 3, "any"), (513, 128, 256, 8, 1, "any"),
+          (200, 120, 128, 4, 1024, "few"), (1000, 512, 48, 16, 16, "any"), (77, 64, 64, 8, 3, "base"), (2049, 64, 72, 16, 9, "few"), (16, 2050, 40, 8, 4, "any"),
+          (700, 256, 1024, 16, 5, "any"), (9, 300, 1000, 9, 3, "any")]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("M,din,dout,r,E,kind", SHAPES)
+def test_adapter_forward_and_gradients(M, din, dout, r, E, kind, dt):
+    g = gen(M * 13 + din)
+    a = adapter_inputs(g, M, din, dout, r, E, dt, kind)
+    gy = randn(g, M, dout, dt=dt)
+    for n in ("x", "down", "up"):
+        a[n].requires_grad_()
+    y = call(a)
+    ref = adapter_reference(**{**a, "relu": False, "gy": gy})
+    dx, ddown, dup = torch.autograd.grad(y, (a["x"], a["down"], a["up"]), gy)
+    within(y, ref["y"], tol(ref["y_terms"], ref["y_low"], din, r, ref["y"], dt))
+    within(dx, ref["dx"], tol(ref["dx_terms"], ref["dx_low"], dout, r, ref["dx"], dt))
+    rows = int((a["offsets"][1:] - a["offsets"][:-1]).max())
+    inner = 0.0 if dt == torch.float32 else half(dt) * 1.01
+    for name, got, K in (("ddown", ddown, dout), ("dup", dup, din)):
+        want, mag = ref[name], ref[name + "_terms"]
+        within(got, want, (TWICE * (K + rows + 8) * U32 + inner) * mag + half(dt) * want.abs() * 1.01 + tiny(dt) * 4)
+    # the same bits again, and alone
+    y2 = call(a)
+    assert torch.equal(y, y2)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y2, (a["x"], a["down"], a["up"]), gy), (dx, ddown, dup)))
+    for i, n in enumerate(("x", "down", "up")):
+        b = {**a, **{m: a[m].detach() for m in ("x", "down", "up") if m != n}}
+        assert torch.equal(torch.autograd.grad(call(b), b[n], gy)[0], (dx, ddown, dup)[i]), n
+    # without gradients the layer is the same, and so it is without a bias
+    b = {n: t.detach() for n, t in a.items()}
+    assert torch.equal(call(b), y)
+    ref0 = adapter_reference(**{**b, "bias": None, "relu": True})
+    within(call(b, bias=None, activation="relu"), ref0["y"], tol(ref0["y_terms"], ref0["y_low"], din, r, ref0["y"], dt))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("M,din,dout,r,E", [(1, 16, 8, 2, 1), (100, 33, 65, 8, 3), (300, 128, 128, 16, 4)])
+def test_adapter_relu_gradient(M, din, dout, r, E, dt):
+    """The mask: rows of x are scaled so that the layer's values stay clear of 0 by more than their tolerance; where one would not, its dy is 0
+    (which adds nothing on either side)."""
+    g = gen(M + din)
+    a = adapter_inputs(g, M, din, dout, r, E, dt)
+    gy = randn(g, M, dout, dt=dt)
+    pre = adapter_reference(**{**a, "relu": False})
+    near = pre["y"].abs() <= tol(pre["y_terms"], pre["y_low"], din, r, pre["y"], dt)
+    gy[near.to(DEV)] = 0
+    for n in ("x", "down", "up"):
+        a[n].requires_grad_()
+    ref = adapter_reference(**{**a, "relu": True, "gy": gy})
+    y = call(a, activation="relu")
+    within(y, ref["y"], tol(pre["y_terms"], pre["y_low"], din, r, pre["y"], dt))
+    dx, ddown, dup = torch.autograd.grad(y, (a["x"], a["down"], a["up"]), gy)
+    within(dx, ref["dx"], tol(ref["dx_terms"], ref["dx_low"], dout, r, ref["dx"], dt))
+    inner = 0.0 if dt == torch.float32 else half(dt) * 1.01
+    for name, got, K in (("ddown", ddown, dout), ("dup", dup, din)):
+        within(got, ref[name], (TWICE * (K + M + 8) * U32 + inner) * ref[name + "_terms"] + half(dt) * ref[name].abs() * 1.01 + tiny(dt) * 4)
+
+
+def test_adapter_gradients_against_differences():
+    """The layer is linear in x, down and up each, so a central difference is exact but for rounding: half of each loss's error bound
+    (the forward tolerance times |gy|, summed), twice, and the gradients' own."""
+    g = gen(8)
+    M, din, dout, r, E = 90, 48, 40, 8, 4
+    a = adapter_inputs(g, M, din, dout, r, E, torch.float32)
+    gy = randn(g, M, dout)
+    for n in ("x", "down", "up"):
+        leaf = a[n].clone().requires_grad_()
+        d = randn(g, *leaf.shape) * 0.3
+        grad = torch.autograd.grad(call(a, **{n: leaf}), leaf, gy)[0]
+        loss, err = [], 0.0
+        for sign in (1, -1):
+            b = {**a, n: a[n] + sign * d}
+            ref = adapter_reference(**{**b, "relu": False})
+            err += float((tol(ref["y_terms"], ref["y_low"], din, r, ref["y"], torch.float32) * gy.cpu().double().abs()).sum()) + 4 * U32 * float(
+                ((ref["y_terms"] + ref["y_low"]) * gy.cpu().double().abs()).sum())  # a +- d is rounded too
+            loss.append(float((call(b).double() * gy.double()).sum()))
+        own = TWICE * (din + dout + M + r + 16) * U32 * float((grad.double().abs() * d.double().abs()).sum()) * 8
+        assert abs((loss[0] - loss[1]) / 2 - float((grad.double() * d.double()).sum())) <= err + own, n
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("M", [3, 200])
+def test_a_diverged_model_leaves_the_others_alone(M, dt):
+    """Infinite and NaN factors, rows and gradients of one model: every other model's rows and gradients keep their bits."""
+    g = gen(17)
+    din, dout, r, E = 72, 80, 8, 3
+    a = adapter_inputs(g, M, din, dout, r, E, dt)
+    a["offsets"] = torch.tensor([0, M // 3, 2 * M // 3, M], dtype=torch.int32, device=DEV)
+    gy = randn(g, M, dout, dt=dt)
+
+    def run(b, gy):
+        b = {n: t.clone() for n, t in b.items()}
+        for n in ("x", "down", "up"):
+            b[n].requires_grad_()
+        y = call(b)
+        return (y.detach(),) + torch.autograd.grad(y, (b["x"], b["down"], b["up"]), gy)
+
+    clean = run(a, gy)
+    rows = slice(M // 3, 2 * M // 3)
+    rest = torch.ones(M, dtype=torch.bool)
+    rest[rows] = False
+    for what in ("down", "up", "x", "gy"):
+        for value in (float("inf"), float("nan")):
+            b, gz = {n: t.clone() for n, t in a.items()}, gy.clone()
+            if what == "gy":
+                gz[rows] = value
+            elif what == "x":
+                b["x"][rows] = value
+            else:
+                b[what][1] = value
+            y, dx, dd, du = run(b, gz)
+            assert torch.equal(y.cpu()[rest], clean[0].cpu()[rest]) and torch.equal(dx.cpu()[rest], clean[1].cpu()[rest]), (what, value)
+            for got, want in ((dd, clean[2]), (du, clean[3])):
+                assert torch.equal(got[[0, 2]], want[[0, 2]]), (what, value)
+            if what != "gy":
+                assert not bool(torch.isfinite(y[rows]).any()), what
+
+
+def test_adapter_strides_scales_and_plans():
+    g = gen(4)
+    M, din, dout, r, E = 60, 40, 24, 4, 3
+    a = adapter_inputs(g, M, din, dout, r, E, torch.float32)
+    wide = randn(g, M, 2 * din + 3)
+    for x in (wide[:, 3:3 + din], wide[:, ::2][:, :din], wide[:1, :din].expand(M, din), randn(g, din, M).t()):
+        assert torch.equal(call(a, x=x), call(a, x=x.contiguous()))
+    b = {**a, "weight": a["weight"].t().contiguous().t(), "up": a["up"].transpose(1, 2).contiguous().transpose(1, 2)}
+    assert torch.equal(call(b), call(a))
+    assert torch.equal(call(a, scale=2.5), call(a, scale=torch.full((E,), 2.5, device=DEV)))
+    idx = torch.randint(-1, E, (M,), generator=g).to(DEV)
+    plan = mtk.route_rows(idx, E)
+    assert torch.equal(mtk.adapter_linear(a["x"], a["weight"], a["bias"], a["down"], a["up"], plan), call(a, offsets=plan.offsets, scale=1.0))
+    x = wide[:, :din].clone().requires_grad_()
+    call(a, x=x).sum().backward()  # an expanded gradient
+    y = a["x"].clone().requires_grad_()
+    xe = wide[:1, :din].clone().requires_grad_()
+    call(a, x=xe.expand(M, din)).sum().backward()  # a broadcast input: its gradient is the rows' sum
+    full = wide[:1, :din].expand(M, din).clone().requires_grad_()
+    call(a, x=full).sum().backward()
+    assert torch.equal(xe.grad, full.grad.sum(0, keepdim=True)) and y.grad is None
+
+
+def test_adapter_without_rows():
+    g = gen(6)
+    a = adapter_inputs(g, 0, 8, 6, 2, 3, torch.float32)
+    for n in ("x", "down", "up"):
+        a[n].requires_grad_()
+    y = call(a)
+    assert y.shape == (0, 6)
+    dx, dd, du = torch.autograd.grad(y, (a["x"], a["down"], a["up"]), torch.zeros(0, 6, device=DEV))
+    assert dx.shape == (0, 8) and not bool(dd.any()) and not bool(du.any())
+
+
+def test_adapter_refusals():
+    g = gen(7)
+    a = adapter_inputs(g, 6, 8, 6, 2, 3, torch.float32)
+    bad = [dict(x=a["x"][0]), dict(x=a["x"][:, :7]), dict(weight=a["weight"].half()), dict(up=a["up"][:2]), dict(bias=a["bias"][:5]), dict(offsets=a["offsets"].long()),
+           dict(offsets=a["offsets"][:3]), dict(scale=torch.ones(2, device=DEV)), dict(scale=torch.ones(3)), dict(activation="gelu"), dict(x=a["x"].double()),
+           dict(weight=a["weight"].cpu()), dict(down=a["down"][:, :0], up=a["up"][:, :, :0])]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            call(a, **kw)
+    with pytest.raises(NotImplementedError, match="frozen"):
+        call(a, weight=a["weight"].clone().requires_grad_())
+
+
+@pytest.mark.parametrize("off", [[0, 90, 10, 40], [50, 60, 70, 80], [-5, 20, 1000, 2000], [100, 60, 30, 0], [-9, -8, -7, -6], [2**31 - 1] * 4])
+def test_offsets_that_make_no_sense_stay_inside_the_tensors(off):
+    """Offsets live on the device, so the host cannot check them: whatever they hold, no row outside the tensors is touched and the call ends.
+    Rows before the first offset have the shared layer alone."""
+    g = gen(12)
+    M, din, dout, r, E = 64, 32, 48, 4, 3
+    a = adapter_inputs(g, M, din, dout, r, E, torch.float32)
+    a["offsets"] = torch.tensor(off, dtype=torch.int32, device=DEV)
+    for n in ("x", "down", "up"):
+        a[n].requires_grad_()
+    y = call(a)
+    y.sum().backward()
+    assert bool(torch.isfinite(y).all())
+    if off == [50, 60, 70, 80]:
+        fine = a["offsets"].cpu().clamp(max=M)
+        ref = adapter_reference(**{**a, "offsets": fine, "relu": False})
+        within(y, ref["y"], tol(ref["y_terms"], ref["y_low"], din, r, ref["y"], torch.float32))
+
+
+# ------------------------------------------------------------------------------------------------------------------- AdamW
+SIZES = [1, 2, 3, 5, 255, 256, 257, 1000, 1024, 4099]
+
+
+def adamw_lists(g, sizes, dt, odd):
+    """tensors of their own, or (odd) views that start anywhere in one buffer"""
+    def cut(scale):
+        if not odd:
+            return [(randn(g, n) * scale).to(dt) for n in sizes]
+        flat = (randn(g, sum(sizes) + len(sizes)) * scale).to(dt)
+        at, out = 1, []
+        for n in sizes:
+            out.append(flat[at:at + n])
+            at += n + 1
+        return out
+    return cut(0.1), cut(0.01)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("odd", [False, True])
+def test_adamw_32_bit(dt, odd):
+    """Six fp32 roundings lie between the moments and their 64-bit values, some sixteen between p and its own (the moments', a square root, two
+    divisions, four products and sums); p rounds to its type at the end.  The reference continues from the step's own outputs."""
+    g = gen(21)
+    p, _ = adamw_lists(g, SIZES, dt, odd)
+    m = [torch.zeros(n, device=DEV) for n in SIZES]
+    v = [torch.zeros(n, device=DEV) for n in SIZES]
+    lr, b1, b2, eps, wd = 3e-3, 0.9, 0.99, 1e-8, 0.05
+    for t in range(1, 5):
+        _, gr = adamw_lists(g, SIZES, dt, odd)
+        P, M, V = ([q.cpu().double() for q in z] for z in (p, m, v))
+        mtk.adamw_step(p, gr, m, v, t, lr=lr, betas=(b1, b2), eps=eps, weight_decay=wd)
+        for i in range(len(SIZES)):
+            G = gr[i].cpu().double()
+            wm, wv = b1 * M[i] + (1 - b1) * G, b2 * V[i] + (1 - b2) * G * G
+            within(m[i], wm, 6 * U32 * (M[i].abs() + G.abs()))
+            within(v[i], wv, 6 * U32 * (V[i] + G * G) + 2.0**-140)
+            upd = lr / (1 - b1**t) * wm / (torch.sqrt(wv) / math.sqrt(1 - b2**t) + eps)
+            mag = lr / (1 - b1**t) * (M[i].abs() + G.abs()) / (torch.sqrt(wv) / math.sqrt(1 - b2**t) + eps)
+            want = P[i] * (1 - lr * wd) - upd
+            within(p[i], want, 4 * U32 * P[i].abs() + 16 * U32 * mag + half(dt) * (want.abs() + 1e-6) * 1.01 + tiny(dt))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("odd", [False, True])
+def test_adamw_8_bit_codes(dt, odd):
+    """Against the operator's own fp32 operations in numpy: codes, scales and (fp32) parameters are equal, step after step."""
+    g = gen(22)
+    p, _ = adamw_lists(g, SIZES, dt, odd)
+    code = lambda n: torch.zeros(n, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)  # noqa: E731
+    m, v = [code(n) for n in SIZES], [code(n) for n in SIZES]
+    ms, vs = ([torch.ones(-(-n // 256), device=DEV) for n in SIZES] for _ in range(2))
+    for t in range(1, 6):
+        _, gr = adamw_lists(g, SIZES, dt, odd)
+        for q in gr:
+            q *= 10 ** (t - 3)
+            q[::7] *= 1e-3
+            q[3::11] = 0
+        n = lambda z: [q.cpu().float().numpy() for q in z]  # noqa: E731
+        P, M, V, MS, VS = n(p), n(m), n(v), n(ms), n(vs)
+        mtk.adamw_step(p, gr, m, v, t, lr=1e-3, exp_avg_scales=ms, exp_avg_sq_scales=vs)
+        for i in range(len(SIZES)):
+            wp, wm, wms, wv, wvs = adamw8_reference(P[i], gr[i].cpu().float().numpy(), M[i], MS[i], V[i], VS[i], t)
+            assert np.array_equal(ms[i].cpu().numpy(), wms.astype(np.float32)) and np.array_equal(vs[i].cpu().numpy(), wvs.astype(np.float32)), (t, i)
+            assert np.array_equal(m[i].cpu().float().numpy(), wm.astype(np.float32)) and np.array_equal(v[i].cpu().float().numpy(), wv.astype(np.float32)), (t, i)
+            assert torch.equal(p[i].cpu(), torch.from_numpy(wp.astype(np.float32)).to(dt)), (t, i)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_keeps_bad_gradients_to_themselves(bits):
+    n = 700
+    g = gen(9)
+    p0, g0 = randn(g, n), randn(g, n)
+
+    def run(grad):
+        p = torch.nn.Parameter(p0.clone())
+        opt = mtk.AdamW([p], lr=1e-2, state_bits=bits)
+        for _ in range(3):
+            p.grad = grad.clone()
+            opt.step()
+        return p.detach().cpu(), opt.state[p]["exp_avg"].float().cpu(), opt.state[p]["exp_avg_sq"].float().cpu()
+
+    bad = g0.clone()
+    bad[5], bad[300], bad[699] = float("nan"), float("inf"), -float("inf")
+    keep = torch.ones(n, dtype=torch.bool)
+    keep[[5, 300, 699]] = False
+    zeroed = torch.where(keep.to(DEV), g0, torch.zeros_like(g0))
+    a, b = run(bad), run(zeroed)
+    for x, y in zip(a, b):
+        assert torch.equal(x[keep], y[keep])
+    assert bool(torch.isnan(a[0][~keep]).all())
+
+
+def test_adamw_extremes():
+    """Largest and smallest gradients: nothing overflows on the way that the formula does not overflow, and tiny averages keep a code."""
+    for value in (1e-38, 1e-30, 1e-22, 1e18):
+        for bits in (8, 32):
+            p = torch.nn.Parameter(torch.ones(300, device=DEV))
+            opt = mtk.AdamW([p], lr=1e-3, eps=0.0 if value > 1e-20 else 1e-8, weight_decay=0.0, state_bits=bits)
+            for _ in range(4):
+                p.grad = torch.full_like(p, value)
+                opt.step()
+            assert bool(torch.isfinite(p).all()), (value, bits)
+            assert bool((p <= 1).all())
+
+
+def test_adamw_many_tensors_and_empty_ones():
+    g = gen(30)
+    sizes = [int(v) for v in torch.randint(0, 600, (200,), generator=g)] + [0, 0]
+    ps = [torch.nn.Parameter(randn(g, n)) for n in sizes]
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    ours, theirs = mtk.AdamW(ps, lr=1e-2, weight_decay=0.1), torch.optim.AdamW(qs, lr=1e-2, weight_decay=0.1, foreach=False)
+    for _ in range(3):
+        for p, q in zip(ps, qs):
+            p.grad = randn(g, *p.shape)
+            q.grad = p.grad.clone()
+        ours.step()
+        theirs.step()
+    for p, q in zip(ps, qs):  # three steps of 1e-2, each off by some 16 half steps of fp32 at most, and p's own roundings
+        assert torch.allclose(p, q, rtol=3 * 8 * U32, atol=3 * 1e-2 * 32 * U32)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_adamw_state_round_trip(bits, dt):
+    """A saved and loaded state continues with the same bits, in the moments' own types."""
+    g = gen(31)
+    grads = [randn(g, 33, 17).to(dt) for _ in range(6)]
+    p0 = randn(g, 33, 17).to(dt)
+
+    def steps(p, opt, gs):
+        for q in gs:
+            p.grad = q.clone()
+            opt.step()
+
+    for capturable in (False, True):
+        kw = dict(lr=1e-2, state_bits=bits, capturable=capturable)
+        p = torch.nn.Parameter(p0.clone())
+        opt = mtk.AdamW([p], **kw)
+        steps(p, opt, grads)
+        q = torch.nn.Parameter(p0.clone())
+        first = mtk.AdamW([q], **kw)
+        steps(q, first, grads[:3])
+        second = mtk.AdamW([q], **kw)
+        second.load_state_dict(first.state_dict())
+        steps(q, second, grads[3:])
+        assert torch.equal(p, q)
+        for name in ("exp_avg", "exp_avg_sq"):
+            a, b = opt.state[p][name], second.state[q][name]
+            assert a.dtype == b.dtype == (torch.float8_e4m3fn if bits == 8 else torch.float32) and torch.equal(a.float(), b.float())
+        assert int(second.state[q]["step"]) == 6
+
+
+def test_adamw_groups_closures_and_refusals():
+    g = gen(32)
+    a, b, c = (torch.nn.Parameter(randn(g, 4, 5)) for _ in range(3))
+    frozen = c.detach().clone()
+    opt = mtk.AdamW([{"params": [a], "lr": 1e-1, "state_bits": 8}, {"params": [b, c], "weight_decay": 0.0}], lr=1e-3)
+
+    def closure():
+        opt.zero_grad()
+        loss = (a.sum() + (2 * b).sum()) ** 2
+        loss.backward()
+        return loss
+
+    before = (a.detach().clone(), b.detach().clone())
+    v = a._version
+    loss = opt.step(closure)
+    assert loss.requires_grad and a._version > v and torch.equal(c, frozen) and c not in opt.state
+    # a first step is lr * sign(g) but for eps: within a thousandth
+    assert torch.allclose((before[0] * (1 - 1e-1 * 1e-2) - a).abs(), torch.full_like(a, 1e-1), rtol=1e-3) and torch.allclose((before[1] - b).abs(), torch.full_like(b, 1e-3), rtol=1e-3)
+    a.grad = torch.zeros(5, 4, device=DEV).t()  # a gradient of other strides is copied
+    opt.step()
+    t = torch.nn.Parameter(randn(g, 4, 5).t())
+    t.grad = torch.ones_like(t)
+    with pytest.raises(ValueError, match="not contiguous"):
+        mtk.AdamW([t]).step()
+    s = torch.nn.Parameter(randn(g, 4))
+    s.grad = torch.ones(4, device=DEV).to_sparse()
+    with pytest.raises(ValueError, match="sparse"):
+        mtk.AdamW([s]).step()
+    d = torch.nn.Parameter(randn(g, 4).double())
+    d.grad = torch.ones_like(d)
+    with pytest.raises(ValueError):
+        mtk.AdamW([d]).step()
+    x = [torch.zeros(4, device=DEV)]
+    for bad in (dict(grads=[]), dict(grads=[torch.zeros(5, device=DEV)]), dict(grads=[torch.zeros(4, device=DEV).half()]), dict(exp_avgs=[torch.zeros(8, device=DEV)[::2]]),
+                dict(exp_avg_scales=x), dict(exp_avg_sqs=[torch.zeros(4)])):
+        kw = {**dict(params=x, grads=x, exp_avgs=x, exp_avg_sqs=x, step=1, lr=1e-3), **bad}
+        with pytest.raises(ValueError):
+            mtk.adamw_step(**kw)
+    with pytest.raises(AssertionError):
+        mtk.adamw_step(x, x, [torch.zeros(4, device=DEV)], [torch.zeros(4, device=DEV)], 0, lr=1e-3)
+
+
+# --------------------------------------------------------------------------------------------------- streams, graphs, together
+def test_operators_follow_the_current_stream():
+    """Inputs written on a side stream behind a long product, the operators called there: the results are those of the default stream."""
+    g = gen(40)
+    M, din, dout, r, E = 256, 64, 64, 8, 4
+    a = adapter_inputs(g, M, din, dout, r, E, torch.float32)
+    idx = torch.randint(-1, E, (M, 2), generator=g).to(DEV)
+    p0, g0 = randn(g, 1000), randn(g, 1000)
+
+    def work():
+        x = a["x"] * 2.0
+        plan = mtk.route_rows(idx, E)
+        h = mtk.combine_rows(mtk.dispatch_rows(call(a, x=x), plan), plan)
+        p = p0.clone()
+        mtk.adamw_step([p], [g0 * 2.0], [torch.zeros_like(p)], [torch.zeros_like(p)], 1, lr=1e-2)
+        return h, p
+
+    want = work()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    big = torch.randn(4096, 4096, device=DEV)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        for _ in range(8):
+            big = big @ big / 64
+        got = work()
+    s.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def ensemble(g, D=24, layers=(64, 48), E=3, rank=4):
+    torch.manual_seed(11)
+    net = mtk.MLPDiffusion(D, 0, mtk.IsTargetConditioned.NONE, mtk.DiffusionParameters(list(layers), 0.0)).to(DEV)
+    net.num_timesteps = 50
+    for p in net.parameters():
+        p.requires_grad_(False)
+    ens = mtk.LowRankEnsemble(net, E, rank=rank, alpha=2 * rank)
+    return net, ens
+
+
+def ensemble_reference(net, ens, x, t, idx, w):
+    """The ensemble in 64 bits, record by record's model: autograd's own graph on the CPU."""
+    d = lambda q: q.detach().cpu().double()  # noqa: E731
+    down = [d(p).requires_grad_() for p in ens.down]
+    up = [d(p).requires_grad_() for p in ens.up]
+    lin = [net.proj] + [b.linear for b in net.mlp.blocks] + [net.mlp.head]
+    f = mtk.timestep_frequencies(net.timestep_dimension)
+    arg = t.cpu().float()[:, None] * f[None]
+    e = torch.cat([torch.cos(arg), torch.sin(arg)], 1).double()
+    e = torch.nn.functional.silu(e @ d(net.timestep_embedding[0].weight).t() + d(net.timestep_embedding[0].bias))
+    e = e @ d(net.timestep_embedding[2].weight).t() + d(net.timestep_embedding[2].bias)
+    xd = d(x).requires_grad_()
+    out = 0
+    for j in range(idx.shape[1]):
+        h = xd
+        for i, m in enumerate(lin):
+            m_idx = idx[:, j].cpu()
+            on = (m_idx >= 0).double()[:, None] * ens.scale
+            A, B = down[i][m_idx.clamp(min=0)], up[i][m_idx.clamp(min=0)]
+            low = torch.bmm(torch.bmm(h[:, None], A.transpose(1, 2).contiguous()), B.transpose(1, 2).contiguous())[:, 0]
+            h = h @ d(m.weight).t() + d(m.bias) + on * low
+            if i == 0:
+                h = h + e
+            elif i < len(lin) - 1:
+                h = torch.relu(h)
+        out = out + w[:, j].cpu().double()[:, None] * h
+    return out, xd, down, up
+
+
+def close(got, want, rel=2e-4):
+    """Chains of four layers in fp32: some 4 (K + 4) 2^-24 of the magnitudes, against their cancelled sums; 2e-4 of the largest."""
+    got, want = got.detach().cpu().double(), want.detach()
+    assert float((got - want).abs().max()) <= rel * float(want.abs().max()), float((got - want).abs().max() / want.abs().max())
+
+
+def test_ensemble_starts_as_the_base_and_matches_64_bits():
+    g = gen(50)
+    net, ens = ensemble(g)
+    N, D, E = 150, 24, 3
+    x, t = randn(g, N, D), torch.randint(0, 50, (N,), generator=g).to(DEV)
+    idx = torch.randint(-1, E, (N, 2), generator=g).to(DEV)
+    with torch.no_grad():
+        close(ens(x, t, idx[:, 0]), net(x, t).cpu().double())
+        for p in ens.up:
+            p.copy_(randn(g, *p.shape) * 0.1)
+    w = torch.softmax(randn(g, N, 2), 1)
+    xg = x.clone().requires_grad_()
+    y = ens(xg, t, idx, w)
+    gy = randn(g, N, D)
+    grads = torch.autograd.grad(y, [xg, *ens.down, *ens.up], gy)
+    want, xd, down, up = ensemble_reference(net, ens, x, t, idx, w)
+    close(y, want)
+    wants = torch.autograd.grad(want, [xd, *down, *up], gy.cpu().double())
+    for a, b in zip(grads, wants):
+        close(a, b, 1e-3)  # ReLU borders: a record whose value is within rounding of 0 may take the other side
+    # one model per record and the mean of two equal ones agree; bad indices and timesteps are NaN in their records alone
+    one = ens(x, t, idx[:, 0])
+    two = ens(x, t, idx[:, :1].expand(N, 2))
+    assert torch.allclose(one, two, rtol=1e-6, atol=1e-6)
+    t2, idx2 = t.clone(), idx.clone()
+    t2[3], t2[4], idx2[5, 1] = 50, -1, E
+    bad = ens(x, t2, idx2, w)
+    rest = torch.ones(N, dtype=torch.bool)
+    rest[[3, 4, 5]] = False
+    assert bool(torch.isnan(bad[[3, 4, 5]]).all()) and torch.allclose(bad.cpu()[rest], y.detach().cpu()[rest], rtol=1e-5, atol=1e-5)
+
+
+def train(ens, opt, x, t, idx, noise, steps):
+    for _ in range(steps):
+        opt.zero_grad(set_to_none=False)
+        loss = ((ens(x, t, idx) - noise) ** 2).mean()
+        loss.backward()
+        opt.step()
+    return [p.detach().clone() for p in ens.parameters()]
+
+
+def test_training_the_ensemble_with_our_step_and_torchs():
+    """The operators as they are used: routed rows, adapted layers, their gradients, the step.  All optimizers see gradients of the same bits at
+    the first step; eps = 1 keeps the update proportional to them.  The update, at most lr |g|, is then off by some 16 half steps of
+    fp32 on either side, p by 4 of its own."""
+    g = gen(51)
+    N, D, E, kw = 120, 24, 3, dict(lr=1e-1, eps=1.0)
+    x, noise = randn(g, N, D), randn(g, N, D)
+    t, idx = torch.randint(0, 50, (N,), generator=g).to(DEV), torch.randint(0, E, (N,), generator=g).to(DEV)
+    results = []
+    for make in (lambda p: mtk.AdamW(p, **kw), lambda p: torch.optim.AdamW(p, **kw), lambda p: mtk.AdamW(p, **kw, capturable=True)):
+        _, ens = ensemble(gen(1))
+        start = [p.detach().clone() for p in ens.parameters()]
+        results.append(train(ens, make(ens.parameters()), x, t, idx, noise, 1))
+        grads = [p.grad for p in ens.parameters()]
+    for a, b, c, s, gr in zip(*results, start, grads):
+        assert torch.equal(a, c)
+        assert bool(((a - b).abs() <= 32 * U32 * 1e-1 * gr.abs() + 8 * U32 * s.abs() + 2.0**-149).all())
+    assert any(bool(gr.any()) for gr in grads)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_captured_training_step_replays_like_the_eager_one(bits):
+    g = gen(52)
+    N, D, E = 100, 24, 3
+    x, noise = randn(g, N, D), randn(g, N, D)
+    t, idx = torch.randint(0, 50, (N,), generator=g).to(DEV), torch.randint(0, E, (N,), generator=g).to(DEV)
+
+    def one(ens, opt):
+        grads = torch.autograd.grad(((ens(x, t, idx) - noise) ** 2).sum() / N, list(ens.parameters()))
+        for p, q in zip(ens.parameters(), grads):
+            p.grad = q
+        opt.step()
+
+    _, eager = ensemble(gen(1))
+    _, graph = ensemble(gen(1))
+    with torch.no_grad():
+        for a, b in zip(eager.parameters(), graph.parameters()):
+            b.copy_(a)
+    lr = torch.tensor(1e-3, device=DEV)
+    oe, og = (mtk.AdamW(m.parameters(), lr=lr, state_bits=bits, capturable=True) for m in (eager, graph))
+    plain = mtk.AdamW(graph.parameters(), lr=1e-3)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        one(graph, og)
+    torch.cuda.current_stream().wait_stream(side)
+    one(eager, oe)
+    cg = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(cg):
+        one(graph, og)
+    for i in range(4):
+        lr.fill_(1e-3 / (i + 1))
+        x.copy_(randn(gen(60 + i), N, D))
+        idx.copy_(torch.randint(-1, E, (N,), generator=gen(70 + i)))
+        one(eager, oe)
+        cg.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(eager.parameters(), graph.parameters()):
+            assert torch.equal(a, b), i
+        assert int(og.state[next(graph.parameters())]["step"]) == i + 2
+    refused = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captur"):
+        with torch.cuda.graph(refused):
+            plain.step()
+
+
+def test_our_step_refreshes_the_modules_that_cache_their_weights():
+    """TabSyn's denoiser keeps a packed copy keyed by its parameters' versions: after our step its loss is that of the new weights."""
+    torch.manual_seed(0)
+    model = mtk.tabsyn.Model(mtk.tabsyn.MLPDiffusion(12, dim_t=64)).to(DEV)
+    twin = mtk.tabsyn.Model(mtk.tabsyn.MLPDiffusion(12, dim_t=64)).to(DEV)
+    twin.load_state_dict(model.state_dict())
+    g = gen(61)
+    data, inj = randn(g, 40, 12), (randn(g, 40), randn(g, 40, 12))
+    opt = mtk.AdamW(model.parameters(), lr=1e-2)
+    losses = []
+    for _ in range(3):
+        loss = model(data, inj)
+        opt.zero_grad()
+        loss.backward()
+        opt.step()
+        losses.append(float(loss.detach()))
+    twin.load_state_dict(model.state_dict())
+    with torch.no_grad():
+        assert torch.equal(model(data, inj), twin(data, inj))
+    assert len(set(losses)) == 3
