@@ -519,17 +519,18 @@ int mtk_rows_combine(int64_t n_rows, int k, int64_t D, int dtype, const void* y,
  * dense; all of `dtype`.  s_e = scales[e] (fp32), or `scale` where scales is NULL.  act: enum mtk_activation.
  * saved (mtk_adapter_saved_bytes, 256-byte aligned): holds s_e x down_e^T; mtk_adapter_backward reads it, and with keep = 0 it is
  * scratch.  mtk_adapter_backward: dx [M, din], ddown, dup (each may be NULL) from dy [M, dout] dense, for the same arguments;
- * y is read under an activation only.  W and bias are frozen and get no gradient.  work: mtk_adapter_work_bytes, 256-byte aligned.
+ * y is read under an activation only.  W and bias are frozen and get no gradient.  work: mtk_adapter_work_bytes of the direction, 256-byte
+ * aligned (0: may be NULL).
  * Sums in fp32; identical run to run. */
 #define MTK_ADAPTER_MAX_RANK 256
 #define MTK_ADAPTER_MAX_WIDTH 8192
 #define MTK_ADAPTER_MAX_ROWS 16777216
 enum mtk_activation { MTK_ACT_NONE = 0, MTK_ACT_RELU = 1 };
 int64_t mtk_adapter_saved_bytes(int64_t M, int r, int dtype);
-int64_t mtk_adapter_work_bytes(int64_t M, int din, int dout, int r, int n_models, int dtype, int act);
+int64_t mtk_adapter_work_bytes(int64_t M, int din, int dout, int r, int n_models, int dtype, int act, int backward);
 int mtk_adapter_forward(int64_t M, int din, int dout, int r, int n_models, int dtype, const void* x, int64_t x_ld, const void* W, const void* bias,
                         const void* down, const void* up, const int32_t* offsets, const float* scales, double scale, int act, int keep, void* y,
-                        void* saved, int64_t saved_bytes, mtk_stream stream);
+                        void* saved, int64_t saved_bytes, void* work, int64_t work_bytes, mtk_stream stream);
 int mtk_adapter_backward(int64_t M, int din, int dout, int r, int n_models, int dtype, const void* x, int64_t x_ld, const void* W, const void* down,
                          const void* up, const int32_t* offsets, const float* scales, double scale, int act, const void* y, const void* dy,
                          const void* saved, void* dx, void* ddown, void* dup, void* work, int64_t work_bytes, mtk_stream stream);

@@ -100,8 +100,8 @@ _SIGS = {
     "mtk_rows_dispatch": (C.c_int, [_i64, _i32, _i64, _i32, _p, _i64, _p, _p, _p, _p, _p, _p]),
     "mtk_rows_combine": (C.c_int, [_i64, _i32, _i64, _i32, _p, _i64, _p, _p, _p, _p]),
     "mtk_adapter_saved_bytes": (_i64, [_i64, _i32, _i32]),
-    "mtk_adapter_work_bytes": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32, _i32]),
-    "mtk_adapter_forward": (C.c_int, [_i64, _i32, _i32, _i32, _i32, _i32, _p, _i64, _p, _p, _p, _p, _p, _p, C.c_double, _i32, _i32, _p, _p, _i64, _p]),
+    "mtk_adapter_work_bytes": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "mtk_adapter_forward": (C.c_int, [_i64, _i32, _i32, _i32, _i32, _i32, _p, _i64, _p, _p, _p, _p, _p, _p, C.c_double, _i32, _i32, _p, _p, _i64, _p, _i64, _p]),
     "mtk_adapter_backward": (C.c_int, [_i64, _i32, _i32, _i32, _i32, _i32, _p, _i64, _p, _p, _p, _p, _p, C.c_double, _i32, _p, _p, _p, _p, _p, _p, _p,
                                        _i64, _p]),
     "mtk_adamw_scales": (_i64, [_i64]),
@@ -159,6 +159,17 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def launch(device: torch.device, fn, *args) -> None:
+    """``fn(*args, stream)`` with ``device`` current and its current stream, checked.  For entry points of a few microseconds: the device guard
+    and torch's stream object cost as much as the launch, so the guard is taken only where another device is current."""
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
 
 
 def require_cuda(t: torch.Tensor, what: str) -> None:

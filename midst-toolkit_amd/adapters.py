@@ -18,33 +18,36 @@ from torch import Tensor, nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import check
+from ._lib import launch
 from .model import MLPDiffusion, timestep_frequencies
-from .routing import MAX_GROUPS, RowPlan, combine_rows, dispatch_rows, dtype_code, route_rows, rows_of
+from .routing import DTYPES, MAX_GROUPS, RowPlan, combine_rows, dispatch_rows, dtype_code, route_rows, rows_of
 
 MAX_RANK, MAX_WIDTH, MAX_ROWS = 256, 8192, 16777216  # MTK_ADAPTER_MAX_* of include/mtk.h
 ACTIVATIONS = {"none": 0, "relu": 1}  # enum mtk_activation
 
 
+def _forward(x, weight, bias, down, up, offsets, scales, scale, act, keep):
+    """mtk_adapter_forward: (y, what the backward reads of it)"""
+    dev, (M, din), (E, r, _), dout = x.device, x.shape, down.shape, weight.shape[0]
+    l, dt = _lib.lib(), DTYPES[x.dtype]
+    y = torch.empty((M, dout), dtype=x.dtype, device=dev)
+    saved = torch.empty(l.mtk_adapter_saved_bytes(M, r, dt), dtype=torch.uint8, device=dev)
+    if M:
+        need = l.mtk_adapter_work_bytes(M, din, dout, r, E, dt, act, 0)
+        work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        launch(dev, l.mtk_adapter_forward, M, din, dout, r, E, dt, x.data_ptr(), x.stride(0), weight.data_ptr(), None if bias is None else bias.data_ptr(),
+               down.data_ptr(), up.data_ptr(), offsets.data_ptr(), None if scales is None else scales.data_ptr(), scale, act, int(keep), y.data_ptr(),
+               saved.data_ptr(), saved.numel(), None if work is None else work.data_ptr(), need)
+    return y, saved
+
+
 class _AdapterLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, down, up, offsets, scales, scale, act):
-        dev, (M, din), (E, r, _), dout = x.device, x.shape, down.shape, weight.shape[0]
-        l = _lib.lib()
-        dt = dtype_code(x, "adapter_linear")
         xr = rows_of(x)
-        keep = any(ctx.needs_input_grad)
-        y = torch.empty((M, dout), dtype=x.dtype, device=dev)
-        saved = torch.empty(l.mtk_adapter_saved_bytes(M, r, dt), dtype=torch.uint8, device=dev)
-        if M:
-            with torch.cuda.device(dev):
-                check(l.mtk_adapter_forward(M, din, dout, r, E, dt, xr.data_ptr(), xr.stride(0), weight.data_ptr(),
-                                            None if bias is None else bias.data_ptr(), down.data_ptr(), up.data_ptr(), offsets.data_ptr(),
-                                            None if scales is None else scales.data_ptr(), scale, act, int(keep), y.data_ptr(), saved.data_ptr(),
-                                            saved.numel(), _lib.stream_handle(dev)))
-        if keep:
-            ctx.save_for_backward(xr, weight, down, up, offsets, scales, y if act else None, saved)
-            ctx.scale, ctx.act, ctx.dt = scale, act, dt
+        y, saved = _forward(xr, weight, bias, down, up, offsets, scales, scale, act, True)
+        ctx.save_for_backward(xr, weight, down, up, offsets, scales, y if act else None, saved)
+        ctx.scale, ctx.act = scale, act
         return y
 
     @staticmethod
@@ -52,7 +55,7 @@ class _AdapterLinear(torch.autograd.Function):
     def backward(ctx, g):
         x, weight, down, up, offsets, scales, y, saved = ctx.saved_tensors
         dev, (M, din), (E, r, _), dout = x.device, x.shape, down.shape, weight.shape[0]
-        l = _lib.lib()
+        l, dt = _lib.lib(), DTYPES[x.dtype]
         want = ctx.needs_input_grad
         dx = torch.empty((M, din), dtype=x.dtype, device=dev) if want[0] else None
         if M == 0:
@@ -60,12 +63,10 @@ class _AdapterLinear(torch.autograd.Function):
         ddown = torch.empty_like(down) if want[3] else None
         dup = torch.empty_like(up) if want[4] else None
         g = g.contiguous()
-        work = torch.empty(l.mtk_adapter_work_bytes(M, din, dout, r, E, ctx.dt, ctx.act), dtype=torch.uint8, device=dev)
+        work = torch.empty(l.mtk_adapter_work_bytes(M, din, dout, r, E, dt, ctx.act, 1), dtype=torch.uint8, device=dev)
         p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        with torch.cuda.device(dev):
-            check(l.mtk_adapter_backward(M, din, dout, r, E, ctx.dt, x.data_ptr(), x.stride(0), weight.data_ptr(), down.data_ptr(), up.data_ptr(),
-                                         offsets.data_ptr(), p(scales), ctx.scale, ctx.act, p(y), g.data_ptr(), saved.data_ptr(), p(dx), p(ddown), p(dup),
-                                         work.data_ptr(), work.numel(), _lib.stream_handle(dev)))
+        launch(dev, l.mtk_adapter_backward, M, din, dout, r, E, dt, x.data_ptr(), x.stride(0), weight.data_ptr(), down.data_ptr(), up.data_ptr(),
+               offsets.data_ptr(), p(scales), ctx.scale, ctx.act, p(y), g.data_ptr(), saved.data_ptr(), p(dx), p(ddown), p(dup), work.data_ptr(), work.numel())
         return dx, None, None, ddown, dup, None, None, None, None
 
 
@@ -81,7 +82,7 @@ def adapter_linear(x: Tensor, weight: Tensor, bias: Tensor | None, down: Tensor,
         offsets = offsets.offsets
     if not x.is_cuda:
         raise RuntimeError("adapter_linear: midst_toolkit_amd has no CPU path; move the rows to the MI355X")
-    code = dtype_code(x, "adapter_linear")
+    dtype_code(x, "adapter_linear")
     if x.dim() != 2 or weight.dim() != 2 or down.dim() != 3 or up.dim() != 3:
         raise ValueError("adapter_linear: x [M, din], weight [dout, din], down [E, r, din], up [E, dout, r]")
     (M, din), (E, r, _), dout = x.shape, down.shape, weight.shape[0]
@@ -100,16 +101,20 @@ def adapter_linear(x: Tensor, weight: Tensor, bias: Tensor | None, down: Tensor,
         if scale.dtype != torch.float32 or tuple(scale.shape) != (E,):
             raise ValueError(f"adapter_linear: scale is a number or float32 [{E}], got {scale.dtype} {tuple(scale.shape)}")
         scales, scale = scale.detach().contiguous(), 1.0
-    for t, name in ((weight, "weight"), (bias, "bias"), (down, "down"), (up, "up"), (offsets, "offsets"), (scales, "scale")):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"adapter_linear: x on {x.device}, {name} on {t.device}")
+    at, dt = x.get_device(), x.dtype
     for t, name in ((weight, "weight"), (bias, "bias"), (down, "down"), (up, "up")):
-        if t is not None and t.dtype != x.dtype:
-            raise ValueError(f"adapter_linear: x is {x.dtype}, {name} {t.dtype}")
-    if torch.is_grad_enabled() and (weight.requires_grad or (bias is not None and bias.requires_grad)):
-        raise NotImplementedError("adapter_linear: the shared layer is frozen; detach weight and bias")
+        if t is not None and (t.get_device() != at or t.dtype != dt):
+            raise ValueError(f"adapter_linear: x is {dt} on {x.device}, {name} {t.dtype} on {t.device}")
+    if offsets.get_device() != at or (scales is not None and scales.get_device() != at):
+        raise ValueError(f"adapter_linear: x on {x.device}, offsets on {offsets.device}" + ("" if scales is None else f", scale on {scales.device}"))
     c = lambda t: t if t is None or t.is_contiguous() else t.contiguous()  # noqa: E731
-    return _AdapterLinear.apply(x, c(weight), c(bias), c(down), c(up), c(offsets), scales, float(scale), ACTIVATIONS[activation])
+    args = (c(weight), c(bias), c(down), c(up), c(offsets), scales, float(scale), ACTIVATIONS[activation])
+    if torch.is_grad_enabled():
+        if weight.requires_grad or (bias is not None and bias.requires_grad):
+            raise NotImplementedError("adapter_linear: the shared layer is frozen; detach weight and bias")
+        if x.requires_grad or down.requires_grad or up.requires_grad:
+            return _AdapterLinear.apply(x, *args)
+    return _forward(rows_of(x), *args, False)[0]
 
 
 class LowRankEnsemble(nn.Module):

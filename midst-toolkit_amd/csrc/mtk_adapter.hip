@@ -13,11 +13,14 @@
 // A row's product never meets another model's factors in an accumulator (0 x inf is NaN): products are made per model and
 // SELECTED by row, so one diverged model leaves the others' rows alone.
 // u and t = s_e g B_e are rounded to the rows' type (they are MFMA operands); every sum is in fp32.
+#include <type_traits>
+
 #include "mtk_lowp.h"
 
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef mtk_bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef mtk_f16 f16x8 __attribute__((ext_vector_type(8)));
@@ -49,10 +52,9 @@ template <typename T> __device__ __forceinline__ mtk_vec<T> zero_piece() {
     return v;
 }
 
-// elements of the low rank as stored in u: whole MFMA steps
-template <typename T> constexpr int kRankStep = 32 / (int)sizeof(T);
-template <typename T> __host__ __device__ constexpr int rank_pad(int r) { return (r + kRankStep<T> - 1) / kRankStep<T> * kRankStep<T>; }
-inline int rank_pad_of(int r, int dtype) { return dtype == MTK_DT_F32 ? rank_pad<float>(r) : rank_pad<mtk_bf16>(r); }
+// A k-block is one 128-byte line of a row; the low-rank rows u are stored in whole k-blocks, zeros behind the rank
+template <typename T> constexpr int kLine = 128 / (int)sizeof(T);
+inline int rank_pad(int r, int dtype) { return (int)mtk_up(r, 128 / mtk_dtype_size(dtype)); }
 constexpr int kRankT = 16;  // rows of u^T come in whole 16s
 
 // The models that own rows [at, end): each call yields one (e, first row, behind its last row).  Offsets are clamped and every step moves
@@ -96,25 +98,33 @@ struct ShrinkArgs {
     int64_t Mp;  // row stride of uT
 };
 
-// u[row][j] = s_e sum_k x[row][k] F_e[j][k] (F: [E][r][K]); with uT also its transpose, which the factors' gradients multiply
+// u[row][j] = s_e sum_k x[row][k] F_e[j][k] (F: [E][r][K]); with uT also its transpose, which the factors' gradients multiply.
+// A workgroup takes 32 rows, its waves split k.  Where there are few rows, gridDim.y workgroups share a tile's models in turn (one model's
+// product is a chain of loads of some microseconds); the first of them clears what no model owns.
 template <typename T, int NW>
 __global__ __launch_bounds__(64 * NW) void k_shrink(ShrinkArgs g, const T* __restrict__ x, const T* __restrict__ F, T* __restrict__ u, T* __restrict__ uT) {
-    constexpr int V = mtk_piece<T>::n, KB = 8 * V;  // a k-block is a 128-byte line of a row
+    constexpr int V = mtk_piece<T>::n, KB = kLine<T>, PT = 32 * 32 / (64 * NW);
     __shared__ float part[NW][32][33];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hh = lane >> 5;
     const int64_t m0 = (int64_t)blockIdx.x * 32;
     const int64_t end = m0 + 32 < g.M ? m0 + 32 : g.M;
     const int64_t row = m0 + li < g.M ? m0 + li : g.M - 1;
     const T* xr = x + row * g.x_ld;
-    const int jw = uT ? (int)mtk_up(g.rp, kRankT) : g.rp;
+    const int jt = (int)mtk_up(g.r, kRankT), jw = uT && jt > g.rp ? jt : g.rp;
     for (int j0 = 0; j0 < jw; j0 += 32) {
         Owners own{g.offsets, g.E, m0, end};
-        int e;
+        int e, turn = 0;
         int64_t a, b;
-        float keep[32 * 32 / (64 * NW)];
+        float keep[PT];
+        unsigned mine = 0, all = 0;  // rows computed here / owned by any model
 #pragma unroll
-        for (int i = 0; i < 32 * 32 / (64 * NW); ++i) keep[i] = 0.f;
+        for (int i = 0; i < PT; ++i) keep[i] = 0.f;
         while (own.next(e, a, b)) {
+            const unsigned bits = (unsigned)(((1ull << (b - a)) - 1) << (a - m0));
+            all |= bits;
+            if (turn++ % (int)gridDim.y != (int)blockIdx.y) continue;
+            mine |= bits;
+            if (j0 >= g.r) continue;
             const int j = j0 + li < g.r ? j0 + li : g.r - 1;
             const T* fr = F + ((int64_t)e * g.r + j) * g.K;
             f32x16 acc = {};
@@ -144,27 +154,28 @@ __global__ __launch_bounds__(64 * NW) void k_shrink(ShrinkArgs g, const T* __res
             __syncthreads();
             const float s = g.scales ? g.scales[e] : g.scale;
 #pragma unroll
-            for (int i = 0; i < 32 * 32 / (64 * NW); ++i) {
+            for (int i = 0; i < PT; ++i) {
                 const int q = tid + i * 64 * NW, rr = q >> 5, jj = q & 31;
                 float v = 0.f;
 #pragma unroll
                 for (int w = 0; w < NW; ++w) v += part[w][rr][jj];
-                if (m0 + rr >= a && m0 + rr < b && j0 + jj < g.r) keep[i] = s * v;
+                if ((bits >> rr & 1) && j0 + jj < g.r) keep[i] = s * v;
             }
             __syncthreads();
         }
+        if (blockIdx.y == 0) mine |= ~all;  // rows without a model: zeros
 #pragma unroll
-        for (int i = 0; i < 32 * 32 / (64 * NW); ++i) {
+        for (int i = 0; i < PT; ++i) {
             const int q = tid + i * 64 * NW, rr = q >> 5, jj = q & 31;
-            if (m0 + rr < g.M && j0 + jj < g.rp) u[(m0 + rr) * g.rp + j0 + jj] = (T)keep[i];
+            if ((mine >> rr & 1) && m0 + rr < g.M && j0 + jj < g.rp) u[(m0 + rr) * g.rp + j0 + jj] = (T)keep[i];
             if (uT) part[0][rr][jj] = keep[i];
         }
         if (uT) {  // through LDS: a thread per (j, record), records fastest
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 32 * 32 / (64 * NW); ++i) {
+            for (int i = 0; i < PT; ++i) {
                 const int q = tid + i * 64 * NW, rr = q & 31, jj = q >> 5;
-                if (j0 + jj < jw) uT[(int64_t)(j0 + jj) * g.Mp + m0 + rr] = (T)part[0][rr][jj];  // Mp covers whole tiles of 32 rows
+                if ((mine >> rr & 1) && j0 + jj < jt) uT[(int64_t)(j0 + jj) * g.Mp + m0 + rr] = (T)part[0][rr][jj];  // Mp covers whole tiles of 32 rows
             }
             __syncthreads();
         }
@@ -172,144 +183,391 @@ __global__ __launch_bounds__(64 * NW) void k_shrink(ShrinkArgs g, const T* __res
 }
 
 // ------------------------------------------------------------------------------------------------------------------ linear
+// y = act(x W^T + b + u B_e^T).  Weights are the MFMA's A operand: a lane then holds consecutive features of one record.
+//
+// k_linear, for more than a few rows: persistent workgroups walk tiles of BM rows x BN features; the k-blocks of ALL their tiles form one
+// stream of LDS-DMA (three buffers for rows, two for weights), so a tile's epilogue runs with the next tile's first blocks in flight.
+// The low-rank product is the last k-blocks of a tile: rows of u against rows of B_e (both zero behind the rank), the same
+// instructions through the same buffers.  That needs one model per tile; a tile with several (or none) takes a block of zeros there and a
+// several-model tile adds its products in the epilogue, made per model and selected by row.  With fewer rows a model than a tile
+// has (nkx = 0) all tiles do.
+// The stream wants whole, 16-byte aligned lines: k_prep pads what is not, and lays out B, the bias in fp32 and the tiles' models.
 struct LinearArgs {
-    int64_t M, x_ld;
-    int N, K, r, rp, E;
+    int64_t M, MT;        // rows, row tiles
+    int N, nb_n;          // features, feature tiles
+    int nkb, nkx;         // k-blocks of the shared and of the low-rank product
+    int64_t x_ld, w_ld;   // row strides, in bytes
+    const void *X, *W, *U, *Bp;  // U [M][nkx lines], Bp [E + 1][N][nkx lines], model E: zeros
+    const float* bias;    // [nb_n * BN]
+    const int32_t* owner; // [MT] the tile's model; E: none; -1: several
     const int32_t* offsets;
-    int relu;
+    int E, relu;
+    const void* low;      // [E][N][low_ld] B_e for the epilogue: the padded Bp, or B itself
+    int low_ld, rp;       // rp: elements of a row of U
 };
 
-constexpr int TM = 128, TN = 128;
+template <int WR, int MW, int NT> struct Geo {  // eight waves as WR x WC, each MW x NT tiles of 32 x 32
+    static constexpr int WC = 8 / WR, WN = NT * 32, BM = WR * MW * 32, BN = WC * WN;
+    static constexpr int kTileX = BM * 128, kTileW = BN * 128;   // bytes of a k-block
+    static constexpr int XPW = BM / 64, WPW = BN / 64;           // 8-row, 1 KiB pieces per wave
+    static constexpr int kLds = 3 * kTileX + 2 * kTileW;
+};
 
-// y = act(x W^T + b + u B_e^T): tiles of 128 rows x 128 features, four waves of 64 x 64, k-blocks of 128 bytes double buffered in LDS.
-// Weights are the MFMA's A operand: a lane then holds consecutive features of one record, which leave as 8- or 16-byte pieces.
-template <typename T>
-__global__ __launch_bounds__(256) void k_linear(LinearArgs g, const T* __restrict__ x, const T* __restrict__ W, const T* __restrict__ bias, const T* __restrict__ u,
-                                                const T* __restrict__ up, T* __restrict__ y) {
-    constexpr int V = mtk_piece<T>::n, KB = 8 * V;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2][2][TM * 128];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hh = lane >> 5;
-    const int wr = wave >> 1, wc = wave & 1;
-    const int nb = (g.N + TN - 1) / TN;
-    const int64_t m0 = (int64_t)(blockIdx.x / nb) * TM;
-    const int n0 = (int)(blockIdx.x % nb) * TN;
+extern __shared__ __attribute__((aligned(16))) unsigned char ad_smem[];
 
-    mtk_vec<T> px[4], pw[4];
-    auto fetch = [&](int k0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int p = tid + i * 256, rr = p >> 3, k = k0 + (p & 7) * V;
-            const int64_t row = m0 + rr < g.M ? m0 + rr : g.M - 1;
-            const int n = n0 + rr < g.N ? n0 + rr : g.N - 1;
-            const T *xp = x + row * g.x_ld + k, *wp = W + (int64_t)n * g.K + k;
-            if (k0 + KB <= g.K) {
-                px[i] = mtk_ld(xp);
-                pw[i] = mtk_ld(wp);
-            } else {
-                px[i] = mtk_ld_n(xp, g.K - k);
-                pw[i] = mtk_ld_n(wp, g.K - k);
-            }
+// a uniform value through the scalar cache: a vector load would wait for all the DMA requested before it
+__device__ __forceinline__ int scalar_load(const int32_t* p) {
+    int v;
+    asm volatile("s_load_dword %0, %1, 0x0\n\ts_waitcnt lgkmcnt(0)" : "=&s"(v) : "s"(p) : "memory");
+    return v;
+}
+
+template <typename T, int WR, int MW, int NT>
+__global__ __launch_bounds__(512, 1) void k_linear(LinearArgs g, T* __restrict__ y) {
+    typedef Geo<WR, MW, NT> G;
+    constexpr int V = mtk_piece<T>::n, kWBase = 3 * G::kTileX;
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    const int wv = __builtin_amdgcn_readfirstlane(wid);
+    const int wr = wv / G::WC, wc = wv % G::WC, li = lane & 31, hh = lane >> 5;
+    // workgroups go round-robin over the 8 XCDs: each XCD takes a contiguous eighth of the tiles (features fastest), so a row tile's
+    // feature tiles run side by side on one XCD's L2 and every XCD has work
+    const int xcd = blockIdx.x & 7, wq = blockIdx.x >> 3, wstride = gridDim.x >> 3;
+    const int64_t tiles = g.MT * g.nb_n, per = (tiles + 7) / 8, first = xcd * per;
+    const int64_t slots = tiles - first < per ? tiles - first : per;
+    if (wq >= slots) return;
+    const int nk = g.nkb + g.nkx;
+
+    // DMA of one 8-row piece (64 lanes x 16 bytes): lane -> row lane >> 3, piece slot lane & 7.  The LDS image is linear in the lane, so the
+    // bank swizzle (slot s of row r holds piece s ^ ((r >> 1) & 7)) is applied to the global address.  Rows behind the last are
+    // clamped: they are read again, never stored.  M0 (the LDS address) is written with every piece; the compiler puts nothing there.
+    const int lr = lane >> 3;
+    auto dma = [&](const unsigned char* base, int64_t ld, int64_t rows, int chunk, int64_t kbyte, unsigned dst) {
+        const int lc = ((lane & 7) ^ ((lr >> 1) | ((chunk & 1) << 2))) * 16;
+        const unsigned char* gp = base + kbyte;
+        unsigned voff;
+        if (rows >= chunk * 8 + 8) {
+            gp += (int64_t)chunk * 8 * ld;
+            voff = (unsigned)(lr * (int)ld + lc);
+        } else {
+            const int rr = chunk * 8 + lr, last = (int)rows - 1;
+            voff = (unsigned)((rr < last ? rr : last) * (int)ld + lc);
+        }
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(gp), "s"(dst) : "memory");
+    };
+    struct Cursor { int64_t slot; int kb; int buf; };
+    Cursor cx{wq, 0, 0}, cw{wq, 0, 0};
+    // sources of the tiles at the cursors
+    const unsigned char *xb = nullptr, *ub = nullptr, *wb = nullptr, *bb = nullptr;
+    int64_t xrows = 0, wrows = 0;
+    const int64_t lo_ld = (int64_t)g.nkx * 128;
+    auto x_tile = [&]() {
+        const int64_t m0 = ((first + cx.slot) / g.nb_n) * G::BM;
+        xb = (const unsigned char*)g.X + m0 * g.x_ld;
+        ub = (const unsigned char*)g.U + m0 * lo_ld;
+        xrows = g.M - m0;
+    };
+    auto w_tile = [&]() {
+        const int64_t id = first + cw.slot, mt = id / g.nb_n;
+        const int64_t n0 = (id - mt * g.nb_n) * G::BN;
+        int e = g.E;
+        if (g.nkx) e = scalar_load(g.owner + mt);
+        e = e < 0 || e > g.E ? g.E : e;
+        wb = (const unsigned char*)g.W + n0 * g.w_ld;
+        bb = (const unsigned char*)g.Bp + ((int64_t)e * g.N + n0) * lo_ld;
+        wrows = g.N - n0;
+    };
+    auto x_op = [&](int j) {
+        if (cx.slot >= slots) return;
+        const int chunk = wv * G::XPW + j;
+        const unsigned dst = (unsigned)(cx.buf * G::kTileX + chunk * 1024);
+        if (cx.kb < g.nkb) dma(xb, g.x_ld, xrows, chunk, (int64_t)cx.kb * 128, dst);
+        else dma(ub, lo_ld, xrows, chunk, (int64_t)(cx.kb - g.nkb) * 128, dst);
+    };
+    auto w_op = [&](int j) {
+        if (cw.slot >= slots) return;
+        const int chunk = wv * G::WPW + j;
+        const unsigned dst = (unsigned)(kWBase + cw.buf * G::kTileW + chunk * 1024);
+        if (cw.kb < g.nkb) dma(wb, g.w_ld, wrows, chunk, (int64_t)cw.kb * 128, dst);
+        else dma(bb, lo_ld, wrows, chunk, (int64_t)(cw.kb - g.nkb) * 128, dst);
+    };
+    auto x_advance = [&]() {
+        if (cx.slot >= slots) return;
+        cx.buf = cx.buf == 2 ? 0 : cx.buf + 1;
+        if (++cx.kb == nk) {
+            cx.kb = 0;
+            cx.slot += wstride;
+            if (cx.slot < slots) x_tile();
         }
     };
-    // piece p of row r sits at slot p ^ ((r >> 1) & 7): the 16 lanes that ds_read_b128 serves together then touch 16 different slots
-    auto put = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int p = tid + i * 256, rr = p >> 3, at = rr * 128 + (((p & 7) ^ ((rr >> 1) & 7)) * 16);
-            *reinterpret_cast<uint4*>(&lds[buf][0][at]) = __builtin_bit_cast(uint4, px[i]);
-            *reinterpret_cast<uint4*>(&lds[buf][1][at]) = __builtin_bit_cast(uint4, pw[i]);
+    auto w_advance = [&]() {
+        if (cw.slot >= slots) return;
+        cw.buf ^= 1;
+        if (++cw.kb == nk) {
+            cw.kb = 0;
+            cw.slot += wstride;
+            if (cw.slot < slots) w_tile();
         }
     };
-    auto frag = [&](int buf, int op, int rr, int kp) {
-        return __builtin_bit_cast(mtk_vec<T>, *reinterpret_cast<const uint4*>(&lds[buf][op][rr * 128 + ((kp ^ ((rr >> 1) & 7)) * 16)]));
+    const unsigned char* lds = ad_smem;
+    struct Frags { mtk_vec<T> x[MW], w[NT]; };
+    auto read_frags = [&](Frags& f, int xi, int wi, int ks) {
+#pragma unroll
+        for (int q = 0; q < MW; ++q) {
+            const int ra = (wr * MW + q) * 32 + li, kp = ks * 2 + hh;
+            f.x[q] = __builtin_bit_cast(mtk_vec<T>, *reinterpret_cast<const uint4*>(lds + xi * G::kTileX + ra * 128 + ((kp ^ ((ra >> 1) & 7)) * 16)));
+        }
+#pragma unroll
+        for (int q = 0; q < NT; ++q) {
+            const int rb = wc * G::WN + q * 32 + li, kp = ks * 2 + hh;
+            f.w[q] = __builtin_bit_cast(mtk_vec<T>, *reinterpret_cast<const uint4*>(lds + kWBase + wi * G::kTileW + rb * 128 + ((kp ^ ((rb >> 1) & 7)) * 16)));
+        }
+    };
+    f32x16 acc[MW][NT];
+    auto mma_row = [&](const Frags& f, int mt) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = mma32(f.w[nt], f.x[mt], acc[mt][nt]);
+    };
+    auto mma_all = [&](const Frags& f) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int mt = 0; mt < MW; ++mt) mma_row(f, mt);
+        __builtin_amdgcn_sched_barrier(0);
     };
 
-    f32x16 acc[2][2] = {};
-    const int nkb = (g.K + KB - 1) / KB;
-    fetch(0);
-    put(0);
-    __syncthreads();
-    for (int kb = 0; kb < nkb; ++kb) {
-        if (kb + 1 < nkb) fetch((kb + 1) * KB);
-        const int buf = kb & 1;
+    // One k-block: four steps of two pieces, fragments read one step ahead.  The barrier sits before the last step's MFMAs; the fragment reads
+    // and the DMA requests behind it ride under them.  After the barrier of block c a wave requests its pieces of weight block c + 2,
+    // THEN of row block c + 3: loads return in order, so at the next wait vmcnt(XPW) - all but those last row pieces - means that
+    // weight block c + 2 and row block c + 2 (requested a block earlier) have landed.
+    Frags F0, F1;
+    x_tile();
+    w_tile();
+    for (int b = 0; b < 3; ++b) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            mtk_vec<T> fx[2], fw[2];
+        for (int j = 0; j < G::XPW; ++j) x_op(j);
+        x_advance();
+        if (b < 2) {
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                fx[q] = frag(buf, 0, wr * 64 + q * 32 + li, 2 * s + hh);
-                fw[q] = frag(buf, 1, wc * 64 + q * 32 + li, 2 * s + hh);
-            }
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-                for (int nt = 0; nt < 2; ++nt) acc[mt][nt] = mma32(fw[nt], fx[mt], acc[mt][nt]);
+            for (int j = 0; j < G::WPW; ++j) w_op(j);
+            w_advance();
         }
-        if (kb + 1 < nkb) put(buf ^ 1);
-        __syncthreads();
     }
-
-    int64_t rows[2];
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    int xi = 0, wi = 0;   // buffers of the block being consumed
+    bool x_tail = false;  // the previous block's tail requested row pieces after its weight pieces
+    for (int64_t slot = wq; slot < slots; slot += wstride) {
+        const int64_t id = first + slot, mtile = id / g.nb_n;
+        const int64_t m0 = mtile * G::BM;
+        const int n0 = (int)(id - mtile * g.nb_n) * G::BN;
+        // the accumulators start from the bias, through the SCALAR cache: vector loads here would queue behind the DMA in flight
+        {
+            const float* bp = g.bias + n0 + wc * G::WN;
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) rows[mt] = m0 + wr * 64 + mt * 32 + li;
-    if (up) {
-        const int64_t w0 = m0 + wr * 64;
-        Owners own{g.offsets, g.E, w0, w0 + 64 < g.M ? w0 + 64 : g.M};
+            for (int nt = 0; nt < NT; ++nt) {
+                f32x8 b0, b1, b2, b3;
+                asm volatile("s_load_dwordx8 %0, %4, 0x0\n\ts_load_dwordx8 %1, %4, 0x20\n\ts_load_dwordx8 %2, %4, 0x40\n\ts_load_dwordx8 %3, %4, 0x60\n\t"
+                             "s_waitcnt lgkmcnt(0)"
+                             : "=&s"(b0), "=&s"(b1), "=&s"(b2), "=&s"(b3)
+                             : "s"(bp + nt * 32)
+                             : "memory");
+                const f32x8 bq[4] = {b0, b1, b2, b3};
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float bv = hh ? bq[q][4 + j] : bq[q][j];
+#pragma unroll
+                        for (int a = 0; a < MW; ++a) acc[a][nt][4 * q + j] = bv;
+                    }
+            }
+        }
+        read_frags(F0, xi, wi, 0);
+        for (int kb = 0; kb < nk; ++kb) {
+            read_frags(F1, xi, wi, 1);
+            mma_all(F0);
+            read_frags(F0, xi, wi, 2);
+            mma_all(F1);
+            read_frags(F1, xi, wi, 3);
+            mma_all(F0);
+            // Stores of the previous tile may be outstanding too and do not return in order with the loads, but the count still holds: with S
+            // stores, the weight pieces and XPW younger row pieces in flight, "at most XPW outstanding" needs S + WPW completions,
+            // and fewer than WPW loads done (weights come first) would leave at most S + WPW - 1.
+            if (x_tail) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(G::XPW) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __syncthreads();  // everyone's share has landed, and this block's buffers have no readers left
+            __builtin_amdgcn_sched_barrier(0);
+            const int xn = xi == 2 ? 0 : xi + 1;
+            if (kb + 1 < nk) read_frags(F0, xn, wi ^ 1, 0);
+            constexpr int OPW = G::XPW + G::WPW;
+#pragma unroll
+            for (int mt = 0; mt < MW; ++mt) {
+                __builtin_amdgcn_sched_barrier(0);
+                mma_row(F1, mt);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = mt * OPW / MW; j < (mt + 1) * OPW / MW; ++j) {
+                    if (j < G::WPW) w_op(j);
+                    else x_op(j - G::WPW);
+                }
+            }
+            w_advance();
+            x_tail = cx.slot < slots;
+            x_advance();
+            xi = xn;
+            wi ^= 1;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+
+        // opaque copy of the lane id: what the epilogue derives from it is recomputed per tile instead of being kept alive across the k-loop
+        int lane_e = lane;
+        asm volatile("" : "+v"(lane_e));
+        const int li_e = lane_e & 31, hh_e = lane_e >> 5;
+        if (g.low && (!g.nkx || scalar_load(g.owner + mtile) < 0)) {  // several models in this tile
+            const int64_t w0 = m0 + wr * MW * 32, w1 = w0 + MW * 32;
+            Owners own{g.offsets, g.E, w0, w1 < g.M ? w1 : g.M};
+            int e;
+            int64_t a, b;
+            const T* u = (const T*)g.U;
+            while (own.next(e, a, b)) {
+                const T* be = (const T*)g.low + (int64_t)e * g.N * g.low_ld;
+#pragma unroll
+                for (int mt = 0; mt < MW; ++mt) {
+                    const int64_t row = w0 + mt * 32 + li_e, rc = row < g.M ? row : g.M - 1;
+                    const bool mine = row >= a && row < b;
+                    if (a >= w0 + mt * 32 + 32 || b <= w0 + mt * 32) continue;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const int n = n0 + wc * G::WN + nt * 32 + li_e, nc = n < g.N ? n : g.N - 1;
+                        f32x16 low = {};
+                        const T* bn = be + (int64_t)nc * g.low_ld;
+                        for (int j = hh_e * V; j - hh_e * V < g.low_ld; j += 2 * V)
+                            low = mma32(j + V <= g.low_ld ? mtk_ld(bn + j) : mtk_ld_n(bn + j, g.low_ld - j), mtk_ld(u + rc * g.rp + j), low);
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) acc[mt][nt][q] += mine ? low[q] : 0.f;
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int mt = 0; mt < MW; ++mt) {
+            const int64_t row = m0 + (wr * MW + mt) * 32 + li_e;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                if (g.relu) {
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) acc[mt][nt][q] = acc[mt][nt][q] < 0.f ? 0.f : acc[mt][nt][q];  // NaN stays
+                }
+                const int nb = n0 + wc * G::WN + nt * 32;
+                if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int n = nb + 8 * q + 4 * hh_e;
+                        mtk_vec<T> o;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o.v[j] = acc[mt][nt][4 * q + j];
+                        if (row < g.M) {
+                            if (n + 4 <= g.N) mtk_st(y + row * g.N + n, o);
+                            else mtk_st_n(y + row * g.N + n, o, g.N - n);
+                        }
+                    }
+                } else {
+                    // lanes l and l + 32 hold the two halves of every 8-feature piece: v_permlane32_swap gives each a whole 16-byte piece
+#pragma unroll
+                    for (int p2 = 0; p2 < 2; ++p2) {
+                        unsigned pk[2][2];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            T h[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) h[j] = (T)acc[mt][nt][4 * (2 * p2 + i) + j];
+                            pk[i][0] = reinterpret_cast<const unsigned*>(h)[0];
+                            pk[i][1] = reinterpret_cast<const unsigned*>(h)[1];
+                        }
+                        const auto r0 = __builtin_amdgcn_permlane32_swap(pk[1][0], pk[0][0], false, false);
+                        const auto r1 = __builtin_amdgcn_permlane32_swap(pk[1][1], pk[0][1], false, false);
+                        const int n = nb + 8 * (2 * p2 + (hh_e ? 0 : 1));
+                        const mtk_vec<T> o = __builtin_bit_cast(mtk_vec<T>, make_uint4(r0[0], r1[0], r0[1], r1[1]));
+                        if (row < g.M) {
+                            if (n + 8 <= g.N) mtk_st(y + row * g.N + n, o);
+                            else mtk_st_n(y + row * g.N + n, o, g.N - n);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// k_linear_few, for few rows: bound by the latency of streaming W once.  32 rows x 32 features a workgroup, its eight waves split k and take their
+// fragments straight from memory (every load of a wave is in flight at once), partial sums meet in LDS.  The low-rank product is plain
+// FMAs there, each row with its own model.
+struct FewArgs {
+    int64_t M, x_ld;
+    int N, K, r, rp, E, relu;
+    const int32_t* offsets;
+};
+
+template <typename T>
+__global__ __launch_bounds__(512) void k_linear_few(FewArgs g, const T* __restrict__ x, const T* __restrict__ W, const T* __restrict__ bias, const T* __restrict__ u,
+                                                    const T* __restrict__ up, T* __restrict__ y) {
+    constexpr int V = mtk_piece<T>::n, KB = kLine<T>, NW = 8;
+    __shared__ float part[NW][32][33];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hh = lane >> 5;
+    const int nb = (g.N + 31) / 32;
+    const int64_t m0 = (int64_t)(blockIdx.x / nb) * 32;
+    const int n0 = (int)(blockIdx.x % nb) * 32;
+    const T* xr = x + (m0 + li < g.M ? m0 + li : g.M - 1) * g.x_ld;
+    const T* wr = W + (int64_t)(n0 + li < g.N ? n0 + li : g.N - 1) * g.K;
+    f32x16 acc = {};
+    for (int k0 = wave * KB; k0 < g.K; k0 += NW * KB) {
+        mtk_vec<T> xa[4], wa[4];
+        if (k0 + KB <= g.K) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int k = k0 + (2 * s + hh) * V;
+                xa[s] = mtk_ld(xr + k);
+                wa[s] = mtk_ld(wr + k);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int k = k0 + (2 * s + hh) * V;
+                xa[s] = mtk_ld_n(xr + k, g.K - k);
+                wa[s] = mtk_ld_n(wr + k, g.K - k);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) acc = mma32(wa[s], xa[s], acc);
+    }
+#pragma unroll
+    for (int q = 0; q < 16; ++q) part[wave][li][(q & 3) + 8 * (q >> 2) + 4 * hh] = acc[q];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int q = tid + i * 512, rr = q >> 5, jj = q & 31, n = n0 + jj;
+        const int64_t row = m0 + rr;
+        if (row >= g.M || n >= g.N) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) v += part[w][rr][jj];
+        if (bias) v += (float)bias[n];
+        Owners own{g.offsets, g.E, row, row + 1};
         int e;
         int64_t a, b;
-        while (own.next(e, a, b)) {
-            f32x16 low[2][2] = {};
-            for (int j = hh * V; j < g.rp; j += 2 * V) {
-                mtk_vec<T> fu[2], fb[2];
+        if (own.next(e, a, b)) {
+            const T *ur = u + row * g.rp, *br = up + ((int64_t)e * g.N + n) * g.r;
+            float low = 0.f;
+            for (int j = 0; j < g.r; j += V) {
+                const mtk_vec<T> uv = mtk_ld(ur + j), bv = j + V <= g.r ? mtk_ld(br + j) : mtk_ld_n(br + j, g.r - j);
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const int64_t row = rows[q] < g.M ? rows[q] : g.M - 1;
-                    const int n = n0 + wc * 64 + q * 32 + li, nc = n < g.N ? n : g.N - 1;
-                    const T* bp = up + ((int64_t)e * g.N + nc) * g.r + j;
-                    fu[q] = mtk_ld(u + row * g.rp + j);
-                    fb[q] = j + V <= g.r ? mtk_ld(bp) : mtk_ld_n(bp, g.r - j);
-                }
-#pragma unroll
-                for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) low[mt][nt] = mma32(fb[nt], fu[mt], low[mt][nt]);
+                for (int c = 0; c < V; ++c) low += (float)uv.v[c] * (float)bv.v[c];
             }
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
-                const bool mine = rows[mt] >= a && rows[mt] < b;
-#pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                    for (int q = 0; q < 16; ++q) acc[mt][nt][q] += mine ? low[mt][nt][q] : 0.f;
-            }
+            v += low;
         }
+        if (g.relu) v = v < 0.f ? 0.f : v;
+        y[row * g.N + n] = (T)v;
     }
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int n = n0 + wc * 64 + nt * 32 + 8 * q + 4 * hh;
-            float bv[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) bv[j] = bias && n + j < g.N ? (float)bias[n + j] : 0.f;
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
-                if (rows[mt] >= g.M) continue;
-                T* yp = y + rows[mt] * g.N + n;
-                struct __attribute__((packed, aligned(alignof(T)), may_alias)) Quad { T v[4]; } o;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float v = acc[mt][nt][4 * q + j] + bv[j];
-                    if (g.relu) v = v < 0.f ? 0.f : v;  // NaN stays
-                    o.v[j] = (T)v;
-                }
-                if (n + 4 <= g.N) *reinterpret_cast<Quad*>(yp) = o;
-                else
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (n + j < g.N) yp[j] = o.v[j];
-            }
-        }
 }
 
 // ------------------------------------------------------------------------------------------------- the factors' gradients
@@ -459,17 +717,71 @@ __global__ __launch_bounds__(256) void k_wgrad_join(WgradArgs g, int turn, const
 }
 
 // ------------------------------------------------------------------------------------------------------------------ helpers
-// [batch][R][C] -> [batch][C][R]
+// k_prep: everything that has to be laid out before the products, in one launch.  A job owns consecutive workgroups.
+enum { JOB_TURN, JOB_PAD, JOB_BIAS, JOB_OWNER };
+struct Job {
+    int type, first;      // first workgroup
+    const void* src;
+    void* dst;
+    int64_t rows, ld;     // PAD: rows and source row stride; OWNER: rows of x; BIAS: padded length
+    int R, C, ldo;        // TURN: [batch][R][C] -> [batch][C][ldo]; PAD: [rows][C] -> [rows][ldo]; zeros behind; BIAS: C values; OWNER: C tiles of R rows
+    int E;                // OWNER
+};
+constexpr int kJobs = 8;
+struct Jobs {
+    Job job[kJobs];
+    int n = 0, blocks = 0;
+    void add(Job j, int64_t nblocks) {
+        j.first = blocks;
+        blocks += (int)nblocks;
+        job[n++] = j;
+    }
+};
+constexpr int kPadPieces = 1024;  // 16-byte pieces of a PAD workgroup
+
 template <typename T>
-__global__ __launch_bounds__(256) void k_turn(const T* __restrict__ in, T* __restrict__ out, int R, int C) {
+__global__ __launch_bounds__(256) void k_prep(Jobs jobs) {
+    constexpr int V = mtk_piece<T>::n;
     __shared__ T tile[32][33];
-    const int64_t base = (int64_t)blockIdx.z * R * C;
-    const int c0 = blockIdx.x * 32, r0 = blockIdx.y * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    for (int i = ty; i < 32; i += 8)
-        if (r0 + i < R && c0 + tx < C) tile[i][tx] = in[base + (int64_t)(r0 + i) * C + c0 + tx];
-    __syncthreads();
-    for (int i = ty; i < 32; i += 8)
-        if (c0 + i < C && r0 + tx < R) out[base + (int64_t)(c0 + i) * R + r0 + tx] = tile[tx][i];
+    int q = 0;
+    while (q + 1 < jobs.n && (int)blockIdx.x >= jobs.job[q + 1].first) ++q;
+    const Job& j = jobs.job[q];
+    const int64_t blk = blockIdx.x - j.first;
+    if (j.type == JOB_TURN) {
+        const int nc = (j.C + 31) / 32, nr = (j.ldo + 31) / 32;
+        const int64_t bat = blk / (nc * nr);
+        const int rest = (int)(blk - bat * nc * nr), c0 = rest % nc * 32, r0 = rest / nc * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+        const T* in = (const T*)j.src + bat * j.R * j.C;
+        T* out = (T*)j.dst + bat * j.C * j.ldo;
+        for (int i = ty; i < 32; i += 8) tile[i][tx] = r0 + i < j.R && c0 + tx < j.C ? in[(int64_t)(r0 + i) * j.C + c0 + tx] : T(0);
+        __syncthreads();
+        for (int i = ty; i < 32; i += 8)
+            if (c0 + i < j.C && r0 + tx < j.ldo) out[(int64_t)(c0 + i) * j.ldo + r0 + tx] = tile[tx][i];
+    } else if (j.type == JOB_PAD) {  // ldo is a multiple of a piece, dst 16-byte aligned
+        const int ppr = j.ldo / V;
+        const int64_t n = j.rows * ppr;
+        for (int64_t p = blk * kPadPieces + threadIdx.x; p < n && p < (blk + 1) * kPadPieces; p += 256) {
+            const int64_t row = p / ppr;
+            const int c = (int)(p - row * ppr) * V;
+            const T* in = (const T*)j.src + row * j.ld + c;
+            const mtk_vec<T> v = c + V <= j.C ? mtk_ld(in) : mtk_ld_n(in, j.C - c);
+            *reinterpret_cast<uint4*>((T*)j.dst + p * V) = __builtin_bit_cast(uint4, v);
+        }
+    } else if (j.type == JOB_BIAS) {
+        const int64_t i = blk * 256 + threadIdx.x;
+        if (i < j.rows) ((float*)j.dst)[i] = i < j.C ? (float)((const T*)j.src)[i] : 0.f;
+    } else {
+        const int64_t i = blk * 256 + threadIdx.x;
+        if (i < j.C) {
+            const int64_t a0 = i * j.R, a1 = a0 + j.R < j.rows ? a0 + j.R : j.rows;
+            Owners own{(const int32_t*)j.src, j.E, a0, a1};
+            int e;
+            int64_t a, b;
+            int who = j.E;
+            if (own.next(e, a, b)) who = a == a0 && b == a1 ? e : -1;
+            ((int32_t*)j.dst)[i] = who;
+        }
+    }
 }
 
 // g = dy, 0 where y <= 0
@@ -498,12 +810,9 @@ int64_t wgrad_part(int64_t M, int D, int r, int E) {
 
 template <typename T>
 void shrink(const ShrinkArgs& g, const T* x, const T* F, T* u, T* uT, hipStream_t s) {
-    k_shrink<T, 4><<<(unsigned)((g.M + 31) / 32), 256, 0, s>>>(g, x, F, u, uT);
-}
-template <typename T>
-void linear(const LinearArgs& g, const T* x, const T* W, const T* bias, const T* u, const T* up, T* y, hipStream_t s) {
-    const unsigned grid = (unsigned)((g.M + TM - 1) / TM * ((g.N + TN - 1) / TN));
-    k_linear<T><<<grid, 256, 0, s>>>(g, x, W, bias, u, up, y);
+    const int64_t tiles = (g.M + 31) / 32;
+    const int64_t walkers = tiles >= 256 ? 1 : (g.E < 16 ? g.E : 16);
+    k_shrink<T, 4><<<dim3((unsigned)tiles, (unsigned)walkers), 256, 0, s>>>(g, x, F, u, uT);
 }
 template <typename T, int JT>
 void wgrad_launch(const WgradArgs& g, int j0, const T* u, const T* uT, const T* x, float* part, hipStream_t s) {
@@ -522,11 +831,6 @@ void wgrad(const WgradArgs& g, int turn, const T* u, const T* uT, const T* x, fl
     const unsigned nx = (unsigned)((n + 255) / 256 < 1024 ? (n + 255) / 256 : 1024);
     k_wgrad_join<T><<<dim3(nx, g.E), 256, 0, s>>>(g, turn, part, out);
 }
-template <typename T>
-void turn(const T* in, T* out, int R, int C, int batch, hipStream_t s) {
-    k_turn<T><<<dim3((C + 31) / 32, (R + 31) / 32, batch), 256, 0, s>>>(in, out, R, C);
-}
-
 // where the parts of a buffer lie, in bytes, each on 256
 struct Layout {
     int64_t at = 0;
@@ -541,19 +845,70 @@ struct Saved {
     Saved(int64_t M, int r, int dtype) {
         Layout l;
         Mp = mtk_up(M, 32);
-        u = l.take(M * rank_pad_of(r, dtype) * mtk_dtype_size(dtype));
+        u = l.take(M * rank_pad(r, dtype) * mtk_dtype_size(dtype));
         uT = dtype == MTK_DT_F32 ? l.at : l.take(Mp * mtk_up(r, 64) * mtk_dtype_size(dtype));
         bytes = l.at;
     }
 };
-struct Work {
-    int64_t Wt, At, Bt, t, g, part, bytes;
-    Work(int64_t M, int din, int dout, int r, int E, int dtype, bool relu) {
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// How a product [M x K] [N x K]^T runs.  few: k_linear_few; else a tile of k_linear.
+struct Shape {
+    bool few, blocks;  // blocks: the low-rank product as k-blocks (a model owns a tile's rows on average)
+    int kind, BM, BN;  // 0: 256 x 256, 1: 128 x 128, 2: 64 x 128
+    int line, rp, Kp;  // elements of a line; u's row; K in whole lines
+    int64_t MT;
+    int nb_n;
+    Shape(int64_t M, int N, int K, int r, int E, int dtype) {
+        line = 128 / mtk_dtype_size(dtype);
+        rp = rank_pad(r, dtype);
+        Kp = (int)mtk_up(K, line);
+        few = M <= 256;
+        if (dtype == MTK_DT_F32) kind = cdiv(M, 128) * cdiv(N, 128) >= 1024 ? 1 : 2;
+        else kind = cdiv(M, 256) * cdiv(N, 256) >= 512 ? 0 : 1;
+        BM = kind == 0 ? 256 : kind == 1 ? 128 : 64;
+        BN = kind == 0 ? 256 : 128;
+        blocks = M >= (int64_t)E * BM;
+        MT = cdiv(M, BM);
+        nb_n = (int)cdiv(N, BN);
+    }
+};
+// what k_linear reads beside its operands, and their padded copies where they need one
+struct Packed {
+    int64_t X, W, Bp, bias, owner;
+    Packed(Layout& l, const Shape& sh, int64_t M, int N, int E, int dtype) {
         const int64_t z = mtk_dtype_size(dtype);
-        Layout l;
-        Wt = l.take((int64_t)din * dout * z);
-        At = l.take((int64_t)E * r * din * z);
+        X = l.take(sh.few ? 0 : M * sh.Kp * z);
+        W = l.take(sh.few ? 0 : (int64_t)N * sh.Kp * z);
+        Bp = l.take(sh.blocks ? (int64_t)(E + 1) * N * sh.rp * z : 0);
+        bias = l.take((int64_t)sh.nb_n * sh.BN * 4);
+        owner = l.take(sh.blocks ? sh.MT * 4 : 0);
+    }
+};
+// rows that LDS-DMA can stream as they are: whole lines, 16-byte aligned, offsets inside a tile in 32 bits
+bool streams(const void* p, int64_t ld, int K, int dtype) {
+    const int64_t z = mtk_dtype_size(dtype);
+    return (uintptr_t)p % 16 == 0 && ld * z % 16 == 0 && K % (128 / z) == 0 && ld * z < (1 << 22);
+}
+// forward: the padded operands (sized as if both needed it, where their sizes allow that they do not)
+struct ForwardWork {
+    int64_t bytes;
+    Shape sh;
+    Packed pk;
+    ForwardWork(Layout l, int64_t M, int din, int dout, int r, int E, int dtype) : sh(M, dout, din, r, E, dtype), pk(l, sh, M, dout, E, dtype) {
+        bytes = sh.few ? 0 : l.at;
+    }
+};
+struct BackwardWork {
+    int64_t Bt, Wt, At, t, g, part, bytes;
+    Shape sh;
+    Packed pk;
+    BackwardWork(Layout l, int64_t M, int din, int dout, int r, int E, int dtype, bool relu) : sh(M, din, dout, r, E, dtype), pk(l, sh, M, din, E, dtype) {
+        const int64_t z = mtk_dtype_size(dtype);
         Bt = l.take((int64_t)E * r * dout * z);
+        Wt = l.take(sh.few ? (int64_t)din * dout * z : 0);  // else pk.W
+        At = l.take(sh.blocks && !sh.few ? 0 : (int64_t)E * r * din * z);
         t = l.take(Saved(M, r, dtype).bytes);
         g = l.take(relu ? M * dout * z : 0);
         const int64_t pa = wgrad_part(M, din, r, E), pb = wgrad_part(M, dout, r, E);
@@ -561,6 +916,92 @@ struct Work {
         bytes = l.at;
     }
 };
+
+void job_turn(Jobs& jobs, const void* src, void* dst, int R, int C, int ldo, int batch) {
+    jobs.add(Job{JOB_TURN, 0, src, dst, 0, 0, R, C, ldo, 0}, cdiv(C, 32) * cdiv(ldo, 32) * batch);
+}
+void job_pad(Jobs& jobs, const void* src, int64_t ld, void* dst, int64_t rows, int C, int ldo, int V) {
+    jobs.add(Job{JOB_PAD, 0, src, dst, rows, ld, 0, C, ldo, 0}, cdiv(rows * (ldo / V), kPadPieces));
+}
+template <typename T> void prep(const Jobs& jobs, hipStream_t s) {
+    if (jobs.blocks) k_prep<T><<<(unsigned)jobs.blocks, 256, 0, s>>>(jobs);
+}
+
+// CUs of the current device, and whether a kernel's LDS limit has been raised there
+struct DeviceState {
+    int cus = 0;
+    bool lds[8] = {};
+};
+DeviceState* device_state() {
+    static DeviceState st[64];
+    int d = 0;
+    if (hipGetDevice(&d) != hipSuccess || d < 0 || d >= 64) return nullptr;
+    if (!st[d].cus) {
+        int n = 0;
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, d) != hipSuccess || n < 8) return nullptr;
+        st[d].cus = n;
+    }
+    return &st[d];
+}
+
+template <typename T, int WR, int MW, int NT>
+int launch_linear(LinearArgs& g, T* y, int which, hipStream_t s) {
+    typedef Geo<WR, MW, NT> G;
+    DeviceState* st = device_state();
+    if (!st) MTK_FAIL(MTK_ERR_HIP, "adapter product: no device properties");
+    if (!st->lds[which]) {
+        MTK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear<T, WR, MW, NT>), hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds));
+        st->lds[which] = true;
+    }
+    const int64_t per_xcd = cdiv(g.MT * g.nb_n, 8), room = (int64_t)st->cus / 8 * (163840 / G::kLds < 2 ? 1 : 2);
+    k_linear<T, WR, MW, NT><<<(unsigned)(8 * (per_xcd < room ? per_xcd : room)), 512, G::kLds, s>>>(g, y);
+    return MTK_OK;
+}
+template <typename T> int linear(const Shape& sh, LinearArgs& g, T* y, hipStream_t s) {
+    constexpr int base = sizeof(T) == 4 ? 0 : std::is_same<T, mtk_bf16>::value ? 2 : 4;
+    if constexpr (sizeof(T) == 4) return sh.kind == 1 ? launch_linear<T, 4, 1, 2>(g, y, base, s) : launch_linear<T, 2, 1, 1>(g, y, base + 1, s);
+    else return sh.kind == 0 ? launch_linear<T, 2, 4, 2>(g, y, base, s) : launch_linear<T, 4, 1, 2>(g, y, base + 1, s);
+}
+template <typename T>
+void linear_few(const FewArgs& g, const T* x, const T* W, const T* bias, const T* u, const T* up, T* y, hipStream_t s) {
+    k_linear_few<T><<<(unsigned)(cdiv(g.M, 32) * cdiv(g.N, 32)), 512, 0, s>>>(g, x, W, bias, u, up, y);
+}
+// the jobs of a k_linear product: x and W padded where they do not stream, B_e in whole lines and a block of zeros, bias, tiles' models.
+// F: W [N][K], or its transpose [K][N] when `turned`; L: B [E][N][r], or [E][r][N]
+template <typename T>
+LinearArgs plan_linear(Jobs& jobs, const Shape& sh, const Packed& pk, char* wb, int64_t M, int N, int K, int r, int E, int dtype, const T* x, int64_t x_ld,
+                       const T* F, bool turned, const T* bias, const T* L, const T* u, const int32_t* offsets, int relu) {
+    constexpr int V = mtk_piece<T>::n;
+    LinearArgs g{};
+    g.M = M; g.MT = sh.MT; g.N = N; g.nb_n = sh.nb_n;
+    g.nkb = sh.Kp / sh.line; g.nkx = sh.blocks ? sh.rp / sh.line : 0;
+    g.offsets = offsets; g.E = E; g.relu = relu; g.U = u; g.rp = sh.rp;
+    g.X = x;
+    g.x_ld = x_ld * sizeof(T);
+    if (!streams(x, x_ld, K, dtype)) {
+        job_pad(jobs, x, x_ld, wb + pk.X, M, K, sh.Kp, V);
+        g.X = wb + pk.X;
+        g.x_ld = sh.Kp * sizeof(T);
+    }
+    g.W = F;
+    g.w_ld = sh.Kp * sizeof(T);
+    if (turned) job_turn(jobs, F, wb + pk.W, K, N, sh.Kp, 1);
+    else if (!streams(F, K, K, dtype)) job_pad(jobs, F, K, wb + pk.W, N, K, sh.Kp, V);
+    if (turned || !streams(F, K, K, dtype)) g.W = wb + pk.W;
+    g.bias = (const float*)(wb + pk.bias);
+    const int64_t nbias = (int64_t)sh.nb_n * sh.BN;
+    jobs.add(Job{JOB_BIAS, 0, bias, wb + pk.bias, nbias, 0, 0, bias ? N : 0, 0, 0}, cdiv(nbias, 256));
+    if (sh.blocks) {
+        if (turned) job_turn(jobs, L, wb + pk.Bp, r, N, sh.rp, E);
+        else job_pad(jobs, L, r, wb + pk.Bp, (int64_t)E * N, r, sh.rp, V);
+        job_pad(jobs, L, 0, wb + pk.Bp + (int64_t)E * N * sh.rp * sizeof(T), N, 0, sh.rp, V);
+        jobs.add(Job{JOB_OWNER, 0, offsets, wb + pk.owner, M, 0, sh.BM, (int)sh.MT, 0, E}, cdiv(sh.MT, 256));
+        g.owner = (const int32_t*)(wb + pk.owner);
+        g.Bp = g.low = wb + pk.Bp;
+        g.low_ld = sh.rp;
+    }
+    return g;
+}
 
 int adapter_check(const char* who, int64_t M, int din, int dout, int r, int E, int dtype, int64_t x_ld, int act) {
     if (M < 0 || din < 1 || dout < 1 || r < 1 || E < 1 || x_ld < 0) MTK_FAIL(MTK_ERR_ARG, "%s: bad sizes (rows %lld, %d -> %d, rank %d, %d models)", who, (long long)M, din, dout, r, E);
@@ -578,26 +1019,44 @@ int adapter_check(const char* who, int64_t M, int din, int dout, int r, int E, i
 extern "C" int64_t mtk_adapter_saved_bytes(int64_t M, int r, int dtype) {
     return M > 0 && r > 0 && mtk_dtype_ok(dtype) ? Saved(M, r, dtype).bytes : 0;
 }
-extern "C" int64_t mtk_adapter_work_bytes(int64_t M, int din, int dout, int r, int E, int dtype, int act) {
-    return M > 0 && din > 0 && dout > 0 && r > 0 && E > 0 && mtk_dtype_ok(dtype) ? Work(M, din, dout, r, E, dtype, act == 1).bytes : 0;
+extern "C" int64_t mtk_adapter_work_bytes(int64_t M, int din, int dout, int r, int E, int dtype, int act, int backward) {
+    if (M <= 0 || din <= 0 || dout <= 0 || r <= 0 || E <= 0 || !mtk_dtype_ok(dtype)) return 0;
+    return backward ? BackwardWork(Layout(), M, din, dout, r, E, dtype, act == 1).bytes : ForwardWork(Layout(), M, din, dout, r, E, dtype).bytes;
 }
 
 extern "C" int mtk_adapter_forward(int64_t M, int din, int dout, int r, int E, int dtype, const void* x, int64_t x_ld, const void* W, const void* bias,
                                    const void* down, const void* up, const int32_t* offsets, const float* scales, double scale, int act, int keep,
-                                   void* y, void* saved, int64_t saved_bytes, mtk_stream stream) {
+                                   void* y, void* saved, int64_t saved_bytes, void* work, int64_t work_bytes, mtk_stream stream) {
     if (const int rc = adapter_check("mtk_adapter_forward", M, din, dout, r, E, dtype, x_ld, act)) return rc;
     if (M == 0) return MTK_OK;
     if (!x || !W || !down || !up || !offsets || !y || !saved) MTK_FAIL(MTK_ERR_ARG, "mtk_adapter_forward: null pointer");
     const Saved sv(M, r, dtype);
     if (saved_bytes < sv.bytes) MTK_FAIL(MTK_ERR_ARG, "mtk_adapter_forward: a buffer of %lld bytes for the low-rank rows, %lld needed", (long long)saved_bytes, (long long)sv.bytes);
+    const ForwardWork wk(Layout(), M, din, dout, r, E, dtype);
+    if (wk.bytes && (!work || work_bytes < wk.bytes)) MTK_FAIL(MTK_ERR_ARG, "mtk_adapter_forward: workspace of %lld bytes, %lld needed", (long long)work_bytes, (long long)wk.bytes);
+    int rc = MTK_OK;
     mtk_by_type(dtype, [&](auto tag) {
         typedef decltype(tag) T;
         const hipStream_t s = (hipStream_t)stream;
+        const Shape& sh = wk.sh;
         T* u = (T*)((char*)saved + sv.u);
         T* uT = keep && sizeof(T) == 2 ? (T*)((char*)saved + sv.uT) : nullptr;
-        shrink<T>(ShrinkArgs{M, din, r, rank_pad<T>(r), E, x_ld, offsets, scales, (float)scale, sv.Mp}, (const T*)x, (const T*)down, u, uT, s);
-        linear<T>(LinearArgs{M, x_ld, dout, din, r, rank_pad<T>(r), E, offsets, act}, (const T*)x, (const T*)W, (const T*)bias, u, (const T*)up, (T*)y, s);
+        shrink<T>(ShrinkArgs{M, din, r, sh.rp, E, x_ld, offsets, scales, (float)scale, sv.Mp}, (const T*)x, (const T*)down, u, uT, s);
+        if (sh.few) {
+            linear_few<T>(FewArgs{M, x_ld, dout, din, r, sh.rp, E, act, offsets}, (const T*)x, (const T*)W, (const T*)bias, u, (const T*)up, (T*)y, s);
+            return;
+        }
+        Jobs jobs;
+        LinearArgs g = plan_linear<T>(jobs, sh, wk.pk, (char*)work, M, dout, din, r, E, dtype, (const T*)x, x_ld, (const T*)W, false, (const T*)bias, (const T*)up, u,
+                                      offsets, act);
+        if (!sh.blocks) {
+            g.low = up;
+            g.low_ld = r;
+        }
+        prep<T>(jobs, s);
+        rc = linear<T>(sh, g, (T*)y, s);
     });
+    if (rc) return rc;
     MTK_HIP(hipGetLastError());
     return MTK_OK;
 }
@@ -609,37 +1068,47 @@ extern "C" int mtk_adapter_backward(int64_t M, int din, int dout, int r, int E, 
     if (M == 0) return MTK_OK;
     if (!x || !W || !down || !up || !offsets || !dy || !saved || !work || (act && !y)) MTK_FAIL(MTK_ERR_ARG, "mtk_adapter_backward: null pointer");
     const Saved sv(M, r, dtype);
-    const Work wk(M, din, dout, r, E, dtype, act == 1);
+    const BackwardWork wk(Layout(), M, din, dout, r, E, dtype, act == 1);
     if (work_bytes < wk.bytes) MTK_FAIL(MTK_ERR_ARG, "mtk_adapter_backward: workspace of %lld bytes, %lld needed", (long long)work_bytes, (long long)wk.bytes);
+    int rc = MTK_OK;
     mtk_by_type(dtype, [&](auto tag) {
         typedef decltype(tag) T;
         const hipStream_t s = (hipStream_t)stream;
+        const Shape& sh = wk.sh;
         char* wb = (char*)work;
-        const int rp = rank_pad<T>(r);
         const T *u = (const T*)((const char*)saved + sv.u), *uT = (const T*)((const char*)saved + sv.uT);
         T *t = (T*)(wb + wk.t + sv.u), *tT = (T*)(wb + wk.t + sv.uT);
         const T* g = (const T*)dy;
         if (act) {
             T* gz = (T*)(wb + wk.g);
-            const int64_t n = M * dout, nb = (n + 256 * mtk_piece<T>::n - 1) / (256 * mtk_piece<T>::n);
+            const int64_t n = M * dout, nb = cdiv(n, 256 * mtk_piece<T>::n);
             k_relu_grad<T><<<(unsigned)(nb < 65536 ? nb : 65536), 256, 0, s>>>(n, (const T*)y, g, gz);
             g = gz;
         }
-        if (dx || ddown) {
-            T* Bt = (T*)(wb + wk.Bt);
-            turn<T>((const T*)up, Bt, dout, r, E, s);
-            shrink<T>(ShrinkArgs{M, dout, r, rp, E, dout, offsets, scales, (float)scale, sv.Mp}, g, Bt, t, ddown && sizeof(T) == 2 ? tT : nullptr, s);
-        }
+        Jobs jobs;
+        LinearArgs lin{};
+        if (dx || ddown) job_turn(jobs, up, wb + wk.Bt, dout, r, dout, E);
         if (dx) {
-            T *Wt = (T*)(wb + wk.Wt), *At = (T*)(wb + wk.At);
-            turn<T>((const T*)W, Wt, dout, din, 1, s);
-            turn<T>((const T*)down, At, r, din, E, s);
-            linear<T>(LinearArgs{M, dout, din, dout, r, rp, E, offsets, 0}, g, Wt, nullptr, t, At, (T*)dx, s);
+            if (sh.few) job_turn(jobs, W, wb + wk.Wt, dout, din, dout, 1);
+            else lin = plan_linear<T>(jobs, sh, wk.pk, wb, M, din, dout, r, E, dtype, g, dout, (const T*)W, true, nullptr, (const T*)down, t, offsets, 0);
+            if (sh.few || !sh.blocks) {
+                job_turn(jobs, down, wb + wk.At, r, din, r, E);
+                lin.low = wb + wk.At;
+                lin.low_ld = r;
+            }
+        }
+        prep<T>(jobs, s);
+        if (dx || ddown)
+            shrink<T>(ShrinkArgs{M, dout, r, sh.rp, E, dout, offsets, scales, (float)scale, sv.Mp}, g, (const T*)(wb + wk.Bt), t, ddown && sizeof(T) == 2 ? tT : nullptr, s);
+        if (dx) {
+            if (sh.few) linear_few<T>(FewArgs{M, dout, din, dout, r, sh.rp, E, 0, offsets}, g, (const T*)(wb + wk.Wt), nullptr, t, (const T*)(wb + wk.At), (T*)dx, s);
+            else rc = linear<T>(sh, lin, (T*)dx, s);
         }
         float* part = (float*)(wb + wk.part);
-        if (ddown) wgrad<T>(WgradArgs{M, x_ld, sv.Mp, din, r, rp, E, wgrad_chunk(M, din), offsets}, 0, t, tT, (const T*)x, part, (T*)ddown, s);
-        if (dup) wgrad<T>(WgradArgs{M, dout, sv.Mp, dout, r, rp, E, wgrad_chunk(M, dout), offsets}, 1, u, uT, g, part, (T*)dup, s);
+        if (ddown) wgrad<T>(WgradArgs{M, x_ld, sv.Mp, din, r, sh.rp, E, wgrad_chunk(M, din), offsets}, 0, t, tT, (const T*)x, part, (T*)ddown, s);
+        if (dup) wgrad<T>(WgradArgs{M, dout, sv.Mp, dout, r, sh.rp, E, wgrad_chunk(M, dout), offsets}, 1, u, uT, g, part, (T*)dup, s);
     });
+    if (rc) return rc;
     MTK_HIP(hipGetLastError());
     return MTK_OK;
 }

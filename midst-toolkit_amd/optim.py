@@ -10,33 +10,38 @@ memory of 32-bit ones; rounded up or down by a dither that depends on a value's 
 """
 from __future__ import annotations
 
-import ctypes as C
 from array import array
+from operator import attrgetter
 from typing import Sequence
 
 import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import check
+from ._lib import launch
 from .routing import DTYPES
 
 SCALE_BLOCK = 256  # values per scale of the 8-bit moments
 
 
+_dtype, _numel, _device, _dense, _address = attrgetter("dtype"), Tensor.numel, Tensor.get_device, Tensor.is_contiguous, Tensor.data_ptr
+
+
 def _addresses(ts: Sequence[Tensor]):
-    a = array("Q", [t.data_ptr() for t in ts])
+    a = array("Q", map(_address, ts))
     return a, a.buffer_info()[0]
 
 
-def _check_list(what: str, ts: Sequence[Tensor], params: Sequence[Tensor], dtype: torch.dtype, sizes: list[int]) -> None:
-    if len(ts) != len(params):
-        raise ValueError(f"adamw_step: {len(ts)} {what} for {len(params)} params")
-    dev = params[0].device
+def _check_list(what: str, ts: Sequence[Tensor], dtype: torch.dtype, device: int, sizes: list[int]) -> None:
+    # whole-list passes in C: a step over hundreds of tensors is otherwise bound by these checks
+    if len(ts) != len(sizes):
+        raise ValueError(f"adamw_step: {len(ts)} {what} for {len(sizes)} params")
+    if list(map(_numel, ts)) == sizes and set(map(_dtype, ts)) == {dtype} and set(map(_device, ts)) == {device} and all(map(_dense, ts)):
+        return
     for t, n in zip(ts, sizes):
-        if t.dtype != dtype or t.device != dev or t.numel() != n or not t.is_contiguous():
-            raise ValueError(f"adamw_step: {what}: expected contiguous {dtype} tensors of the params' sizes on {dev}, got {tuple(t.shape)} {t.dtype} on {t.device}"
-                             + ("" if t.is_contiguous() else ", not contiguous"))
+        if t.dtype != dtype or t.get_device() != device or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"adamw_step: {what}: expected contiguous {dtype} tensors of the params' sizes on cuda:{device}, got {tuple(t.shape)} {t.dtype} on "
+                             f"{t.device}" + ("" if t.is_contiguous() else ", not contiguous"))
 
 
 @torch.no_grad()
@@ -57,25 +62,23 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
         raise RuntimeError("adamw_step: midst_toolkit_amd has no CPU path; move the params to the MI355X")
     if p0.dtype not in DTYPES:
         raise ValueError(f"adamw_step: params are {p0.dtype} (float32, bfloat16 or float16)")
-    sizes = [p.numel() for p in params]
-    _check_list("params", params, params, p0.dtype, sizes)
-    _check_list("grads", grads, params, p0.dtype, sizes)
+    sizes, at = list(map(_numel, params)), p0.get_device()
     state = torch.float8_e4m3fn if q8 else torch.float32
-    _check_list("exp_avgs", exp_avgs, params, state, sizes)
-    _check_list("exp_avg_sqs", exp_avg_sqs, params, state, sizes)
+    _check_list("params", params, p0.dtype, at, sizes)
+    _check_list("grads", grads, p0.dtype, at, sizes)
+    _check_list("exp_avgs", exp_avgs, state, at, sizes)
+    _check_list("exp_avg_sqs", exp_avg_sqs, state, at, sizes)
     lists = [params, grads, exp_avgs, exp_avg_sqs]
     if q8:
         blocks = [-(-n // SCALE_BLOCK) for n in sizes]
-        _check_list("exp_avg_scales", exp_avg_scales, params, torch.float32, blocks)
-        _check_list("exp_avg_sq_scales", exp_avg_sq_scales, params, torch.float32, blocks)
+        _check_list("exp_avg_scales", exp_avg_scales, torch.float32, at, blocks)
+        _check_list("exp_avg_sq_scales", exp_avg_sq_scales, torch.float32, at, blocks)
         lists += [exp_avg_scales, exp_avg_sq_scales]
     keep = [_addresses(ts) for ts in lists]
     addr = [a for _, a in keep] + ([] if q8 else [None, None])
     numel = array("q", sizes)
-    dev = p0.device
-    with torch.cuda.device(dev):
-        check(_lib.lib().mtk_adamw_step(len(params), *addr, numel.buffer_info()[0], DTYPES[p0.dtype], 8 if q8 else 32, lr, betas[0], betas[1], eps, weight_decay,
-                                        step, None if _hyper is None else _hyper.data_ptr(), _lib.stream_handle(dev)))
+    launch(p0.device, _lib.lib().mtk_adamw_step, len(params), *addr, numel.buffer_info()[0], DTYPES[p0.dtype], 8 if q8 else 32, lr, betas[0], betas[1], eps,
+           weight_decay, step, None if _hyper is None else _hyper.data_ptr())
     torch.autograd.graph.increment_version(params)  # written through raw pointers: autograd and the modules' caches have to see it
 
 
@@ -179,9 +182,8 @@ class AdamW(torch.optim.Optimizer):
             lr_dev = lr if isinstance(lr, Tensor) else None
             if lr_dev is not None and lr_dev.device != dev:
                 raise ValueError(f"AdamW: lr on {lr_dev.device}, parameters on {dev}")
-            with torch.cuda.device(dev):
-                check(l.mtk_adamw_count(step, None if lr_dev is None else lr_dev.data_ptr(), 0.0 if lr_dev is not None else lr, b1, b2, group["eps"],
-                                        group["weight_decay"], hyper.data_ptr(), _lib.stream_handle(dev)))
+            launch(dev, l.mtk_adamw_count, step, None if lr_dev is None else lr_dev.data_ptr(), 0.0 if lr_dev is not None else lr, b1, b2, group["eps"],
+                   group["weight_decay"], hyper.data_ptr())
             lr, step = 0.0, 1
         adamw_step([p for p, _, _ in items], [g for _, g, _ in items], col("exp_avg"), col("exp_avg_sq"), step, lr=lr, betas=(b1, b2), eps=group["eps"],
                    weight_decay=group["weight_decay"], _hyper=hyper, **scales)

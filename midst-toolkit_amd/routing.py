@@ -12,7 +12,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import check
+from ._lib import launch
 
 MAX_GROUPS = 1024  # MTK_ROUTE_MAX_GROUPS of include/mtk.h
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # enum mtk_dtype
@@ -65,9 +65,8 @@ def route_rows(index: Tensor, n_groups: int) -> RowPlan:
     offsets = torch.empty(n_groups + 1, dtype=torch.int32, device=dev)
     need = l.mtk_route_rows_work(P, n_groups)
     work = torch.empty(need, dtype=torch.int32, device=dev) if need else None
-    with torch.cuda.device(dev):
-        check(l.mtk_route_rows(P, idx.data_ptr(), n_groups, order.data_ptr(), slot.data_ptr(), offsets.data_ptr(),
-                               work.data_ptr() if work is not None else None, need, _lib.stream_handle(dev)))
+    launch(dev, l.mtk_route_rows, P, idx.data_ptr(), n_groups, order.data_ptr(), slot.data_ptr(), offsets.data_ptr(),
+           None if work is None else work.data_ptr(), need)
     return RowPlan(order, slot, offsets, n_groups, index.shape[0], copies)
 
 
@@ -89,10 +88,9 @@ def _dispatch(x: Tensor, plan: RowPlan, w: Tensor | None, y: Tensor | None = Non
     xs = torch.empty((P, D), dtype=x.dtype, device=dev) if want_rows else None
     dw = torch.empty((plan.n_rows, plan.copies), dtype=torch.float32, device=dev) if y is not None else None
     if P:
-        with torch.cuda.device(dev):
-            check(_lib.lib().mtk_rows_dispatch(plan.n_rows, plan.copies, D, DTYPES[x.dtype], x.data_ptr(), x.stride(0), plan.order.data_ptr(),
-                                               None if w is None else w.data_ptr(), None if xs is None else xs.data_ptr(),
-                                               None if y is None else y.data_ptr(), None if dw is None else dw.data_ptr(), _lib.stream_handle(dev)))
+        launch(dev, _lib.lib().mtk_rows_dispatch, plan.n_rows, plan.copies, D, DTYPES[x.dtype], x.data_ptr(), x.stride(0), plan.order.data_ptr(),
+               None if w is None else w.data_ptr(), None if xs is None else xs.data_ptr(), None if y is None else y.data_ptr(),
+               None if dw is None else dw.data_ptr())
     return xs, dw
 
 
@@ -101,9 +99,8 @@ def _combine(y: Tensor, plan: RowPlan, w: Tensor | None) -> Tensor:
     y = rows_of(y)
     out = torch.empty((plan.n_rows, D), dtype=y.dtype, device=dev)
     if plan.n_rows:
-        with torch.cuda.device(dev):
-            check(_lib.lib().mtk_rows_combine(plan.n_rows, plan.copies, D, DTYPES[y.dtype], y.data_ptr(), y.stride(0), plan.slot.data_ptr(),
-                                              None if w is None else w.data_ptr(), out.data_ptr(), _lib.stream_handle(dev)))
+        launch(dev, _lib.lib().mtk_rows_combine, plan.n_rows, plan.copies, D, DTYPES[y.dtype], y.data_ptr(), y.stride(0), plan.slot.data_ptr(),
+               None if w is None else w.data_ptr(), out.data_ptr())
     return out
 
 
@@ -139,7 +136,7 @@ def dispatch_rows(x: Tensor, plan: RowPlan) -> Tensor:
     """``x`` [N, D] -> [N * k, D]: every record's row in the places of its k pairs, sorted by model.  Differentiable in ``x`` (a record's
     gradient is the sum over its pairs, in fp32, in the order of its copies)."""
     _check_rows("dispatch_rows", x, plan.n_rows, plan)
-    return _Dispatch.apply(x, plan)
+    return _Dispatch.apply(x, plan) if x.requires_grad and torch.is_grad_enabled() else _dispatch(x, plan, None)[0]
 
 
 def combine_rows(y: Tensor, plan: RowPlan, weights: Tensor | None = None) -> Tensor:
@@ -151,5 +148,9 @@ def combine_rows(y: Tensor, plan: RowPlan, weights: Tensor | None = None) -> Ten
             raise ValueError(f"combine_rows: weights on {weights.device}, rows on {y.device}")
         if weights.dtype != torch.float32 or weights.numel() != plan.n_rows * plan.copies or weights.shape[0] != plan.n_rows:
             raise ValueError(f"combine_rows: weights are float32 [{plan.n_rows}, {plan.copies}], got {weights.dtype} {tuple(weights.shape)}")
-        weights = weights.reshape(plan.n_rows, plan.copies).contiguous()
-    return _Combine.apply(y, weights, plan)
+        if weights.dim() != 2:
+            weights = weights.reshape(plan.n_rows, plan.copies)
+        weights = weights.contiguous()
+    if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
+        return _Combine.apply(y, weights, plan)
+    return _combine(y, plan, weights)

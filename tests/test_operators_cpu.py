@@ -62,11 +62,12 @@ def test_c_entries_refuse_before_any_launch():
     assert l.mtk_rows_combine(4, 2, 8, 0, one, -1, one, None, one, None) == ARG
     assert l.mtk_rows_combine(4, 2, 8, 0, None, 8, one, None, one, None) == ARG
     fwd = lambda M=4, din=8, dout=8, r=2, E=2, dt=0, act=0, saved=1 << 30, x=one: l.mtk_adapter_forward(  # noqa: E731
-        M, din, dout, r, E, dt, x, din, one, None, one, one, one, None, 1.0, act, 0, one, one, saved, None)
+        M, din, dout, r, E, dt, x, din, one, None, one, one, one, None, 1.0, act, 0, one, one, saved, None, 0, None)
     for kw in (dict(M=-1), dict(din=0), dict(dout=0), dict(r=0), dict(E=0), dict(saved=8), dict(x=None)):
         assert fwd(**kw) == ARG, kw
     for kw in (dict(r=257), dict(E=1025), dict(din=8193), dict(dout=8193), dict(M=(1 << 24) + 1), dict(dt=3), dict(act=2)):
         assert fwd(**kw) == UNS, kw
+    assert fwd(M=5000, din=64, dout=64) == ARG  # no workspace
     assert l.mtk_adapter_backward(4, 8, 8, 2, 2, 0, one, 8, one, one, one, one, None, 1.0, 0, None, one, one, one, one, one, one, 16, None) == ARG
     assert l.mtk_adapter_backward(4, 8, 8, 2, 2, 0, one, 8, one, one, one, one, None, 1.0, 1, None, one, one, one, one, one, one, 1 << 30, None) == ARG
     ptrs, n = (C.c_void_p * 1)(256), (C.c_int64 * 1)(5)
@@ -83,7 +84,7 @@ def test_workspace_sizes_are_monotonic_and_empty_for_nonsense():
     l = _lib.lib()
     assert l.mtk_adapter_saved_bytes(0, 8, 0) == 0 and l.mtk_adapter_saved_bytes(8, 8, 9) == 0
     assert 0 < l.mtk_adapter_saved_bytes(100, 8, 1) <= l.mtk_adapter_saved_bytes(1000, 8, 1)
-    assert 0 < l.mtk_adapter_work_bytes(100, 64, 64, 8, 4, 1, 0) < l.mtk_adapter_work_bytes(100, 64, 64, 8, 4, 1, 1)
+    assert 0 < l.mtk_adapter_work_bytes(100, 64, 64, 8, 4, 1, 0, 1) < l.mtk_adapter_work_bytes(100, 64, 64, 8, 4, 1, 1, 1)
 
 
 def test_dither_rounds_to_neighbours_and_is_unbiased_over_the_steps():
