@@ -45,11 +45,10 @@ __device__ __forceinline__ f32x4 mma16(const mtk_vec<mtk_f16>& a, const mtk_vec<
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-template <typename T> __device__ __forceinline__ mtk_vec<T> zero_piece() {
-    mtk_vec<T> v;
+__device__ __forceinline__ f32x4 mma16(const mtk_vec<float>& a, const mtk_vec<float>& b, f32x4 c) {
 #pragma unroll
-    for (int i = 0; i < mtk_piece<T>::n; ++i) v.v[i] = T(0);
-    return v;
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], c, 0, 0, 0);
+    return c;
 }
 
 // A k-block is one 128-byte line of a row; the low-rank rows u are stored in whole k-blocks, zeros behind the rank
@@ -99,86 +98,126 @@ struct ShrinkArgs {
 };
 
 // u[row][j] = s_e sum_k x[row][k] F_e[j][k] (F: [E][r][K]); with uT also its transpose, which the factors' gradients multiply.
-// A workgroup takes 32 rows, its waves split k.  Where there are few rows, gridDim.y workgroups share a tile's models in turn (one model's
+// Bound by reading x.  16 x 16 MFMA tiles: RR sets of 16 rows against RT tiles of 16 j, so a rank of 16 wastes nothing; a wave streams its rows
+// straight into fragments, two lines at a time.  KS = 1: a wave has 32 rows to itself, which halves what it reads of F.  KS = 4, for few
+// rows: four waves split the lines of 16 rows, their sums meet in LDS, and gridDim.y workgroups share a tile's models in turn (one model's
 // product is a chain of loads of some microseconds); the first of them clears what no model owns.
-template <typename T, int NW>
-__global__ __launch_bounds__(64 * NW) void k_shrink(ShrinkArgs g, const T* __restrict__ x, const T* __restrict__ F, T* __restrict__ u, T* __restrict__ uT) {
-    constexpr int V = mtk_piece<T>::n, KB = kLine<T>, PT = 32 * 32 / (64 * NW);
-    __shared__ float part[NW][32][33];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hh = lane >> 5;
-    const int64_t m0 = (int64_t)blockIdx.x * 32;
-    const int64_t end = m0 + 32 < g.M ? m0 + 32 : g.M;
-    const int64_t row = m0 + li < g.M ? m0 + li : g.M - 1;
-    const T* xr = x + row * g.x_ld;
-    const int jt = (int)mtk_up(g.r, kRankT), jw = uT && jt > g.rp ? jt : g.rp;
-    for (int j0 = 0; j0 < jw; j0 += 32) {
-        Owners own{g.offsets, g.E, m0, end};
-        int e, turn = 0;
-        int64_t a, b;
-        float keep[PT];
-        unsigned mine = 0, all = 0;  // rows computed here / owned by any model
+template <typename T, int RT, int KS>
+__global__ __launch_bounds__(256) void k_shrink(ShrinkArgs g, int j0, const T* __restrict__ x, const T* __restrict__ F, T* __restrict__ u, T* __restrict__ uT) {
+    constexpr int V = mtk_piece<T>::n, KB = kLine<T>, RR = KS > 1 ? 1 : 2;
+    __shared__ float part[KS > 1 ? KS : 1][KS > 1 ? RT * 4 : 1][KS > 1 ? 64 : 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, q = lane >> 4;
+    const int64_t m0 = ((int64_t)blockIdx.x * (4 / KS) + (KS > 1 ? 0 : wave)) * 16 * RR;
+    if (m0 >= g.M) return;
+    const int64_t end = m0 + 16 * RR < g.M ? m0 + 16 * RR : g.M;
+    const T* xr[RR];
 #pragma unroll
-        for (int i = 0; i < PT; ++i) keep[i] = 0.f;
-        while (own.next(e, a, b)) {
-            const unsigned bits = (unsigned)(((1ull << (b - a)) - 1) << (a - m0));
-            all |= bits;
-            if (turn++ % (int)gridDim.y != (int)blockIdx.y) continue;
-            mine |= bits;
-            if (j0 >= g.r) continue;
-            const int j = j0 + li < g.r ? j0 + li : g.r - 1;
-            const T* fr = F + ((int64_t)e * g.r + j) * g.K;
-            f32x16 acc = {};
-            for (int k0 = wave * KB; k0 < g.K; k0 += NW * KB) {
-                mtk_vec<T> xa[4], fa[4];
-                if (k0 + KB <= g.K) {
+    for (int p = 0; p < RR; ++p) xr[p] = x + (m0 + p * 16 + li < g.M ? m0 + p * 16 + li : g.M - 1) * g.x_ld + q * V;
+    f32x4 keep[RR][RT] = {};
+    bool mine[RR] = {}, any[RR] = {};  // this lane's rows: computed here / owned by any model
+    Owners own{g.offsets, g.E, m0, end};
+    int e, turn = 0;
+    int64_t a, b;
+    while (own.next(e, a, b)) {
+        bool in[RR];
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) {
-                        const int k = k0 + (2 * s + hh) * V;
-                        xa[s] = mtk_ld(xr + k);
-                        fa[s] = mtk_ld(fr + k);
-                    }
-                } else {
+        for (int p = 0; p < RR; ++p) {
+            in[p] = m0 + p * 16 + li >= a && m0 + p * 16 + li < b;
+            any[p] |= in[p];
+        }
+        if (KS > 1 && turn++ % (int)gridDim.y != (int)blockIdx.y) continue;
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) {
-                        const int k = k0 + (2 * s + hh) * V;
-                        xa[s] = mtk_ld_n(xr + k, g.K - k);
-                        fa[s] = mtk_ld_n(fr + k, g.K - k);
-                    }
+        for (int p = 0; p < RR; ++p) mine[p] |= in[p];
+        const T* fr[RT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const int j = j0 + t * 16 + li;
+            fr[t] = F + ((int64_t)e * g.r + (j < g.r ? j : g.r - 1)) * g.K + q * V;
+        }
+        f32x4 acc[RR][RT] = {};
+        const int step = KS > 1 ? KS * KB : KB;
+        int k0 = KS > 1 ? wave * KB : 0;
+        auto lines = [&](auto count) {
+            constexpr int L = decltype(count)::value;
+            mtk_vec<T> xv[L][RR][2], fv[L][RT][2];
+#pragma unroll
+            for (int l = 0; l < L; ++l) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int p = 0; p < RR; ++p) xv[l][p][h] = mtk_ld(xr[p] + k0 + l * step + h * 4 * V);
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) fv[l][t][h] = mtk_ld(fr[t] + k0 + l * step + h * 4 * V);
                 }
-#pragma unroll
-                for (int s = 0; s < 4; ++s) acc = mma32(fa[s], xa[s], acc);
             }
-            // D[j][record]: lane -> record, register -> j = (reg & 3) + 8 (reg >> 2) + 4 (lane >> 5)
 #pragma unroll
-            for (int q = 0; q < 16; ++q) part[wave][li][(q & 3) + 8 * (q >> 2) + 4 * hh] = acc[q];
-            __syncthreads();
-            const float s = g.scales ? g.scales[e] : g.scale;
+            for (int l = 0; l < L; ++l)
 #pragma unroll
-            for (int i = 0; i < PT; ++i) {
-                const int q = tid + i * 64 * NW, rr = q >> 5, jj = q & 31;
-                float v = 0.f;
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int w = 0; w < NW; ++w) v += part[w][rr][jj];
-                if ((bits >> rr & 1) && j0 + jj < g.r) keep[i] = s * v;
-            }
-            __syncthreads();
+                    for (int p = 0; p < RR; ++p)
+#pragma unroll
+                        for (int t = 0; t < RT; ++t) acc[p][t] = mma16(fv[l][t][h], xv[l][p][h], acc[p][t]);
+            k0 += L * step;
+        };
+        constexpr int U = RT == 4 ? 2 : 4;
+        while (k0 + (U - 1) * step + KB <= g.K) lines(std::integral_constant<int, U>());
+        while (k0 + KB <= g.K) lines(std::integral_constant<int, 1>());
+        if (k0 < g.K) {  // the last, partial line
+            const int left = g.K - k0 - q * V;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    const mtk_vec<T> f = mtk_ld_n(fr[t] + k0 + h * 4 * V, left - h * 4 * V);
+#pragma unroll
+                    for (int p = 0; p < RR; ++p) acc[p][t] = mma16(f, mtk_ld_n(xr[p] + k0 + h * 4 * V, left - h * 4 * V), acc[p][t]);
+                }
         }
-        if (blockIdx.y == 0) mine |= ~all;  // rows without a model: zeros
-#pragma unroll
-        for (int i = 0; i < PT; ++i) {
-            const int q = tid + i * 64 * NW, rr = q >> 5, jj = q & 31;
-            if ((mine >> rr & 1) && m0 + rr < g.M && j0 + jj < g.rp) u[(m0 + rr) * g.rp + j0 + jj] = (T)keep[i];
-            if (uT) part[0][rr][jj] = keep[i];
-        }
-        if (uT) {  // through LDS: a thread per (j, record), records fastest
+        if (KS > 1) {
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < PT; ++i) {
-                const int q = tid + i * 64 * NW, rr = q & 31, jj = q >> 5;
-                if ((mine >> rr & 1) && j0 + jj < jt) uT[(int64_t)(j0 + jj) * g.Mp + m0 + rr] = (T)part[0][rr][jj];  // Mp covers whole tiles of 32 rows
-            }
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) part[wave][t * 4 + i][lane] = acc[0][t][i];
             __syncthreads();
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float v = 0.f;
+#pragma unroll
+                    for (int w = 0; w < KS; ++w) v += part[w][t * 4 + i][lane];
+                    acc[0][t][i] = v;
+                }
         }
+        const float s = g.scales ? g.scales[e] : g.scale;
+#pragma unroll
+        for (int p = 0; p < RR; ++p)
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) keep[p][t][i] = in[p] ? s * acc[p][t][i] : keep[p][t][i];
+    }
+    if (KS > 1 && wave > 0) return;
+#pragma unroll
+    for (int p = 0; p < RR; ++p) {
+        if (!(mine[p] || ((KS == 1 || blockIdx.y == 0) && !any[p]))) continue;  // a row without a model: zeros
+        const int64_t at = m0 + p * 16 + li;  // D[j][record]: lane & 15 -> record, j = 4 (lane >> 4) + register
+        struct __attribute__((aligned(4 * sizeof(T)), may_alias)) Quad { T v[4]; };
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            Quad o;
+            const int j = j0 + t * 16 + q * 4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o.v[i] = j + i < g.r ? (T)keep[p][t][i] : T(0);
+            if (at < g.M && j < g.rp) *reinterpret_cast<Quad*>(u + at * g.rp + j) = o;
+            if (uT && at < g.Mp)  // mtk_up(r, 64) rows of Mp
+#pragma unroll
+                for (int i = 0; i < 4; ++i) uT[(int64_t)(j + i) * g.Mp + at] = o.v[i];
+        }
+        if (j0 + RT * 16 >= g.r && at < g.M)  // zeros up to the end of the line
+            for (int j = j0 + RT * 16 + q * 4; j < g.rp; j += 16) *reinterpret_cast<Quad*>(u + at * g.rp + j) = Quad{};
     }
 }
 
@@ -206,10 +245,10 @@ struct LinearArgs {
     int low_ld, rp;       // rp: elements of a row of U
 };
 
-template <int WR, int MW, int NT> struct Geo {  // eight waves as WR x WC, each MW x NT tiles of 32 x 32
-    static constexpr int WC = 8 / WR, WN = NT * 32, BM = WR * MW * 32, BN = WC * WN;
-    static constexpr int kTileX = BM * 128, kTileW = BN * 128;   // bytes of a k-block
-    static constexpr int XPW = BM / 64, WPW = BN / 64;           // 8-row, 1 KiB pieces per wave
+template <int WR, int WC_, int MW, int NT> struct Geo {  // WR x WC waves, each MW x NT tiles of 32 x 32
+    static constexpr int WC = WC_, NW = WR * WC, WN = NT * 32, BM = WR * MW * 32, BN = WC * WN;
+    static constexpr int kTileX = BM * 128, kTileW = BN * 128;       // bytes of a k-block
+    static constexpr int XPW = BM / 8 / NW, WPW = BN / 8 / NW;       // 8-row, 1 KiB pieces per wave
     static constexpr int kLds = 3 * kTileX + 2 * kTileW;
 };
 
@@ -222,91 +261,85 @@ __device__ __forceinline__ int scalar_load(const int32_t* p) {
     return v;
 }
 
-template <typename T, int WR, int MW, int NT>
-__global__ __launch_bounds__(512, 1) void k_linear(LinearArgs g, T* __restrict__ y) {
-    typedef Geo<WR, MW, NT> G;
+template <typename T, int WR, int WC, int MW, int NT>
+__global__ __launch_bounds__(64 * WR * WC, 1) void k_linear(LinearArgs g, T* __restrict__ y) {
+    typedef Geo<WR, WC, MW, NT> G;
     constexpr int V = mtk_piece<T>::n, kWBase = 3 * G::kTileX;
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
     const int wv = __builtin_amdgcn_readfirstlane(wid);
-    const int wr = wv / G::WC, wc = wv % G::WC, li = lane & 31, hh = lane >> 5;
+    const int wr = wv / WC, wc = wv % WC, li = lane & 31, hh = lane >> 5;
     // workgroups go round-robin over the 8 XCDs: each XCD takes a contiguous eighth of the tiles (features fastest), so a row tile's
     // feature tiles run side by side on one XCD's L2 and every XCD has work
     const int xcd = blockIdx.x & 7, wq = blockIdx.x >> 3, wstride = gridDim.x >> 3;
-    const int64_t tiles = g.MT * g.nb_n, per = (tiles + 7) / 8, first = xcd * per;
-    const int64_t slots = tiles - first < per ? tiles - first : per;
+    const int tiles = (int)g.MT * g.nb_n, per = (tiles + 7) / 8, first = xcd * per;
+    const int slots = tiles - first < per ? tiles - first : per;
     if (wq >= slots) return;
     const int nk = g.nkb + g.nkx;
 
     // DMA of one 8-row piece (64 lanes x 16 bytes): lane -> row lane >> 3, piece slot lane & 7.  The LDS image is linear in the lane, so the
     // bank swizzle (slot s of row r holds piece s ^ ((r >> 1) & 7)) is applied to the global address.  Rows behind the last are
     // clamped: they are read again, never stored.  M0 (the LDS address) is written with every piece; the compiler puts nothing there.
-    const int lr = lane >> 3;
-    auto dma = [&](const unsigned char* base, int64_t ld, int64_t rows, int chunk, int64_t kbyte, unsigned dst) {
-        const int lc = ((lane & 7) ^ ((lr >> 1) | ((chunk & 1) << 2))) * 16;
-        const unsigned char* gp = base + kbyte;
-        unsigned voff;
-        if (rows >= chunk * 8 + 8) {
-            gp += (int64_t)chunk * 8 * ld;
-            voff = (unsigned)(lr * (int)ld + lc);
-        } else {
-            const int rr = chunk * 8 + lr, last = (int)rows - 1;
-            voff = (unsigned)((rr < last ? rr : last) * (int)ld + lc);
+    // A cursor keeps what its next block needs: a scalar base that moves on by a line a block, and the wave's piece offsets, worked out
+    // anew when the source changes (a tile's operand, then its low-rank lines).
+    const int lr = lane >> 3, lc0 = ((lane & 7) ^ (lr >> 1)) * 16, lc1 = ((lane & 7) ^ ((lr >> 1) | 4)) * 16;
+    auto offsets = [&](unsigned* voff, int n, int chunk0, int rows, unsigned ld) {
+#pragma unroll
+        for (int j = 0; j < n; ++j) {
+            const int rr = (chunk0 + j) * 8 + lr, rc = rr < rows ? rr : rows - 1;
+            voff[j] = (unsigned)rc * ld + (unsigned)((chunk0 + j) & 1 ? lc1 : lc0);
         }
+    };
+    auto dma = [&](const unsigned char* gp, unsigned voff, unsigned dst) {
         asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(gp), "s"(dst) : "memory");
     };
-    struct Cursor { int64_t slot; int kb; int buf; };
-    Cursor cx{wq, 0, 0}, cw{wq, 0, 0};
-    // sources of the tiles at the cursors
-    const unsigned char *xb = nullptr, *ub = nullptr, *wb = nullptr, *bb = nullptr;
-    int64_t xrows = 0, wrows = 0;
-    const int64_t lo_ld = (int64_t)g.nkx * 128;
-    auto x_tile = [&]() {
-        const int64_t m0 = ((first + cx.slot) / g.nb_n) * G::BM;
-        xb = (const unsigned char*)g.X + m0 * g.x_ld;
-        ub = (const unsigned char*)g.U + m0 * lo_ld;
-        xrows = g.M - m0;
+    const unsigned lo_ld = (unsigned)g.nkx * 128, x_ld = (unsigned)g.x_ld, w_ld = (unsigned)g.w_ld;
+    int cx_slot = wq, cx_kb = 0, cx_buf = 0, cw_slot = wq, cw_kb = 0, cw_buf = 0;
+    const unsigned char *xb = nullptr, *wb = nullptr;
+    unsigned xoff[G::XPW], woff[G::WPW];
+    auto x_source = [&](bool low) {
+        const int mt = (first + cx_slot) / g.nb_n;
+        const int64_t m0 = (int64_t)mt * G::BM;
+        const int rows = g.M - m0 < G::BM ? (int)(g.M - m0) : G::BM;
+        xb = low ? (const unsigned char*)g.U + m0 * lo_ld : (const unsigned char*)g.X + m0 * g.x_ld;
+        offsets(xoff, G::XPW, wv * G::XPW, rows, low ? lo_ld : x_ld);
     };
-    auto w_tile = [&]() {
-        const int64_t id = first + cw.slot, mt = id / g.nb_n;
-        const int64_t n0 = (id - mt * g.nb_n) * G::BN;
-        int e = g.E;
-        if (g.nkx) e = scalar_load(g.owner + mt);
-        e = e < 0 || e > g.E ? g.E : e;
-        wb = (const unsigned char*)g.W + n0 * g.w_ld;
-        bb = (const unsigned char*)g.Bp + ((int64_t)e * g.N + n0) * lo_ld;
-        wrows = g.N - n0;
+    auto w_source = [&](bool low) {
+        const int id = first + cw_slot, mt = id / g.nb_n, n0 = (id - mt * g.nb_n) * G::BN;
+        const int rows = g.N - n0 < G::BN ? g.N - n0 : G::BN;
+        if (low) {
+            int e = scalar_load(g.owner + mt);
+            e = e < 0 || e > g.E ? g.E : e;
+            wb = (const unsigned char*)g.Bp + ((int64_t)e * g.N + n0) * lo_ld;
+        } else {
+            wb = (const unsigned char*)g.W + (int64_t)n0 * g.w_ld;
+        }
+        offsets(woff, G::WPW, wv * G::WPW, rows, low ? lo_ld : w_ld);
     };
     auto x_op = [&](int j) {
-        if (cx.slot >= slots) return;
-        const int chunk = wv * G::XPW + j;
-        const unsigned dst = (unsigned)(cx.buf * G::kTileX + chunk * 1024);
-        if (cx.kb < g.nkb) dma(xb, g.x_ld, xrows, chunk, (int64_t)cx.kb * 128, dst);
-        else dma(ub, lo_ld, xrows, chunk, (int64_t)(cx.kb - g.nkb) * 128, dst);
+        if (cx_slot < slots) dma(xb, xoff[j], (unsigned)(cx_buf * G::kTileX + (wv * G::XPW + j) * 1024));
     };
     auto w_op = [&](int j) {
-        if (cw.slot >= slots) return;
-        const int chunk = wv * G::WPW + j;
-        const unsigned dst = (unsigned)(kWBase + cw.buf * G::kTileW + chunk * 1024);
-        if (cw.kb < g.nkb) dma(wb, g.w_ld, wrows, chunk, (int64_t)cw.kb * 128, dst);
-        else dma(bb, lo_ld, wrows, chunk, (int64_t)(cw.kb - g.nkb) * 128, dst);
+        if (cw_slot < slots) dma(wb, woff[j], (unsigned)(kWBase + cw_buf * G::kTileW + (wv * G::WPW + j) * 1024));
     };
     auto x_advance = [&]() {
-        if (cx.slot >= slots) return;
-        cx.buf = cx.buf == 2 ? 0 : cx.buf + 1;
-        if (++cx.kb == nk) {
-            cx.kb = 0;
-            cx.slot += wstride;
-            if (cx.slot < slots) x_tile();
-        }
+        if (cx_slot >= slots) return;
+        cx_buf = cx_buf == 2 ? 0 : cx_buf + 1;
+        xb += 128;
+        if (++cx_kb == nk) {
+            cx_kb = 0;
+            cx_slot += wstride;
+            if (cx_slot < slots) x_source(false);
+        } else if (cx_kb == g.nkb) x_source(true);
     };
     auto w_advance = [&]() {
-        if (cw.slot >= slots) return;
-        cw.buf ^= 1;
-        if (++cw.kb == nk) {
-            cw.kb = 0;
-            cw.slot += wstride;
-            if (cw.slot < slots) w_tile();
-        }
+        if (cw_slot >= slots) return;
+        cw_buf ^= 1;
+        wb += 128;
+        if (++cw_kb == nk) {
+            cw_kb = 0;
+            cw_slot += wstride;
+            if (cw_slot < slots) w_source(false);
+        } else if (cw_kb == g.nkb) w_source(true);
     };
     const unsigned char* lds = ad_smem;
     struct Frags { mtk_vec<T> x[MW], w[NT]; };
@@ -339,8 +372,8 @@ __global__ __launch_bounds__(512, 1) void k_linear(LinearArgs g, T* __restrict__
     // THEN of row block c + 3: loads return in order, so at the next wait vmcnt(XPW) - all but those last row pieces - means that
     // weight block c + 2 and row block c + 2 (requested a block earlier) have landed.
     Frags F0, F1;
-    x_tile();
-    w_tile();
+    x_source(false);
+    w_source(false);
     for (int b = 0; b < 3; ++b) {
 #pragma unroll
         for (int j = 0; j < G::XPW; ++j) x_op(j);
@@ -355,30 +388,25 @@ __global__ __launch_bounds__(512, 1) void k_linear(LinearArgs g, T* __restrict__
     __syncthreads();
     int xi = 0, wi = 0;   // buffers of the block being consumed
     bool x_tail = false;  // the previous block's tail requested row pieces after its weight pieces
-    for (int64_t slot = wq; slot < slots; slot += wstride) {
-        const int64_t id = first + slot, mtile = id / g.nb_n;
-        const int64_t m0 = mtile * G::BM;
-        const int n0 = (int)(id - mtile * g.nb_n) * G::BN;
+    for (int slot = wq; slot < slots; slot += wstride) {
+        const int id = first + slot, mtile = id / g.nb_n, n0 = (id - mtile * g.nb_n) * G::BN;
+        const int64_t m0 = (int64_t)mtile * G::BM;
         // the accumulators start from the bias, through the SCALAR cache: vector loads here would queue behind the DMA in flight
         {
             const float* bp = g.bias + n0 + wc * G::WN;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                f32x8 b0, b1, b2, b3;
-                asm volatile("s_load_dwordx8 %0, %4, 0x0\n\ts_load_dwordx8 %1, %4, 0x20\n\ts_load_dwordx8 %2, %4, 0x40\n\ts_load_dwordx8 %3, %4, 0x60\n\t"
-                             "s_waitcnt lgkmcnt(0)"
-                             : "=&s"(b0), "=&s"(b1), "=&s"(b2), "=&s"(b3)
-                             : "s"(bp + nt * 32)
-                             : "memory");
-                const f32x8 bq[4] = {b0, b1, b2, b3};
+            for (int h = 0; h < 2 * NT; ++h) {  // 16 features at a time: more would spill scalar registers
+                f32x8 b0, b1;
+                asm volatile("s_load_dwordx8 %0, %2, 0x0\n\ts_load_dwordx8 %1, %2, 0x20\n\ts_waitcnt lgkmcnt(0)" : "=&s"(b0), "=&s"(b1) : "s"(bp + h * 16) : "memory");
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
+                for (int j = 0; j < 4; ++j) {
+                    const float v0 = hh ? b0[4 + j] : b0[j], v1 = hh ? b1[4 + j] : b1[j];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float bv = hh ? bq[q][4 + j] : bq[q][j];
-#pragma unroll
-                        for (int a = 0; a < MW; ++a) acc[a][nt][4 * q + j] = bv;
+                    for (int a = 0; a < MW; ++a) {
+                        acc[a][h >> 1][8 * (h & 1) + j] = v0;
+                        acc[a][h >> 1][8 * (h & 1) + 4 + j] = v1;
                     }
+                }
             }
         }
         read_frags(F0, xi, wi, 0);
@@ -411,7 +439,7 @@ __global__ __launch_bounds__(512, 1) void k_linear(LinearArgs g, T* __restrict__
                 }
             }
             w_advance();
-            x_tail = cx.slot < slots;
+            x_tail = cx_slot < slots;
             x_advance();
             xi = xn;
             wi ^= 1;
@@ -579,140 +607,182 @@ struct WgradArgs {
 };
 
 // part[c + e][j][d] = sum over the rows of chunk c that model e owns of u[row][j] x[row][d].  Walking the chunks, each step to the next
-// (chunk, model) pair raises c, e or both, so c + e numbers the pairs without a gap's worth of bookkeeping.
+// (chunk, model) pair raises c, e or both, so c + e numbers the pairs without bookkeeping.  Bound by reading x: four waves share a strip
+// of columns and take the chunk's row groups in turn, the next group's loads in flight under the current one's products; their sums
+// meet in LDS.  Two such products (down's and up's gradient) share a launch.
 // 16-bit types: MFMA 16 x 16 x 32, the rows are its k.  u^T gives a lane's eight rows of one j as one piece; x's eight rows of eight
-// columns come as eight pieces and are turned in registers.  Rows of other models are zeroed in BOTH operands (0 x inf).
+// columns come as eight pieces and are turned in registers.  fp32: 16 x 16 x 4, a lane holds one row's four columns and one j.
+// Rows of other models are zeroed in BOTH operands (0 x inf).
+template <typename T> constexpr int kStrip = sizeof(T) == 4 ? 64 : 128;  // columns of a workgroup
 template <typename T, int JT>
-__global__ __launch_bounds__(256) void k_wgrad16(WgradArgs g, int j0, const T* __restrict__ uT, const T* __restrict__ x, float* __restrict__ part) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, q = lane >> 4;
-    const int c0 = (blockIdx.x * 4 + wave) * 128 + li * 8;
-    if ((blockIdx.x * 4 + wave) * 128 >= g.D) return;
-    const int cols = g.D - c0;
-    const int64_t lo = (int64_t)blockIdx.y * g.chunk, hi = lo + g.chunk < g.M ? lo + g.chunk : g.M;
+__device__ void wgrad_body(const WgradArgs& g, int strip, int c, int j0, const T* __restrict__ u, const T* __restrict__ uT, const T* __restrict__ x, float* __restrict__ part,
+                           float (*sum)[64 * 4]) {
+    constexpr int V = mtk_piece<T>::n, NV = V;  // columns per lane
+    constexpr int GR = sizeof(T) == 4 ? 16 : 32, PL = sizeof(T) == 4 ? 4 : 8;  // rows of a group, pieces of x per lane
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, q = lane >> 4;
+    const int c0 = strip * kStrip<T> + li * NV, cols = g.D - c0;
+    const int64_t lo = (int64_t)c * g.chunk, hi = lo + g.chunk < g.M ? lo + g.chunk : g.M;
     Owners own{g.offsets, g.E, lo, hi};
     int e;
     int64_t a, b;
     const int jp = (int)mtk_up(g.r, kRankT);
     while (own.next(e, a, b)) {
-        f32x4 acc[JT][8] = {};
-        for (int64_t r0 = a / 32 * 32; r0 < b; r0 += 32) {
-            const int64_t rr = r0 + q * 8;
-            mtk_vec<T> xv[8], ut[JT];
+        f32x4 acc[JT][NV] = {};
+        mtk_vec<T> xv[PL];
+        T us[sizeof(T) == 4 ? PL : 1][JT];
+        mtk_vec<T> ut[JT];
+        // a group inside the model's rows and a strip inside the width: a scalar base and one 32-bit offset per lane
+        const bool whole = (strip + 1) * kStrip<T> <= g.D && g.x_ld < (1 << 24);
+        const unsigned lane_off = (unsigned)((sizeof(T) == 4 ? q : q * 8) * (int)g.x_ld + c0) * (unsigned)sizeof(T);
+        auto load = [&](int64_t r0) {
+            if (whole && r0 >= a && r0 + GR <= b) {
+                const char* base = (const char*)(x + r0 * g.x_ld);
+                const int64_t ld = (sizeof(T) == 4 ? 4 : 1) * g.x_ld * (int64_t)sizeof(T);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int64_t row = rr + i;
+                for (int i = 0; i < PL; ++i) xv[i] = mtk_ld((const T*)(base + i * ld + lane_off));
+                if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                    for (int i = 0; i < PL; ++i)
+#pragma unroll
+                        for (int t = 0; t < JT; ++t) {
+                            const int j = j0 + t * 16 + li;
+                            us[i][t] = j < g.rp ? u[(r0 + i * 4 + q) * g.rp + j] : 0.f;
+                        }
+                } else {
+#pragma unroll
+                    for (int t = 0; t < JT; ++t) ut[t] = mtk_ld(uT + (int64_t)(j0 + t * 16 + li) * g.Mp + r0 + q * 8);
+                }
+                return;
+            }
+#pragma unroll
+            for (int i = 0; i < PL; ++i) {
+                const int64_t row = sizeof(T) == 4 ? r0 + i * 4 + q : r0 + q * 8 + i;
                 const bool in = row >= a && row < b;
                 const T* xp = x + row * g.x_ld + c0;
-                xv[i] = in && cols >= 8 ? mtk_ld(xp) : mtk_ld_n(xp, in ? cols : 0);
-            }
+                xv[i] = in && cols >= NV ? mtk_ld(xp) : mtk_ld_n(xp, in ? cols : 0);
+                if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int t = 0; t < JT; ++t) {
-                ut[t] = mtk_ld(uT + (int64_t)(j0 + t * 16 + li) * g.Mp + rr);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) ut[t].v[i] = rr + i >= a && rr + i < b ? ut[t].v[i] : T(0);
-            }
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                mtk_vec<T> col;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) col.v[i] = xv[i].v[c];
-#pragma unroll
-                for (int t = 0; t < JT; ++t) acc[t][c] = mma16(ut[t], col, acc[t][c]);
-            }
-        }
-        // D[j][column lane]: register -> j = 4 (lane >> 4) + reg, column li of the c-th set is c0 + c
-        float* o = part + (int64_t)(blockIdx.y + e) * jp * g.D;
-#pragma unroll
-        for (int t = 0; t < JT; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int j = j0 + t * 16 + q * 4 + i;
-                float* op = o + (int64_t)j * g.D + c0;
-                mtk_vec<float> v0, v1;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    v0.v[c] = acc[t][c][i];
-                    v1.v[c] = acc[t][c + 4][i];
-                }
-                if (j >= g.r) continue;
-                if (cols >= 8) {
-                    mtk_st(op, v0);
-                    mtk_st(op + 4, v1);
-                } else if (cols > 0) {
-                    mtk_st_n(op, v0, cols);
-                    mtk_st_n(op + 4, v1, cols - 4);
+                    for (int t = 0; t < JT; ++t) {
+                        const int j = j0 + t * 16 + li;
+                        us[i][t] = in && j < g.rp ? u[row * g.rp + j] : 0.f;
+                    }
                 }
             }
-    }
-}
-
-// fp32: MFMA 16 x 16 x 4, a lane holds one row's four columns and one j; nothing to turn
-template <int JT>
-__global__ __launch_bounds__(256) void k_wgrad32(WgradArgs g, int j0, const float* __restrict__ u, const float* __restrict__ x, float* __restrict__ part) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, q = lane >> 4;
-    const int c0 = (blockIdx.x * 4 + wave) * 64 + li * 4;
-    if ((blockIdx.x * 4 + wave) * 64 >= g.D) return;
-    const int cols = g.D - c0;
-    const int64_t lo = (int64_t)blockIdx.y * g.chunk, hi = lo + g.chunk < g.M ? lo + g.chunk : g.M;
-    Owners own{g.offsets, g.E, lo, hi};
-    int e;
-    int64_t a, b;
-    const int jp = (int)mtk_up(g.r, kRankT);
-    while (own.next(e, a, b)) {
-        f32x4 acc[JT][4] = {};
-        for (int64_t r0 = a / 16 * 16; r0 < b; r0 += 16) {
-            mtk_vec<float> xv[4];
-            float ut[4][JT];
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int64_t row = r0 + s * 4 + q;
-                const bool in = row >= a && row < b;
-                const float* xp = x + row * g.x_ld + c0;
-                xv[s] = in && cols >= 4 ? mtk_ld(xp) : mtk_ld_n(xp, in ? cols : 0);
+            if constexpr (sizeof(T) == 2) {
+                const int64_t rr = r0 + q * 8;
 #pragma unroll
                 for (int t = 0; t < JT; ++t) {
-                    const int j = j0 + t * 16 + li;
-                    ut[s][t] = in && j < g.rp ? u[row * g.rp + j] : 0.f;
+                    ut[t] = mtk_ld(uT + (int64_t)(j0 + t * 16 + li) * g.Mp + rr);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) ut[t].v[i] = rr + i >= a && rr + i < b ? ut[t].v[i] : T(0);
                 }
             }
+        };
+        const int64_t start = a / GR * GR + wave * GR;
+        if (start < b) load(start);
+        for (int64_t r0 = start; r0 < b; r0 += 4 * GR) {
+            mtk_vec<T> xc[PL], uc[JT];
+            T uu[sizeof(T) == 4 ? PL : 1][JT];
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
+            for (int i = 0; i < PL; ++i) xc[i] = xv[i];
 #pragma unroll
-                for (int t = 0; t < JT; ++t)
+            for (int t = 0; t < JT; ++t) {
+                if constexpr (sizeof(T) == 2) uc[t] = ut[t];
+                else
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) acc[t][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(ut[s][t], xv[s].v[c], acc[t][c], 0, 0, 0);
-        }
-        float* o = part + (int64_t)(blockIdx.y + e) * jp * g.D;
-#pragma unroll
-        for (int t = 0; t < JT; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int j = j0 + t * 16 + q * 4 + i;
-                if (j >= g.r) continue;
-                mtk_vec<float> v;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) v.v[c] = acc[t][c][i];
-                if (cols >= 4) mtk_st(o + (int64_t)j * g.D + c0, v);
-                else if (cols > 0) mtk_st_n(o + (int64_t)j * g.D + c0, v, cols);
+                    for (int i = 0; i < PL; ++i) uu[i][t] = us[i][t];
             }
+            if (r0 + 4 * GR < b) load(r0 + 4 * GR);
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int cc = 0; cc < NV; ++cc) {
+                    mtk_vec<T> col;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) col.v[i] = xc[i].v[cc];
+#pragma unroll
+                    for (int t = 0; t < JT; ++t) acc[t][cc] = mma16(uc[t], col, acc[t][cc]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < PL; ++i)
+#pragma unroll
+                    for (int t = 0; t < JT; ++t)
+#pragma unroll
+                        for (int cc = 0; cc < NV; ++cc) acc[t][cc] = __builtin_amdgcn_mfma_f32_16x16x4f32(uu[i][t], xc[i].v[cc], acc[t][cc], 0, 0, 0);
+            }
+        }
+        // D[j][column lane]: register i -> j = 4 (lane >> 4) + i, column li of set cc is c0 + cc.  Wave w adds up the registers with index w.
+        float* o = part + (int64_t)(c + e) * jp * g.D;
+#pragma unroll
+        for (int t = 0; t < JT; ++t) {
+#pragma unroll
+            for (int h = 0; h < NV; h += 4) {  // four columns at a time through 16 KB
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<float4*>(&sum[wave * 4 + i][lane * 4]) = make_float4(acc[t][h][i], acc[t][h + 1][i], acc[t][h + 2][i], acc[t][h + 3][i]);
+                __syncthreads();
+                float4 v = *reinterpret_cast<float4*>(&sum[wave][lane * 4]);
+#pragma unroll
+                for (int w = 1; w < 4; ++w) {
+                    const float4 p = *reinterpret_cast<float4*>(&sum[w * 4 + wave][lane * 4]);
+                    v.x += p.x; v.y += p.y; v.z += p.z; v.w += p.w;
+                }
+                const int j = j0 + t * 16 + q * 4 + wave, left = cols - h;
+                const mtk_vec<float> ov = {{v.x, v.y, v.z, v.w}};
+                float* op = o + (int64_t)j * g.D + c0 + h;
+                if (j < g.r && left > 0) {
+                    if (left >= 4) mtk_st(op, ov);
+                    else mtk_st_n(op, ov, left);
+                }
+            }
+        }
     }
+}
+template <typename T> struct WgradOne {
+    WgradArgs g;
+    int strips, chunks;
+    const T *u, *uT, *x;
+    float* part;
+    T* out;
+    int turn;
+};
+template <typename T> struct WgradBoth {
+    WgradOne<T> p[2];
+};
+template <typename T, int JT>
+__global__ __launch_bounds__(256) void k_wgrad(WgradBoth<T> both, int j0) {
+    __shared__ float sum[16][64 * 4];
+    const WgradOne<T>& p = both.p[blockIdx.y];
+    const int64_t c = blockIdx.x / (unsigned)p.strips;  // strips of a chunk side by side: they share u
+    if (c >= p.chunks) return;
+    wgrad_body<T, JT>(p.g, (int)(blockIdx.x % (unsigned)p.strips), (int)c, j0, p.u, p.uT, p.x, p.part, sum);
 }
 
 // out[e] = sum of model e's chunks in ascending order; [r][D], or [D][r] when `turn`.  A model without rows gets zeros.
 template <typename T>
-__global__ __launch_bounds__(256) void k_wgrad_join(WgradArgs g, int turn, const float* __restrict__ part, T* __restrict__ out) {
+__global__ __launch_bounds__(256) void k_wgrad_join(WgradBoth<T> both) {
+    const WgradOne<T>& p = both.p[blockIdx.z];
+    const WgradArgs& g = p.g;
+    if (!p.out) return;
     const int e = blockIdx.y;
     const int jp = (int)mtk_up(g.r, kRankT);
-    const int64_t n = (int64_t)g.r * g.D;
+    const int64_t n = (int64_t)g.r * g.D, slice = (int64_t)jp * g.D;
     int64_t a = g.offsets[e], b = g.offsets[e + 1];
     a = a < 0 ? 0 : a;
     b = b < g.M ? b : g.M;
     const int64_t ca = a / g.chunk, cb = b > a ? (b - 1) / g.chunk : ca - 1;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int64_t j = i / g.D, d = i - j * g.D;
-        float s = 0.f;
-        for (int64_t c = ca; c <= cb; ++c) s += part[((c + e) * jp + j) * g.D + d];
-        out[(int64_t)e * n + (turn ? d * g.r + j : i)] = (T)s;
+        const float* s = p.part + (ca + e) * slice + i;
+        float v = 0.f;
+        int64_t c = ca;
+        for (; c + 3 <= cb; c += 4, s += 4 * slice) {
+            const float v0 = s[0], v1 = s[slice], v2 = s[2 * slice], v3 = s[3 * slice];
+            v = ((v + v0) + v1) + v2 + v3;
+        }
+        for (; c <= cb; ++c, s += slice) v += *s;
+        p.out[(int64_t)e * n + (p.turn ? d * g.r + j : i)] = (T)v;
     }
 }
 
@@ -799,38 +869,50 @@ __global__ __launch_bounds__(256) void k_relu_grad(int64_t n, const T* __restric
     }
 }
 
-int wgrad_chunk(int64_t M, int D) {
-    const int64_t want = M * ((D + 127) / 128) / 2048;  // about 2048 waves
-    const int64_t c = mtk_up(want < 1 ? 1 : want, 32);
-    return (int)(c < 64 ? 64 : (c > 1024 ? 1024 : c));
-}
-int64_t wgrad_part(int64_t M, int D, int r, int E) {
-    return ((M + wgrad_chunk(M, D) - 1) / wgrad_chunk(M, D) + E) * mtk_up(r, kRankT) * D;
-}
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// rows of a chunk: about a thousand workgroups in all, each with some row groups for every wave
+int wgrad_chunk(int64_t M, int D, int dtype) {
+    const int strip = dtype == MTK_DT_F32 ? 64 : 128;
+    const int64_t c = mtk_up(M * cdiv(D, strip) / 768 + 1, 64);
+    return (int)(c > 2048 ? 2048 : c);
+}
+int64_t wgrad_part(int64_t M, int D, int r, int E, int dtype) { return (cdiv(M, wgrad_chunk(M, D, dtype)) + E) * mtk_up(r, kRankT) * D; }
+
+template <typename T, int RT>
+void shrink_launch(const ShrinkArgs& g, int j0, const T* x, const T* F, T* u, T* uT, hipStream_t s) {
+    // 32 rows a wave fill the chip from some 16,384 rows on; below, four waves split 16 rows
+    if (g.M >= 16384) k_shrink<T, RT, 1><<<(unsigned)cdiv(g.M, 128), 256, 0, s>>>(g, j0, x, F, u, uT);
+    else k_shrink<T, RT, 4><<<dim3((unsigned)cdiv(g.M, 16), (unsigned)(g.M >= 2048 ? 1 : (g.E < 16 ? g.E : 16))), 256, 0, s>>>(g, j0, x, F, u, uT);
+}
 template <typename T>
 void shrink(const ShrinkArgs& g, const T* x, const T* F, T* u, T* uT, hipStream_t s) {
-    const int64_t tiles = (g.M + 31) / 32;
-    const int64_t walkers = tiles >= 256 ? 1 : (g.E < 16 ? g.E : 16);
-    k_shrink<T, 4><<<dim3((unsigned)tiles, (unsigned)walkers), 256, 0, s>>>(g, x, F, u, uT);
-}
-template <typename T, int JT>
-void wgrad_launch(const WgradArgs& g, int j0, const T* u, const T* uT, const T* x, float* part, hipStream_t s) {
-    const unsigned nch = (unsigned)((g.M + g.chunk - 1) / g.chunk);
-    if constexpr (sizeof(T) == 4) k_wgrad32<JT><<<dim3((g.D + 255) / 256, nch), 256, 0, s>>>(g, j0, u, x, part);
-    else k_wgrad16<T, JT><<<dim3((g.D + 511) / 512, nch), 256, 0, s>>>(g, j0, uT, x, part);
+    for (int j0 = 0; j0 < g.r; j0 += 64) {
+        if (g.r - j0 > 32) shrink_launch<T, 4>(g, j0, x, F, u, uT, s);
+        else if (g.r - j0 > 16) shrink_launch<T, 2>(g, j0, x, F, u, uT, s);
+        else shrink_launch<T, 1>(g, j0, x, F, u, uT, s);
+    }
 }
 template <typename T>
-void wgrad(const WgradArgs& g, int turn, const T* u, const T* uT, const T* x, float* part, T* out, hipStream_t s) {
-    for (int j0 = 0; j0 < g.r; j0 += 64) {
-        if (g.r - j0 > 32) wgrad_launch<T, 4>(g, j0, u, uT, x, part, s);
-        else if (g.r - j0 > 16) wgrad_launch<T, 2>(g, j0, u, uT, x, part, s);
-        else wgrad_launch<T, 1>(g, j0, u, uT, x, part, s);
-    }
-    const int64_t n = (int64_t)g.r * g.D;
-    const unsigned nx = (unsigned)((n + 255) / 256 < 1024 ? (n + 255) / 256 : 1024);
-    k_wgrad_join<T><<<dim3(nx, g.E), 256, 0, s>>>(g, turn, part, out);
+WgradOne<T> wgrad_one(int64_t M, int64_t x_ld, int64_t Mp, int D, int r, int rp, int E, const int32_t* offsets, int dtype, int turn, const T* u, const T* uT, const T* x,
+                      float* part, T* out) {
+    const int chunk = wgrad_chunk(M, D, dtype);
+    return WgradOne<T>{WgradArgs{M, x_ld, Mp, D, r, rp, E, chunk, offsets}, (int)cdiv(D, kStrip<T>), out ? (int)cdiv(M, chunk) : 0, u, uT, x, part, out, turn};
 }
+template <typename T>
+void wgrad(const WgradBoth<T>& w, hipStream_t s) {
+    const WgradOne<T>&p = w.p[0], &q = w.p[1];
+    const int64_t n = (int64_t)p.strips * p.chunks, m = (int64_t)q.strips * q.chunks;
+    const dim3 grid((unsigned)(n > m ? n : m), 2);
+    for (int j0 = 0; j0 < p.g.r; j0 += 64) {
+        if (p.g.r - j0 > 32) k_wgrad<T, 4><<<grid, 256, 0, s>>>(w, j0);
+        else if (p.g.r - j0 > 16) k_wgrad<T, 2><<<grid, 256, 0, s>>>(w, j0);
+        else k_wgrad<T, 1><<<grid, 256, 0, s>>>(w, j0);
+    }
+    const int64_t e = (int64_t)p.g.r * (p.g.D > q.g.D ? p.g.D : q.g.D);
+    k_wgrad_join<T><<<dim3((unsigned)(cdiv(e, 256) < 1024 ? cdiv(e, 256) : 1024), p.g.E, 2), 256, 0, s>>>(w);
+}
+
 // where the parts of a buffer lie, in bytes, each on 256
 struct Layout {
     int64_t at = 0;
@@ -851,12 +933,10 @@ struct Saved {
     }
 };
 
-int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 // How a product [M x K] [N x K]^T runs.  few: k_linear_few; else a tile of k_linear.
 struct Shape {
     bool few, blocks;  // blocks: the low-rank product as k-blocks (a model owns a tile's rows on average)
-    int kind, BM, BN;  // 0: 256 x 256, 1: 128 x 128, 2: 64 x 128
+    int kind, BM, BN;  // 0: 256 x 256, 1: 128 x 128, 2: 64 x 64
     int line, rp, Kp;  // elements of a line; u's row; K in whole lines
     int64_t MT;
     int nb_n;
@@ -865,10 +945,13 @@ struct Shape {
         rp = rank_pad(r, dtype);
         Kp = (int)mtk_up(K, line);
         few = M <= 256;
-        if (dtype == MTK_DT_F32) kind = cdiv(M, 128) * cdiv(N, 128) >= 1024 ? 1 : 2;
-        else kind = cdiv(M, 256) * cdiv(N, 256) >= 512 ? 0 : 1;
-        BM = kind == 0 ? 256 : kind == 1 ? 128 : 64;
-        BN = kind == 0 ? 256 : 128;
+        // 256 x 256 tiles (one workgroup a CU) where they fill their rounds over the CUs to four fifths; 64 x 64 while the chip is not full.  us for
+        // K = N = 1024, 256 / 128 / 64: bf16 65,536 rows 123 / 159 / 232, 20,011 rows 77 / 54 / 71, 8,192 rows 33 / 24 / 31, 2,048 rows
+        // 33 / 16 / 13; fp32 20,011 rows 540 / 338 / 346, 8,192 rows 262 / 144 / 140, 2,048 rows 264 / 79 / 43
+        const int64_t t256 = cdiv(M, 256) * cdiv(N, 256), t128 = cdiv(M, 128) * cdiv(N, 128);
+        if (dtype == MTK_DT_F32) kind = t128 >= 1024 ? 1 : 2;
+        else kind = t256 * 5 >= cdiv(t256, 256) * 256 * 4 ? 0 : t128 > 256 ? 1 : 2;
+        BM = BN = kind == 0 ? 256 : kind == 1 ? 128 : 64;
         blocks = M >= (int64_t)E * BM;
         MT = cdiv(M, BM);
         nb_n = (int)cdiv(N, BN);
@@ -901,7 +984,7 @@ struct ForwardWork {
     }
 };
 struct BackwardWork {
-    int64_t Bt, Wt, At, t, g, part, bytes;
+    int64_t Bt, Wt, At, t, g, part[2], bytes;
     Shape sh;
     Packed pk;
     BackwardWork(Layout l, int64_t M, int din, int dout, int r, int E, int dtype, bool relu) : sh(M, din, dout, r, E, dtype), pk(l, sh, M, din, E, dtype) {
@@ -911,8 +994,8 @@ struct BackwardWork {
         At = l.take(sh.blocks && !sh.few ? 0 : (int64_t)E * r * din * z);
         t = l.take(Saved(M, r, dtype).bytes);
         g = l.take(relu ? M * dout * z : 0);
-        const int64_t pa = wgrad_part(M, din, r, E), pb = wgrad_part(M, dout, r, E);
-        part = l.take((pa > pb ? pa : pb) * 4);
+        part[0] = l.take(wgrad_part(M, din, r, E, dtype) * 4);
+        part[1] = l.take(wgrad_part(M, dout, r, E, dtype) * 4);
         bytes = l.at;
     }
 };
@@ -930,7 +1013,7 @@ template <typename T> void prep(const Jobs& jobs, hipStream_t s) {
 // CUs of the current device, and whether a kernel's LDS limit has been raised there
 struct DeviceState {
     int cus = 0;
-    bool lds[8] = {};
+    bool lds[9] = {};
 };
 DeviceState* device_state() {
     static DeviceState st[64];
@@ -944,23 +1027,25 @@ DeviceState* device_state() {
     return &st[d];
 }
 
-template <typename T, int WR, int MW, int NT>
+template <typename T, int WR, int WC, int MW, int NT>
 int launch_linear(LinearArgs& g, T* y, int which, hipStream_t s) {
-    typedef Geo<WR, MW, NT> G;
+    typedef Geo<WR, WC, MW, NT> G;
     DeviceState* st = device_state();
     if (!st) MTK_FAIL(MTK_ERR_HIP, "adapter product: no device properties");
     if (!st->lds[which]) {
-        MTK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear<T, WR, MW, NT>), hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds));
+        MTK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear<T, WR, WC, MW, NT>), hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds));
         st->lds[which] = true;
     }
-    const int64_t per_xcd = cdiv(g.MT * g.nb_n, 8), room = (int64_t)st->cus / 8 * (163840 / G::kLds < 2 ? 1 : 2);
-    k_linear<T, WR, MW, NT><<<(unsigned)(8 * (per_xcd < room ? per_xcd : room)), 512, G::kLds, s>>>(g, y);
+    const int64_t per_xcd = cdiv(g.MT * g.nb_n, 8), room = (int64_t)st->cus / 8 * (163840 / G::kLds);
+    k_linear<T, WR, WC, MW, NT><<<(unsigned)(8 * (per_xcd < room ? per_xcd : room)), 64 * G::NW, G::kLds, s>>>(g, y);
     return MTK_OK;
 }
 template <typename T> int linear(const Shape& sh, LinearArgs& g, T* y, hipStream_t s) {
-    constexpr int base = sizeof(T) == 4 ? 0 : std::is_same<T, mtk_bf16>::value ? 2 : 4;
-    if constexpr (sizeof(T) == 4) return sh.kind == 1 ? launch_linear<T, 4, 1, 2>(g, y, base, s) : launch_linear<T, 2, 1, 1>(g, y, base + 1, s);
-    else return sh.kind == 0 ? launch_linear<T, 2, 4, 2>(g, y, base, s) : launch_linear<T, 4, 1, 2>(g, y, base + 1, s);
+    constexpr int base = sizeof(T) == 4 ? 0 : std::is_same<T, mtk_bf16>::value ? 3 : 6;
+    if constexpr (sizeof(T) == 2)
+        if (sh.kind == 0) return launch_linear<T, 2, 4, 4, 2>(g, y, base, s);
+    if (sh.kind == 1) return launch_linear<T, 4, 2, 1, 2>(g, y, base + 1, s);
+    return launch_linear<T, 2, 2, 1, 1>(g, y, base + 2, s);
 }
 template <typename T>
 void linear_few(const FewArgs& g, const T* x, const T* W, const T* bias, const T* u, const T* up, T* y, hipStream_t s) {
@@ -1104,9 +1189,9 @@ extern "C" int mtk_adapter_backward(int64_t M, int din, int dout, int r, int E, 
             if (sh.few) linear_few<T>(FewArgs{M, dout, din, dout, r, sh.rp, E, 0, offsets}, g, (const T*)(wb + wk.Wt), nullptr, t, (const T*)(wb + wk.At), (T*)dx, s);
             else rc = linear<T>(sh, lin, (T*)dx, s);
         }
-        float* part = (float*)(wb + wk.part);
-        if (ddown) wgrad<T>(WgradArgs{M, x_ld, sv.Mp, din, r, sh.rp, E, wgrad_chunk(M, din), offsets}, 0, t, tT, (const T*)x, part, (T*)ddown, s);
-        if (dup) wgrad<T>(WgradArgs{M, dout, sv.Mp, dout, r, sh.rp, E, wgrad_chunk(M, dout), offsets}, 1, u, uT, g, part, (T*)dup, s);
+        if (ddown || dup)
+            wgrad<T>(WgradBoth<T>{{wgrad_one<T>(M, x_ld, sv.Mp, din, r, sh.rp, E, offsets, dtype, 0, t, tT, (const T*)x, (float*)(wb + wk.part[0]), (T*)ddown),
+                                   wgrad_one<T>(M, dout, sv.Mp, dout, r, sh.rp, E, offsets, dtype, 1, u, uT, g, (float*)(wb + wk.part[1]), (T*)dup)}}, s);
     });
     if (rc) return rc;
     MTK_HIP(hipGetLastError());
