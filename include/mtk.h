@@ -493,20 +493,20 @@ int mtk_edm_set_weights(mtk_edm* edm, const float* const* W, const float* const*
  * the other (attacks/ensemble/rmia/shadow_model_training.py:308); here the pairs of all models run as one batch.
  *
  * mtk_route_rows plans n_pairs pairs by index[i] in [0, n_groups), or -1 for a pair without a model.  order: the pairs in stable
- * ascending order of their model, those without one last (a pair whose index is out of range too, stored as ~pair); slot: each
- * pair's place in it; offsets [n_groups + 1]: model e's pairs are order[offsets[e]] .. order[offsets[e + 1] - 1].  work: int32,
+ * ascending order of their model, those without one last; slot: each pair's place in it (a pair whose index is out of range goes
+ * last too, and both hold the complement: ~pair, ~place); offsets [n_groups + 1]: model e's pairs are order[offsets[e]] .. order[offsets[e + 1] - 1].  work: int32,
  * mtk_route_rows_work elements (0: may be NULL).
  *
- * mtk_rows_dispatch: xs[s] = x[order[s] / k] for the n_rows * k pairs of n_rows records with k copies each, times w[order[s]] where w
- * is given; pair index = record * k + copy.  x: row stride x_ld; xs: dense, n_rows * k rows.  Rows of out-of-range pairs are NaN.
- * With y (dense, like xs) and dw: dw[order[s]] = <x[order[s] / k], y[s]> too (xs may then be NULL).
+ * mtk_rows_dispatch: xs[slot[n k + j]] = x[n] for the n_rows * k pairs of n_rows records with k copies each, times w[n k + j] where w is
+ * given.  x: row stride x_ld; xs: dense, n_rows * k rows.  Rows of out-of-range pairs are NaN, on both ways.  With y (dense, like xs) and dw:
+ * dw[n k + j] = <x[n], y[slot[n k + j]]> too (xs may then be NULL).
  * mtk_rows_combine: out[n] = sum_j w[n k + j] y[slot[n k + j]], j ascending, in fp32; w NULL: ones.
  * Each of the two is the other's gradient.  dtype: enum mtk_dtype of x / xs / y / out; w and dw are fp32. */
 #define MTK_ROUTE_MAX_GROUPS 1024
 int64_t mtk_route_rows_work(int64_t n_pairs, int n_groups);
 int mtk_route_rows(int64_t n_pairs, const int64_t* index, int n_groups, int32_t* order, int32_t* slot, int32_t* offsets, int32_t* work,
                    int64_t work_elems, mtk_stream stream);
-int mtk_rows_dispatch(int64_t n_rows, int k, int64_t D, int dtype, const void* x, int64_t x_ld, const int32_t* order, const float* w, void* xs,
+int mtk_rows_dispatch(int64_t n_rows, int k, int64_t D, int dtype, const void* x, int64_t x_ld, const int32_t* slot, const float* w, void* xs,
                       const void* y, float* dw, mtk_stream stream);
 int mtk_rows_combine(int64_t n_rows, int k, int64_t D, int dtype, const void* y, int64_t y_ld, const int32_t* slot, const float* w, void* out,
                      mtk_stream stream);

@@ -56,30 +56,44 @@ template <typename T> constexpr int kLine = 128 / (int)sizeof(T);
 inline int rank_pad(int r, int dtype) { return (int)mtk_up(r, 128 / mtk_dtype_size(dtype)); }
 constexpr int kRankT = 16;  // rows of u^T come in whole 16s
 
-// The models that own rows [at, end): each call yields one (e, first row, behind its last row).  Offsets are clamped and every step moves
-// forward, so whatever they hold no row outside [at, end) is named and the walk ends.
+// The models that own rows [at, end): each call yields one (e, first row, behind its last row).  Whatever the offsets hold, every step moves
+// forward and stays inside [at, end), so no other row is named and the walk ends.
+// One lane's search, by bisection:
+__device__ __forceinline__ int owner_of(const int32_t* off, int E, int64_t at) {  // number of offsets <= at, less one
+    int lo = 0, hi = E + 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (off[mid] <= at) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo - 1;
+}
+// A wave's walk: its lanes hold an offset each, so a step is a ballot and not a chain of loads (beyond 64 offsets, one load a 64).
 struct Owners {
     const int32_t* off;
     int E;
     int64_t at, end;
+    int held;  // lane's offset of the first 64
+    __device__ Owners(const int32_t* off_, int E_, int64_t at_, int64_t end_) : off(off_), E(E_), at(at_), end(end_) {
+        const int lane = __lane_id();
+        held = lane <= E ? off[lane] : 0x7fffffff;
+    }
     __device__ bool next(int& e, int64_t& a, int64_t& b) {
         while (at < end) {
-            int lo = 0, hi = E + 1;  // number of offsets <= at
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (off[mid] <= at) lo = mid + 1;
-                else hi = mid;
+            int lo = __popcll(__ballot(held <= at));
+            for (int i = 64; i <= E && lo == i; i += 64) {
+                const int k = i + (int)__lane_id();
+                lo += __popcll(__ballot((k <= E ? off[k] : 0x7fffffff) <= at));
             }
             if (lo > E) return false;  // behind the last model's rows
-            const int64_t to = off[lo] < end ? off[lo] : end;
-            if (lo == 0) {
-                at = to;
-                continue;
-            }
-            e = lo - 1;
+            int64_t to = lo < 64 ? __builtin_amdgcn_readlane(held, lo) : __builtin_amdgcn_readfirstlane(off[lo]);
+            to = to > at ? to : at + 1;
+            to = to < end ? to : end;
             a = at;
             b = to;
             at = to;
+            if (lo == 0) continue;
+            e = lo - 1;
             return true;
         }
         return false;
@@ -115,7 +129,7 @@ __global__ __launch_bounds__(256) void k_shrink(ShrinkArgs g, int j0, const T* _
     for (int p = 0; p < RR; ++p) xr[p] = x + (m0 + p * 16 + li < g.M ? m0 + p * 16 + li : g.M - 1) * g.x_ld + q * V;
     f32x4 keep[RR][RT] = {};
     bool mine[RR] = {}, any[RR] = {};  // this lane's rows: computed here / owned by any model
-    Owners own{g.offsets, g.E, m0, end};
+    Owners own(g.offsets, g.E, m0, end);
     int e, turn = 0;
     int64_t a, b;
     while (own.next(e, a, b)) {
@@ -160,7 +174,7 @@ __global__ __launch_bounds__(256) void k_shrink(ShrinkArgs g, int j0, const T* _
                         for (int t = 0; t < RT; ++t) acc[p][t] = mma16(fv[l][t][h], xv[l][p][h], acc[p][t]);
             k0 += L * step;
         };
-        constexpr int U = RT == 4 ? 2 : 4;
+        constexpr int U = RT == 4 ? 2 : (KS > 1 && RT == 1 ? 8 : 4);
         while (k0 + (U - 1) * step + KB <= g.K) lines(std::integral_constant<int, U>());
         while (k0 + KB <= g.K) lines(std::integral_constant<int, 1>());
         if (k0 < g.K) {  // the last, partial line
@@ -225,7 +239,7 @@ __global__ __launch_bounds__(256) void k_shrink(ShrinkArgs g, int j0, const T* _
 // y = act(x W^T + b + u B_e^T).  Weights are the MFMA's A operand: a lane then holds consecutive features of one record.
 //
 // k_linear, for more than a few rows: persistent workgroups walk tiles of BM rows x BN features; the k-blocks of ALL their tiles form one
-// stream of LDS-DMA (three buffers for rows, two for weights), so a tile's epilogue runs with the next tile's first blocks in flight.
+// stream of LDS-DMA (DX buffers for rows, DW for weights), so a tile's epilogue runs with the next tile's first blocks in flight.
 // The low-rank product is the last k-blocks of a tile: rows of u against rows of B_e (both zero behind the rank), the same
 // instructions through the same buffers.  That needs one model per tile; a tile with several (or none) takes a block of zeros there and a
 // several-model tile adds its products in the epilogue, made per model and selected by row.  With fewer rows a model than a tile
@@ -245,11 +259,13 @@ struct LinearArgs {
     int low_ld, rp;       // rp: elements of a row of U
 };
 
-template <int WR, int WC_, int MW, int NT> struct Geo {  // WR x WC waves, each MW x NT tiles of 32 x 32
+// WR x WC waves, each MW x NT tiles of 32 x 32; DX buffers of rows and DW of weights
+template <int WR, int WC_, int MW, int NT, int DX_, int DW_> struct Geo {
     static constexpr int WC = WC_, NW = WR * WC, WN = NT * 32, BM = WR * MW * 32, BN = WC * WN;
     static constexpr int kTileX = BM * 128, kTileW = BN * 128;       // bytes of a k-block
     static constexpr int XPW = BM / 8 / NW, WPW = BN / 8 / NW;       // 8-row, 1 KiB pieces per wave
-    static constexpr int kLds = 3 * kTileX + 2 * kTileW;
+    static constexpr int DX = DX_, DW = DW_, kLds = DX * kTileX + DW * kTileW;
+    static constexpr int kYounger = XPW + (DW - 2) * (XPW + WPW);    // pieces a wave requests after its last of the next block
 };
 
 extern __shared__ __attribute__((aligned(16))) unsigned char ad_smem[];
@@ -261,10 +277,10 @@ __device__ __forceinline__ int scalar_load(const int32_t* p) {
     return v;
 }
 
-template <typename T, int WR, int WC, int MW, int NT>
+template <typename T, int WR, int WC, int MW, int NT, int DX, int DW>
 __global__ __launch_bounds__(64 * WR * WC, 1) void k_linear(LinearArgs g, T* __restrict__ y) {
-    typedef Geo<WR, WC, MW, NT> G;
-    constexpr int V = mtk_piece<T>::n, kWBase = 3 * G::kTileX;
+    typedef Geo<WR, WC, MW, NT, DX, DW> G;
+    constexpr int V = mtk_piece<T>::n, kWBase = DX * G::kTileX;
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
     const int wv = __builtin_amdgcn_readfirstlane(wid);
     const int wr = wv / WC, wc = wv % WC, li = lane & 31, hh = lane >> 5;
@@ -292,54 +308,84 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void k_linear(LinearArgs g, T* __r
     auto dma = [&](const unsigned char* gp, unsigned voff, unsigned dst) {
         asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(gp), "s"(dst) : "memory");
     };
+    // The common step of a cursor is an addition, a wrap and a countdown: with one or two waves on a SIMD, scalar work between two
+    // barriers is time.
     const unsigned lo_ld = (unsigned)g.nkx * 128, x_ld = (unsigned)g.x_ld, w_ld = (unsigned)g.w_ld;
-    int cx_slot = wq, cx_kb = 0, cx_buf = 0, cw_slot = wq, cw_kb = 0, cw_buf = 0;
+    const unsigned x_dst0 = (unsigned)(wv * G::XPW * 1024), w_dst0 = (unsigned)(kWBase + wv * G::WPW * 1024);
+    unsigned x_dst = x_dst0, w_dst = w_dst0;
+    int cx_slot = wq, cw_slot = wq, x_left = 0, w_left = 0;  // blocks left at the source
+    int x_low = 1, w_low = 1;  // 1: the source is the low-rank lines (an int: a bool that loops is kept as a lane mask, and its selects in vector registers)
     const unsigned char *xb = nullptr, *wb = nullptr;
     unsigned xoff[G::XPW], woff[G::WPW];
-    auto x_source = [&](bool low) {
-        const int mt = (first + cx_slot) / g.nb_n;
-        const int64_t m0 = (int64_t)mt * G::BM;
+    auto x_source = [&]() {  // the next source of the row cursor; none: never counts down again
+        x_low = x_low == 0 && g.nkx > 0 ? 1 : 0;
+        if (x_low == 0) {
+            if (x_left < 0) cx_slot += wstride;
+            if (cx_slot >= slots) {
+                x_left = 0x7fffffff;
+                return;
+            }
+        }
+        const int64_t m0 = (int64_t)((first + cx_slot) / g.nb_n) * G::BM;
         const int rows = g.M - m0 < G::BM ? (int)(g.M - m0) : G::BM;
-        xb = low ? (const unsigned char*)g.U + m0 * lo_ld : (const unsigned char*)g.X + m0 * g.x_ld;
-        offsets(xoff, G::XPW, wv * G::XPW, rows, low ? lo_ld : x_ld);
+        unsigned ld;
+        if (x_low) {
+            x_left = g.nkx;
+            xb = (const unsigned char*)g.U + m0 * lo_ld;
+            ld = lo_ld;
+        } else {
+            x_left = g.nkb;
+            xb = (const unsigned char*)g.X + m0 * g.x_ld;
+            ld = x_ld;
+        }
+        offsets(xoff, G::XPW, wv * G::XPW, rows, ld);
     };
-    auto w_source = [&](bool low) {
+    auto w_source = [&]() {
+        w_low = w_low == 0 && g.nkx > 0 ? 1 : 0;
+        if (w_low == 0) {
+            if (w_left < 0) cw_slot += wstride;
+            if (cw_slot >= slots) {
+                w_left = 0x7fffffff;
+                return;
+            }
+        }
         const int id = first + cw_slot, mt = id / g.nb_n, n0 = (id - mt * g.nb_n) * G::BN;
         const int rows = g.N - n0 < G::BN ? g.N - n0 : G::BN;
-        if (low) {
+        unsigned ld;
+        if (w_low) {
             int e = scalar_load(g.owner + mt);
             e = e < 0 || e > g.E ? g.E : e;
+            w_left = g.nkx;
             wb = (const unsigned char*)g.Bp + ((int64_t)e * g.N + n0) * lo_ld;
+            ld = lo_ld;
         } else {
+            w_left = g.nkb;
             wb = (const unsigned char*)g.W + (int64_t)n0 * g.w_ld;
+            ld = w_ld;
         }
-        offsets(woff, G::WPW, wv * G::WPW, rows, low ? lo_ld : w_ld);
+        offsets(woff, G::WPW, wv * G::WPW, rows, ld);
     };
     auto x_op = [&](int j) {
-        if (cx_slot < slots) dma(xb, xoff[j], (unsigned)(cx_buf * G::kTileX + (wv * G::XPW + j) * 1024));
+        if (cx_slot < slots) dma(xb, xoff[j], x_dst + j * 1024);
     };
     auto w_op = [&](int j) {
-        if (cw_slot < slots) dma(wb, woff[j], (unsigned)(kWBase + cw_buf * G::kTileW + (wv * G::WPW + j) * 1024));
+        if (cw_slot < slots) dma(wb, woff[j], w_dst + j * 1024);
     };
     auto x_advance = [&]() {
-        if (cx_slot >= slots) return;
-        cx_buf = cx_buf == 2 ? 0 : cx_buf + 1;
         xb += 128;
-        if (++cx_kb == nk) {
-            cx_kb = 0;
-            cx_slot += wstride;
-            if (cx_slot < slots) x_source(false);
-        } else if (cx_kb == g.nkb) x_source(true);
+        x_dst = x_dst == x_dst0 + (DX - 1) * G::kTileX ? x_dst0 : x_dst + G::kTileX;
+        if (--x_left == 0) {
+            x_left = -1;
+            x_source();
+        }
     };
     auto w_advance = [&]() {
-        if (cw_slot >= slots) return;
-        cw_buf ^= 1;
         wb += 128;
-        if (++cw_kb == nk) {
-            cw_kb = 0;
-            cw_slot += wstride;
-            if (cw_slot < slots) w_source(false);
-        } else if (cw_kb == g.nkb) w_source(true);
+        w_dst = w_dst == w_dst0 + (DW - 1) * G::kTileW ? w_dst0 : w_dst + G::kTileW;
+        if (--w_left == 0) {
+            w_left = -1;
+            w_source();
+        }
     };
     const unsigned char* lds = ad_smem;
     struct Frags { mtk_vec<T> x[MW], w[NT]; };
@@ -368,17 +414,17 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void k_linear(LinearArgs g, T* __r
     };
 
     // One k-block: four steps of two pieces, fragments read one step ahead.  The barrier sits before the last step's MFMAs; the fragment reads
-    // and the DMA requests behind it ride under them.  After the barrier of block c a wave requests its pieces of weight block c + 2,
-    // THEN of row block c + 3: loads return in order, so at the next wait vmcnt(XPW) - all but those last row pieces - means that
-    // weight block c + 2 and row block c + 2 (requested a block earlier) have landed.
+    // and the DMA requests behind it ride under them.  After the barrier of block c a wave requests its pieces of weight block c + DW,
+    // THEN of row block c + DX (DX >= DW).  Loads return in order, so at the end of block c all but the kYounger pieces requested after
+    // weight block c + 1 (row block c + 1 is older still) done means that block c + 1 has landed.
     Frags F0, F1;
-    x_source(false);
-    w_source(false);
-    for (int b = 0; b < 3; ++b) {
+    x_source();
+    w_source();
+    for (int b = 0; b < DX; ++b) {
 #pragma unroll
         for (int j = 0; j < G::XPW; ++j) x_op(j);
         x_advance();
-        if (b < 2) {
+        if (b < DW) {
 #pragma unroll
             for (int j = 0; j < G::WPW; ++j) w_op(j);
             w_advance();
@@ -417,15 +463,15 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void k_linear(LinearArgs g, T* __r
             mma_all(F1);
             read_frags(F1, xi, wi, 3);
             mma_all(F0);
-            // Stores of the previous tile may be outstanding too and do not return in order with the loads, but the count still holds: with S
-            // stores, the weight pieces and XPW younger row pieces in flight, "at most XPW outstanding" needs S + WPW completions,
-            // and fewer than WPW loads done (weights come first) would leave at most S + WPW - 1.
-            if (x_tail) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(G::XPW) : "memory");
+            // Stores of the previous tile may be outstanding too and do not return in order with the loads, but the count still holds: with S stores,
+            // N needed and kYounger younger pieces in flight, "at most kYounger outstanding" needs S + N completions, and fewer than
+            // N loads done (the needed ones come first) would leave at most S + N - 1.
+            if (x_tail) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(G::kYounger) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __syncthreads();  // everyone's share has landed, and this block's buffers have no readers left
             __builtin_amdgcn_sched_barrier(0);
-            const int xn = xi == 2 ? 0 : xi + 1;
-            if (kb + 1 < nk) read_frags(F0, xn, wi ^ 1, 0);
+            const int xn = xi == DX - 1 ? 0 : xi + 1, wn = wi == DW - 1 ? 0 : wi + 1;
+            if (kb + 1 < nk) read_frags(F0, xn, wn, 0);
             constexpr int OPW = G::XPW + G::WPW;
 #pragma unroll
             for (int mt = 0; mt < MW; ++mt) {
@@ -442,7 +488,7 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void k_linear(LinearArgs g, T* __r
             x_tail = cx_slot < slots;
             x_advance();
             xi = xn;
-            wi ^= 1;
+            wi = wn;
             __builtin_amdgcn_sched_barrier(0);
         }
 
@@ -452,7 +498,7 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void k_linear(LinearArgs g, T* __r
         const int li_e = lane_e & 31, hh_e = lane_e >> 5;
         if (g.low && (!g.nkx || scalar_load(g.owner + mtile) < 0)) {  // several models in this tile
             const int64_t w0 = m0 + wr * MW * 32, w1 = w0 + MW * 32;
-            Owners own{g.offsets, g.E, w0, w1 < g.M ? w1 : g.M};
+            Owners own(g.offsets, g.E, w0, w1 < g.M ? w1 : g.M);
             int e;
             int64_t a, b;
             const T* u = (const T*)g.U;
@@ -547,6 +593,12 @@ __global__ __launch_bounds__(512) void k_linear_few(FewArgs g, const T* __restri
     const int n0 = (int)(blockIdx.x % nb) * 32;
     const T* xr = x + (m0 + li < g.M ? m0 + li : g.M - 1) * g.x_ld;
     const T* wr = W + (int64_t)(n0 + li < g.N ? n0 + li : g.N - 1) * g.K;
+    int who[2];  // the models of this thread's two outputs' rows: a chain of loads, begun before the product's
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int64_t row = m0 + ((tid + i * 512) >> 5);
+        who[i] = owner_of(g.offsets, g.E, row < g.M ? row : g.M - 1);
+    }
     f32x16 acc = {};
     for (int k0 = wave * KB; k0 < g.K; k0 += NW * KB) {
         mtk_vec<T> xa[4], wa[4];
@@ -580,10 +632,8 @@ __global__ __launch_bounds__(512) void k_linear_few(FewArgs g, const T* __restri
 #pragma unroll
         for (int w = 0; w < NW; ++w) v += part[w][rr][jj];
         if (bias) v += (float)bias[n];
-        Owners own{g.offsets, g.E, row, row + 1};
-        int e;
-        int64_t a, b;
-        if (own.next(e, a, b)) {
+        const int e = who[i];
+        if (e >= 0 && e < g.E) {
             const T *ur = u + row * g.rp, *br = up + ((int64_t)e * g.N + n) * g.r;
             float low = 0.f;
             for (int j = 0; j < g.r; j += V) {
@@ -622,7 +672,7 @@ __device__ void wgrad_body(const WgradArgs& g, int strip, int c, int j0, const T
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, q = lane >> 4;
     const int c0 = strip * kStrip<T> + li * NV, cols = g.D - c0;
     const int64_t lo = (int64_t)c * g.chunk, hi = lo + g.chunk < g.M ? lo + g.chunk : g.M;
-    Owners own{g.offsets, g.E, lo, hi};
+    Owners own(g.offsets, g.E, lo, hi);
     int e;
     int64_t a, b;
     const int jp = (int)mtk_up(g.r, kRankT);
@@ -844,11 +894,10 @@ __global__ __launch_bounds__(256) void k_prep(Jobs jobs) {
         const int64_t i = blk * 256 + threadIdx.x;
         if (i < j.C) {
             const int64_t a0 = i * j.R, a1 = a0 + j.R < j.rows ? a0 + j.R : j.rows;
-            Owners own{(const int32_t*)j.src, j.E, a0, a1};
-            int e;
-            int64_t a, b;
-            int who = j.E;
-            if (own.next(e, a, b)) who = a == a0 && b == a1 ? e : -1;
+            const int32_t* off = (const int32_t*)j.src;
+            const int e0 = owner_of(off, j.E, a0), e1 = owner_of(off, j.E, a1 - 1);
+            // rows before the first offset (-1) and behind the last (E) have no model
+            const int who = e0 == e1 ? (e0 < 0 ? j.E : e0) : -1;
             ((int32_t*)j.dst)[i] = who;
         }
     }
@@ -944,7 +993,9 @@ struct Shape {
         line = 128 / mtk_dtype_size(dtype);
         rp = rank_pad(r, dtype);
         Kp = (int)mtk_up(K, line);
-        few = M <= 256;
+        // us for K = N = 1024, few rows / 64 x 64 tiles (and some 5 for their k_prep): bf16 256 rows 9.0 / 9.9, 512 rows 13.9 / 9.4, 1,024 rows
+        // 26 / 9.3; fp32 256 rows 14 / 26, 512 rows 24 / 26, 1,024 rows 45 / 27
+        few = M <= 512;
         // 256 x 256 tiles (one workgroup a CU) where they fill their rounds over the CUs to four fifths; 64 x 64 while the chip is not full.  us for
         // K = N = 1024, 256 / 128 / 64: bf16 65,536 rows 123 / 159 / 232, 20,011 rows 77 / 54 / 71, 8,192 rows 33 / 24 / 31, 2,048 rows
         // 33 / 16 / 13; fp32 20,011 rows 540 / 338 / 346, 8,192 rows 262 / 144 / 140, 2,048 rows 264 / 79 / 43
@@ -1027,25 +1078,25 @@ DeviceState* device_state() {
     return &st[d];
 }
 
-template <typename T, int WR, int WC, int MW, int NT>
+template <typename T, int WR, int WC, int MW, int NT, int DX, int DW>
 int launch_linear(LinearArgs& g, T* y, int which, hipStream_t s) {
-    typedef Geo<WR, WC, MW, NT> G;
+    typedef Geo<WR, WC, MW, NT, DX, DW> G;
     DeviceState* st = device_state();
     if (!st) MTK_FAIL(MTK_ERR_HIP, "adapter product: no device properties");
     if (!st->lds[which]) {
-        MTK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear<T, WR, WC, MW, NT>), hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds));
+        MTK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear<T, WR, WC, MW, NT, DX, DW>), hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds));
         st->lds[which] = true;
     }
     const int64_t per_xcd = cdiv(g.MT * g.nb_n, 8), room = (int64_t)st->cus / 8 * (163840 / G::kLds);
-    k_linear<T, WR, WC, MW, NT><<<(unsigned)(8 * (per_xcd < room ? per_xcd : room)), 64 * G::NW, G::kLds, s>>>(g, y);
+    k_linear<T, WR, WC, MW, NT, DX, DW><<<(unsigned)(8 * (per_xcd < room ? per_xcd : room)), 64 * G::NW, G::kLds, s>>>(g, y);
     return MTK_OK;
 }
 template <typename T> int linear(const Shape& sh, LinearArgs& g, T* y, hipStream_t s) {
     constexpr int base = sizeof(T) == 4 ? 0 : std::is_same<T, mtk_bf16>::value ? 3 : 6;
     if constexpr (sizeof(T) == 2)
-        if (sh.kind == 0) return launch_linear<T, 2, 4, 4, 2>(g, y, base, s);
-    if (sh.kind == 1) return launch_linear<T, 4, 2, 1, 2>(g, y, base + 1, s);
-    return launch_linear<T, 2, 2, 1, 1>(g, y, base + 2, s);
+        if (sh.kind == 0) return launch_linear<T, 2, 4, 4, 2, 3, 2>(g, y, base, s);
+    if (sh.kind == 1) return launch_linear<T, 4, 2, 1, 2, 3, 2>(g, y, base + 1, s);
+    return launch_linear<T, 2, 2, 1, 1, 3, 2>(g, y, base + 2, s);
 }
 template <typename T>
 void linear_few(const FewArgs& g, const T* x, const T* W, const T* bias, const T* u, const T* up, T* y, hipStream_t s) {

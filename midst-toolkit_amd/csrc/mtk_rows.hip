@@ -5,12 +5,14 @@
 //   dispatch  xs[s] = x[order[s] / k] (times w[order[s]])      combine  out[n] = sum_j w[n, j] y[slot[n, j]]
 // and each is the other's gradient, so two row kernels serve the four directions; the gradient of the weights, <gout[n], y[s]>, rides
 // in the dispatch of gout.  Sums run over j (or along the row in a fixed tree) in fp32: no atomics, the same bits every run.
+#include <type_traits>
+
 #include "mtk_lowp.h"
 
 namespace {
 
 constexpr int RT = 512, RW = RT / 64;      // threads / waves of a routing workgroup
-constexpr int64_t kRouteChunk = 8192;      // pairs of a workgroup, until there are kRouteBlocks of them
+constexpr int64_t kRouteChunk = 2048;      // pairs of a workgroup, until there are kRouteBlocks of them
 constexpr int kRouteBlocks = 128;
 
 struct RouteArgs {
@@ -50,19 +52,19 @@ __global__ __launch_bounds__(RT) void k_route_place(RouteArgs a) {
     const int64_t per = a.chunk / RW, wlo = lo + wave * per, whi = wlo + per < hi ? wlo + per : hi;
     for (int64_t i = wlo + lane; i < whi; i += 64) atomicAdd(&ctr[wave * bins + route_key(a.index[i], a.E)], 1);
     __syncthreads();
-    for (int b = tid; b < bins; b += RT) {
-        int before = 0, all = 0;
-        if (a.nblk > 1) {
-            for (int q = 0; q < a.nblk; ++q) {
-                const int c = a.counts[(int64_t)q * bins + b];
-                before += q < (int)blockIdx.x ? c : 0;
-                all += c;
+    for (int b = tid; b < bins; b += RT) base[b] = tot[b] = 0;
+    __syncthreads();
+    if (a.nblk > 1) {
+        for (int i = tid; i < a.nblk * bins; i += RT) {
+            const int q = i / bins, b = i - q * bins, c = a.counts[i];
+            if (c) {
+                atomicAdd(&tot[b], c);
+                if (q < (int)blockIdx.x) atomicAdd(&base[b], c);
             }
-        } else {
-            for (int w = 0; w < RW; ++w) all += ctr[w * bins + b];
         }
-        base[b] = before;
-        tot[b] = all;
+    } else {
+        for (int i = tid; i < RW * bins; i += RT)
+            if (ctr[i]) atomicAdd(&tot[i % bins], ctr[i]);
     }
     __syncthreads();
     // exclusive prefix over the keys: a wave scans 64 at a time, carrying the sum (at most 17 rounds)
@@ -94,10 +96,12 @@ __global__ __launch_bounds__(RT) void k_route_place(RouteArgs a) {
     int bits = 0;
     while ((1 << bits) < bins) ++bits;
     volatile int32_t* my = ctr + wave * bins;  // one wave's LDS operations complete in order: no barrier inside the loop
+    int64_t ahead = wlo + lane < whi ? a.index[wlo + lane] : -1;
     for (int64_t i0 = wlo; i0 < whi; i0 += 64) {
         const int64_t i = i0 + lane;
         const bool live = i < whi;
-        const int64_t v = live ? a.index[i] : -1;
+        const int64_t v = ahead;
+        ahead = i + 64 < whi ? a.index[i + 64] : -1;
         const int key = route_key(v, a.E);
         unsigned long long same = __ballot(live);
         for (int b = 0; b < bits; ++b) {
@@ -107,92 +111,163 @@ __global__ __launch_bounds__(RT) void k_route_place(RouteArgs a) {
         const unsigned long long below = same & ((1ull << lane) - 1);
         if (live) {
             const int s = my[key] + __popcll(below);
-            a.slot[i] = s;
-            a.order[s] = v < -1 || v >= a.E ? ~(int32_t)i : (int32_t)i;
+            const bool bad = v < -1 || v >= a.E;
+            a.slot[i] = bad ? ~s : s;
+            a.order[s] = bad ? ~(int32_t)i : (int32_t)i;
             if (below == 0) my[key] = s + __popcll(same);
         }
     }
 }
 
 struct RowsArgs {
-    int64_t n;        // rows written
-    int64_t other;    // rows of the tensor that is read
+    int64_t n;        // records
+    int64_t other;    // pairs
     int64_t D, ld;    // width; row stride of the tensor that is read
     int k;            // copies per record
-    const int32_t* map;  // order [n] (dispatch) or slot [n][k] (combine)
+    const int32_t* map;  // slot [n][k]
     const float* w;      // [pairs] or null
     int lpr;             // lanes of a row: a power of two up to 64
+    bool nt;             // stores past the caches
 };
 
-// xs[s] = x[pair / k] (times w[pair]); pair = order[s].  A row of a pair whose index was out of range (stored as ~pair) is NaN: loud,
-// never an out-of-range read.  With y: dw[pair] = <x[pair / k], y[s]> as well (x is the gradient of the combined rows then).
-// Bound by bandwidth: a row belongs to lpr lanes, each moving 16-byte pieces, so a wave reads whole lines.
-template <typename T, bool W, bool DOT>
+// A pair whose index was out of range has ~place for a slot: its rows are NaN on both ways, loud, and never an out-of-range access.
+// KC: copies at a time, 1, 2 or 4.
+template <int KC> struct Copies {
+    int32_t s[KC];
+    float w[KC];
+};
+// the slots and weights of record n's copies j0 ..; behind the last copy, the first again.  Loaded a record ahead of their use: they would
+// otherwise be a round trip to memory in front of every row.
+template <bool W, int KC> __device__ __forceinline__ Copies<KC> copies_of(const RowsArgs& a, int64_t n, int j0) {
+    Copies<KC> c;
+    n = n < a.n ? n : a.n - 1;
+#pragma unroll
+    for (int j = 0; j < KC; ++j) {
+        const int64_t pair = n * a.k + (j0 + j < a.k ? j0 + j : j0);
+        c.s[j] = a.map[pair];
+        c.w[j] = W ? a.w[pair] : 1.f;
+    }
+    return c;
+}
+__device__ __forceinline__ int64_t place_of(int32_t s, int64_t pairs, bool& bad) {
+    bad = s < 0;
+    s = bad ? ~s : s;
+    return s < pairs ? s : pairs - 1;
+}
+
+// xs[slot[n, j]] = x[n] (times w[n, j]) for all copies j: a record's row is read once and written k times.  With y: dw[n, j] =
+// <x[n], y[slot[n, j]]> as well (x is the gradient of the combined rows then).  Bound by bandwidth: a row belongs to lpr lanes, each moving
+// 16-byte pieces, so a wave touches whole lines.
+template <typename T, bool W, bool DOT, int KC>
 __global__ __launch_bounds__(256) void k_dispatch(RowsArgs a, const T* __restrict__ x, T* __restrict__ xs, const T* __restrict__ y, float* __restrict__ dw) {
     constexpr int V = mtk_piece<T>::n;
     const int sub = threadIdx.x & (a.lpr - 1);
-    for (int64_t s = (int64_t)blockIdx.x * (256 / a.lpr) + threadIdx.x / a.lpr; s < a.n; s += (int64_t)gridDim.x * (256 / a.lpr)) {
-        float dot = 0.f;
-        int p = a.map[s];
-        const bool bad = p < 0;
-        p = bad ? ~p : p;
-        int64_t row = p / a.k;
-        row = row < a.other ? row : a.other - 1;
-        const float w = bad ? __builtin_nanf("") : (W ? a.w[p] : 1.f);
-        const T* src = x + row * a.ld;
-        T* dst = xs ? xs + s * a.D : nullptr;
-        const T* ys = DOT ? y + s * a.D : nullptr;
-        for (int64_t c = (int64_t)sub * V; c < a.D; c += (int64_t)a.lpr * V) {
-            const int left = a.D - c < V ? (int)(a.D - c) : V;
-            mtk_vec<T> v = left == V ? mtk_ld(src + c) : mtk_ld_n(src + c, left);
-            if (DOT) {
-                const mtk_vec<T> q = left == V ? mtk_ld(ys + c) : mtk_ld_n(ys + c, left);
+    const int64_t pairs = a.n * a.k, stride = (int64_t)gridDim.x * (256 / a.lpr);
+    int64_t n = (int64_t)blockIdx.x * (256 / a.lpr) + threadIdx.x / a.lpr;
+    Copies<KC> next = copies_of<W, KC>(a, n, 0);
+    for (; n < a.n; n += stride) {
+        const T* src = x + n * a.ld;
+        for (int j0 = 0; j0 < a.k; j0 += KC) {
+            const int nj = a.k - j0 < KC ? a.k - j0 : KC;
+            const Copies<KC> cur = next;
+            next = j0 + KC < a.k ? copies_of<W, KC>(a, n, j0 + KC) : copies_of<W, KC>(a, n + stride, 0);
+            int64_t at[KC];
+            float w[KC], dot[KC];
+            bool scaled = W;
 #pragma unroll
-                for (int i = 0; i < V; ++i) dot += (float)v.v[i] * (float)q.v[i];
+            for (int j = 0; j < KC; ++j) {
+                bool bad;
+                at[j] = place_of(cur.s[j], pairs, bad) * a.D;
+                w[j] = bad ? __builtin_nanf("") : cur.w[j];
+                scaled |= bad;
+                dot[j] = 0.f;
             }
-            if (W || bad) {
+#pragma unroll 2
+            for (int64_t c = (int64_t)sub * V; c < a.D; c += (int64_t)a.lpr * V) {
+                const int left = a.D - c < V ? (int)(a.D - c) : V;
+                const mtk_vec<T> v = left == V ? mtk_ld(src + c) : mtk_ld_n(src + c, left);
+                if (DOT) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) v.v[i] = (T)((float)v.v[i] * w);
+                    for (int j = 0; j < KC; ++j) {
+                        if (j >= nj) break;
+                        const T* ys = y + at[j] + c;
+                        const mtk_vec<T> q = left == V ? mtk_ld(ys) : mtk_ld_n(ys, left);
+#pragma unroll
+                        for (int i = 0; i < V; ++i) dot[j] += (float)v.v[i] * (float)q.v[i];
+                    }
+                }
+                if (!DOT || xs) {
+#pragma unroll
+                    for (int j = 0; j < KC; ++j) {
+                        if (j >= nj) break;
+                        mtk_vec<T> o = v;
+                        if (scaled) {
+#pragma unroll
+                            for (int i = 0; i < V; ++i) o.v[i] = (T)((float)v.v[i] * w[j]);
+                        }
+                        T* op = xs + at[j] + c;
+                        if (left < V) mtk_st_n(op, o, left);
+                        else if (a.nt) mtk_st_nt(op, o);
+                        else mtk_st(op, o);
+                    }
+                }
             }
-            if (!DOT || dst) {
-                if (left == V) mtk_st(dst + c, v);
-                else mtk_st_n(dst + c, v, left);
+            if (DOT) {  // the lanes of a row leave the loop together, and the exchange stays among them
+#pragma unroll
+                for (int j = 0; j < KC; ++j) {
+                    for (int d = a.lpr >> 1; d > 0; d >>= 1) dot[j] += __shfl_xor(dot[j], d);
+                    if (sub == 0 && j < nj) dw[n * a.k + j0 + j] = dot[j];
+                }
             }
-        }
-        if (DOT) {  // the lanes of a row leave the loop together, and the exchange stays among them
-            for (int d = a.lpr >> 1; d > 0; d >>= 1) dot += __shfl_xor(dot, d);
-            if (sub == 0) dw[p] = dot;
         }
     }
 }
 
-// out[n] = sum_j (w[n, j]) y[slot[n, j]], j ascending, fp32, rounded once
-template <typename T, bool W>
+// out[n] = sum_j (w[n, j]) y[slot[n, j]], j ascending, fp32, rounded once; four copies' loads in flight
+template <typename T, bool W, int KC>
 __global__ __launch_bounds__(256) void k_combine(RowsArgs a, const T* __restrict__ y, T* __restrict__ out) {
     constexpr int V = mtk_piece<T>::n;
     const int sub = threadIdx.x & (a.lpr - 1);
-    for (int64_t n = (int64_t)blockIdx.x * (256 / a.lpr) + threadIdx.x / a.lpr; n < a.n; n += (int64_t)gridDim.x * (256 / a.lpr))
-    for (int64_t c = (int64_t)sub * V; c < a.D; c += (int64_t)a.lpr * V) {
-        const int32_t* slots = a.map + n * a.k;
-        const float* ws = W ? a.w + n * a.k : nullptr;
-        const int left = a.D - c < V ? (int)(a.D - c) : V;
-        float acc[V];
+    const int64_t stride = (int64_t)gridDim.x * (256 / a.lpr);
+    int64_t n = (int64_t)blockIdx.x * (256 / a.lpr) + threadIdx.x / a.lpr;
+    Copies<KC> next = copies_of<W, KC>(a, n, 0);
+    for (; n < a.n; n += stride) {
+        const Copies<KC> first = next;
+        next = copies_of<W, KC>(a, n + stride, 0);
+#pragma unroll 2
+        for (int64_t c = (int64_t)sub * V; c < a.D; c += (int64_t)a.lpr * V) {
+            const int left = a.D - c < V ? (int)(a.D - c) : V;
+            float acc[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = 0.f;
-        for (int j = 0; j < a.k; ++j) {
-            int64_t s = slots[j];
-            s = s < 0 ? 0 : (s < a.other ? s : a.other - 1);
-            const float w = W ? ws[j] : 1.f;
-            const T* src = y + s * a.ld + c;
-            const mtk_vec<T> v = left == V ? mtk_ld(src) : mtk_ld_n(src, left);
+            for (int i = 0; i < V; ++i) acc[i] = 0.f;
+            auto add = [&](const Copies<KC>& cp, int nj) {
+                mtk_vec<T> v[KC];
+                float w[KC];
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] += W ? w * (float)v.v[i] : (float)v.v[i];
+                for (int j = 0; j < KC; ++j) {
+                    if (j >= nj) break;
+                    bool bad;
+                    const T* src = y + place_of(cp.s[j], a.other, bad) * a.ld + c;
+                    w[j] = bad ? __builtin_nanf("") : cp.w[j];
+                    v[j] = left == V ? mtk_ld(src) : mtk_ld_n(src, left);
+                }
+#pragma unroll
+                for (int j = 0; j < KC; ++j) {
+                    if (j >= nj) break;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) acc[i] += w[j] * (float)v[j].v[i];
+                }
+            };
+            add(first, a.k < KC ? a.k : KC);
+            for (int j0 = KC; j0 < a.k; j0 += KC) add(copies_of<W, KC>(a, n, j0), a.k - j0 < KC ? a.k - j0 : KC);
+            mtk_vec<T> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] = (T)acc[i];
+            T* op = out + n * a.D + c;
+            if (left < V) mtk_st_n(op, o, left);
+            else if (a.nt) mtk_st_nt(op, o);
+            else mtk_st(op, o);
         }
-        mtk_vec<T> o;
-#pragma unroll
-        for (int i = 0; i < V; ++i) o.v[i] = (T)acc[i];
-        if (left == V) mtk_st(out + n * a.D + c, o);
-        else mtk_st_n(out + n * a.D + c, o, left);
     }
 }
 
@@ -202,10 +277,23 @@ int lanes_per_row(int64_t D, int V) {
     return l;
 }
 
-// one row per lane group, up to 2^22 workgroups (a launch holds fewer than 2^32 threads)
+// Stores go past the caches where what a call reads and writes exceeds what they hold (256 MB): the result's readers would find nothing there.
+// us, past them / through them: 100,000 rows of 1024 bf16, two copies, out 128 / 221.
+constexpr int64_t kCaches = 256ll << 20;
+template <typename F> void by_flags(bool a, bool b, int k, F f) {
+    auto third = [&](auto ta, auto tb) {
+        if (k == 1) f(ta, tb, std::integral_constant<int, 1>());
+        else if (k == 2) f(ta, tb, std::integral_constant<int, 2>());
+        else f(ta, tb, std::integral_constant<int, 4>());
+    };
+    auto second = [&](auto ta) { b ? third(ta, std::true_type()) : third(ta, std::false_type()); };
+    a ? second(std::true_type()) : second(std::false_type());
+}
+
+// a row per lane group; from 16 workgroups a CU on they walk
 unsigned rows_grid(const RowsArgs& a) {
     const int64_t nb = (a.n + 256 / a.lpr - 1) / (256 / a.lpr);
-    return (unsigned)(nb < (1 << 22) ? nb : (1 << 22));
+    return (unsigned)(nb < 4096 ? nb : 4096);
 }
 
 int route_blocks(int64_t P, int64_t* chunk) {
@@ -249,23 +337,21 @@ extern "C" int mtk_route_rows(int64_t n_pairs, const int64_t* index, int n_group
     return MTK_OK;
 }
 
-extern "C" int mtk_rows_dispatch(int64_t n_rows, int k, int64_t D, int dtype, const void* x, int64_t x_ld, const int32_t* order, const float* w,
+extern "C" int mtk_rows_dispatch(int64_t n_rows, int k, int64_t D, int dtype, const void* x, int64_t x_ld, const int32_t* slot, const float* w,
                                  void* xs, const void* y, float* dw, mtk_stream stream) {
     if (const int rc = rows_check("mtk_rows_dispatch", n_rows, k, D, x_ld, dtype)) return rc;
     if (n_rows == 0) return MTK_OK;
-    if (!x || !order || (!xs && !dw) || ((y != nullptr) != (dw != nullptr))) MTK_FAIL(MTK_ERR_ARG, "mtk_rows_dispatch: null pointer");
+    if (!x || !slot || (!xs && !dw) || ((y != nullptr) != (dw != nullptr))) MTK_FAIL(MTK_ERR_ARG, "mtk_rows_dispatch: null pointer");
     mtk_by_type(dtype, [&](auto t) {
         typedef decltype(t) T;
-        RowsArgs a{n_rows * k, n_rows, D, x_ld, k, order, w, lanes_per_row(D, mtk_piece<T>::n)};
+        const int64_t touched = n_rows * D * (int64_t)sizeof(T) * (1 + k + (y ? k : 0));
+        RowsArgs a{n_rows, n_rows * k, D, x_ld, k, slot, w, lanes_per_row(D, mtk_piece<T>::n), touched > kCaches};
         const unsigned grid = rows_grid(a);
         const T* xp = (const T*)x;
-        if (dw) {
-            if (w) k_dispatch<T, true, true><<<grid, 256, 0, (hipStream_t)stream>>>(a, xp, (T*)xs, (const T*)y, dw);
-            else k_dispatch<T, false, true><<<grid, 256, 0, (hipStream_t)stream>>>(a, xp, (T*)xs, (const T*)y, dw);
-        } else {
-            if (w) k_dispatch<T, true, false><<<grid, 256, 0, (hipStream_t)stream>>>(a, xp, (T*)xs, nullptr, nullptr);
-            else k_dispatch<T, false, false><<<grid, 256, 0, (hipStream_t)stream>>>(a, xp, (T*)xs, nullptr, nullptr);
-        }
+        const hipStream_t s = (hipStream_t)stream;
+        by_flags(w != nullptr, dw != nullptr, k, [&](auto tw, auto td, auto tk) {
+            k_dispatch<T, decltype(tw)::value, decltype(td)::value, decltype(tk)::value><<<grid, 256, 0, s>>>(a, xp, (T*)xs, (const T*)y, dw);
+        });
     });
     MTK_HIP(hipGetLastError());
     return MTK_OK;
@@ -278,10 +364,10 @@ extern "C" int mtk_rows_combine(int64_t n_rows, int k, int64_t D, int dtype, con
     if (!y || !slot || !out) MTK_FAIL(MTK_ERR_ARG, "mtk_rows_combine: null pointer");
     mtk_by_type(dtype, [&](auto t) {
         typedef decltype(t) T;
-        RowsArgs a{n_rows, n_rows * k, D, y_ld, k, slot, w, lanes_per_row(D, mtk_piece<T>::n)};
+        RowsArgs a{n_rows, n_rows * k, D, y_ld, k, slot, w, lanes_per_row(D, mtk_piece<T>::n), n_rows * D * (int64_t)sizeof(T) * (1 + k) > kCaches};
         const unsigned grid = rows_grid(a);
-        if (w) k_combine<T, true><<<grid, 256, 0, (hipStream_t)stream>>>(a, (const T*)y, (T*)out);
-        else k_combine<T, false><<<grid, 256, 0, (hipStream_t)stream>>>(a, (const T*)y, (T*)out);
+        const hipStream_t s = (hipStream_t)stream;
+        by_flags(w != nullptr, false, k, [&](auto tw, auto, auto tk) { k_combine<T, decltype(tw)::value, decltype(tk)::value><<<grid, 256, 0, s>>>(a, (const T*)y, (T*)out); });
     });
     MTK_HIP(hipGetLastError());
     return MTK_OK;

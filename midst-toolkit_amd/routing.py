@@ -31,8 +31,8 @@ def rows_of(t: Tensor) -> Tensor:
 
 
 class RowPlan:
-    """Where the pairs go: what ``route_rows`` returns.  ``order`` [P] int32: the pair in each place (``~pair`` for one whose index was out
-    of range), ``slot`` (the shape of ``index``) int32: the place of each pair, ``offsets`` [n_groups + 1] int32: model e's pairs are in
+    """Where the pairs go: what ``route_rows`` returns.  ``order`` [P] int32: the pair in each place, ``slot`` (the shape of ``index``) int32: the
+    place of each pair (for a pair whose index was out of range both hold the complement, ``~pair`` and ``~place``), ``offsets`` [n_groups + 1] int32: model e's pairs are in
     places ``offsets[e]`` to ``offsets[e + 1] - 1``, pairs without a model behind them all."""
 
     __slots__ = ("order", "slot", "offsets", "n_groups", "n_rows", "copies")
@@ -45,7 +45,7 @@ class RowPlan:
 def route_rows(index: Tensor, n_groups: int) -> RowPlan:
     """Plan for ``index`` [N] or [N, k] (whole numbers): the model of record n's copy j, in [0, n_groups), or -1 for a copy without a
     model.  The same model twice in a record is two pairs.  Pairs keep their order within a model.  A pair whose index is out of
-    range is treated like -1 and its dispatched row is NaN."""
+    range goes where -1 goes, and its rows are NaN: dispatched, combined and in gradients."""
     if not index.is_cuda:
         raise RuntimeError("route_rows: midst_toolkit_amd has no CPU path; move the indices to the MI355X")
     if index.dim() not in (1, 2) or index.dtype.is_floating_point or index.dtype.is_complex or index.dtype == torch.bool:
@@ -88,7 +88,7 @@ def _dispatch(x: Tensor, plan: RowPlan, w: Tensor | None, y: Tensor | None = Non
     xs = torch.empty((P, D), dtype=x.dtype, device=dev) if want_rows else None
     dw = torch.empty((plan.n_rows, plan.copies), dtype=torch.float32, device=dev) if y is not None else None
     if P:
-        launch(dev, _lib.lib().mtk_rows_dispatch, plan.n_rows, plan.copies, D, DTYPES[x.dtype], x.data_ptr(), x.stride(0), plan.order.data_ptr(),
+        launch(dev, _lib.lib().mtk_rows_dispatch, plan.n_rows, plan.copies, D, DTYPES[x.dtype], x.data_ptr(), x.stride(0), plan.slot.data_ptr(),
                None if w is None else w.data_ptr(), None if xs is None else xs.data_ptr(), None if y is None else y.data_ptr(),
                None if dw is None else dw.data_ptr())
     return xs, dw

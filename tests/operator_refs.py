@@ -8,7 +8,7 @@ import torch
 
 
 def route_reference(index: np.ndarray, groups: int):
-    """(order with ~pair for out-of-range indices, slot, offsets)"""
+    """(order, slot, offsets); an out-of-range index has ~pair and ~place"""
     flat = index.reshape(-1)
     bad = (flat < -1) | (flat >= groups)
     key = np.where((flat < 0) | bad, groups, flat)
@@ -16,7 +16,7 @@ def route_reference(index: np.ndarray, groups: int):
     slot = np.empty_like(order)
     slot[order] = np.arange(len(order))
     offsets = np.array([int((key < e).sum()) for e in range(groups + 1)])
-    return np.where(bad[order], ~order, order), slot.reshape(index.shape), offsets
+    return np.where(bad[order], ~order, order), np.where(bad, ~slot, slot).reshape(index.shape), offsets
 
 
 def adapter_reference(x, weight, bias, down, up, offsets, scale, relu, gy=None):

@@ -151,12 +151,31 @@ def test_rows_keep_bad_values_to_themselves(dt):
     assert torch.equal(torch.nan_to_num(xs[~bad].float()), torch.nan_to_num(x.cpu()[src[~bad]].float()))
     y = randn(g, N * k, D, dt=dt)
     clean = mtk.combine_rows(y, plan)
+    lost = torch.zeros(N, dtype=torch.bool)  # a record with a pair out of range is NaN on the way back, and in its gradient, too
+    lost[[N // 2, N - 1]] = True
+    assert bool(torch.isnan(clean.cpu()[lost]).all()) and bool(torch.isfinite(clean.cpu()[~lost]).all())
+    leaf = torch.zeros(N, D, dtype=dt, device=DEV, requires_grad=True)
+    mtk.dispatch_rows(leaf, plan).backward(y)
+    assert bool(torch.isnan(leaf.grad.cpu()[lost]).all()) and torch.equal(leaf.grad.cpu()[~lost], clean.cpu()[~lost])
     s = int(slot[11, 1])
     y[s] = float("nan")
     got = mtk.combine_rows(y, plan)
     assert bool(torch.isnan(got[11]).all())
-    rest = torch.arange(N) != 11
+    rest = (torch.arange(N) != 11) & ~lost
     assert torch.equal(got.cpu()[rest], clean.cpu()[rest])
+
+
+def test_rows_past_the_caches():
+    """A result larger than 256 MB is stored another way: the same values."""
+    N, k, D = 70000, 2, 512
+    x = torch.arange(N * D, device=DEV, dtype=torch.int32).remainder(8191).float().view(N, D)
+    idx = torch.randint(-1, 7, (N, k), generator=gen(1)).to(DEV)
+    plan = mtk.route_rows(idx, 7)
+    xs = mtk.dispatch_rows(x, plan)
+    assert xs.numel() * 4 > 256 << 20
+    assert torch.equal(xs, x[plan.order.long() // k])
+    big = torch.cat([xs, xs], 1)
+    assert torch.equal(mtk.combine_rows(big, plan), torch.cat([2 * x, 2 * x], 1))
 
 
 def test_rows_strides_and_shapes():
