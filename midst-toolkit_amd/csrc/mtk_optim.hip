@@ -44,30 +44,27 @@ struct AdamwArgs {
 
 constexpr uint32_t kPhi = 0x9E3779B1u, kPlaceM = 0x6A09E667u, kPlaceR = 0xBB67AE85u;
 
-__device__ __forceinline__ float absmax_finite(float a, float x) {
-    const float b = fabsf(x);
-    return b <= 3.402823466e38f ? fmaxf(a, b) : a;
-}
-
-// exponent (unbiased) of the block scale of a largest magnitude a > 0: a 2^-k in (224, 448]
-__device__ __forceinline__ int scale_exp(float a) {
-    const uint32_t b = __float_as_uint(a);
+// exponent (unbiased) of the block scale of a largest magnitude with bits b > 0: the magnitude times 2^-k is in (224, 448]
+__device__ __forceinline__ int scale_exp(uint32_t b) {
     const int k = (int)(b >> 23) - 135 + ((b & 0x7fffff) > 0x600000 ? 1 : 0);
     return k < -126 ? -126 : k;
 }
 __device__ __forceinline__ float pow2(int k) { return __uint_as_float((uint32_t)(k + 127) << 23); }
 
-// the e4m3 neighbour of |x| 2^-k that the dither u20 (20 bits) selects, as a float with x's sign: exact in e4m3
+// |x| 2^-k rounded to the e4m3 neighbour that the dither w (its upper 20 bits) selects; exact in e4m3.  The dither is added to the 20 bits of the
+// float behind e4m3's three and the sum cut: a carry is the step up.  Codes below 2^-6 are equally spaced, as those in [2^-6, 2^-5) are:
+// such a value is moved there and back.
 __device__ __forceinline__ float dither(float x, float inv_scale, uint32_t w, float lowest) {
     const float y = fabsf(x) * inv_scale;
-    uint32_t eb = __float_as_uint(y) >> 23;  // codes below 2^-6 are equally spaced
-    eb = eb < 121 ? 121 : eb;
-    const float step = __uint_as_float((eb - 3) << 23), inv = __uint_as_float((257 - eb) << 23);
-    float q = floorf(y * inv + (float)(w >> 12) * 0x1p-20f) * step;
-    q = fminf(q, 448.f);
-    q = y != 0.f ? fmaxf(q, lowest) : q;
-    q = fabsf(x) <= 3.402823466e38f ? q : __builtin_nanf("");  // infinities have no code: they and NaN become NaN, alone in their block
-    return copysignf(q, x);
+    const float lift = y < 0x1p-6f ? 0x1p-6f : 0.f;
+    const float q = __uint_as_float((__float_as_uint(y + lift) + (w >> 12)) & 0xfff00000u) - lift;
+    return __builtin_amdgcn_fmed3f(q, lowest, 448.f);
+}
+// sqrt(v), correctly rounded but for rare ties, in six instructions: the hardware's reciprocal root and one correction.  Roots of zero (the cap)
+// and of numbers below 2^-126 (counted as 0 by the instruction) stay small.
+__device__ __forceinline__ float fast_sqrt(float v) {
+    const float y = fminf(__builtin_amdgcn_rsqf(v), 0x1p60f), r = v * y;
+    return __builtin_fmaf(__builtin_fmaf(-r, r, v) * 0.5f, y, r);
 }
 
 template <int N> struct __attribute__((packed, aligned(1), may_alias)) CodeVec { uint32_t w[N / 4]; };
@@ -156,17 +153,22 @@ __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
         ld_f32<V>((const float*)a.v[lo] + i0, left, v);
     }
     mtk_vec<T> p1;
-    float r[V], am = 0.f, ar = 0.f;
+    float r[V];
+    uint32_t am = 0, ar = 0;  // largest magnitudes, as bits: what is not finite comes out on top
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const float g = (float)g0.v[i];
         m[i] = h.b1 * m[i] + h.c1 * g;
         v[i] = h.b2 * v[i] + h.c2 * (g * g);
-        r[i] = sqrtf(v[i]);
-        p1.v[i] = (T)((float)p0.v[i] * h.decay - h.step_size * (m[i] / (r[i] * h.inv_bc2 + h.eps)));
-        if (Q8) {
-            am = absmax_finite(am, m[i]);
-            ar = absmax_finite(ar, r[i]);
+        if (Q8) {  // bound by its instructions: the quotient by a reciprocal (one unit in its last place), the root as above
+            r[i] = fast_sqrt(v[i]);
+            p1.v[i] = (T)((float)p0.v[i] * h.decay - h.step_size * (m[i] * __builtin_amdgcn_rcpf(r[i] * h.inv_bc2 + h.eps)));
+            const uint32_t bm = __float_as_uint(m[i]) & 0x7fffffffu, br = __float_as_uint(r[i]) & 0x7fffffffu;
+            am = am > bm ? am : bm;
+            ar = ar > br ? ar : br;
+        } else {
+            r[i] = sqrtf(v[i]);
+            p1.v[i] = (T)((float)p0.v[i] * h.decay - h.step_size * (m[i] / (r[i] * h.inv_bc2 + h.eps)));
         }
     }
     if (left == V) mtk_st(pp, p1);
@@ -176,21 +178,49 @@ __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
         st_f32<V>((float*)a.v[lo] + i0, left, v);
         return;
     }
+    auto block_max = [](uint32_t a) {
 #pragma unroll
-    for (int d = 1; d < QB / V; d <<= 1) {
-        am = fmaxf(am, __shfl_xor(am, d));
-        ar = fmaxf(ar, __shfl_xor(ar, d));
+        for (int d = 1; d < QB / V; d <<= 1) {
+            const uint32_t o = (uint32_t)__shfl_xor((int)a, d);
+            a = a > o ? a : o;
+        }
+        return a;
+    };
+    am = block_max(am);
+    ar = block_max(ar);
+    constexpr uint32_t kInf = 0x7f800000u;
+    const bool bad = am >= kInf || ar >= kInf;  // the same in all lanes of a block
+    if (__any(bad)) {  // rare: the scales go by the finite values (blocks without others keep theirs)
+        uint32_t fm = 0, fr = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const uint32_t bm = __float_as_uint(m[i]) & 0x7fffffffu, br = __float_as_uint(r[i]) & 0x7fffffffu;
+            fm = bm < kInf && bm > fm ? bm : fm;
+            fr = br < kInf && br > fr ? br : fr;
+        }
+        am = block_max(fm);
+        ar = block_max(fr);
     }
-    const int km = am > 0.f ? scale_exp(am) : 0, kr = ar > 0.f ? scale_exp(ar) : 0;
+    const int km = am ? scale_exp(am) : 0, kr = ar ? scale_exp(ar) : 0;
     const float im = pow2(-km), ir = pow2(-kr);
+    uint32_t wm = (uint32_t)i0 * kPlaceM + h.phase, wr = (uint32_t)i0 * kPlaceR + h.phase;
+    float qm[V], qr[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const uint32_t at = (uint32_t)(i0 + i);
-        m[i] = dither(m[i], im, at * kPlaceM + h.phase, 0.f);
-        r[i] = dither(r[i], ir, at * kPlaceR + h.phase, 0x1p-9f);
+        qm[i] = copysignf(dither(m[i], im, wm, 0.f), m[i]);
+        qr[i] = dither(r[i], ir, wr, r[i] > 0.f ? 0x1p-9f : 0.f);
+        wm += kPlaceM;
+        wr += kPlaceR;
     }
-    st_codes<V>((uint8_t*)a.m[lo] + i0, left, m);
-    st_codes<V>((uint8_t*)a.v[lo] + i0, left, r);
+    if (bad) {  // infinities have no code: they and NaN become NaN, alone in their block
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            qm[i] = (__float_as_uint(m[i]) & 0x7fffffffu) < kInf ? qm[i] : __builtin_nanf("");
+            qr[i] = (__float_as_uint(r[i]) & 0x7fffffffu) < kInf ? qr[i] : __builtin_nanf("");
+        }
+    }
+    st_codes<V>((uint8_t*)a.m[lo] + i0, left, qm);
+    st_codes<V>((uint8_t*)a.v[lo] + i0, left, qr);
     if (left && (threadIdx.x & (QB / V - 1)) == 0) {
         a.ms[lo][blk] = pow2(km);
         a.vs[lo][blk] = pow2(kr);

@@ -463,7 +463,9 @@ def test_adamw_32_bit(dt, odd):
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("odd", [False, True])
 def test_adamw_8_bit_codes(dt, odd):
-    """Against the operator's own fp32 operations in numpy: codes, scales and (fp32) parameters are equal, step after step."""
+    """Against the operator's own fp32 operations in numpy, step after step: codes and scales are equal.  The parameters' quotient goes by a
+    reciprocal of one unit in the last place (2^-23) and a product: three half steps of the update more than an exact quotient, one half
+    step on each side for the sum, and the type's own."""
     g = gen(22)
     p, _ = adamw_lists(g, SIZES, dt, odd)
     code = lambda n: torch.zeros(n, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)  # noqa: E731
@@ -482,7 +484,9 @@ def test_adamw_8_bit_codes(dt, odd):
             wp, wm, wms, wv, wvs = adamw8_reference(P[i], gr[i].cpu().float().numpy(), M[i], MS[i], V[i], VS[i], t)
             assert np.array_equal(ms[i].cpu().numpy(), wms.astype(np.float32)) and np.array_equal(vs[i].cpu().numpy(), wvs.astype(np.float32)), (t, i)
             assert np.array_equal(m[i].cpu().float().numpy(), wm.astype(np.float32)) and np.array_equal(v[i].cpu().float().numpy(), wv.astype(np.float32)), (t, i)
-            assert torch.equal(p[i].cpu(), torch.from_numpy(wp.astype(np.float32)).to(dt)), (t, i)
+            want = torch.from_numpy(wp.astype(np.float64))
+            upd = (want - torch.from_numpy(P[i]).double() * (1 - 1e-5)).abs()
+            within(p[i], want, 4 * U32 * (upd + want.abs() + 1e-6) + half(dt) * 1.01 * want.abs() * (dt != torch.float32) + tiny(dt))
 
 
 @pytest.mark.parametrize("bits", [8, 32])
