@@ -26,6 +26,10 @@ TABLE_ORDER = [
 ]
 
 _lib = None
+_native = None
+# the library functions that _mtk_torch calls, in the order of its table
+_NATIVE = ["mtk_route_rows_work", "mtk_route_rows", "mtk_rows_dispatch", "mtk_rows_combine", "mtk_adapter_saved_bytes", "mtk_adapter_work_bytes",
+           "mtk_adapter_forward", "mtk_adapter_backward", "mtk_adamw_step"]
 
 _p, _i64, _i32, _u64 = C.c_void_p, C.c_int64, C.c_int, C.c_uint64
 _SIGS = {
@@ -129,6 +133,26 @@ def lib() -> C.CDLL:
             fn.argtypes = args
         _lib = l
     return _lib
+
+
+def native():
+    """The module that checks tensors, allocates results and calls the small entry points in one go (csrc/mtk_torch.cpp): its functions return
+    None for a call that is not the ordinary case, which the caller then makes through :func:`launch`."""
+    global _native
+    if _native is None:
+        l = lib()
+        try:
+            from . import _mtk_torch as module
+        except ImportError as e:
+            raise RuntimeError(f"{_HERE}/_mtk_torch.so is missing or does not load ({e}): build it with `python -c 'import __graft_entry__ as g; g.build()'`") from e
+        module.bind(*(C.cast(getattr(l, name), C.c_void_p).value for name in _NATIVE))
+        _native = module
+    return _native
+
+
+def raw_stream(index: int) -> int:
+    """Handle of the current stream of device ``index``."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def exported_symbols() -> list[str]:

@@ -18,7 +18,7 @@ from torch import Tensor, nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import launch
+from ._lib import launch, native, raw_stream
 from .model import MLPDiffusion, timestep_frequencies
 from .routing import DTYPES, MAX_GROUPS, RowPlan, combine_rows, dispatch_rows, dtype_code, route_rows, rows_of
 
@@ -28,6 +28,9 @@ ACTIVATIONS = {"none": 0, "relu": 1}  # enum mtk_activation
 
 def _forward(x, weight, bias, down, up, offsets, scales, scale, act, keep):
     """mtk_adapter_forward: (y, what the backward reads of it)"""
+    got = native().adapter_forward(x, weight, bias, down, up, offsets, scale if scales is None else scales, act, 1, raw_stream(x.get_device())) if keep else None
+    if got is not None:
+        return got
     dev, (M, din), (E, r, _), dout = x.device, x.shape, down.shape, weight.shape[0]
     l, dt = _lib.lib(), DTYPES[x.dtype]
     y = torch.empty((M, dout), dtype=x.dtype, device=dev)
@@ -57,12 +60,16 @@ class _AdapterLinear(torch.autograd.Function):
         dev, (M, din), (E, r, _), dout = x.device, x.shape, down.shape, weight.shape[0]
         l, dt = _lib.lib(), DTYPES[x.dtype]
         want = ctx.needs_input_grad
+        g = g.contiguous()
+        got = native().adapter_backward(x, weight, down, up, offsets, ctx.scale if scales is None else scales, ctx.act, y, g, saved,
+                                        want[0] + 2 * want[3] + 4 * want[4], raw_stream(x.get_device()))
+        if got is not None:
+            return got[0], None, None, got[1], got[2], None, None, None, None
         dx = torch.empty((M, din), dtype=x.dtype, device=dev) if want[0] else None
         if M == 0:
             return dx, None, None, torch.zeros_like(down) if want[3] else None, torch.zeros_like(up) if want[4] else None, None, None, None, None
         ddown = torch.empty_like(down) if want[3] else None
         dup = torch.empty_like(up) if want[4] else None
-        g = g.contiguous()
         work = torch.empty(l.mtk_adapter_work_bytes(M, din, dout, r, E, dt, ctx.act, 1), dtype=torch.uint8, device=dev)
         p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         launch(dev, l.mtk_adapter_backward, M, din, dout, r, E, dt, x.data_ptr(), x.stride(0), weight.data_ptr(), down.data_ptr(), up.data_ptr(),
@@ -82,6 +89,10 @@ def adapter_linear(x: Tensor, weight: Tensor, bias: Tensor | None, down: Tensor,
         offsets = offsets.offsets
     if not x.is_cuda:
         raise RuntimeError("adapter_linear: midst_toolkit_amd has no CPU path; move the rows to the MI355X")
+    if activation in ACTIVATIONS:
+        got = native().adapter_forward(x, weight, bias, down, up, offsets, scale, ACTIVATIONS[activation], 0, raw_stream(x.get_device()))
+        if got is not None:
+            return got
     dtype_code(x, "adapter_linear")
     if x.dim() != 2 or weight.dim() != 2 or down.dim() != 3 or up.dim() != 3:
         raise ValueError("adapter_linear: x [M, din], weight [dout, din], down [E, r, din], up [E, dout, r]")

@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import launch
+from ._lib import launch, native, raw_stream
 from .routing import DTYPES
 
 SCALE_BLOCK = 256  # values per scale of the 8-bit moments
@@ -44,7 +44,6 @@ def _check_list(what: str, ts: Sequence[Tensor], dtype: torch.dtype, device: int
                              f"{t.device}" + ("" if t.is_contiguous() else ", not contiguous"))
 
 
-@torch.no_grad()
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor], exp_avg_sqs: Sequence[Tensor], step: int, *, lr: float,
                betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, exp_avg_scales: Sequence[Tensor] | None = None,
                exp_avg_sq_scales: Sequence[Tensor] | None = None, _hyper: Tensor | None = None) -> None:
@@ -60,6 +59,9 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     p0 = params[0]
     if not p0.is_cuda:
         raise RuntimeError("adamw_step: midst_toolkit_amd has no CPU path; move the params to the MI355X")
+    if native().adamw(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, step, lr, betas[0], betas[1], eps, weight_decay, _hyper,
+                      raw_stream(p0.get_device())):
+        return
     if p0.dtype not in DTYPES:
         raise ValueError(f"adamw_step: params are {p0.dtype} (float32, bfloat16 or float16)")
     sizes, at = list(map(_numel, params)), p0.get_device()

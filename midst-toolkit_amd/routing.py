@@ -12,7 +12,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import launch
+from ._lib import launch, native, raw_stream
 
 MAX_GROUPS = 1024  # MTK_ROUTE_MAX_GROUPS of include/mtk.h
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # enum mtk_dtype
@@ -48,6 +48,9 @@ def route_rows(index: Tensor, n_groups: int) -> RowPlan:
     range goes where -1 goes, and its rows are NaN: dispatched, combined and in gradients."""
     if not index.is_cuda:
         raise RuntimeError("route_rows: midst_toolkit_amd has no CPU path; move the indices to the MI355X")
+    got = native().route(index, n_groups, raw_stream(index.get_device()))
+    if got is not None:
+        return RowPlan(*got, n_groups, index.shape[0], 1 if index.dim() == 1 else index.shape[1])
     if index.dim() not in (1, 2) or index.dtype.is_floating_point or index.dtype.is_complex or index.dtype == torch.bool:
         raise ValueError(f"route_rows: index is [N] or [N, k] whole numbers, got {tuple(index.shape)} {index.dtype}")
     if not 1 <= n_groups <= MAX_GROUPS:
@@ -82,6 +85,9 @@ def _check_rows(what: str, t: Tensor, rows: int, plan: RowPlan) -> int:
 
 def _dispatch(x: Tensor, plan: RowPlan, w: Tensor | None, y: Tensor | None = None, want_rows: bool = True):
     """mtk_rows_dispatch: (xs, dw)."""
+    got = native().dispatch(x, plan.slot, plan.n_rows, plan.copies, w, y, int(want_rows), raw_stream(x.get_device()))
+    if got is not None:
+        return got
     dev, D = x.device, x.shape[1]
     x = rows_of(x)
     P = plan.n_rows * plan.copies
@@ -95,6 +101,9 @@ def _dispatch(x: Tensor, plan: RowPlan, w: Tensor | None, y: Tensor | None = Non
 
 
 def _combine(y: Tensor, plan: RowPlan, w: Tensor | None) -> Tensor:
+    got = native().combine(y, plan.slot, plan.n_rows, plan.copies, w, raw_stream(y.get_device()))
+    if got is not None:
+        return got
     dev, D = y.device, y.shape[1]
     y = rows_of(y)
     out = torch.empty((plan.n_rows, D), dtype=y.dtype, device=dev)
@@ -135,13 +144,23 @@ class _Combine(torch.autograd.Function):
 def dispatch_rows(x: Tensor, plan: RowPlan) -> Tensor:
     """``x`` [N, D] -> [N * k, D]: every record's row in the places of its k pairs, sorted by model.  Differentiable in ``x`` (a record's
     gradient is the sum over its pairs, in fp32, in the order of its copies)."""
+    track = x.requires_grad and torch.is_grad_enabled()
+    if not track and x.is_cuda:
+        got = native().dispatch(x, plan.slot, plan.n_rows, plan.copies, None, None, 1, raw_stream(x.get_device()))
+        if got is not None:
+            return got[0]
     _check_rows("dispatch_rows", x, plan.n_rows, plan)
-    return _Dispatch.apply(x, plan) if x.requires_grad and torch.is_grad_enabled() else _dispatch(x, plan, None)[0]
+    return _Dispatch.apply(x, plan) if track else _dispatch(x, plan, None)[0]
 
 
 def combine_rows(y: Tensor, plan: RowPlan, weights: Tensor | None = None) -> Tensor:
     """``y`` [N * k, D] in the plan's order -> [N, D]: ``sum_j weights[n, j] * y[slot[n, j]]`` (``weights`` None: ones), summed in fp32 and
     rounded once.  ``weights``: float32 of ``index``'s shape.  Differentiable in both."""
+    track = torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad))
+    if not track and y.is_cuda and (weights is None or weights.dim() == 2):
+        got = native().combine(y, plan.slot, plan.n_rows, plan.copies, weights, raw_stream(y.get_device()))
+        if got is not None:
+            return got
     _check_rows("combine_rows", y, plan.n_rows * plan.copies, plan)
     if weights is not None:
         if weights.device != y.device:
@@ -151,6 +170,4 @@ def combine_rows(y: Tensor, plan: RowPlan, weights: Tensor | None = None) -> Ten
         if weights.dim() != 2:
             weights = weights.reshape(plan.n_rows, plan.copies)
         weights = weights.contiguous()
-    if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
-        return _Combine.apply(y, weights, plan)
-    return _combine(y, plan, weights)
+    return _Combine.apply(y, weights, plan) if track else _combine(y, plan, weights)
