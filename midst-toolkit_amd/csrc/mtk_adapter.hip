@@ -573,73 +573,131 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void k_linear(LinearArgs g, T* __r
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// k_linear_few, for few rows: bound by the latency of streaming W once.  32 rows x 32 features a workgroup, its eight waves split k and take their
-// fragments straight from memory (every load of a wave is in flight at once), partial sums meet in LDS.  The low-rank product is plain
-// FMAs there, each row with its own model.
+// k_linear_few, for few rows: bound by the latency of streaming W once.  TS rows x TS features a workgroup (16 up to 64 rows, else 32), its eight
+// waves split k and take their fragments straight from memory; partial sums meet in LDS.  The low-rank product is plain FMAs there, each row
+// with its own model.  What the end needs (offsets, bias, the low-rank operands) is requested between the first lines' loads and their
+// products: each would be a round trip of its own otherwise.
 struct FewArgs {
     int64_t M, x_ld;
     int N, K, r, rp, E, relu;
     const int32_t* offsets;
 };
 
-template <typename T>
+template <typename T, int TS>
 __global__ __launch_bounds__(512) void k_linear_few(FewArgs g, const T* __restrict__ x, const T* __restrict__ W, const T* __restrict__ bias, const T* __restrict__ u,
                                                     const T* __restrict__ up, T* __restrict__ y) {
     constexpr int V = mtk_piece<T>::n, KB = kLine<T>, NW = 8;
-    __shared__ float part[NW][32][33];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hh = lane >> 5;
-    const int nb = (g.N + 31) / 32;
-    const int64_t m0 = (int64_t)(blockIdx.x / nb) * 32;
-    const int n0 = (int)(blockIdx.x % nb) * 32;
-    const T* xr = x + (m0 + li < g.M ? m0 + li : g.M - 1) * g.x_ld;
-    const T* wr = W + (int64_t)(n0 + li < g.N ? n0 + li : g.N - 1) * g.K;
-    int who[2];  // the models of this thread's two outputs' rows: a chain of loads, begun before the product's
+    constexpr int LANES = 64 / TS, S = 8 / LANES;  // lanes that share a row, steps of a line
+    constexpr int OUT = TS * TS > 512 ? 2 : 1;     // outputs of a thread
+    typedef typename std::conditional<TS == 32, f32x16, f32x4>::type Acc;
+    __shared__ float part[NW][TS][TS + 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & (TS - 1), hh = lane / TS;
+    const int nb = (g.N + TS - 1) / TS;
+    const int64_t m0 = (int64_t)(blockIdx.x / nb) * TS;
+    const int n0 = (int)(blockIdx.x % nb) * TS;
+    const T* xr = x + (m0 + li < g.M ? m0 + li : g.M - 1) * g.x_ld + hh * V;
+    const T* wr = W + (int64_t)(n0 + li < g.N ? n0 + li : g.N - 1) * g.K + hh * V;
+    auto mma = [](const mtk_vec<T>& a, const mtk_vec<T>& b, Acc c) {
+        if constexpr (TS == 32) return mma32(a, b, c);
+        else return mma16(a, b, c);
+    };
+    const int held = lane <= g.E ? g.offsets[lane] : 0x7fffffff;
+    // the wave's first two lines, zeros where there are none
+    mtk_vec<T> xa[2][S], wa[2][S];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int64_t row = m0 + ((tid + i * 512) >> 5);
-        who[i] = owner_of(g.offsets, g.E, row < g.M ? row : g.M - 1);
-    }
-    f32x16 acc = {};
-    for (int k0 = wave * KB; k0 < g.K; k0 += NW * KB) {
-        mtk_vec<T> xa[4], wa[4];
-        if (k0 + KB <= g.K) {
+    for (int l = 0; l < 2; ++l) {
+        const int k0 = (wave + l * NW) * KB;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int k = k0 + (2 * s + hh) * V;
-                xa[s] = mtk_ld(xr + k);
-                wa[s] = mtk_ld(wr + k);
+        for (int s = 0; s < S; ++s) {
+            const int k = k0 + s * LANES * V, left = g.K - k - hh * V;
+            if (k0 + KB <= g.K) {
+                xa[l][s] = mtk_ld(xr + k);
+                wa[l][s] = mtk_ld(wr + k);
+            } else {
+                xa[l][s] = mtk_ld_n(xr + k, left);
+                wa[l][s] = mtk_ld_n(wr + k, left);
             }
-        } else {
+        }
+    }
+    // this thread's outputs: row rr + 16 i, feature n; models by ballots over the offsets
+    const int rr = tid / TS, n = n0 + (tid & (TS - 1)), nc = n < g.N ? n : g.N - 1;
+    constexpr int LP = 16 / V < 2 ? 1 : 16 / V;  // pieces of the rank requested ahead: 16 values
+    const float bv = bias ? (float)bias[nc] : 0.f;
+    int who[OUT];
+    mtk_vec<T> ua[OUT][LP], ba[OUT][LP];
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int k = k0 + (2 * s + hh) * V;
-                xa[s] = mtk_ld_n(xr + k, g.K - k);
-                wa[s] = mtk_ld_n(wr + k, g.K - k);
+    for (int i = 0; i < OUT; ++i) {
+        const int64_t row = m0 + rr + 16 * i, rc = row < g.M ? row : g.M - 1;
+        int c = 0;
+#pragma unroll
+        for (int q = 0; q < LANES; ++q) {  // the wave's rows
+            const int64_t at = m0 + wave * LANES + q + 16 * i;
+            int cq = __popcll(__ballot(held <= at));
+            for (int e0 = 64; e0 <= g.E; e0 += 64) cq += __popcll(__ballot((e0 + lane <= g.E ? g.offsets[e0 + lane] : 0x7fffffff) <= at));
+            c = hh == q ? cq : c;
+        }
+        who[i] = c - 1;
+        if (who[i] < 0 || who[i] >= g.E || row >= g.M || rr + 16 * i >= TS) who[i] = -1;
+        const T *ur = u + rc * g.rp, *br = up + ((int64_t)(who[i] < 0 ? 0 : who[i]) * g.N + nc) * g.r;
+#pragma unroll
+        for (int p = 0; p < LP; ++p) {
+            ua[i][p] = mtk_ld(ur + p * V);  // a whole line, zeros behind the rank
+            ba[i][p] = p * V + V <= g.r ? mtk_ld(br + p * V) : mtk_ld_n(br + p * V, g.r - p * V);
+        }
+    }
+    Acc acc = {};
+#pragma unroll
+    for (int l = 0; l < 2; ++l)
+#pragma unroll
+        for (int s = 0; s < S; ++s) acc = mma(wa[l][s], xa[l][s], acc);
+    for (int k0 = (wave + 2 * NW) * KB; k0 < g.K; k0 += 2 * NW * KB) {
+#pragma unroll
+        for (int l = 0; l < 2; ++l) {
+            const int kl = k0 + l * NW * KB;
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                const int k = kl + s * LANES * V, left = g.K - k - hh * V;
+                if (kl + KB <= g.K) {
+                    xa[l][s] = mtk_ld(xr + k);
+                    wa[l][s] = mtk_ld(wr + k);
+                } else {
+                    xa[l][s] = mtk_ld_n(xr + k, left);
+                    wa[l][s] = mtk_ld_n(wr + k, left);
+                }
             }
         }
 #pragma unroll
-        for (int s = 0; s < 4; ++s) acc = mma32(wa[s], xa[s], acc);
-    }
+        for (int l = 0; l < 2; ++l)
 #pragma unroll
-    for (int q = 0; q < 16; ++q) part[wave][li][(q & 3) + 8 * (q >> 2) + 4 * hh] = acc[q];
+            for (int s = 0; s < S; ++s) acc = mma(wa[l][s], xa[l][s], acc);
+    }
+    // D[feature][row]: lane -> row; 32: register -> feature (reg & 3) + 8 (reg >> 2) + 4 (lane >> 5), 16: 4 (lane >> 4) + reg
+    if constexpr (TS == 32) {
+#pragma unroll
+        for (int q = 0; q < 16; ++q) part[wave][li][(q & 3) + 8 * (q >> 2) + 4 * hh] = acc[q];
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) part[wave][li][4 * hh + q] = acc[q];
+    }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int q = tid + i * 512, rr = q >> 5, jj = q & 31, n = n0 + jj;
-        const int64_t row = m0 + rr;
-        if (row >= g.M || n >= g.N) continue;
-        float v = 0.f;
+    for (int i = 0; i < OUT; ++i) {
+        const int64_t row = m0 + rr + 16 * i;
+        if (rr + 16 * i >= TS || row >= g.M || n >= g.N) continue;
+        float v = bv;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) v += part[w][rr][jj];
-        if (bias) v += (float)bias[n];
-        const int e = who[i];
-        if (e >= 0 && e < g.E) {
-            const T *ur = u + row * g.rp, *br = up + ((int64_t)e * g.N + n) * g.r;
+        for (int w = 0; w < NW; ++w) v += part[w][rr + 16 * i][tid & (TS - 1)];
+        if (who[i] >= 0) {
             float low = 0.f;
-            for (int j = 0; j < g.r; j += V) {
-                const mtk_vec<T> uv = mtk_ld(ur + j), bv = j + V <= g.r ? mtk_ld(br + j) : mtk_ld_n(br + j, g.r - j);
 #pragma unroll
-                for (int c = 0; c < V; ++c) low += (float)uv.v[c] * (float)bv.v[c];
+            for (int p = 0; p < LP; ++p)
+#pragma unroll
+                for (int c = 0; c < V; ++c) low += (float)ua[i][p].v[c] * (float)ba[i][p].v[c];
+            const T *ur = u + row * g.rp, *br = up + ((int64_t)who[i] * g.N + n) * g.r;
+            for (int j = LP * V; j < g.r; j += V) {
+                const mtk_vec<T> uv = mtk_ld(ur + j), bq = j + V <= g.r ? mtk_ld(br + j) : mtk_ld_n(br + j, g.r - j);
+#pragma unroll
+                for (int c = 0; c < V; ++c) low += (float)uv.v[c] * (float)bq.v[c];
             }
             v += low;
         }
@@ -847,7 +905,7 @@ struct Job {
     int R, C, ldo;        // TURN: [batch][R][C] -> [batch][C][ldo]; PAD: [rows][C] -> [rows][ldo]; zeros behind; BIAS: C values; OWNER: C tiles of R rows
     int E;                // OWNER
 };
-constexpr int kJobs = 8;
+constexpr int kJobs = 9;
 struct Jobs {
     Job job[kJobs];
     int n = 0, blocks = 0;
@@ -1010,11 +1068,12 @@ struct Shape {
 };
 // what k_linear reads beside its operands, and their padded copies where they need one
 struct Packed {
-    int64_t X, W, Bp, bias, owner;
-    Packed(Layout& l, const Shape& sh, int64_t M, int N, int E, int dtype) {
+    int64_t X, W, F, Bp, bias, owner;  // F: the factors that the shrink multiplies, in whole lines like X
+    Packed(Layout& l, const Shape& sh, int64_t M, int N, int r, int E, int dtype) {
         const int64_t z = mtk_dtype_size(dtype);
         X = l.take(sh.few ? 0 : M * sh.Kp * z);
         W = l.take(sh.few ? 0 : (int64_t)N * sh.Kp * z);
+        F = l.take(sh.few ? 0 : (int64_t)E * r * sh.Kp * z);
         Bp = l.take(sh.blocks ? (int64_t)(E + 1) * N * sh.rp * z : 0);
         bias = l.take((int64_t)sh.nb_n * sh.BN * 4);
         owner = l.take(sh.blocks ? sh.MT * 4 : 0);
@@ -1030,7 +1089,7 @@ struct ForwardWork {
     int64_t bytes;
     Shape sh;
     Packed pk;
-    ForwardWork(Layout l, int64_t M, int din, int dout, int r, int E, int dtype) : sh(M, dout, din, r, E, dtype), pk(l, sh, M, dout, E, dtype) {
+    ForwardWork(Layout l, int64_t M, int din, int dout, int r, int E, int dtype) : sh(M, dout, din, r, E, dtype), pk(l, sh, M, dout, r, E, dtype) {
         bytes = sh.few ? 0 : l.at;
     }
 };
@@ -1038,9 +1097,9 @@ struct BackwardWork {
     int64_t Bt, Wt, At, t, g, part[2], bytes;
     Shape sh;
     Packed pk;
-    BackwardWork(Layout l, int64_t M, int din, int dout, int r, int E, int dtype, bool relu) : sh(M, din, dout, r, E, dtype), pk(l, sh, M, din, E, dtype) {
+    BackwardWork(Layout l, int64_t M, int din, int dout, int r, int E, int dtype, bool relu) : sh(M, din, dout, r, E, dtype), pk(l, sh, M, din, r, E, dtype) {
         const int64_t z = mtk_dtype_size(dtype);
-        Bt = l.take((int64_t)E * r * dout * z);
+        Bt = l.take((int64_t)E * r * sh.Kp * z);
         Wt = l.take(sh.few ? (int64_t)din * dout * z : 0);  // else pk.W
         At = l.take(sh.blocks && !sh.few ? 0 : (int64_t)E * r * din * z);
         t = l.take(Saved(M, r, dtype).bytes);
@@ -1100,7 +1159,8 @@ template <typename T> int linear(const Shape& sh, LinearArgs& g, T* y, hipStream
 }
 template <typename T>
 void linear_few(const FewArgs& g, const T* x, const T* W, const T* bias, const T* u, const T* up, T* y, hipStream_t s) {
-    k_linear_few<T><<<(unsigned)(cdiv(g.M, 32) * cdiv(g.N, 32)), 512, 0, s>>>(g, x, W, bias, u, up, y);
+    if (g.M <= 64) k_linear_few<T, 16><<<(unsigned)(cdiv(g.M, 16) * cdiv(g.N, 16)), 512, 0, s>>>(g, x, W, bias, u, up, y);
+    else k_linear_few<T, 32><<<(unsigned)(cdiv(g.M, 32) * cdiv(g.N, 32)), 512, 0, s>>>(g, x, W, bias, u, up, y);
 }
 // the jobs of a k_linear product: x and W padded where they do not stream, B_e in whole lines and a block of zeros, bias, tiles' models.
 // F: W [N][K], or its transpose [K][N] when `turned`; L: B [E][N][r], or [E][r][N]
@@ -1177,8 +1237,9 @@ extern "C" int mtk_adapter_forward(int64_t M, int din, int dout, int r, int E, i
         const Shape& sh = wk.sh;
         T* u = (T*)((char*)saved + sv.u);
         T* uT = keep && sizeof(T) == 2 ? (T*)((char*)saved + sv.uT) : nullptr;
-        shrink<T>(ShrinkArgs{M, din, r, sh.rp, E, x_ld, offsets, scales, (float)scale, sv.Mp}, (const T*)x, (const T*)down, u, uT, s);
+        ShrinkArgs sa{M, din, r, sh.rp, E, x_ld, offsets, scales, (float)scale, sv.Mp};
         if (sh.few) {
+            shrink<T>(sa, (const T*)x, (const T*)down, u, uT, s);
             linear_few<T>(FewArgs{M, x_ld, dout, din, r, sh.rp, E, act, offsets}, (const T*)x, (const T*)W, (const T*)bias, u, (const T*)up, (T*)y, s);
             return;
         }
@@ -1189,7 +1250,16 @@ extern "C" int mtk_adapter_forward(int64_t M, int din, int dout, int r, int E, i
             g.low = up;
             g.low_ld = r;
         }
+        const T *sx = (const T*)x, *sf = (const T*)down;
+        if (g.X != x) {  // x was padded to whole lines: the shrink reads them too
+            job_pad(jobs, down, din, (char*)work + wk.pk.F, (int64_t)E * r, din, sh.Kp, mtk_piece<T>::n);
+            sx = (const T*)g.X;
+            sf = (const T*)((char*)work + wk.pk.F);
+            sa.K = sh.Kp;
+            sa.x_ld = sh.Kp;
+        }
         prep<T>(jobs, s);
+        shrink<T>(sa, sx, sf, u, uT, s);
         rc = linear<T>(sh, g, (T*)y, s);
     });
     if (rc) return rc;
@@ -1223,10 +1293,14 @@ extern "C" int mtk_adapter_backward(int64_t M, int din, int dout, int r, int E, 
         }
         Jobs jobs;
         LinearArgs lin{};
-        if (dx || ddown) job_turn(jobs, up, wb + wk.Bt, dout, r, dout, E);
+        const bool padded = dx && !sh.few && !streams(g, dout, dout, dtype);  // g in whole lines, for all that reads it from here on
+        const int gk = padded ? sh.Kp : dout;
+        const T* graw = g;
+        if (padded) g = (const T*)(wb + wk.pk.X);
+        if (dx || ddown) job_turn(jobs, up, wb + wk.Bt, dout, r, gk, E);
         if (dx) {
             if (sh.few) job_turn(jobs, W, wb + wk.Wt, dout, din, dout, 1);
-            else lin = plan_linear<T>(jobs, sh, wk.pk, wb, M, din, dout, r, E, dtype, g, dout, (const T*)W, true, nullptr, (const T*)down, t, offsets, 0);
+            else lin = plan_linear<T>(jobs, sh, wk.pk, wb, M, din, dout, r, E, dtype, graw, dout, (const T*)W, true, nullptr, (const T*)down, t, offsets, 0);
             if (sh.few || !sh.blocks) {
                 job_turn(jobs, down, wb + wk.At, r, din, r, E);
                 lin.low = wb + wk.At;
@@ -1235,14 +1309,14 @@ extern "C" int mtk_adapter_backward(int64_t M, int din, int dout, int r, int E, 
         }
         prep<T>(jobs, s);
         if (dx || ddown)
-            shrink<T>(ShrinkArgs{M, dout, r, sh.rp, E, dout, offsets, scales, (float)scale, sv.Mp}, g, (const T*)(wb + wk.Bt), t, ddown && sizeof(T) == 2 ? tT : nullptr, s);
+            shrink<T>(ShrinkArgs{M, gk, r, sh.rp, E, gk, offsets, scales, (float)scale, sv.Mp}, g, (const T*)(wb + wk.Bt), t, ddown && sizeof(T) == 2 ? tT : nullptr, s);
         if (dx) {
             if (sh.few) linear_few<T>(FewArgs{M, dout, din, dout, r, sh.rp, E, 0, offsets}, g, (const T*)(wb + wk.Wt), nullptr, t, (const T*)(wb + wk.At), (T*)dx, s);
             else rc = linear<T>(sh, lin, (T*)dx, s);
         }
         if (ddown || dup)
             wgrad<T>(WgradBoth<T>{{wgrad_one<T>(M, x_ld, sv.Mp, din, r, sh.rp, E, offsets, dtype, 0, t, tT, (const T*)x, (float*)(wb + wk.part[0]), (T*)ddown),
-                                   wgrad_one<T>(M, dout, sv.Mp, dout, r, sh.rp, E, offsets, dtype, 1, u, uT, g, (float*)(wb + wk.part[1]), (T*)dup)}}, s);
+                                   wgrad_one<T>(M, gk, sv.Mp, dout, r, sh.rp, E, offsets, dtype, 1, u, uT, g, (float*)(wb + wk.part[1]), (T*)dup)}}, s);
     });
     if (rc) return rc;
     MTK_HIP(hipGetLastError());
