@@ -12,7 +12,9 @@
 // The backward of x is the same two kernels on g with W, A_e, B_e transposed first (W is small beside the rows).
 // A row's product never meets another model's factors in an accumulator (0 x inf is NaN): products are made per model and
 // SELECTED by row, so one diverged model leaves the others' rows alone.
-// u and t = s_e g B_e are rounded to the rows' type (they are MFMA operands); every sum is in fp32.
+// Every sum is in fp32.  u and t = s_e g B_e are MFMA operands, so with 16-bit rows they are 16-bit numbers: two each, u = hi + lo, which keeps
+// 16 bits of u or more (one rounded number would add as much error as the result's own rounding, and all of a row's at once).  The line of
+// a row of u holds both halves side by side, against B_e twice: for ranks up to 32 that costs nothing.
 #include <type_traits>
 
 #include "mtk_lowp.h"
@@ -51,9 +53,10 @@ __device__ __forceinline__ f32x4 mma16(const mtk_vec<float>& a, const mtk_vec<fl
     return c;
 }
 
-// A k-block is one 128-byte line of a row; the low-rank rows u are stored in whole k-blocks, zeros behind the rank
+// A k-block is one 128-byte line of a row.  A row of u is rank_pad elements, whole k-blocks: fp32 [u, zeros], 16 bits [hi, zeros | lo, zeros]
 template <typename T> constexpr int kLine = 128 / (int)sizeof(T);
-inline int rank_pad(int r, int dtype) { return (int)mtk_up(r, 128 / mtk_dtype_size(dtype)); }
+inline int rank_pad(int r, int dtype) { return (int)mtk_up(r, 32) * (dtype == MTK_DT_F32 ? 1 : 2); }
+template <typename T> __device__ __forceinline__ T low_half(float v, T hi) { return fabsf((float)hi) <= 3.0e38f ? (T)(v - (float)hi) : T(0); }
 constexpr int kRankT = 16;  // rows of u^T come in whole 16s
 
 // The models that own rows [at, end): each call yields one (e, first row, behind its last row).  Whatever the offsets hold, every step moves
@@ -219,19 +222,36 @@ __global__ __launch_bounds__(256) void k_shrink(ShrinkArgs g, int j0, const T* _
         if (!(mine[p] || ((KS == 1 || blockIdx.y == 0) && !any[p]))) continue;  // a row without a model: zeros
         const int64_t at = m0 + p * 16 + li;  // D[j][record]: lane & 15 -> record, j = 4 (lane >> 4) + register
         struct __attribute__((aligned(4 * sizeof(T)), may_alias)) Quad { T v[4]; };
+        constexpr bool kSplit = sizeof(T) == 2;
+        const int half = kSplit ? g.rp / 2 : g.rp;
+        const int64_t plane = mtk_up(g.r, 64) * g.Mp;  // of u^T: hi, then lo
+        T* ur = u + at * g.rp;
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            Quad o;
+            Quad o, l;
             const int j = j0 + t * 16 + q * 4;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o.v[i] = j + i < g.r ? (T)keep[p][t][i] : T(0);
-            if (at < g.M && j < g.rp) *reinterpret_cast<Quad*>(u + at * g.rp + j) = o;
+            for (int i = 0; i < 4; ++i) {
+                const float v = j + i < g.r ? keep[p][t][i] : 0.f;
+                o.v[i] = (T)v;
+                l.v[i] = low_half(v, o.v[i]);
+            }
+            if (at < g.M && j < half) {
+                *reinterpret_cast<Quad*>(ur + j) = o;
+                if (kSplit) *reinterpret_cast<Quad*>(ur + half + j) = l;
+            }
             if (uT && at < g.Mp)  // mtk_up(r, 64) rows of Mp
 #pragma unroll
-                for (int i = 0; i < 4; ++i) uT[(int64_t)(j + i) * g.Mp + at] = o.v[i];
+                for (int i = 0; i < 4; ++i) {
+                    uT[(int64_t)(j + i) * g.Mp + at] = o.v[i];
+                    uT[plane + (int64_t)(j + i) * g.Mp + at] = l.v[i];
+                }
         }
-        if (j0 + RT * 16 >= g.r && at < g.M)  // zeros up to the end of the line
-            for (int j = j0 + RT * 16 + q * 4; j < g.rp; j += 16) *reinterpret_cast<Quad*>(u + at * g.rp + j) = Quad{};
+        if (j0 + RT * 16 >= g.r && at < g.M)  // zeros up to the end of the half
+            for (int j = j0 + RT * 16 + q * 4; j < half; j += 16) {
+                *reinterpret_cast<Quad*>(ur + j) = Quad{};
+                if (kSplit) *reinterpret_cast<Quad*>(ur + half + j) = Quad{};
+            }
     }
 }
 
@@ -514,8 +534,11 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void k_linear(LinearArgs g, T* __r
                         const int n = n0 + wc * G::WN + nt * 32 + li_e, nc = n < g.N ? n : g.N - 1;
                         f32x16 low = {};
                         const T* bn = be + (int64_t)nc * g.low_ld;
-                        for (int j = hh_e * V; j - hh_e * V < g.low_ld; j += 2 * V)
-                            low = mma32(j + V <= g.low_ld ? mtk_ld(bn + j) : mtk_ld_n(bn + j, g.low_ld - j), mtk_ld(u + rc * g.rp + j), low);
+                        for (int j = hh_e * V; j - hh_e * V < g.low_ld; j += 2 * V) {
+                            const mtk_vec<T> bv = j + V <= g.low_ld ? mtk_ld(bn + j) : mtk_ld_n(bn + j, g.low_ld - j);
+                            low = mma32(bv, mtk_ld(u + rc * g.rp + j), low);
+                            if (sizeof(T) == 2 && g.low_ld < g.rp) low = mma32(bv, mtk_ld(u + rc * g.rp + g.rp / 2 + j), low);  // B once: both halves of u
+                        }
 #pragma unroll
                         for (int q = 0; q < 16; ++q) acc[mt][nt][q] += mine ? low[q] : 0.f;
                     }
@@ -621,10 +644,12 @@ __global__ __launch_bounds__(512) void k_linear_few(FewArgs g, const T* __restri
     }
     // this thread's outputs: row rr + 16 i, feature n; models by ballots over the offsets
     const int rr = tid / TS, n = n0 + (tid & (TS - 1)), nc = n < g.N ? n : g.N - 1;
-    constexpr int LP = 16 / V < 2 ? 1 : 16 / V;  // pieces of the rank requested ahead: 16 values
+    constexpr int LP = 16 / V;  // pieces of the rank requested ahead: 16 values
+    constexpr int H = sizeof(T) == 2 ? 2 : 1;  // halves of u
+    const int half = g.rp / H;
     const float bv = bias ? (float)bias[nc] : 0.f;
     int who[OUT];
-    mtk_vec<T> ua[OUT][LP], ba[OUT][LP];
+    mtk_vec<T> ua[OUT][LP][H], ba[OUT][LP];
 #pragma unroll
     for (int i = 0; i < OUT; ++i) {
         const int64_t row = m0 + rr + 16 * i, rc = row < g.M ? row : g.M - 1;
@@ -641,7 +666,8 @@ __global__ __launch_bounds__(512) void k_linear_few(FewArgs g, const T* __restri
         const T *ur = u + rc * g.rp, *br = up + ((int64_t)(who[i] < 0 ? 0 : who[i]) * g.N + nc) * g.r;
 #pragma unroll
         for (int p = 0; p < LP; ++p) {
-            ua[i][p] = mtk_ld(ur + p * V);  // a whole line, zeros behind the rank
+#pragma unroll
+            for (int h = 0; h < H; ++h) ua[i][p][h] = mtk_ld(ur + h * half + p * V);  // whole lines, zeros behind the rank
             ba[i][p] = p * V + V <= g.r ? mtk_ld(br + p * V) : mtk_ld_n(br + p * V, g.r - p * V);
         }
     }
@@ -692,12 +718,12 @@ __global__ __launch_bounds__(512) void k_linear_few(FewArgs g, const T* __restri
 #pragma unroll
             for (int p = 0; p < LP; ++p)
 #pragma unroll
-                for (int c = 0; c < V; ++c) low += (float)ua[i][p].v[c] * (float)ba[i][p].v[c];
+                for (int c = 0; c < V; ++c) low += (H == 2 ? (float)ua[i][p][0].v[c] + (float)ua[i][p][H - 1].v[c] : (float)ua[i][p][0].v[c]) * (float)ba[i][p].v[c];
             const T *ur = u + row * g.rp, *br = up + ((int64_t)who[i] * g.N + n) * g.r;
             for (int j = LP * V; j < g.r; j += V) {
-                const mtk_vec<T> uv = mtk_ld(ur + j), bq = j + V <= g.r ? mtk_ld(br + j) : mtk_ld_n(br + j, g.r - j);
+                const mtk_vec<T> uv = mtk_ld(ur + j), ul = mtk_ld(ur + (H - 1) * half + j), bq = j + V <= g.r ? mtk_ld(br + j) : mtk_ld_n(br + j, g.r - j);
 #pragma unroll
-                for (int c = 0; c < V; ++c) low += (float)uv.v[c] * (float)bq.v[c];
+                for (int c = 0; c < V; ++c) low += (H == 2 ? (float)uv.v[c] + (float)ul.v[c] : (float)uv.v[c]) * (float)bq.v[c];
             }
             v += low;
         }
@@ -738,8 +764,9 @@ __device__ void wgrad_body(const WgradArgs& g, int strip, int c, int j0, const T
         f32x4 acc[JT][NV] = {};
         mtk_vec<T> xv[PL];
         T us[sizeof(T) == 4 ? PL : 1][JT];
-        mtk_vec<T> ut[JT];
+        mtk_vec<T> ut[2][JT];  // hi, lo
         // a group inside the model's rows and a strip inside the width: a scalar base and one 32-bit offset per lane
+        const int64_t plane = mtk_up(g.r, 64) * g.Mp;
         const bool whole = (strip + 1) * kStrip<T> <= g.D && g.x_ld < (1 << 24);
         const unsigned lane_off = (unsigned)((sizeof(T) == 4 ? q : q * 8) * (int)g.x_ld + c0) * (unsigned)sizeof(T);
         auto load = [&](int64_t r0) {
@@ -758,7 +785,9 @@ __device__ void wgrad_body(const WgradArgs& g, int strip, int c, int j0, const T
                         }
                 } else {
 #pragma unroll
-                    for (int t = 0; t < JT; ++t) ut[t] = mtk_ld(uT + (int64_t)(j0 + t * 16 + li) * g.Mp + r0 + q * 8);
+                    for (int t = 0; t < JT; ++t)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) ut[h][t] = mtk_ld(uT + h * plane + (int64_t)(j0 + t * 16 + li) * g.Mp + r0 + q * 8);
                 }
                 return;
             }
@@ -779,23 +808,25 @@ __device__ void wgrad_body(const WgradArgs& g, int strip, int c, int j0, const T
             if constexpr (sizeof(T) == 2) {
                 const int64_t rr = r0 + q * 8;
 #pragma unroll
-                for (int t = 0; t < JT; ++t) {
-                    ut[t] = mtk_ld(uT + (int64_t)(j0 + t * 16 + li) * g.Mp + rr);
+                for (int t = 0; t < JT; ++t)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) ut[t].v[i] = rr + i >= a && rr + i < b ? ut[t].v[i] : T(0);
-                }
+                    for (int h = 0; h < 2; ++h) {
+                        ut[h][t] = mtk_ld(uT + h * plane + (int64_t)(j0 + t * 16 + li) * g.Mp + rr);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) ut[h][t].v[i] = rr + i >= a && rr + i < b ? ut[h][t].v[i] : T(0);
+                    }
             }
         };
         const int64_t start = a / GR * GR + wave * GR;
         if (start < b) load(start);
         for (int64_t r0 = start; r0 < b; r0 += 4 * GR) {
-            mtk_vec<T> xc[PL], uc[JT];
+            mtk_vec<T> xc[PL], uc[2][JT];
             T uu[sizeof(T) == 4 ? PL : 1][JT];
 #pragma unroll
             for (int i = 0; i < PL; ++i) xc[i] = xv[i];
 #pragma unroll
             for (int t = 0; t < JT; ++t) {
-                if constexpr (sizeof(T) == 2) uc[t] = ut[t];
+                if constexpr (sizeof(T) == 2) uc[0][t] = ut[0][t], uc[1][t] = ut[1][t];
                 else
 #pragma unroll
                     for (int i = 0; i < PL; ++i) uu[i][t] = us[i][t];
@@ -808,7 +839,7 @@ __device__ void wgrad_body(const WgradArgs& g, int strip, int c, int j0, const T
 #pragma unroll
                     for (int i = 0; i < 8; ++i) col.v[i] = xc[i].v[cc];
 #pragma unroll
-                    for (int t = 0; t < JT; ++t) acc[t][cc] = mma16(uc[t], col, acc[t][cc]);
+                    for (int t = 0; t < JT; ++t) acc[t][cc] = mma16(uc[0][t], col, mma16(uc[1][t], col, acc[t][cc]));
                 }
             } else {
 #pragma unroll
@@ -904,6 +935,7 @@ struct Job {
     int64_t rows, ld;     // PAD: rows and source row stride; OWNER: rows of x; BIAS: padded length
     int R, C, ldo;        // TURN: [batch][R][C] -> [batch][C][ldo]; PAD: [rows][C] -> [rows][ldo]; zeros behind; BIAS: C values; OWNER: C tiles of R rows
     int E;                // OWNER
+    int rep;              // TURN, PAD: a row repeats every rep elements (a multiple of 32)
 };
 constexpr int kJobs = 9;
 struct Jobs {
@@ -931,7 +963,8 @@ __global__ __launch_bounds__(256) void k_prep(Jobs jobs) {
         const int rest = (int)(blk - bat * nc * nr), c0 = rest % nc * 32, r0 = rest / nc * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
         const T* in = (const T*)j.src + bat * j.R * j.C;
         T* out = (T*)j.dst + bat * j.C * j.ldo;
-        for (int i = ty; i < 32; i += 8) tile[i][tx] = r0 + i < j.R && c0 + tx < j.C ? in[(int64_t)(r0 + i) * j.C + c0 + tx] : T(0);
+        const int rs = r0 % j.rep;
+        for (int i = ty; i < 32; i += 8) tile[i][tx] = rs + i < j.R && c0 + tx < j.C ? in[(int64_t)(rs + i) * j.C + c0 + tx] : T(0);
         __syncthreads();
         for (int i = ty; i < 32; i += 8)
             if (c0 + i < j.C && r0 + tx < j.ldo) out[(int64_t)(c0 + i) * j.ldo + r0 + tx] = tile[tx][i];
@@ -940,7 +973,7 @@ __global__ __launch_bounds__(256) void k_prep(Jobs jobs) {
         const int64_t n = j.rows * ppr;
         for (int64_t p = blk * kPadPieces + threadIdx.x; p < n && p < (blk + 1) * kPadPieces; p += 256) {
             const int64_t row = p / ppr;
-            const int c = (int)(p - row * ppr) * V;
+            const int c = (int)(p - row * ppr) * V % j.rep;
             const T* in = (const T*)j.src + row * j.ld + c;
             const mtk_vec<T> v = c + V <= j.C ? mtk_ld(in) : mtk_ld_n(in, j.C - c);
             *reinterpret_cast<uint4*>((T*)j.dst + p * V) = __builtin_bit_cast(uint4, v);
@@ -1035,7 +1068,7 @@ struct Saved {
         Layout l;
         Mp = mtk_up(M, 32);
         u = l.take(M * rank_pad(r, dtype) * mtk_dtype_size(dtype));
-        uT = dtype == MTK_DT_F32 ? l.at : l.take(Mp * mtk_up(r, 64) * mtk_dtype_size(dtype));
+        uT = dtype == MTK_DT_F32 ? l.at : l.take(2 * Mp * mtk_up(r, 64) * mtk_dtype_size(dtype));
         bytes = l.at;
     }
 };
@@ -1110,11 +1143,11 @@ struct BackwardWork {
     }
 };
 
-void job_turn(Jobs& jobs, const void* src, void* dst, int R, int C, int ldo, int batch) {
-    jobs.add(Job{JOB_TURN, 0, src, dst, 0, 0, R, C, ldo, 0}, cdiv(C, 32) * cdiv(ldo, 32) * batch);
+void job_turn(Jobs& jobs, const void* src, void* dst, int R, int C, int ldo, int batch, int rep = 1 << 30) {
+    jobs.add(Job{JOB_TURN, 0, src, dst, 0, 0, R, C, ldo, 0, rep}, cdiv(C, 32) * cdiv(ldo, 32) * batch);
 }
-void job_pad(Jobs& jobs, const void* src, int64_t ld, void* dst, int64_t rows, int C, int ldo, int V) {
-    jobs.add(Job{JOB_PAD, 0, src, dst, rows, ld, 0, C, ldo, 0}, cdiv(rows * (ldo / V), kPadPieces));
+void job_pad(Jobs& jobs, const void* src, int64_t ld, void* dst, int64_t rows, int C, int ldo, int V, int rep = 1 << 30) {
+    jobs.add(Job{JOB_PAD, 0, src, dst, rows, ld, 0, C, ldo, 0, rep}, cdiv(rows * (ldo / V), kPadPieces));
 }
 template <typename T> void prep(const Jobs& jobs, hipStream_t s) {
     if (jobs.blocks) k_prep<T><<<(unsigned)jobs.blocks, 256, 0, s>>>(jobs);
@@ -1186,12 +1219,13 @@ LinearArgs plan_linear(Jobs& jobs, const Shape& sh, const Packed& pk, char* wb, 
     if (turned || !streams(F, K, K, dtype)) g.W = wb + pk.W;
     g.bias = (const float*)(wb + pk.bias);
     const int64_t nbias = (int64_t)sh.nb_n * sh.BN;
-    jobs.add(Job{JOB_BIAS, 0, bias, wb + pk.bias, nbias, 0, 0, bias ? N : 0, 0, 0}, cdiv(nbias, 256));
+    jobs.add(Job{JOB_BIAS, 0, bias, wb + pk.bias, nbias, 0, 0, bias ? N : 0, 0, 0, 1}, cdiv(nbias, 256));
     if (sh.blocks) {
-        if (turned) job_turn(jobs, L, wb + pk.Bp, r, N, sh.rp, E);
-        else job_pad(jobs, L, r, wb + pk.Bp, (int64_t)E * N, r, sh.rp, V);
+        const int half = sizeof(T) == 2 ? sh.rp / 2 : sh.rp;
+        if (turned) job_turn(jobs, L, wb + pk.Bp, r, N, sh.rp, E, half);
+        else job_pad(jobs, L, r, wb + pk.Bp, (int64_t)E * N, r, sh.rp, V, half);
         job_pad(jobs, L, 0, wb + pk.Bp + (int64_t)E * N * sh.rp * sizeof(T), N, 0, sh.rp, V);
-        jobs.add(Job{JOB_OWNER, 0, offsets, wb + pk.owner, M, 0, sh.BM, (int)sh.MT, 0, E}, cdiv(sh.MT, 256));
+        jobs.add(Job{JOB_OWNER, 0, offsets, wb + pk.owner, M, 0, sh.BM, (int)sh.MT, 0, E, 1}, cdiv(sh.MT, 256));
         g.owner = (const int32_t*)(wb + pk.owner);
         g.Bp = g.low = wb + pk.Bp;
         g.low_ld = sh.rp;

@@ -223,15 +223,26 @@ def call(a, **kw):
     return mtk.adapter_linear(a["x"], a["weight"], a["bias"], a["down"], a["up"], a["offsets"], a["scale"], kw.get("activation", "none"))
 
 
-def tol(terms, low, K, r, want, dt):
-    """Sums of K products over `terms`; the low-rank part sums K, then r, and its inner value is rounded to the type once (and to fp32's
-    denormals: nothing).  The stored value rounds once more."""
-    inner = 0.0 if dt == torch.float32 else half(dt) * 1.01
-    return TWICE * (K + 2) * U32 * terms + (TWICE * (K + r + 8) * U32 + inner) * low + half(dt) * want.abs() * 1.01 + tiny(dt) * 4
+def inner(dt):
+    """The low-rank rows between their two products: a 16-bit type keeps them as hi + lo, and lo, at most half a step of the value, is rounded to
+    half a step of its own."""
+    return 0.0 if dt == torch.float32 else half(dt) ** 2 * 1.05
+
+
+def tol(terms, low, K, r, want, dt, factor):
+    """Sums of K products over `terms`; the low-rank part sums K, then r, with its inner value rounded (by half the smallest step at least, times
+    the second factor).  The stored value rounds once more."""
+    return (TWICE * (K + 2) * U32 * terms + (TWICE * (K + r + 8) * U32 + inner(dt)) * low + tiny(dt) * r * float(factor.abs().max()) * 1.5
+            + half(dt) * want.abs() * 1.01 + tiny(dt) * 4)
+
+
+def tol_factor(mag, K, rows, want, dt, other):
+    """A factor's gradient: sums over K features, then over a model's rows."""
+    return (TWICE * (K + rows + 8) * U32 + inner(dt)) * mag + tiny(dt) * rows * float(other.abs().max()) * 1.5 + half(dt) * want.abs() * 1.01 + tiny(dt) * 4
 
 
 SHAPES = [(1, 1, 1, 1, 1, "any"), (1, 64, 64, 8, 4, "any"), (2, 7, 5, 3, 2, "any"), (31, 130, 67, 12, 5, "any"), (33, 64, 128, 16, 3, "last"), (64, 33, 130, 17, 64, "any"),
-          (127, 257, 129, 33, 7, "few"), (130, 96, 200, 64, 4, "any"), (300, 70, 66, 100, 2, "any"), (129, 40, 24, 256, 3, "any"), (513, 128, 256, 8, 1, "any"),
+          (127, 257, 129, 33, 7, "few"), (130, 96, 200, 64, 4, "any"), (300, 70, 66, 100, 2, "any"), (700, 128, 192, 40, 2, "last"), (1100, 100, 130, 70, 3, "any"), (129, 40, 24, 256, 3, "any"), (513, 128, 256, 8, 1, "any"),
           (200, 120, 128, 4, 1024, "few"), (1000, 512, 48, 16, 16, "any"), (77, 64, 64, 8, 3, "base"), (2049, 64, 72, 16, 9, "few"), (16, 2050, 40, 8, 4, "any"),
           (700, 256, 1024, 16, 5, "any"), (9, 300, 1000, 9, 3, "any")]
 
@@ -247,13 +258,11 @@ def test_adapter_forward_and_gradients(M, din, dout, r, E, kind, dt):
     y = call(a)
     ref = adapter_reference(**{**a, "relu": False, "gy": gy})
     dx, ddown, dup = torch.autograd.grad(y, (a["x"], a["down"], a["up"]), gy)
-    within(y, ref["y"], tol(ref["y_terms"], ref["y_low"], din, r, ref["y"], dt))
-    within(dx, ref["dx"], tol(ref["dx_terms"], ref["dx_low"], dout, r, ref["dx"], dt))
+    within(y, ref["y"], tol(ref["y_terms"], ref["y_low"], din, r, ref["y"], dt, a["up"]))
+    within(dx, ref["dx"], tol(ref["dx_terms"], ref["dx_low"], dout, r, ref["dx"], dt, a["down"]))
     rows = int((a["offsets"][1:] - a["offsets"][:-1]).max())
-    inner = 0.0 if dt == torch.float32 else half(dt) * 1.01
-    for name, got, K in (("ddown", ddown, dout), ("dup", dup, din)):
-        want, mag = ref[name], ref[name + "_terms"]
-        within(got, want, (TWICE * (K + rows + 8) * U32 + inner) * mag + half(dt) * want.abs() * 1.01 + tiny(dt) * 4)
+    for name, got, K, other in (("ddown", ddown, dout, a["x"]), ("dup", dup, din, gy)):
+        within(got, ref[name], tol_factor(ref[name + "_terms"], K, rows, ref[name], dt, other))
     # the same bits again, and alone
     y2 = call(a)
     assert torch.equal(y, y2)
@@ -265,7 +274,7 @@ def test_adapter_forward_and_gradients(M, din, dout, r, E, kind, dt):
     b = {n: t.detach() for n, t in a.items()}
     assert torch.equal(call(b), y)
     ref0 = adapter_reference(**{**b, "bias": None, "relu": True})
-    within(call(b, bias=None, activation="relu"), ref0["y"], tol(ref0["y_terms"], ref0["y_low"], din, r, ref0["y"], dt))
+    within(call(b, bias=None, activation="relu"), ref0["y"], tol(ref0["y_terms"], ref0["y_low"], din, r, ref0["y"], dt, b["up"]))
 
 
 @pytest.mark.parametrize("dt", DTYPES)
@@ -277,18 +286,17 @@ def test_adapter_relu_gradient(M, din, dout, r, E, dt):
     a = adapter_inputs(g, M, din, dout, r, E, dt)
     gy = randn(g, M, dout, dt=dt)
     pre = adapter_reference(**{**a, "relu": False})
-    near = pre["y"].abs() <= tol(pre["y_terms"], pre["y_low"], din, r, pre["y"], dt)
+    near = pre["y"].abs() <= tol(pre["y_terms"], pre["y_low"], din, r, pre["y"], dt, a["up"])
     gy[near.to(DEV)] = 0
     for n in ("x", "down", "up"):
         a[n].requires_grad_()
     ref = adapter_reference(**{**a, "relu": True, "gy": gy})
     y = call(a, activation="relu")
-    within(y, ref["y"], tol(pre["y_terms"], pre["y_low"], din, r, pre["y"], dt))
+    within(y, ref["y"], tol(pre["y_terms"], pre["y_low"], din, r, pre["y"], dt, a["up"]))
     dx, ddown, dup = torch.autograd.grad(y, (a["x"], a["down"], a["up"]), gy)
-    within(dx, ref["dx"], tol(ref["dx_terms"], ref["dx_low"], dout, r, ref["dx"], dt))
-    inner = 0.0 if dt == torch.float32 else half(dt) * 1.01
-    for name, got, K in (("ddown", ddown, dout), ("dup", dup, din)):
-        within(got, ref[name], (TWICE * (K + M + 8) * U32 + inner) * ref[name + "_terms"] + half(dt) * ref[name].abs() * 1.01 + tiny(dt) * 4)
+    within(dx, ref["dx"], tol(ref["dx_terms"], ref["dx_low"], dout, r, ref["dx"], dt, a["down"]))
+    for name, got, K, other in (("ddown", ddown, dout, a["x"]), ("dup", dup, din, gy)):
+        within(got, ref[name], tol_factor(ref[name + "_terms"], K, M, ref[name], dt, other))
 
 
 def test_adapter_gradients_against_differences():
@@ -306,7 +314,7 @@ def test_adapter_gradients_against_differences():
         for sign in (1, -1):
             b = {**a, n: a[n] + sign * d}
             ref = adapter_reference(**{**b, "relu": False})
-            err += float((tol(ref["y_terms"], ref["y_low"], din, r, ref["y"], torch.float32) * gy.cpu().double().abs()).sum()) + 4 * U32 * float(
+            err += float((tol(ref["y_terms"], ref["y_low"], din, r, ref["y"], torch.float32, b["up"]) * gy.cpu().double().abs()).sum()) + 4 * U32 * float(
                 ((ref["y_terms"] + ref["y_low"]) * gy.cpu().double().abs()).sum())  # a +- d is rounded too
             loss.append(float((call(b).double() * gy.double()).sum()))
         own = TWICE * (din + dout + M + r + 16) * U32 * float((grad.double().abs() * d.double().abs()).sum()) * 8
@@ -414,7 +422,7 @@ def test_offsets_that_make_no_sense_stay_inside_the_tensors(off):
     if off == [50, 60, 70, 80]:
         fine = a["offsets"].cpu().clamp(max=M)
         ref = adapter_reference(**{**a, "offsets": fine, "relu": False})
-        within(y, ref["y"], tol(ref["y_terms"], ref["y_low"], din, r, ref["y"], torch.float32))
+        within(y, ref["y"], tol(ref["y_terms"], ref["y_low"], din, r, ref["y"], torch.float32, a["up"]))
 
 
 # ------------------------------------------------------------------------------------------------------------------- AdamW
