@@ -28,7 +28,7 @@ TABLE_ORDER = [
 _lib = None
 _native = None
 # the library functions that _mtk_torch calls, in the order of its table
-_NATIVE = ["mtk_route_rows_work", "mtk_route_rows", "mtk_rows_dispatch", "mtk_rows_combine", "mtk_adapter_saved_bytes", "mtk_adapter_work_bytes",
+_NATIVE = ["mtk_last_error", "mtk_route_rows_work", "mtk_route_rows", "mtk_rows_dispatch", "mtk_rows_combine", "mtk_adapter_saved_bytes", "mtk_adapter_work_bytes",
            "mtk_adapter_forward", "mtk_adapter_backward", "mtk_adamw_step"]
 
 _p, _i64, _i32, _u64 = C.c_void_p, C.c_int64, C.c_int, C.c_uint64
@@ -136,8 +136,9 @@ def lib() -> C.CDLL:
 
 
 def native():
-    """The module that checks tensors, allocates results and calls the small entry points in one go (csrc/mtk_torch.cpp): its functions return
-    None for a call that is not the ordinary case, which the caller then makes through :func:`launch`."""
+    """The module that checks tensors, allocates results, calls the small entry points and is their autograd node (csrc/mtk_torch.cpp).  Its
+    functions return None for a call that is not the ordinary case: on another device than the current one, with strides to copy, or
+    with arguments that do not fit."""
     global _native
     if _native is None:
         l = lib()
@@ -148,11 +149,6 @@ def native():
         module.bind(*(C.cast(getattr(l, name), C.c_void_p).value for name in _NATIVE))
         _native = module
     return _native
-
-
-def raw_stream(index: int) -> int:
-    """Handle of the current stream of device ``index``."""
-    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def exported_symbols() -> list[str]:
@@ -194,6 +190,15 @@ def launch(device: torch.device, fn, *args) -> None:
     else:
         with torch.cuda.device(device):
             check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+
+
+def ordinary(what: str, device: torch.device, fn, *args):
+    """``fn`` of :func:`native` on arguments that the caller has checked and made ordinary, with ``device`` current."""
+    with torch.cuda.device(device):
+        got = fn(*args)
+    if got is None:
+        raise RuntimeError(f"{what}: libmtk_hip: {lib().mtk_last_error().decode()}")
+    return got
 
 
 def require_cuda(t: torch.Tensor, what: str) -> None:

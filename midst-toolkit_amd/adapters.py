@@ -7,7 +7,7 @@ model is a low-rank update of every linear layer, and the rows of all models run
   ``adapter_linear``   y = act(x W^T + b + s_e (x A_e^T) B_e^T) on rows sorted by model, with the gradients of x and of all A_e, B_e
   ``LowRankEnsemble``  an ``MLPDiffusion`` denoiser with E such fine-tunes: ``forward(x, timesteps, index, weights)``
 
-Everything runs in libmtk_hip.so (mtk_adapter_forward / mtk_adapter_backward, mtk_route_rows ...).  There is no CPU path.
+Everything runs in libmtk_hip.so (mtk_adapter_forward / mtk_adapter_backward, mtk_route_rows ...), the autograd nodes in csrc/mtk_torch.cpp.  There is no CPU path.
 """
 from __future__ import annotations
 
@@ -15,66 +15,13 @@ import math
 
 import torch
 from torch import Tensor, nn
-from torch.autograd.function import once_differentiable
 
-from . import _lib
-from ._lib import launch, native, raw_stream
+from ._lib import native, ordinary
 from .model import MLPDiffusion, timestep_frequencies
-from .routing import DTYPES, MAX_GROUPS, RowPlan, combine_rows, dispatch_rows, dtype_code, route_rows, rows_of
+from .routing import MAX_GROUPS, RowPlan, combine_rows, dispatch_rows, dtype_code, route_rows, rows_of
 
 MAX_RANK, MAX_WIDTH, MAX_ROWS = 256, 8192, 16777216  # MTK_ADAPTER_MAX_* of include/mtk.h
 ACTIVATIONS = {"none": 0, "relu": 1}  # enum mtk_activation
-
-
-def _forward(x, weight, bias, down, up, offsets, scales, scale, act, keep):
-    """mtk_adapter_forward: (y, what the backward reads of it)"""
-    got = native().adapter_forward(x, weight, bias, down, up, offsets, scale if scales is None else scales, act, 1, raw_stream(x.get_device())) if keep else None
-    if got is not None:
-        return got
-    dev, (M, din), (E, r, _), dout = x.device, x.shape, down.shape, weight.shape[0]
-    l, dt = _lib.lib(), DTYPES[x.dtype]
-    y = torch.empty((M, dout), dtype=x.dtype, device=dev)
-    saved = torch.empty(l.mtk_adapter_saved_bytes(M, r, dt), dtype=torch.uint8, device=dev)
-    if M:
-        need = l.mtk_adapter_work_bytes(M, din, dout, r, E, dt, act, 0)
-        work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        launch(dev, l.mtk_adapter_forward, M, din, dout, r, E, dt, x.data_ptr(), x.stride(0), weight.data_ptr(), None if bias is None else bias.data_ptr(),
-               down.data_ptr(), up.data_ptr(), offsets.data_ptr(), None if scales is None else scales.data_ptr(), scale, act, int(keep), y.data_ptr(),
-               saved.data_ptr(), saved.numel(), None if work is None else work.data_ptr(), need)
-    return y, saved
-
-
-class _AdapterLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, down, up, offsets, scales, scale, act):
-        xr = rows_of(x)
-        y, saved = _forward(xr, weight, bias, down, up, offsets, scales, scale, act, True)
-        ctx.save_for_backward(xr, weight, down, up, offsets, scales, y if act else None, saved)
-        ctx.scale, ctx.act = scale, act
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        x, weight, down, up, offsets, scales, y, saved = ctx.saved_tensors
-        dev, (M, din), (E, r, _), dout = x.device, x.shape, down.shape, weight.shape[0]
-        l, dt = _lib.lib(), DTYPES[x.dtype]
-        want = ctx.needs_input_grad
-        g = g.contiguous()
-        got = native().adapter_backward(x, weight, down, up, offsets, ctx.scale if scales is None else scales, ctx.act, y, g, saved,
-                                        want[0] + 2 * want[3] + 4 * want[4], raw_stream(x.get_device()))
-        if got is not None:
-            return got[0], None, None, got[1], got[2], None, None, None, None
-        dx = torch.empty((M, din), dtype=x.dtype, device=dev) if want[0] else None
-        if M == 0:
-            return dx, None, None, torch.zeros_like(down) if want[3] else None, torch.zeros_like(up) if want[4] else None, None, None, None, None
-        ddown = torch.empty_like(down) if want[3] else None
-        dup = torch.empty_like(up) if want[4] else None
-        work = torch.empty(l.mtk_adapter_work_bytes(M, din, dout, r, E, dt, ctx.act, 1), dtype=torch.uint8, device=dev)
-        p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        launch(dev, l.mtk_adapter_backward, M, din, dout, r, E, dt, x.data_ptr(), x.stride(0), weight.data_ptr(), down.data_ptr(), up.data_ptr(),
-               offsets.data_ptr(), p(scales), ctx.scale, ctx.act, p(y), g.data_ptr(), saved.data_ptr(), p(dx), p(ddown), p(dup), work.data_ptr(), work.numel())
-        return dx, None, None, ddown, dup, None, None, None, None
 
 
 def adapter_linear(x: Tensor, weight: Tensor, bias: Tensor | None, down: Tensor, up: Tensor, offsets: Tensor | RowPlan, scale: float | Tensor = 1.0,
@@ -90,7 +37,7 @@ def adapter_linear(x: Tensor, weight: Tensor, bias: Tensor | None, down: Tensor,
     if not x.is_cuda:
         raise RuntimeError("adapter_linear: midst_toolkit_amd has no CPU path; move the rows to the MI355X")
     if activation in ACTIVATIONS:
-        got = native().adapter_forward(x, weight, bias, down, up, offsets, scale, ACTIVATIONS[activation], 0, raw_stream(x.get_device()))
+        got = native().adapter(x, weight, bias, down, up, offsets, scale, ACTIVATIONS[activation])
         if got is not None:
             return got
     dtype_code(x, "adapter_linear")
@@ -107,25 +54,20 @@ def adapter_linear(x: Tensor, weight: Tensor, bias: Tensor | None, down: Tensor,
         raise ValueError(f"adapter_linear: offsets are int32 [{E + 1}], got {offsets.dtype} {tuple(offsets.shape)}")
     if activation not in ACTIVATIONS:
         raise ValueError(f"adapter_linear: activation {activation!r} (none or relu)")
-    scales = None
-    if isinstance(scale, Tensor):
-        if scale.dtype != torch.float32 or tuple(scale.shape) != (E,):
-            raise ValueError(f"adapter_linear: scale is a number or float32 [{E}], got {scale.dtype} {tuple(scale.shape)}")
-        scales, scale = scale.detach().contiguous(), 1.0
+    scales = scale if isinstance(scale, Tensor) else None
+    if scales is not None and (scales.dtype != torch.float32 or tuple(scales.shape) != (E,)):
+        raise ValueError(f"adapter_linear: scale is a number or float32 [{E}], got {scales.dtype} {tuple(scales.shape)}")
     at, dt = x.get_device(), x.dtype
     for t, name in ((weight, "weight"), (bias, "bias"), (down, "down"), (up, "up")):
         if t is not None and (t.get_device() != at or t.dtype != dt):
             raise ValueError(f"adapter_linear: x is {dt} on {x.device}, {name} {t.dtype} on {t.device}")
     if offsets.get_device() != at or (scales is not None and scales.get_device() != at):
         raise ValueError(f"adapter_linear: x on {x.device}, offsets on {offsets.device}" + ("" if scales is None else f", scale on {scales.device}"))
-    c = lambda t: t if t is None or t.is_contiguous() else t.contiguous()  # noqa: E731
-    args = (c(weight), c(bias), c(down), c(up), c(offsets), scales, float(scale), ACTIVATIONS[activation])
-    if torch.is_grad_enabled():
-        if weight.requires_grad or (bias is not None and bias.requires_grad):
-            raise NotImplementedError("adapter_linear: the shared layer is frozen; detach weight and bias")
-        if x.requires_grad or down.requires_grad or up.requires_grad:
-            return _AdapterLinear.apply(x, *args)
-    return _forward(rows_of(x), *args, False)[0]
+    if torch.is_grad_enabled() and (weight.requires_grad or (bias is not None and bias.requires_grad)):
+        raise NotImplementedError("adapter_linear: the shared layer is frozen; detach weight and bias")
+    c = lambda t: t if t is None else t.contiguous()  # noqa: E731
+    return ordinary("adapter_linear", x.device, native().adapter, rows_of(x), c(weight), c(bias), c(down), c(up), c(offsets),
+                    float(scale) if scales is None else c(scales), ACTIVATIONS[activation])
 
 
 class LowRankEnsemble(nn.Module):

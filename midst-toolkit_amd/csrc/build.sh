@@ -23,8 +23,8 @@ hipcc $FLAGS -c mtk_adapter.hip -o _build/mtk_adapter.o & pids+=($!)
 hipcc $FLAGS -ffp-contract=off -c mtk_optim.hip -o _build/mtk_optim.o & pids+=($!)
 # torch's side of the small entry points (host code only; the library's functions reach it by address)
 read -r TORCH PYINC CXX11 < <(python3 -c "import os, sysconfig, torch; print(os.path.dirname(torch.__file__), sysconfig.get_paths()['include'], int(torch._C._GLIBCXX_USE_CXX11_ABI))")
-g++ -O2 -std=c++17 -fPIC -shared -Wall -D_GLIBCXX_USE_CXX11_ABI=$CXX11 -I$INC -isystem $TORCH/include -isystem $TORCH/include/torch/csrc/api/include -isystem $PYINC \
-    mtk_torch.cpp -o ../_mtk_torch.so -L$TORCH/lib -lc10 -ltorch_cpu -ltorch_python & pids+=($!)
+g++ -O2 -std=c++17 -fPIC -shared -Wall -D_GLIBCXX_USE_CXX11_ABI=$CXX11 -D__HIP_PLATFORM_AMD__=1 -DUSE_ROCM -I$INC -isystem $TORCH/include -isystem $TORCH/include/torch/csrc/api/include -isystem $PYINC -isystem /opt/rocm/include \
+    mtk_torch.cpp -o ../_mtk_torch.so -L$TORCH/lib -lc10 -lc10_hip -ltorch_cpu -ltorch_python & pids+=($!)
 for p in "${pids[@]}"; do wait "$p"; done
 hipcc --offload-arch=gfx950 -shared -fPIC _build/*.o -o ../libmtk_hip.so
 echo "built $(cd .. && pwd)/libmtk_hip.so"

@@ -1,16 +1,26 @@
-// mtk_torch.cpp — torch's side of the small entry points: a CPython module that checks tensors, allocates results and calls the C ABI.
+// mtk_torch.cpp — torch's side of the small entry points: a CPython module that checks tensors, allocates results, calls the C ABI and, where
+// autograd asks, is the node of the graph.
 //
 // A launch costs some microseconds; reading the shapes, types and addresses of a call's tensors in Python and converting twenty arguments costs
-// several times that, and a step over hundreds of tensors more than its kernels.  Each function here takes the ordinary case of a call and
-// does it all at once.  Whatever it does not recognise (another device than the current one, strides it would have to copy, shapes that
-// do not fit, a refusal by the library) it leaves alone and returns None: the Python layer then checks, copies or raises, in full.
+// several times that, a backward pass through a Python node more again (its thread waits for the interpreter), and a step over hundreds of
+// tensors more than its kernels.  Each function here takes the ordinary case of a call and does it all at once.  Whatever it does not
+// recognise (another device than the current one, strides it would have to copy, shapes that do not fit, a refusal by the library's
+// checks) it leaves alone and returns None: the Python layer then makes the arguments ordinary and calls again, or raises.
 // The library's functions come by address (bind), so there is one copy of it, wherever it was loaded from.
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
-#include <c10/core/impl/VirtualGuardImpl.h>
+#include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <optional>
+#include <stdexcept>
+#include <string>
 #include <vector>
 
 #include "mtk.h"
@@ -18,6 +28,7 @@
 namespace {
 
 struct Table {
+    decltype(&mtk_last_error) last_error;
     decltype(&mtk_route_rows_work) route_rows_work;
     decltype(&mtk_route_rows) route_rows;
     decltype(&mtk_rows_dispatch) rows_dispatch;
@@ -43,7 +54,7 @@ const at::Tensor& tensor(PyObject* o) {
     need(THPVariable_Check(o));
     return THPVariable_Unpack(o);
 }
-const at::Tensor* maybe(PyObject* o) { return o == Py_None ? nullptr : &tensor(o); }
+at::Tensor maybe(PyObject* o) { return o == Py_None ? at::Tensor() : tensor(o); }  // undefined for None
 int code(const at::Tensor& t) {
     switch (t.scalar_type()) {
         case at::kFloat: return MTK_DT_F32;
@@ -60,18 +71,17 @@ void dense(const at::Tensor& t, int device) {
 }
 int current(const at::Tensor& t) {
     need(t.is_cuda());
-    static const c10::impl::VirtualGuardImpl guard(c10::DeviceType::CUDA);
-    const int d = guard.getDevice().index();
+    const int d = c10::hip::current_device();
     need(t.device().index() == d);
     return d;
 }
+mtk_stream stream_of(int device) { return (mtk_stream)c10::hip::getCurrentHIPStream((c10::DeviceIndex)device).stream(); }
 // rows whose elements lie side by side, at any distance from each other
 void rows(const at::Tensor& t, int device) {
     here(t, device);
     need(t.dim() == 2 && t.size(1) >= 1 && (t.stride(1) == 1 || t.size(1) == 1 || t.size(0) == 0) && t.stride(0) >= 0);
 }
-void* ptr(const at::Tensor& t) { return t.data_ptr(); }
-void* ptr(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
+void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 at::Tensor like(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType type) { return at::empty(sizes, t.options().dtype(type).requires_grad(false)); }
 int64_t integer(PyObject* o) {
     const long long v = PyLong_AsLongLong(o);
@@ -89,12 +99,19 @@ double real(PyObject* o) {
     }
     return v;
 }
-template <typename F> void call(F f) {  // a library call without the interpreter's lock
+template <typename F> void call(F f) {  // a library call without the interpreter's lock, where this thread has it
     int rc;
-    Py_BEGIN_ALLOW_THREADS;
-    rc = f();
-    Py_END_ALLOW_THREADS;
-    need(rc == MTK_OK);
+    {
+        struct Unlocked {
+            PyThreadState* s = PyGILState_Check() ? PyEval_SaveThread() : nullptr;
+            ~Unlocked() {
+                if (s) PyEval_RestoreThread(s);
+            }
+        } unlocked;
+        rc = f();
+    }
+    need(rc != MTK_ERR_ARG && rc != MTK_ERR_UNSUPPORTED);
+    if (rc != MTK_OK) throw std::runtime_error(std::string("libmtk_hip: ") + lib.fn.last_error());
 }
 PyObject* pack(std::initializer_list<at::Tensor> ts) {
     PyObject* out = PyTuple_New((Py_ssize_t)ts.size());
@@ -120,11 +137,30 @@ template <typename F> PyObject* guarded(Py_ssize_t n, Py_ssize_t want, F f) {
         return nullptr;
     }
 }
-bool tracked(std::initializer_list<const at::Tensor*> ts) {
+bool tracked(std::initializer_list<at::Tensor> ts) {
     if (!c10::GradMode::is_enabled()) return false;
-    for (const at::Tensor* t : ts)
-        if (t && t->requires_grad()) return true;
+    for (const at::Tensor& t : ts)
+        if (t.defined() && t.requires_grad()) return true;
     return false;
+}
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+// The nodes differentiate once: a second time raises where it is tried.
+variable_list once(const variable_list& grads, variable_list out, const char* what) {
+    bool again = false;
+    for (const at::Tensor& g : grads) again |= g.defined() && g.requires_grad();
+    if (!again || !c10::GradMode::is_enabled()) return out;
+    for (at::Tensor& t : out)
+        if (t.defined()) t = t.detach().requires_grad_(true);
+    return (*std::make_shared<torch::autograd::DelayedError>(std::string(what) + " differentiates once only", (int64_t)out.size()))(std::move(out));
+}
+template <typename F> variable_list backward_of(const char* what, const at::Tensor& like_, F f) {
+    const c10::DeviceGuard guard(like_.device());
+    try {
+        return f();
+    } catch (const Decline&) {
+        throw std::runtime_error(std::string(what) + ": a gradient or saved tensor does not fit the layer");
+    }
 }
 
 // bind((address, ...)): the library's functions in Table's order
@@ -135,13 +171,13 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// route(index, n_groups, stream) -> (order, slot, offsets)
+// route(index, n_groups) -> (order, slot, offsets)
 PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded(n, 3, [&]() -> PyObject* {
+    return guarded(n, 2, [&]() -> PyObject* {
         const at::Tensor& index = tensor(a[0]);
         const int64_t groups = integer(a[1]);
-        const mtk_stream s = (mtk_stream)(intptr_t)integer(a[2]);
-        dense(index, current(index));
+        const int d = current(index);
+        dense(index, d);
         need(index.scalar_type() == at::kLong && (index.dim() == 1 || (index.dim() == 2 && index.size(1) >= 1)) && groups >= 1 && groups <= MTK_ROUTE_MAX_GROUPS);
         const int64_t P = index.numel();
         need(P <= 0x7fffffff);
@@ -149,72 +185,121 @@ PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
         at::Tensor order = like(index, {P}, at::kInt), slot = like(index, index.sizes(), at::kInt), offsets = like(index, {groups + 1}, at::kInt), work;
         if (w) work = like(index, {w}, at::kInt);
         call([&] {
-            return lib.fn.route_rows(P, index.const_data_ptr<int64_t>(), (int)groups, (int32_t*)ptr(order), (int32_t*)ptr(slot), (int32_t*)ptr(offsets),
-                                     w ? (int32_t*)work.data_ptr() : nullptr, w, s);
+            return lib.fn.route_rows(P, index.const_data_ptr<int64_t>(), (int)groups, (int32_t*)ptr(order), (int32_t*)ptr(slot), (int32_t*)ptr(offsets), (int32_t*)ptr(work), w,
+                                     stream_of(d));
         });
         return pack({order, slot, offsets});
     });
 }
 
-// dispatch(x, slot, n_rows, copies, weights | None, y | None, want_rows, stream) -> (xs | None, dw | None)
-PyObject* dispatch(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded(n, 8, [&]() -> PyObject* {
-        const at::Tensor &x = tensor(a[0]), &slot = tensor(a[1]);
-        const int64_t N = integer(a[2]), k = integer(a[3]);
-        const at::Tensor *w = maybe(a[4]), *y = maybe(a[5]);
-        const bool want = integer(a[6]) != 0;
-        const mtk_stream s = (mtk_stream)(intptr_t)integer(a[7]);
-        const int d = current(x), dt = code(x);
-        rows(x, d);
-        dense(slot, d);
-        need(k >= 1 && x.size(0) == N && N >= 1 && slot.numel() == N * k && slot.scalar_type() == at::kInt);
-        const int64_t D = x.size(1);
-        if (w) {
-            dense(*w, d);
-            need(w->scalar_type() == at::kFloat && w->numel() == N * k);
-        }
-        if (y) {
-            dense(*y, d);
-            need(y->scalar_type() == x.scalar_type() && y->dim() == 2 && y->size(0) == N * k && y->size(1) == D);
-        }
-        at::Tensor xs, dw;
-        if (want) xs = like(x, {N * k, D}, x.scalar_type());
-        if (y) dw = like(x, {N, k}, at::kFloat);
+struct Pairs {  // of a plan
+    at::Tensor slot;
+    int64_t N, k;
+    void check(int device) const {
+        dense(slot, device);
+        need(k >= 1 && N >= 0 && slot.numel() == N * k && slot.scalar_type() == at::kInt);
+    }
+    void weights(const at::Tensor& w, int device) const {
+        if (!w.defined()) return;
+        dense(w, device);
+        need(w.scalar_type() == at::kFloat && w.dim() == 2 && w.size(0) == N && w.size(1) == k);
+    }
+};
+// (xs if wanted, dw if y is given)
+std::pair<at::Tensor, at::Tensor> rows_out(const at::Tensor& x, const Pairs& p, const at::Tensor& w, const at::Tensor& y, bool want) {
+    const int d = current(x), dt = code(x);
+    rows(x, d);
+    p.check(d);
+    p.weights(w, d);
+    const int64_t D = x.size(1);
+    need(x.size(0) == p.N);
+    if (y.defined()) {
+        dense(y, d);
+        need(y.scalar_type() == x.scalar_type() && y.dim() == 2 && y.size(0) == p.N * p.k && y.size(1) == D);
+    }
+    at::Tensor xs, dw;
+    if (want) xs = like(x, {p.N * p.k, D}, x.scalar_type());
+    if (y.defined()) dw = like(x, {p.N, p.k}, at::kFloat);
+    if (p.N && (want || y.defined()))
         call([&] {
-            return lib.fn.rows_dispatch(N, (int)k, D, dt, ptr(x), x.stride(0), (const int32_t*)ptr(slot), (const float*)ptr(w), want ? xs.data_ptr() : nullptr, ptr(y),
-                                        y ? (float*)dw.data_ptr() : nullptr, s);
+            return lib.fn.rows_dispatch(p.N, (int)p.k, D, dt, ptr(x), x.stride(0), (const int32_t*)ptr(p.slot), (const float*)ptr(w), ptr(xs), ptr(y), (float*)ptr(dw), stream_of(d));
         });
-        return pack({xs, dw});
+    return {xs, dw};
+}
+at::Tensor rows_back(const at::Tensor& y, const Pairs& p, const at::Tensor& w) {
+    const int d = current(y), dt = code(y);
+    rows(y, d);
+    p.check(d);
+    p.weights(w, d);
+    need(y.size(0) == p.N * p.k);
+    at::Tensor out = like(y, {p.N, y.size(1)}, y.scalar_type());
+    if (p.N)
+        call([&] {
+            return lib.fn.rows_combine(p.N, (int)p.k, y.size(1), dt, ptr(y), y.stride(0), (const int32_t*)ptr(p.slot), (const float*)ptr(w), ptr(out), stream_of(d));
+        });
+    return out;
+}
+at::Tensor as_rows(const at::Tensor& g) { return g.size(0) == 0 || ((g.stride(1) == 1 || g.size(1) == 1) && g.stride(0) >= 0) ? g : g.contiguous(); }
+
+struct DispatchNode : torch::autograd::Function<DispatchNode> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& slot, int64_t N, int64_t k) {
+        ctx->save_for_backward({slot});
+        ctx->saved_data["N"] = N;
+        ctx->saved_data["k"] = k;
+        return rows_out(x, Pairs{slot, N, k}, {}, {}, true).first;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const Pairs p{ctx->get_saved_variables()[0], ctx->saved_data["N"].toInt(), ctx->saved_data["k"].toInt()};
+        return backward_of("dispatch_rows", p.slot, [&] { return once(grads, {rows_back(as_rows(grads[0]), p, {}), {}, {}, {}}, "dispatch_rows"); });
+    }
+};
+std::optional<at::Tensor> given(const at::Tensor& t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; }
+// (needs_input_grad counts the tensors that are given: what may be absent comes last)
+struct CombineNode : torch::autograd::Function<CombineNode> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& y, const at::Tensor& slot, const std::optional<at::Tensor>& weights, int64_t N, int64_t k) {
+        const at::Tensor w = weights.value_or(at::Tensor());
+        at::Tensor keep;
+        if (w.defined() && w.requires_grad()) keep = y;
+        ctx->save_for_backward({keep, w, slot});
+        ctx->saved_data["N"] = N;
+        ctx->saved_data["k"] = k;
+        return rows_back(y, Pairs{slot, N, k}, w);
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const Pairs p{saved[2], ctx->saved_data["N"].toInt(), ctx->saved_data["k"].toInt()};
+        return backward_of("combine_rows", p.slot, [&] {
+            const bool want_w = saved[1].defined() && saved[0].defined() && ctx->needs_input_grad(2);
+            auto got = rows_out(as_rows(grads[0]), p, saved[1], want_w ? saved[0].contiguous() : at::Tensor(), ctx->needs_input_grad(0));
+            return once(grads, {got.first, {}, got.second, {}, {}}, "combine_rows");
+        });
+    }
+};
+
+// dispatch(x, slot, n_rows, copies) -> xs
+PyObject* dispatch(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 4, [&]() -> PyObject* {
+        const at::Tensor& x = tensor(a[0]);
+        const Pairs p{tensor(a[1]), integer(a[2]), integer(a[3])};
+        return THPVariable_Wrap(tracked({x}) ? DispatchNode::apply(x, p.slot, p.N, p.k) : rows_out(x, p, {}, {}, true).first);
     });
 }
-
-// combine(y, slot, n_rows, copies, weights | None, stream) -> out
+// combine(y, slot, n_rows, copies, weights | None) -> out
 PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded(n, 6, [&]() -> PyObject* {
-        const at::Tensor &y = tensor(a[0]), &slot = tensor(a[1]);
-        const int64_t N = integer(a[2]), k = integer(a[3]);
-        const at::Tensor* w = maybe(a[4]);
-        const mtk_stream s = (mtk_stream)(intptr_t)integer(a[5]);
-        const int d = current(y), dt = code(y);
-        rows(y, d);
-        dense(slot, d);
-        need(k >= 1 && N >= 1 && y.size(0) == N * k && slot.numel() == N * k && slot.scalar_type() == at::kInt);
-        if (w) {
-            dense(*w, d);
-            need(w->scalar_type() == at::kFloat && w->numel() == N * k);
-        }
-        at::Tensor out = like(y, {N, y.size(1)}, y.scalar_type());
-        call([&] { return lib.fn.rows_combine(N, (int)k, y.size(1), dt, ptr(y), y.stride(0), (const int32_t*)ptr(slot), (const float*)ptr(w), out.data_ptr(), s); });
-        return THPVariable_Wrap(out);
+    return guarded(n, 5, [&]() -> PyObject* {
+        const at::Tensor& y = tensor(a[0]);
+        const Pairs p{tensor(a[1]), integer(a[2]), integer(a[3])};
+        const at::Tensor w = maybe(a[4]);
+        return THPVariable_Wrap(tracked({y, w}) ? CombineNode::apply(y, p.slot, given(w), p.N, p.k) : rows_back(y, p, w));
     });
 }
 
-struct Layer {  // the arguments that the two directions of an adapted layer share, checked
-    int device, dt, din, dout, r, E;
-    int64_t M, x_ld;
-    const float* scales = nullptr;
-    double scale = 1.0;
-    Layer(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& down, const at::Tensor& up, const at::Tensor& offsets, PyObject* scale_) {
+struct Layer {  // an adapted layer's arguments, checked
+    at::Tensor x, weight, down, up, offsets, bias, scales;
+    double scale;
+    int act, device, dt, din, dout, r, E;
+    int64_t M;
+    void check() {
         device = current(x);
         dt = code(x);
         rows(x, device);
@@ -226,77 +311,90 @@ struct Layer {  // the arguments that the two directions of an adapted layer sha
         need(weight.dim() == 2 && down.dim() == 3 && up.dim() == 3 && offsets.dim() == 1 && offsets.scalar_type() == at::kInt);
         need(weight.size(0) <= MTK_ADAPTER_MAX_WIDTH && weight.size(1) <= MTK_ADAPTER_MAX_WIDTH && down.size(0) <= MTK_ROUTE_MAX_GROUPS && down.size(1) <= MTK_ADAPTER_MAX_RANK);
         M = x.size(0);
-        x_ld = x.stride(0);
         din = (int)x.size(1), dout = (int)weight.size(0), E = (int)down.size(0), r = (int)down.size(1);
-        need(M >= 1 && dout >= 1 && E >= 1 && r >= 1 && weight.size(1) == din && down.size(2) == din && up.size(0) == E && up.size(1) == dout && up.size(2) == r &&
-             offsets.size(0) == E + 1);
-        if (THPVariable_Check(scale_)) {
-            const at::Tensor& s = THPVariable_Unpack(scale_);
-            dense(s, device);
-            need(s.scalar_type() == at::kFloat && s.dim() == 1 && s.size(0) == E);
-            scales = s.const_data_ptr<float>();
-        } else {
-            scale = real(scale_);
+        need(dout >= 1 && E >= 1 && r >= 1 && weight.size(1) == din && down.size(2) == din && up.size(0) == E && up.size(1) == dout && up.size(2) == r && offsets.size(0) == E + 1);
+        if (bias.defined()) {
+            dense(bias, device);
+            need(bias.scalar_type() == x.scalar_type() && bias.dim() == 1 && bias.size(0) == dout);
+        }
+        if (scales.defined()) {
+            dense(scales, device);
+            need(scales.scalar_type() == at::kFloat && scales.dim() == 1 && scales.size(0) == E);
         }
     }
-    at::Tensor bytes(const at::Tensor& x, int64_t n) const { return n ? like(x, {n}, at::kByte) : at::Tensor(); }
+    at::Tensor bytes(int64_t n) const { return n ? like(x, {n}, at::kByte) : at::Tensor(); }
+    // y, and in `saved` what the backward reads
+    at::Tensor forward(bool keep, at::Tensor& saved) {
+        check();
+        at::Tensor y = like(x, {M, dout}, x.scalar_type());
+        const int64_t saved_bytes = lib.fn.saved_bytes(M, r, dt), work_bytes = lib.fn.work_bytes(M, din, dout, r, E, dt, act, 0);
+        saved = like(x, {saved_bytes}, at::kByte);
+        const at::Tensor work = bytes(work_bytes);
+        if (M)
+            call([&] {
+                return lib.fn.adapter_forward(M, din, dout, r, E, dt, ptr(x), x.stride(0), ptr(weight), ptr(bias), ptr(down), ptr(up), (const int32_t*)ptr(offsets), (const float*)ptr(scales),
+                                              scale, act, keep, ptr(y), ptr(saved), saved_bytes, ptr(work), work_bytes, stream_of(device));
+            });
+        return y;
+    }
+    variable_list backward(const at::Tensor& y, const at::Tensor& dy, const at::Tensor& saved, bool want_x, bool want_down, bool want_up) {
+        check();
+        need(dy.scalar_type() == x.scalar_type() && dy.dim() == 2 && dy.size(0) == M && dy.size(1) == dout && dy.is_contiguous() && dy.device() == x.device());
+        need(act == MTK_ACT_NONE || (y.defined() && y.is_contiguous() && y.sizes() == dy.sizes() && y.scalar_type() == x.scalar_type()));
+        at::Tensor dx, ddown, dup;
+        if (want_x) dx = like(x, {M, din}, x.scalar_type());
+        if (want_down) ddown = M ? like(x, down.sizes(), x.scalar_type()) : at::zeros(down.sizes(), x.options().requires_grad(false));
+        if (want_up) dup = M ? like(x, up.sizes(), x.scalar_type()) : at::zeros(up.sizes(), x.options().requires_grad(false));
+        const int64_t work_bytes = lib.fn.work_bytes(M, din, dout, r, E, dt, act, 1);
+        const at::Tensor work = bytes(work_bytes);
+        if (M && (want_x || want_down || want_up))
+            call([&] {
+                return lib.fn.adapter_backward(M, din, dout, r, E, dt, ptr(x), x.stride(0), ptr(weight), ptr(down), ptr(up), (const int32_t*)ptr(offsets), (const float*)ptr(scales), scale, act,
+                                               ptr(y), ptr(dy), ptr(saved), ptr(dx), ptr(ddown), ptr(dup), ptr(work), work_bytes, stream_of(device));
+            });
+        return {dx, ddown, dup};
+    }
 };
 
-// adapter_forward(x, weight, bias | None, down, up, offsets, scale, act, keep, stream) -> y, or (y, saved) with keep.  Without keep, inputs
-// that autograd tracks are declined.
-PyObject* adapter_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded(n, 10, [&]() -> PyObject* {
-        const at::Tensor &x = tensor(a[0]), &weight = tensor(a[1]), &down = tensor(a[3]), &up = tensor(a[4]), &offsets = tensor(a[5]);
-        const at::Tensor* bias = maybe(a[2]);
-        const int act = (int)integer(a[7]);
-        const bool keep = integer(a[8]) != 0;
-        const mtk_stream s = (mtk_stream)(intptr_t)integer(a[9]);
-        need(keep || !tracked({&x, &weight, bias, &down, &up}));
-        const Layer l(x, weight, down, up, offsets, a[6]);
-        if (bias) {
-            dense(*bias, l.device);
-            need(bias->scalar_type() == x.scalar_type() && bias->dim() == 1 && bias->size(0) == l.dout);
-        }
-        const int64_t saved_bytes = lib.fn.saved_bytes(l.M, l.r, l.dt), work_bytes = lib.fn.work_bytes(l.M, l.din, l.dout, l.r, l.E, l.dt, act, 0);
-        at::Tensor y = like(x, {l.M, l.dout}, x.scalar_type()), saved = l.bytes(x, saved_bytes), work = l.bytes(x, work_bytes);
-        call([&] {
-            return lib.fn.adapter_forward(l.M, l.din, l.dout, l.r, l.E, l.dt, ptr(x), l.x_ld, ptr(weight), ptr(bias), ptr(down), ptr(up), (const int32_t*)ptr(offsets), l.scales,
-                                          l.scale, act, keep, y.data_ptr(), saved.data_ptr(), saved_bytes, work.defined() ? work.data_ptr() : nullptr, work_bytes, s);
+struct AdapterNode : torch::autograd::Function<AdapterNode> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& down, const at::Tensor& up, const at::Tensor& weight, const at::Tensor& offsets,
+                              const std::optional<at::Tensor>& bias, const std::optional<at::Tensor>& scales_, double scale, int64_t act) {
+        const at::Tensor scales = scales_.value_or(at::Tensor());
+        Layer l{x, weight, down, up, offsets, bias.value_or(at::Tensor()), scales, scale, (int)act};
+        at::Tensor saved;
+        const at::Tensor y = l.forward(true, saved);
+        ctx->save_for_backward({x, down, up, weight, offsets, scales, act ? y : at::Tensor(), saved});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["act"] = act;
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list s = ctx->get_saved_variables();
+        return backward_of("adapter_linear", s[0], [&] {
+            Layer l{s[0], s[3], s[1], s[2], s[4], {}, s[5], ctx->saved_data["scale"].toDouble(), (int)ctx->saved_data["act"].toInt()};
+            variable_list out = l.backward(s[6], grads[0].contiguous(), s[7], ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2));
+            out.resize(9);
+            return once(grads, std::move(out), "adapter_linear");
         });
-        return keep ? pack({y, saved}) : THPVariable_Wrap(y);
+    }
+};
+
+// adapter(x, weight, bias | None, down, up, offsets, scale, act) -> y.  A shared layer that autograd tracks is declined.
+PyObject* adapter(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 8, [&]() -> PyObject* {
+        Layer l{tensor(a[0]), tensor(a[1]), tensor(a[3]), tensor(a[4]), tensor(a[5]), maybe(a[2]), {}, 1.0, (int)integer(a[7])};
+        if (THPVariable_Check(a[6])) l.scales = tensor(a[6]);
+        else l.scale = real(a[6]);
+        need(!tracked({l.weight, l.bias}));
+        at::Tensor saved;
+        if (!tracked({l.x, l.down, l.up})) return THPVariable_Wrap(l.forward(false, saved));
+        return THPVariable_Wrap(AdapterNode::apply(l.x, l.down, l.up, l.weight, l.offsets, given(l.bias), given(l.scales.defined() ? l.scales.detach() : l.scales), l.scale, (int64_t)l.act));
     });
 }
 
-// adapter_backward(x, weight, down, up, offsets, scale, act, y | None, dy, saved, want (1: dx, 2: ddown, 4: dup), stream) -> (dx, ddown, dup)
-PyObject* adapter_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded(n, 12, [&]() -> PyObject* {
-        const at::Tensor &x = tensor(a[0]), &weight = tensor(a[1]), &down = tensor(a[2]), &up = tensor(a[3]), &offsets = tensor(a[4]), &dy = tensor(a[8]), &saved = tensor(a[9]);
-        const int act = (int)integer(a[6]);
-        const at::Tensor* y = maybe(a[7]);
-        const int64_t want = integer(a[10]);
-        const mtk_stream s = (mtk_stream)(intptr_t)integer(a[11]);
-        const Layer l(x, weight, down, up, offsets, a[5]);
-        dense(dy, l.device);
-        dense(saved, l.device);
-        need(dy.scalar_type() == x.scalar_type() && dy.dim() == 2 && dy.size(0) == l.M && dy.size(1) == l.dout && saved.numel() >= lib.fn.saved_bytes(l.M, l.r, l.dt));
-        need(act == MTK_ACT_NONE || (y && y->is_contiguous() && y->sizes() == dy.sizes() && y->scalar_type() == x.scalar_type()));
-        const int64_t work_bytes = lib.fn.work_bytes(l.M, l.din, l.dout, l.r, l.E, l.dt, act, 1);
-        at::Tensor dx, ddown, dup, work = l.bytes(x, work_bytes);
-        if (want & 1) dx = like(x, {l.M, l.din}, x.scalar_type());
-        if (want & 2) ddown = like(x, down.sizes(), x.scalar_type());
-        if (want & 4) dup = like(x, up.sizes(), x.scalar_type());
-        call([&] {
-            return lib.fn.adapter_backward(l.M, l.din, l.dout, l.r, l.E, l.dt, ptr(x), l.x_ld, ptr(weight), ptr(down), ptr(up), (const int32_t*)ptr(offsets), l.scales, l.scale, act,
-                                           ptr(y), ptr(dy), ptr(saved), want & 1 ? dx.data_ptr() : nullptr, want & 2 ? ddown.data_ptr() : nullptr,
-                                           want & 4 ? dup.data_ptr() : nullptr, work.data_ptr(), work_bytes, s);
-        });
-        return pack({dx, ddown, dup});
-    });
-}
-
-// adamw(params, grads, exp_avgs, exp_avg_sqs, scales | None, scales | None, step, lr, beta1, beta2, eps, weight_decay, hyper | None, stream) -> True
+// adamw(params, grads, exp_avgs, exp_avg_sqs, scales | None, scales | None, step, lr, beta1, beta2, eps, weight_decay, hyper | None) -> True
 PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded(n, 14, [&]() -> PyObject* {
+    return guarded(n, 13, [&]() -> PyObject* {
         const bool q8 = a[4] != Py_None;
         need(q8 == (a[5] != Py_None));
         const int lists = q8 ? 6 : 4;
@@ -334,11 +432,10 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
         }
         const int64_t step = integer(a[6]);
         const double lr = real(a[7]), b1 = real(a[8]), b2 = real(a[9]), eps = real(a[10]), wd = real(a[11]);
-        const at::Tensor* hyper = maybe(a[12]);
-        const mtk_stream s = (mtk_stream)(intptr_t)integer(a[13]);
+        const at::Tensor hyper = maybe(a[12]);
         call([&] {
             return lib.fn.adamw_step((int)count, at[0].data(), at[1].data(), at[2].data(), at[3].data(), q8 ? (float* const*)at[4].data() : nullptr,
-                                     q8 ? (float* const*)at[5].data() : nullptr, numel.data(), dt, q8 ? 8 : 32, lr, b1, b2, eps, wd, step, ptr(hyper), s);
+                                     q8 ? (float* const*)at[5].data() : nullptr, numel.data(), dt, q8 ? 8 : 32, lr, b1, b2, eps, wd, step, ptr(hyper), stream_of(d));
         });
         // written through raw pointers: autograd and the modules' caches have to see it
         for (Py_ssize_t j = 0; j < count; ++j) {
@@ -350,7 +447,7 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 #define ENTRY(name) {#name, (PyCFunction)(void (*)())name, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {ENTRY(bind), ENTRY(route), ENTRY(dispatch), ENTRY(combine), ENTRY(adapter_forward), ENTRY(adapter_backward), ENTRY(adamw), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {ENTRY(bind), ENTRY(route), ENTRY(dispatch), ENTRY(combine), ENTRY(adapter), ENTRY(adamw), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mtk_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import launch, native, raw_stream
+from ._lib import launch, native
 from .routing import DTYPES
 
 SCALE_BLOCK = 256  # values per scale of the 8-bit moments
@@ -59,8 +59,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     p0 = params[0]
     if not p0.is_cuda:
         raise RuntimeError("adamw_step: midst_toolkit_amd has no CPU path; move the params to the MI355X")
-    if native().adamw(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, step, lr, betas[0], betas[1], eps, weight_decay, _hyper,
-                      raw_stream(p0.get_device())):
+    if native().adamw(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, step, lr, betas[0], betas[1], eps, weight_decay, _hyper):
         return
     if p0.dtype not in DTYPES:
         raise ValueError(f"adamw_step: params are {p0.dtype} (float32, bfloat16 or float16)")

@@ -9,10 +9,8 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
-from . import _lib
-from ._lib import launch, native, raw_stream
+from ._lib import native, ordinary
 
 MAX_GROUPS = 1024  # MTK_ROUTE_MAX_GROUPS of include/mtk.h
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # enum mtk_dtype
@@ -48,7 +46,7 @@ def route_rows(index: Tensor, n_groups: int) -> RowPlan:
     range goes where -1 goes, and its rows are NaN: dispatched, combined and in gradients."""
     if not index.is_cuda:
         raise RuntimeError("route_rows: midst_toolkit_amd has no CPU path; move the indices to the MI355X")
-    got = native().route(index, n_groups, raw_stream(index.get_device()))
+    got = native().route(index, n_groups)
     if got is not None:
         return RowPlan(*got, n_groups, index.shape[0], 1 if index.dim() == 1 else index.shape[1])
     if index.dim() not in (1, 2) or index.dtype.is_floating_point or index.dtype.is_complex or index.dtype == torch.bool:
@@ -58,107 +56,38 @@ def route_rows(index: Tensor, n_groups: int) -> RowPlan:
     copies = 1 if index.dim() == 1 else index.shape[1]
     if copies < 1:
         raise ValueError("route_rows: index has no copies")
-    dev, P = index.device, index.numel()
-    if P > 0x7FFFFFFF:
-        raise ValueError(f"route_rows: {P} pairs exceed 2^31 - 1")
-    idx = index.to(torch.int64).contiguous()
-    l = _lib.lib()
-    order = torch.empty(P, dtype=torch.int32, device=dev)
-    slot = torch.empty(index.shape, dtype=torch.int32, device=dev)
-    offsets = torch.empty(n_groups + 1, dtype=torch.int32, device=dev)
-    need = l.mtk_route_rows_work(P, n_groups)
-    work = torch.empty(need, dtype=torch.int32, device=dev) if need else None
-    launch(dev, l.mtk_route_rows, P, idx.data_ptr(), n_groups, order.data_ptr(), slot.data_ptr(), offsets.data_ptr(),
-           None if work is None else work.data_ptr(), need)
-    return RowPlan(order, slot, offsets, n_groups, index.shape[0], copies)
+    if index.numel() > 0x7FFFFFFF:
+        raise ValueError(f"route_rows: {index.numel()} pairs exceed 2^31 - 1")
+    got = ordinary("route_rows", index.device, native().route, index.to(torch.int64).contiguous(), int(n_groups))
+    return RowPlan(*got, int(n_groups), index.shape[0], copies)
 
 
-def _check_rows(what: str, t: Tensor, rows: int, plan: RowPlan) -> int:
+def _check_rows(what: str, t: Tensor, rows: int, plan: RowPlan) -> None:
     if not t.is_cuda:
         raise RuntimeError(f"{what}: midst_toolkit_amd has no CPU path; move the rows to the MI355X")
     if t.device != plan.order.device:
         raise ValueError(f"{what}: rows on {t.device}, plan on {plan.order.device}")
     if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1:
         raise ValueError(f"{what}: expected [{rows}, width] rows, got {tuple(t.shape)}")
-    return dtype_code(t, what)
-
-
-def _dispatch(x: Tensor, plan: RowPlan, w: Tensor | None, y: Tensor | None = None, want_rows: bool = True):
-    """mtk_rows_dispatch: (xs, dw)."""
-    got = native().dispatch(x, plan.slot, plan.n_rows, plan.copies, w, y, int(want_rows), raw_stream(x.get_device()))
-    if got is not None:
-        return got
-    dev, D = x.device, x.shape[1]
-    x = rows_of(x)
-    P = plan.n_rows * plan.copies
-    xs = torch.empty((P, D), dtype=x.dtype, device=dev) if want_rows else None
-    dw = torch.empty((plan.n_rows, plan.copies), dtype=torch.float32, device=dev) if y is not None else None
-    if P:
-        launch(dev, _lib.lib().mtk_rows_dispatch, plan.n_rows, plan.copies, D, DTYPES[x.dtype], x.data_ptr(), x.stride(0), plan.slot.data_ptr(),
-               None if w is None else w.data_ptr(), None if xs is None else xs.data_ptr(), None if y is None else y.data_ptr(),
-               None if dw is None else dw.data_ptr())
-    return xs, dw
-
-
-def _combine(y: Tensor, plan: RowPlan, w: Tensor | None) -> Tensor:
-    got = native().combine(y, plan.slot, plan.n_rows, plan.copies, w, raw_stream(y.get_device()))
-    if got is not None:
-        return got
-    dev, D = y.device, y.shape[1]
-    y = rows_of(y)
-    out = torch.empty((plan.n_rows, D), dtype=y.dtype, device=dev)
-    if plan.n_rows:
-        launch(dev, _lib.lib().mtk_rows_combine, plan.n_rows, plan.copies, D, DTYPES[y.dtype], y.data_ptr(), y.stride(0), plan.slot.data_ptr(),
-               None if w is None else w.data_ptr(), out.data_ptr())
-    return out
-
-
-class _Dispatch(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, plan):
-        ctx.plan = plan
-        return _dispatch(x, plan, None)[0]
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        return _combine(g, ctx.plan, None), None
-
-
-class _Combine(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, weights, plan):
-        ctx.plan = plan
-        ctx.save_for_backward(y if weights is not None and ctx.needs_input_grad[1] else None, weights)
-        return _combine(y, plan, weights)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        y, w = ctx.saved_tensors
-        want_w = w is not None and ctx.needs_input_grad[1]
-        gy, gw = _dispatch(g, ctx.plan, w, y.contiguous() if want_w else None, ctx.needs_input_grad[0])
-        return gy, gw, None
+    dtype_code(t, what)
 
 
 def dispatch_rows(x: Tensor, plan: RowPlan) -> Tensor:
     """``x`` [N, D] -> [N * k, D]: every record's row in the places of its k pairs, sorted by model.  Differentiable in ``x`` (a record's
     gradient is the sum over its pairs, in fp32, in the order of its copies)."""
-    track = x.requires_grad and torch.is_grad_enabled()
-    if not track and x.is_cuda:
-        got = native().dispatch(x, plan.slot, plan.n_rows, plan.copies, None, None, 1, raw_stream(x.get_device()))
+    if x.is_cuda:
+        got = native().dispatch(x, plan.slot, plan.n_rows, plan.copies)
         if got is not None:
-            return got[0]
+            return got
     _check_rows("dispatch_rows", x, plan.n_rows, plan)
-    return _Dispatch.apply(x, plan) if track else _dispatch(x, plan, None)[0]
+    return ordinary("dispatch_rows", x.device, native().dispatch, rows_of(x), plan.slot, plan.n_rows, plan.copies)
 
 
 def combine_rows(y: Tensor, plan: RowPlan, weights: Tensor | None = None) -> Tensor:
     """``y`` [N * k, D] in the plan's order -> [N, D]: ``sum_j weights[n, j] * y[slot[n, j]]`` (``weights`` None: ones), summed in fp32 and
     rounded once.  ``weights``: float32 of ``index``'s shape.  Differentiable in both."""
-    track = torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad))
-    if not track and y.is_cuda and (weights is None or weights.dim() == 2):
-        got = native().combine(y, plan.slot, plan.n_rows, plan.copies, weights, raw_stream(y.get_device()))
+    if y.is_cuda:
+        got = native().combine(y, plan.slot, plan.n_rows, plan.copies, weights)
         if got is not None:
             return got
     _check_rows("combine_rows", y, plan.n_rows * plan.copies, plan)
@@ -167,7 +96,5 @@ def combine_rows(y: Tensor, plan: RowPlan, weights: Tensor | None = None) -> Ten
             raise ValueError(f"combine_rows: weights on {weights.device}, rows on {y.device}")
         if weights.dtype != torch.float32 or weights.numel() != plan.n_rows * plan.copies or weights.shape[0] != plan.n_rows:
             raise ValueError(f"combine_rows: weights are float32 [{plan.n_rows}, {plan.copies}], got {weights.dtype} {tuple(weights.shape)}")
-        if weights.dim() != 2:
-            weights = weights.reshape(plan.n_rows, plan.copies)
-        weights = weights.contiguous()
-    return _Combine.apply(y, weights, plan) if track else _combine(y, plan, weights)
+        weights = weights.reshape(plan.n_rows, plan.copies).contiguous()
+    return ordinary("combine_rows", y.device, native().combine, rows_of(y), plan.slot, plan.n_rows, plan.copies, weights)

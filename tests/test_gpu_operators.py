@@ -232,13 +232,13 @@ def inner(dt):
 def tol(terms, low, K, r, want, dt, factor):
     """Sums of K products over `terms`; the low-rank part sums K, then r, with its inner value rounded (by half the smallest step at least, times
     the second factor).  The stored value rounds once more."""
-    return (TWICE * (K + 2) * U32 * terms + (TWICE * (K + r + 8) * U32 + inner(dt)) * low + tiny(dt) * r * float(factor.abs().max()) * 1.5
+    return (TWICE * (K + 2) * U32 * terms + (TWICE * (K + r + 8) * U32 + inner(dt)) * low + tiny(dt) * r * float(factor.detach().abs().max()) * 1.5
             + half(dt) * want.abs() * 1.01 + tiny(dt) * 4)
 
 
 def tol_factor(mag, K, rows, want, dt, other):
     """A factor's gradient: sums over K features, then over a model's rows."""
-    return (TWICE * (K + rows + 8) * U32 + inner(dt)) * mag + tiny(dt) * rows * float(other.abs().max()) * 1.5 + half(dt) * want.abs() * 1.01 + tiny(dt) * 4
+    return (TWICE * (K + rows + 8) * U32 + inner(dt)) * mag + tiny(dt) * rows * float(other.detach().abs().max()) * 1.5 + half(dt) * want.abs() * 1.01 + tiny(dt) * 4
 
 
 SHAPES = [(1, 1, 1, 1, 1, "any"), (1, 64, 64, 8, 4, "any"), (2, 7, 5, 3, 2, "any"), (31, 130, 67, 12, 5, "any"), (33, 64, 128, 16, 3, "last"), (64, 33, 130, 17, 64, "any"),
