@@ -520,14 +520,16 @@ int mtk_rows_combine(int64_t n_rows, int k, int64_t D, int dtype, const void* y,
  * saved (mtk_adapter_saved_bytes, 256-byte aligned): holds s_e x down_e^T; mtk_adapter_backward reads it, and with keep = 0 it is
  * scratch.  mtk_adapter_backward: dx [M, din], ddown, dup (each may be NULL) from dy [M, dout] dense, for the same arguments;
  * y is read under an activation only.  W and bias are frozen and get no gradient.  work: mtk_adapter_work_bytes of the direction, 256-byte
- * aligned (0: may be NULL).
+ * aligned (0: may be NULL).  mtk_adapter_streams says whether K values a row at p, ld apart, can be read as they lie; rows_stream (of x, or of
+ * dy; under an activation, of an aligned dense dy) and weight_streams say so of a call's operands, padded copies need room otherwise.
  * Sums in fp32; identical run to run. */
 #define MTK_ADAPTER_MAX_RANK 256
 #define MTK_ADAPTER_MAX_WIDTH 8192
 #define MTK_ADAPTER_MAX_ROWS 16777216
 enum mtk_activation { MTK_ACT_NONE = 0, MTK_ACT_RELU = 1 };
 int64_t mtk_adapter_saved_bytes(int64_t M, int r, int dtype);
-int64_t mtk_adapter_work_bytes(int64_t M, int din, int dout, int r, int n_models, int dtype, int act, int backward);
+int mtk_adapter_streams(const void* p, int64_t ld, int K, int dtype);
+int64_t mtk_adapter_work_bytes(int64_t M, int din, int dout, int r, int n_models, int dtype, int act, int backward, int rows_stream, int weight_streams);
 int mtk_adapter_forward(int64_t M, int din, int dout, int r, int n_models, int dtype, const void* x, int64_t x_ld, const void* W, const void* bias,
                         const void* down, const void* up, const int32_t* offsets, const float* scales, double scale, int act, int keep, void* y,
                         void* saved, int64_t saved_bytes, void* work, int64_t work_bytes, mtk_stream stream);

@@ -28,7 +28,7 @@ TABLE_ORDER = [
 _lib = None
 _native = None
 # the library functions that _mtk_torch calls, in the order of its table
-_NATIVE = ["mtk_last_error", "mtk_route_rows_work", "mtk_route_rows", "mtk_rows_dispatch", "mtk_rows_combine", "mtk_adapter_saved_bytes", "mtk_adapter_work_bytes",
+_NATIVE = ["mtk_last_error", "mtk_route_rows_work", "mtk_route_rows", "mtk_rows_dispatch", "mtk_rows_combine", "mtk_adapter_saved_bytes", "mtk_adapter_streams", "mtk_adapter_work_bytes",
            "mtk_adapter_forward", "mtk_adapter_backward", "mtk_adamw_step"]
 
 _p, _i64, _i32, _u64 = C.c_void_p, C.c_int64, C.c_int, C.c_uint64
@@ -104,7 +104,8 @@ _SIGS = {
     "mtk_rows_dispatch": (C.c_int, [_i64, _i32, _i64, _i32, _p, _i64, _p, _p, _p, _p, _p, _p]),
     "mtk_rows_combine": (C.c_int, [_i64, _i32, _i64, _i32, _p, _i64, _p, _p, _p, _p]),
     "mtk_adapter_saved_bytes": (_i64, [_i64, _i32, _i32]),
-    "mtk_adapter_work_bytes": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "mtk_adapter_streams": (C.c_int, [_p, _i64, _i32, _i32]),
+    "mtk_adapter_work_bytes": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "mtk_adapter_forward": (C.c_int, [_i64, _i32, _i32, _i32, _i32, _i32, _p, _i64, _p, _p, _p, _p, _p, _p, C.c_double, _i32, _i32, _p, _p, _i64, _p, _i64, _p]),
     "mtk_adapter_backward": (C.c_int, [_i64, _i32, _i32, _i32, _i32, _i32, _p, _i64, _p, _p, _p, _p, _p, C.c_double, _i32, _p, _p, _p, _p, _p, _p, _p,
                                        _i64, _p]),

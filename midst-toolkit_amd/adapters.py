@@ -116,7 +116,7 @@ class LowRankEnsemble(nn.Module):
             raise ValueError(f"LowRankEnsemble: x is [N, {self.weight0.shape[1]}], got {tuple(x.shape)}")
         if timesteps.shape != x.shape[:1] or index.shape[:1] != x.shape[:1]:
             raise ValueError(f"LowRankEnsemble: {x.shape[0]} records, timesteps {tuple(timesteps.shape)}, index {tuple(index.shape)}")
-        plan = route_rows(index, self.n_models)
+        plan = route_rows(index.to(x.device), self.n_models)
         t = timesteps.to(device=x.device, dtype=torch.int64)
         emb = self.time_table[t.clamp(0, self.num_timesteps - 1)]
         emb = torch.where(((t < 0) | (t >= self.num_timesteps))[:, None], float("nan"), emb)

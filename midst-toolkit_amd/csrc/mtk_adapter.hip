@@ -1102,11 +1102,11 @@ struct Shape {
 // what k_linear reads beside its operands, and their padded copies where they need one
 struct Packed {
     int64_t X, W, F, Bp, bias, owner;  // F: the factors that the shrink multiplies, in whole lines like X
-    Packed(Layout& l, const Shape& sh, int64_t M, int N, int r, int E, int dtype) {
+    Packed(Layout& l, const Shape& sh, int64_t M, int N, int r, int E, int dtype, bool pad_x, bool pad_w) {
         const int64_t z = mtk_dtype_size(dtype);
-        X = l.take(sh.few ? 0 : M * sh.Kp * z);
-        W = l.take(sh.few ? 0 : (int64_t)N * sh.Kp * z);
-        F = l.take(sh.few ? 0 : (int64_t)E * r * sh.Kp * z);
+        X = l.take(!sh.few && pad_x ? M * sh.Kp * z : 0);
+        W = l.take(!sh.few && pad_w ? (int64_t)N * sh.Kp * z : 0);
+        F = l.take(!sh.few && pad_x ? (int64_t)E * r * sh.Kp * z : 0);
         Bp = l.take(sh.blocks ? (int64_t)(E + 1) * N * sh.rp * z : 0);
         bias = l.take((int64_t)sh.nb_n * sh.BN * 4);
         owner = l.take(sh.blocks ? sh.MT * 4 : 0);
@@ -1117,12 +1117,12 @@ bool streams(const void* p, int64_t ld, int K, int dtype) {
     const int64_t z = mtk_dtype_size(dtype);
     return (uintptr_t)p % 16 == 0 && ld * z % 16 == 0 && K % (128 / z) == 0 && ld * z < (1 << 22);
 }
-// forward: the padded operands (sized as if both needed it, where their sizes allow that they do not)
 struct ForwardWork {
     int64_t bytes;
     Shape sh;
     Packed pk;
-    ForwardWork(Layout l, int64_t M, int din, int dout, int r, int E, int dtype) : sh(M, dout, din, r, E, dtype), pk(l, sh, M, dout, r, E, dtype) {
+    ForwardWork(Layout l, int64_t M, int din, int dout, int r, int E, int dtype, bool pad_x, bool pad_w)
+        : sh(M, dout, din, r, E, dtype), pk(l, sh, M, dout, r, E, dtype, pad_x, pad_w) {
         bytes = sh.few ? 0 : l.at;
     }
 };
@@ -1130,7 +1130,8 @@ struct BackwardWork {
     int64_t Bt, Wt, At, t, g, part[2], bytes;
     Shape sh;
     Packed pk;
-    BackwardWork(Layout l, int64_t M, int din, int dout, int r, int E, int dtype, bool relu) : sh(M, din, dout, r, E, dtype), pk(l, sh, M, din, r, E, dtype) {
+    BackwardWork(Layout l, int64_t M, int din, int dout, int r, int E, int dtype, bool relu, bool pad_g)
+        : sh(M, din, dout, r, E, dtype), pk(l, sh, M, din, r, E, dtype, pad_g, true) {  // the weights are turned, so laid out anew
         const int64_t z = mtk_dtype_size(dtype);
         Bt = l.take((int64_t)E * r * sh.Kp * z);
         Wt = l.take(sh.few ? (int64_t)din * dout * z : 0);  // else pk.W
@@ -1249,9 +1250,11 @@ int adapter_check(const char* who, int64_t M, int din, int dout, int r, int E, i
 extern "C" int64_t mtk_adapter_saved_bytes(int64_t M, int r, int dtype) {
     return M > 0 && r > 0 && mtk_dtype_ok(dtype) ? Saved(M, r, dtype).bytes : 0;
 }
-extern "C" int64_t mtk_adapter_work_bytes(int64_t M, int din, int dout, int r, int E, int dtype, int act, int backward) {
+extern "C" int mtk_adapter_streams(const void* p, int64_t ld, int K, int dtype) { return mtk_dtype_ok(dtype) && K > 0 && streams(p, ld, K, dtype); }
+extern "C" int64_t mtk_adapter_work_bytes(int64_t M, int din, int dout, int r, int E, int dtype, int act, int backward, int rows_stream, int weight_streams) {
     if (M <= 0 || din <= 0 || dout <= 0 || r <= 0 || E <= 0 || !mtk_dtype_ok(dtype)) return 0;
-    return backward ? BackwardWork(Layout(), M, din, dout, r, E, dtype, act == 1).bytes : ForwardWork(Layout(), M, din, dout, r, E, dtype).bytes;
+    return backward ? BackwardWork(Layout(), M, din, dout, r, E, dtype, act == 1, !rows_stream).bytes
+                    : ForwardWork(Layout(), M, din, dout, r, E, dtype, !rows_stream, !weight_streams).bytes;
 }
 
 extern "C" int mtk_adapter_forward(int64_t M, int din, int dout, int r, int E, int dtype, const void* x, int64_t x_ld, const void* W, const void* bias,
@@ -1262,7 +1265,7 @@ extern "C" int mtk_adapter_forward(int64_t M, int din, int dout, int r, int E, i
     if (!x || !W || !down || !up || !offsets || !y || !saved) MTK_FAIL(MTK_ERR_ARG, "mtk_adapter_forward: null pointer");
     const Saved sv(M, r, dtype);
     if (saved_bytes < sv.bytes) MTK_FAIL(MTK_ERR_ARG, "mtk_adapter_forward: a buffer of %lld bytes for the low-rank rows, %lld needed", (long long)saved_bytes, (long long)sv.bytes);
-    const ForwardWork wk(Layout(), M, din, dout, r, E, dtype);
+    const ForwardWork wk(Layout(), M, din, dout, r, E, dtype, !streams(x, x_ld, din, dtype), !streams(W, din, din, dtype));
     if (wk.bytes && (!work || work_bytes < wk.bytes)) MTK_FAIL(MTK_ERR_ARG, "mtk_adapter_forward: workspace of %lld bytes, %lld needed", (long long)work_bytes, (long long)wk.bytes);
     int rc = MTK_OK;
     mtk_by_type(dtype, [&](auto tag) {
@@ -1308,7 +1311,8 @@ extern "C" int mtk_adapter_backward(int64_t M, int din, int dout, int r, int E, 
     if (M == 0) return MTK_OK;
     if (!x || !W || !down || !up || !offsets || !dy || !saved || !work || (act && !y)) MTK_FAIL(MTK_ERR_ARG, "mtk_adapter_backward: null pointer");
     const Saved sv(M, r, dtype);
-    const BackwardWork wk(Layout(), M, din, dout, r, E, dtype, act == 1);
+    // (under an activation the masked gradient is a copy in the workspace, aligned)
+    const BackwardWork wk(Layout(), M, din, dout, r, E, dtype, act == 1, act ? !streams(nullptr, dout, dout, dtype) : !streams(dy, dout, dout, dtype));
     if (work_bytes < wk.bytes) MTK_FAIL(MTK_ERR_ARG, "mtk_adapter_backward: workspace of %lld bytes, %lld needed", (long long)work_bytes, (long long)wk.bytes);
     int rc = MTK_OK;
     mtk_by_type(dtype, [&](auto tag) {

@@ -18,6 +18,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -34,6 +35,7 @@ struct Table {
     decltype(&mtk_rows_dispatch) rows_dispatch;
     decltype(&mtk_rows_combine) rows_combine;
     decltype(&mtk_adapter_saved_bytes) saved_bytes;
+    decltype(&mtk_adapter_streams) streams;
     decltype(&mtk_adapter_work_bytes) work_bytes;
     decltype(&mtk_adapter_forward) adapter_forward;
     decltype(&mtk_adapter_backward) adapter_backward;
@@ -327,7 +329,8 @@ struct Layer {  // an adapted layer's arguments, checked
     at::Tensor forward(bool keep, at::Tensor& saved) {
         check();
         at::Tensor y = like(x, {M, dout}, x.scalar_type());
-        const int64_t saved_bytes = lib.fn.saved_bytes(M, r, dt), work_bytes = lib.fn.work_bytes(M, din, dout, r, E, dt, act, 0);
+        const int64_t saved_bytes = lib.fn.saved_bytes(M, r, dt), work_bytes = lib.fn.work_bytes(M, din, dout, r, E, dt, act, 0, lib.fn.streams(ptr(x), x.stride(0), din, dt),
+                                                                                                              lib.fn.streams(ptr(weight), din, din, dt));
         saved = like(x, {saved_bytes}, at::kByte);
         const at::Tensor work = bytes(work_bytes);
         if (M)
@@ -345,7 +348,7 @@ struct Layer {  // an adapted layer's arguments, checked
         if (want_x) dx = like(x, {M, din}, x.scalar_type());
         if (want_down) ddown = M ? like(x, down.sizes(), x.scalar_type()) : at::zeros(down.sizes(), x.options().requires_grad(false));
         if (want_up) dup = M ? like(x, up.sizes(), x.scalar_type()) : at::zeros(up.sizes(), x.options().requires_grad(false));
-        const int64_t work_bytes = lib.fn.work_bytes(M, din, dout, r, E, dt, act, 1);
+        const int64_t work_bytes = lib.fn.work_bytes(M, din, dout, r, E, dt, act, 1, lib.fn.streams(act ? nullptr : ptr(dy), dout, dout, dt), 0);
         const at::Tensor work = bytes(work_bytes);
         if (M && (want_x || want_down || want_up))
             call([&] {
@@ -430,6 +433,9 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 at[i][(size_t)j] = t.data_ptr();
             }
         }
+        std::vector<void*> seen = at[0];
+        std::sort(seen.begin(), seen.end());
+        need(std::adjacent_find(seen.begin(), seen.end(), [](void* p, void* q) { return p && p == q; }) == seen.end());
         const int64_t step = integer(a[6]);
         const double lr = real(a[7]), b1 = real(a[8]), b2 = real(a[9]), eps = real(a[10]), wd = real(a[11]);
         const at::Tensor hyper = maybe(a[12]);

@@ -75,6 +75,8 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
         _check_list("exp_avg_scales", exp_avg_scales, torch.float32, at, blocks)
         _check_list("exp_avg_sq_scales", exp_avg_sq_scales, torch.float32, at, blocks)
         lists += [exp_avg_scales, exp_avg_sq_scales]
+    if len({p.data_ptr() for p in params if p.numel()}) < sum(n > 0 for n in sizes):
+        raise ValueError("adamw_step: the same tensor twice among params")
     keep = [_addresses(ts) for ts in lists]
     addr = [a for _, a in keep] + ([] if q8 else [None, None])
     numel = array("q", sizes)

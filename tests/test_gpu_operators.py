@@ -407,11 +407,12 @@ def test_adapter_refusals():
 
 
 @pytest.mark.parametrize("off", [[0, 90, 10, 40], [50, 60, 70, 80], [-5, 20, 1000, 2000], [100, 60, 30, 0], [-9, -8, -7, -6], [2**31 - 1] * 4])
-def test_offsets_that_make_no_sense_stay_inside_the_tensors(off):
+@pytest.mark.parametrize("M", [64, 700])
+def test_offsets_that_make_no_sense_stay_inside_the_tensors(M, off):
     """Offsets live on the device, so the host cannot check them: whatever they hold, no row outside the tensors is touched and the call ends.
     Rows before the first offset have the shared layer alone."""
     g = gen(12)
-    M, din, dout, r, E = 64, 32, 48, 4, 3
+    din, dout, r, E = 32, 48, 4, 3
     a = adapter_inputs(g, M, din, dout, r, E, torch.float32)
     a["offsets"] = torch.tensor(off, dtype=torch.int32, device=DEV)
     for n in ("x", "down", "up"):
@@ -423,6 +424,77 @@ def test_offsets_that_make_no_sense_stay_inside_the_tensors(off):
         fine = a["offsets"].cpu().clamp(max=M)
         ref = adapter_reference(**{**a, "offsets": fine, "relu": False})
         within(y, ref["y"], tol(ref["y_terms"], ref["y_low"], din, r, ref["y"], torch.float32, a["up"]))
+
+
+# one shape for each tile of the products: 256 x 256 and 128 x 128 with 16 bits, 128 x 128 with fp32, both directions; 32 rows a wave in the shrink
+BIG = [(16384, 64, 1024, 8, 3), (16384, 1024, 64, 20, 2), (20011, 131, 1000, 12, 33), (16500, 1000, 131, 33, 40), (16384, 96, 1024, 40, 70)]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("M,din,dout,r,E", BIG)
+def test_adapter_with_many_rows(M, din, dout, r, E, dt):
+    g = gen(M + din + r)
+    a = adapter_inputs(g, M, din, dout, r, E, dt)
+    gy = randn(g, M, dout, dt=dt)
+    for n in ("x", "down", "up"):
+        a[n].requires_grad_()
+    y = call(a)
+    ref = adapter_reference(**{**a, "relu": False, "gy": gy})
+    dx, ddown, dup = torch.autograd.grad(y, (a["x"], a["down"], a["up"]), gy)
+    within(y, ref["y"], tol(ref["y_terms"], ref["y_low"], din, r, ref["y"], dt, a["up"]))
+    within(dx, ref["dx"], tol(ref["dx_terms"], ref["dx_low"], dout, r, ref["dx"], dt, a["down"]))
+    rows = int((a["offsets"][1:] - a["offsets"][:-1]).max())
+    for name, got, K, other in (("ddown", ddown, dout, a["x"]), ("dup", dup, din, gy)):
+        within(got, ref[name], tol_factor(ref[name + "_terms"], K, rows, ref[name], dt, other))
+    y2 = call(a)
+    assert torch.equal(y, y2)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y2, (a["x"], a["down"], a["up"]), gy), (dx, ddown, dup)))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("M", [40, 700])
+def test_adapter_operands_that_start_anywhere(M, dt):
+    """Views at odd offsets, odd distances between rows, an expanded row: the values of aligned copies, bit for bit."""
+    g = gen(M)
+    din, dout, r, E = 128, 192, 8, 3
+    a = adapter_inputs(g, M, din, dout, r, E, dt)
+    gy = randn(g, M, dout, dt=dt)
+
+    def moved(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=DEV)
+        flat[1:] = t.reshape(-1)
+        return flat[1:].view(t.shape)
+
+    def run(b, gy):
+        b = {n: t.detach() for n, t in b.items()}
+        for n in ("x", "down", "up"):
+            b[n].requires_grad_()
+        y = call(b)
+        return (y,) + torch.autograd.grad(y, (b["x"], b["down"], b["up"]), gy)
+
+    want = run(a, gy)
+    for names in (("x",), ("weight",), ("down", "up", "bias"), ("x", "weight", "down", "up", "bias")):
+        assert all(torch.equal(p, q) for p, q in zip(run({**a, **{n: moved(a[n]) for n in names}}, gy), want)), names
+    assert all(torch.equal(p, q) for p, q in zip(run(a, moved(gy)), want))
+    wide = torch.empty(M, din + 1, dtype=dt, device=DEV)
+    wide[:, 1:] = a["x"]
+    assert all(torch.equal(p, q) for p, q in zip(run({**a, "x": wide[:, 1:]}, gy), want))
+    row = a["x"][:1]
+    assert torch.equal(call(a, x=row.expand(M, din)), call(a, x=row.expand(M, din).contiguous()))
+
+
+def test_nodes_differentiate_once():
+    g = gen(90)
+    a = adapter_inputs(g, 20, 8, 6, 2, 3, torch.float32)
+    plan = mtk.route_rows(torch.randint(0, 3, (10, 2), generator=g).to(DEV), 3)
+    w = randn(g, 10, 2)
+    for f, leaf in ((lambda t: call(a, x=t), randn(g, 20, 8)), (lambda t: mtk.dispatch_rows(t, plan), randn(g, 10, 5)), (lambda t: mtk.combine_rows(t, plan, w), randn(g, 20, 5))):
+        leaf.requires_grad_()
+        first = torch.autograd.grad((f(leaf) ** 2).sum(), leaf, create_graph=True)[0]
+        with pytest.raises(RuntimeError, match="differentiates once only"):
+            first.sum().backward()
+        plain = torch.autograd.grad((f(leaf) ** 2).sum(), leaf)[0]
+        assert torch.equal(plain, first.detach())
 
 
 # ------------------------------------------------------------------------------------------------------------------- AdamW
@@ -616,7 +688,7 @@ def test_adamw_groups_closures_and_refusals():
         mtk.AdamW([d]).step()
     x = [torch.zeros(4, device=DEV)]
     for bad in (dict(grads=[]), dict(grads=[torch.zeros(5, device=DEV)]), dict(grads=[torch.zeros(4, device=DEV).half()]), dict(exp_avgs=[torch.zeros(8, device=DEV)[::2]]),
-                dict(exp_avg_scales=x), dict(exp_avg_sqs=[torch.zeros(4)])):
+                dict(exp_avg_scales=x), dict(exp_avg_sqs=[torch.zeros(4)]), dict(params=x * 2, grads=x * 2, exp_avgs=x * 2, exp_avg_sqs=x * 2)):
         kw = {**dict(params=x, grads=x, exp_avgs=x, exp_avg_sqs=x, step=1, lr=1e-3), **bad}
         with pytest.raises(ValueError):
             mtk.adamw_step(**kw)

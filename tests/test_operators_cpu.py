@@ -84,7 +84,12 @@ def test_workspace_sizes_are_monotonic_and_empty_for_nonsense():
     l = _lib.lib()
     assert l.mtk_adapter_saved_bytes(0, 8, 0) == 0 and l.mtk_adapter_saved_bytes(8, 8, 9) == 0
     assert 0 < l.mtk_adapter_saved_bytes(100, 8, 1) <= l.mtk_adapter_saved_bytes(1000, 8, 1)
-    assert 0 < l.mtk_adapter_work_bytes(100, 64, 64, 8, 4, 1, 0, 1) < l.mtk_adapter_work_bytes(100, 64, 64, 8, 4, 1, 1, 1)
+    assert 0 < l.mtk_adapter_work_bytes(100, 64, 64, 8, 4, 1, 0, 1, 1, 1) < l.mtk_adapter_work_bytes(100, 64, 64, 8, 4, 1, 1, 1, 1, 1)
+    assert l.mtk_adapter_work_bytes(100, 64, 64, 8, 4, 1, 0, 0, 0, 0) == 0  # few rows: nothing is laid out
+    assert l.mtk_adapter_work_bytes(5000, 64, 64, 8, 4, 1, 0, 0, 1, 1) + 5000 * 64 * 2 <= l.mtk_adapter_work_bytes(5000, 64, 64, 8, 4, 1, 0, 0, 0, 1)
+    ok = lambda p, ld, K, dt: l.mtk_adapter_streams(C.c_void_p(p), ld, K, dt)  # noqa: E731
+    assert ok(256, 64, 64, 1) and ok(256, 0, 64, 1) and ok(256, 72, 64, 1) and ok(256, 32, 32, 0)
+    assert not ok(258, 64, 64, 1) and not ok(256, 65, 64, 1) and not ok(256, 64, 32, 1) and not ok(256, 1 << 21, 64, 1) and not ok(256, 64, 64, 5)
 
 
 def test_dither_rounds_to_neighbours_and_is_unbiased_over_the_steps():
