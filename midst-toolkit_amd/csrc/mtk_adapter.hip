@@ -275,8 +275,8 @@ struct LinearArgs {
     const int32_t* owner; // [MT] the tile's model; E: none; -1: several
     const int32_t* offsets;
     int E, relu;
-    const void* low;      // [E][N][low_ld] B_e for the epilogue: the padded Bp, or B itself
-    int low_ld, rp;       // rp: elements of a row of U
+    const void* low;      // [E][N][low_ld] B_e for the epilogue, in whole pieces, zeros behind the rank
+    int low_ld, rp, r;    // rp: elements of a row of U
 };
 
 // WR x WC waves, each MW x NT tiles of 32 x 32; DX buffers of rows and DW of weights
@@ -285,6 +285,7 @@ template <int WR, int WC_, int MW, int NT, int DX_, int DW_> struct Geo {
     static constexpr int kTileX = BM * 128, kTileW = BN * 128;       // bytes of a k-block
     static constexpr int XPW = BM / 8 / NW, WPW = BN / 8 / NW;       // 8-row, 1 KiB pieces per wave
     static constexpr int DX = DX_, DW = DW_, kLds = DX * kTileX + DW * kTileW;
+    static constexpr int kRoom = 163840 / kLds, kWaves = kRoom * NW / 4;  // workgroups of a CU, waves of a SIMD: a register too many halves them
     static constexpr int kYounger = XPW + (DW - 2) * (XPW + WPW);    // pieces a wave requests after its last of the next block
 };
 
@@ -298,7 +299,7 @@ __device__ __forceinline__ int scalar_load(const int32_t* p) {
 }
 
 template <typename T, int WR, int WC, int MW, int NT, int DX, int DW>
-__global__ __launch_bounds__(64 * WR * WC, 1) void k_linear(LinearArgs g, T* __restrict__ y) {
+__global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)) void k_linear(LinearArgs g, T* __restrict__ y) {
     typedef Geo<WR, WC, MW, NT, DX, DW> G;
     constexpr int V = mtk_piece<T>::n, kWBase = DX * G::kTileX;
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
@@ -522,25 +523,45 @@ __global__ __launch_bounds__(64 * WR * WC, 1) void k_linear(LinearArgs g, T* __r
             int e;
             int64_t a, b;
             const T* u = (const T*)g.U;
+            constexpr int H = sizeof(T) == 2 ? 2 : 1, S = 32 / (2 * V);  // halves of u; steps of 32 values of the rank
+            const int half = g.rp / H, low_n = g.low_ld < half ? g.low_ld : half;  // B_e's values, once
             while (own.next(e, a, b)) {
-                const T* be = (const T*)g.low + (int64_t)e * g.N * g.low_ld;
+                const T* be = (const T*)g.low + (int64_t)e * g.N * g.low_ld + hh_e * V;
 #pragma unroll
                 for (int mt = 0; mt < MW; ++mt) {
                     const int64_t row = w0 + mt * 32 + li_e, rc = row < g.M ? row : g.M - 1;
                     const bool mine = row >= a && row < b;
                     if (a >= w0 + mt * 32 + 32 || b <= w0 + mt * 32) continue;
+                    const T* ur = u + rc * g.rp + hh_e * V;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        const int n = n0 + wc * G::WN + nt * 32 + li_e, nc = n < g.N ? n : g.N - 1;
+                        const int n = n0 + wc * G::WN + nt * 32 + li_e;
+                        const T* bn = be + (int64_t)(n < g.N ? n : g.N - 1) * g.low_ld;
                         f32x16 low = {};
-                        const T* bn = be + (int64_t)nc * g.low_ld;
-                        for (int j = hh_e * V; j - hh_e * V < g.low_ld; j += 2 * V) {
-                            const mtk_vec<T> bv = j + V <= g.low_ld ? mtk_ld(bn + j) : mtk_ld_n(bn + j, g.low_ld - j);
-                            low = mma32(bv, mtk_ld(u + rc * g.rp + j), low);
-                            if (sizeof(T) == 2 && g.low_ld < g.rp) low = mma32(bv, mtk_ld(u + rc * g.rp + g.rp / 2 + j), low);  // B once: both halves of u
+                        auto steps = [&](int j0, auto count) {  // requested together: one round trip
+                            constexpr int C = decltype(count)::value;
+                            mtk_vec<T> uv[C][H], bv[C];
+#pragma unroll
+                            for (int s = 0; s < C; ++s) {
+                                const int j = j0 + s * 2 * V;
+                                const bool in = j + hh_e * V < low_n;
+                                const uint4 w = __builtin_bit_cast(uint4, mtk_ld(in ? bn + j : be));
+                                bv[s] = __builtin_bit_cast(mtk_vec<T>, make_uint4(in ? w.x : 0u, in ? w.y : 0u, in ? w.z : 0u, in ? w.w : 0u));
+#pragma unroll
+                                for (int h = 0; h < H; ++h) uv[s][h] = mtk_ld(ur + h * half + j);
+                            }
+#pragma unroll
+                            for (int s = 0; s < C; ++s)
+#pragma unroll
+                                for (int h = 0; h < H; ++h) low = mma32(bv[s], uv[s][h], low);
+                        };
+                        for (int j0 = 0; j0 < g.r; j0 += 32) {
+                            if (g.r - j0 <= 16) steps(j0, std::integral_constant<int, S / 2>());
+                            else steps(j0, std::integral_constant<int, S>());
                         }
 #pragma unroll
                         for (int q = 0; q < 16; ++q) acc[mt][nt][q] += mine ? low[q] : 0.f;
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
             }
@@ -1077,12 +1098,13 @@ struct Saved {
 struct Shape {
     bool few, blocks;  // blocks: the low-rank product as k-blocks (a model owns a tile's rows on average)
     int kind, BM, BN;  // 0: 256 x 256, 1: 128 x 128, 2: 64 x 64
-    int line, rp, Kp;  // elements of a line; u's row; K in whole lines
+    int line, rp, low_ld, Kp;  // elements of a line; u's row; a row of B_e for the epilogue, in whole 16-byte pieces; K in whole lines
     int64_t MT;
     int nb_n;
     Shape(int64_t M, int N, int K, int r, int E, int dtype) {
         line = 128 / mtk_dtype_size(dtype);
         rp = rank_pad(r, dtype);
+        low_ld = (int)mtk_up(r, 16 / mtk_dtype_size(dtype));
         Kp = (int)mtk_up(K, line);
         // us for K = N = 1024, few rows / 64 x 64 tiles (and some 5 for their k_prep): bf16 256 rows 9.0 / 9.9, 512 rows 13.9 / 9.4, 1,024 rows
         // 26 / 9.3; fp32 256 rows 14 / 26, 512 rows 24 / 26, 1,024 rows 45 / 27
@@ -1102,12 +1124,12 @@ struct Shape {
 // what k_linear reads beside its operands, and their padded copies where they need one
 struct Packed {
     int64_t X, W, F, Bp, bias, owner;  // F: the factors that the shrink multiplies, in whole lines like X
-    Packed(Layout& l, const Shape& sh, int64_t M, int N, int r, int E, int dtype, bool pad_x, bool pad_w) {
+    Packed(Layout& l, const Shape& sh, int64_t M, int N, int r, int E, int dtype, bool pad_x, bool pad_w, bool pad_low) {
         const int64_t z = mtk_dtype_size(dtype);
         X = l.take(!sh.few && pad_x ? M * sh.Kp * z : 0);
         W = l.take(!sh.few && pad_w ? (int64_t)N * sh.Kp * z : 0);
         F = l.take(!sh.few && pad_x ? (int64_t)E * r * sh.Kp * z : 0);
-        Bp = l.take(sh.blocks ? (int64_t)(E + 1) * N * sh.rp * z : 0);
+        Bp = l.take(sh.blocks ? (int64_t)(E + 1) * N * sh.rp * z : pad_low ? (int64_t)E * N * sh.low_ld * z : 0);
         bias = l.take((int64_t)sh.nb_n * sh.BN * 4);
         owner = l.take(sh.blocks ? sh.MT * 4 : 0);
     }
@@ -1122,7 +1144,7 @@ struct ForwardWork {
     Shape sh;
     Packed pk;
     ForwardWork(Layout l, int64_t M, int din, int dout, int r, int E, int dtype, bool pad_x, bool pad_w)
-        : sh(M, dout, din, r, E, dtype), pk(l, sh, M, dout, r, E, dtype, pad_x, pad_w) {
+        : sh(M, dout, din, r, E, dtype), pk(l, sh, M, dout, r, E, dtype, pad_x, pad_w, !sh.few && r != sh.low_ld) {
         bytes = sh.few ? 0 : l.at;
     }
 };
@@ -1131,11 +1153,11 @@ struct BackwardWork {
     Shape sh;
     Packed pk;
     BackwardWork(Layout l, int64_t M, int din, int dout, int r, int E, int dtype, bool relu, bool pad_g)
-        : sh(M, din, dout, r, E, dtype), pk(l, sh, M, din, r, E, dtype, pad_g, true) {  // the weights are turned, so laid out anew
+        : sh(M, din, dout, r, E, dtype), pk(l, sh, M, din, r, E, dtype, pad_g, true, false) {  // the weights are turned, so laid out anew
         const int64_t z = mtk_dtype_size(dtype);
         Bt = l.take((int64_t)E * r * sh.Kp * z);
         Wt = l.take(sh.few ? (int64_t)din * dout * z : 0);  // else pk.W
-        At = l.take(sh.blocks && !sh.few ? 0 : (int64_t)E * r * din * z);
+        At = l.take(sh.blocks && !sh.few ? 0 : (int64_t)E * sh.low_ld * din * z);
         t = l.take(Saved(M, r, dtype).bytes);
         g = l.take(relu ? M * dout * z : 0);
         part[0] = l.take(wgrad_part(M, din, r, E, dtype) * 4);
@@ -1180,7 +1202,7 @@ int launch_linear(LinearArgs& g, T* y, int which, hipStream_t s) {
         MTK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear<T, WR, WC, MW, NT, DX, DW>), hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds));
         st->lds[which] = true;
     }
-    const int64_t per_xcd = cdiv(g.MT * g.nb_n, 8), room = (int64_t)st->cus / 8 * (163840 / G::kLds);
+    const int64_t per_xcd = cdiv(g.MT * g.nb_n, 8), room = (int64_t)st->cus / 8 * G::kRoom;
     k_linear<T, WR, WC, MW, NT, DX, DW><<<(unsigned)(8 * (per_xcd < room ? per_xcd : room)), 64 * G::NW, G::kLds, s>>>(g, y);
     return MTK_OK;
 }
@@ -1205,7 +1227,7 @@ LinearArgs plan_linear(Jobs& jobs, const Shape& sh, const Packed& pk, char* wb, 
     LinearArgs g{};
     g.M = M; g.MT = sh.MT; g.N = N; g.nb_n = sh.nb_n;
     g.nkb = sh.Kp / sh.line; g.nkx = sh.blocks ? sh.rp / sh.line : 0;
-    g.offsets = offsets; g.E = E; g.relu = relu; g.U = u; g.rp = sh.rp;
+    g.offsets = offsets; g.E = E; g.relu = relu; g.U = u; g.rp = sh.rp; g.r = r;
     g.X = x;
     g.x_ld = x_ld * sizeof(T);
     if (!streams(x, x_ld, K, dtype)) {
@@ -1285,7 +1307,11 @@ extern "C" int mtk_adapter_forward(int64_t M, int din, int dout, int r, int E, i
                                       offsets, act);
         if (!sh.blocks) {
             g.low = up;
-            g.low_ld = r;
+            g.low_ld = sh.low_ld;
+            if (r != sh.low_ld) {
+                job_pad(jobs, up, r, (char*)work + wk.pk.Bp, (int64_t)E * dout, r, sh.low_ld, mtk_piece<T>::n);
+                g.low = (char*)work + wk.pk.Bp;
+            }
         }
         const T *sx = (const T*)x, *sf = (const T*)down;
         if (g.X != x) {  // x was padded to whole lines: the shrink reads them too
@@ -1340,9 +1366,9 @@ extern "C" int mtk_adapter_backward(int64_t M, int din, int dout, int r, int E, 
             if (sh.few) job_turn(jobs, W, wb + wk.Wt, dout, din, dout, 1);
             else lin = plan_linear<T>(jobs, sh, wk.pk, wb, M, din, dout, r, E, dtype, graw, dout, (const T*)W, true, nullptr, (const T*)down, t, offsets, 0);
             if (sh.few || !sh.blocks) {
-                job_turn(jobs, down, wb + wk.At, r, din, r, E);
+                job_turn(jobs, down, wb + wk.At, r, din, sh.few ? r : sh.low_ld, E);
                 lin.low = wb + wk.At;
-                lin.low_ld = r;
+                lin.low_ld = sh.low_ld;
             }
         }
         prep<T>(jobs, s);
