@@ -112,19 +112,22 @@ struct ShrinkArgs {
     const float* scales;
     float scale;
     int64_t Mp;  // row stride of uT
+    int turns, tiles;  // workgroups: turns x tiles
 };
 
 // u[row][j] = s_e sum_k x[row][k] F_e[j][k] (F: [E][r][K]); with uT also its transpose, which the factors' gradients multiply.
 // Bound by reading x.  16 x 16 MFMA tiles: RR sets of 16 rows against RT tiles of 16 j, so a rank of 16 wastes nothing; a wave streams its rows
 // straight into fragments, two lines at a time.  KS = 1: a wave has 32 rows to itself, which halves what it reads of F.  KS = 4, for few
-// rows: four waves split the lines of 16 rows, their sums meet in LDS, and gridDim.y workgroups share a tile's models in turn (one model's
-// product is a chain of loads of some microseconds); the first of them clears what no model owns.
+// rows: four waves split the lines of 16 rows, their sums meet in LDS.  g.turns workgroups share a tile's models in turn (one model's product is
+// a chain of loads of some microseconds); the first of them clears what no model owns.
+template <int RT, int KS> constexpr int kShrinkLds = KS > 1 ? KS * RT * 4 * 64 : 1;  // floats
 template <typename T, int RT, int KS>
-__global__ __launch_bounds__(256) void k_shrink(ShrinkArgs g, int j0, const T* __restrict__ x, const T* __restrict__ F, T* __restrict__ u, T* __restrict__ uT) {
+__device__ void shrink_body(const ShrinkArgs& g, unsigned block, int j0, const T* __restrict__ x, const T* __restrict__ F, T* __restrict__ u, T* __restrict__ uT, float* lds) {
     constexpr int V = mtk_piece<T>::n, KB = kLine<T>, RR = KS > 1 ? 1 : 2;
-    __shared__ float part[KS > 1 ? KS : 1][KS > 1 ? RT * 4 : 1][KS > 1 ? 64 : 1];
+    float (*part)[KS > 1 ? RT * 4 : 1][64] = reinterpret_cast<float (*)[KS > 1 ? RT * 4 : 1][64]>(lds);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, q = lane >> 4;
-    const int64_t m0 = ((int64_t)blockIdx.x * (4 / KS) + (KS > 1 ? 0 : wave)) * 16 * RR;
+    const int my_turn = block / (unsigned)g.tiles;  // neighbours go to different XCDs, so the turns must not alternate
+    const int64_t m0 = ((int64_t)(block % (unsigned)g.tiles) * (4 / KS) + (KS > 1 ? 0 : wave)) * 16 * RR;
     if (m0 >= g.M) return;
     const int64_t end = m0 + 16 * RR < g.M ? m0 + 16 * RR : g.M;
     const T* xr[RR];
@@ -142,7 +145,7 @@ __global__ __launch_bounds__(256) void k_shrink(ShrinkArgs g, int j0, const T* _
             in[p] = m0 + p * 16 + li >= a && m0 + p * 16 + li < b;
             any[p] |= in[p];
         }
-        if (KS > 1 && turn++ % (int)gridDim.y != (int)blockIdx.y) continue;
+        if (turn++ % g.turns != my_turn) continue;
 #pragma unroll
         for (int p = 0; p < RR; ++p) mine[p] |= in[p];
         const T* fr[RT];
@@ -219,7 +222,7 @@ __global__ __launch_bounds__(256) void k_shrink(ShrinkArgs g, int j0, const T* _
     if (KS > 1 && wave > 0) return;
 #pragma unroll
     for (int p = 0; p < RR; ++p) {
-        if (!(mine[p] || ((KS == 1 || blockIdx.y == 0) && !any[p]))) continue;  // a row without a model: zeros
+        if (!(mine[p] || (my_turn == 0 && !any[p]))) continue;  // a row without a model: zeros
         const int64_t at = m0 + p * 16 + li;  // D[j][record]: lane & 15 -> record, j = 4 (lane >> 4) + register
         struct __attribute__((aligned(4 * sizeof(T)), may_alias)) Quad { T v[4]; };
         constexpr bool kSplit = sizeof(T) == 2;
@@ -971,13 +974,13 @@ struct Jobs {
 constexpr int kPadPieces = 1024;  // 16-byte pieces of a PAD workgroup
 
 template <typename T>
-__global__ __launch_bounds__(256) void k_prep(Jobs jobs) {
+__device__ void prep_body(const Jobs& jobs, int block, float* lds) {
     constexpr int V = mtk_piece<T>::n;
-    __shared__ T tile[32][33];
+    T (*tile)[33] = reinterpret_cast<T (*)[33]>(lds);
     int q = 0;
-    while (q + 1 < jobs.n && (int)blockIdx.x >= jobs.job[q + 1].first) ++q;
+    while (q + 1 < jobs.n && block >= jobs.job[q + 1].first) ++q;
     const Job& j = jobs.job[q];
-    const int64_t blk = blockIdx.x - j.first;
+    const int64_t blk = block - j.first;
     if (j.type == JOB_TURN) {
         const int nc = (j.C + 31) / 32, nr = (j.ldo + 31) / 32;
         const int64_t bat = blk / (nc * nr);
@@ -1015,6 +1018,19 @@ __global__ __launch_bounds__(256) void k_prep(Jobs jobs) {
     }
 }
 
+template <typename T>
+__global__ __launch_bounds__(256) void k_prep(Jobs jobs) {
+    __shared__ float lds[32 * 33];
+    prep_body<T>(jobs, (int)blockIdx.x, lds);
+}
+// the shrink, in front of it what does not depend on it and it does not depend on: the jobs' workgroups run under its own
+template <typename T, int RT, int KS>
+__global__ __launch_bounds__(256) void k_shrink(ShrinkArgs g, Jobs jobs, int j0, const T* __restrict__ x, const T* __restrict__ F, T* __restrict__ u, T* __restrict__ uT) {
+    __shared__ float lds[kShrinkLds<RT, KS> > 32 * 33 ? kShrinkLds<RT, KS> : 32 * 33];
+    if ((int)blockIdx.x < jobs.blocks) prep_body<T>(jobs, (int)blockIdx.x, lds);
+    else shrink_body<T, RT, KS>(g, blockIdx.x - (unsigned)jobs.blocks, j0, x, F, u, uT, lds);
+}
+
 // g = dy, 0 where y <= 0
 template <typename T>
 __global__ __launch_bounds__(256) void k_relu_grad(int64_t n, const T* __restrict__ y, const T* __restrict__ dy, T* __restrict__ gz) {
@@ -1041,17 +1057,21 @@ int wgrad_chunk(int64_t M, int D, int dtype) {
 int64_t wgrad_part(int64_t M, int D, int r, int E, int dtype) { return (cdiv(M, wgrad_chunk(M, D, dtype)) + E) * mtk_up(r, kRankT) * D; }
 
 template <typename T, int RT>
-void shrink_launch(const ShrinkArgs& g, int j0, const T* x, const T* F, T* u, T* uT, hipStream_t s) {
+void shrink_launch(ShrinkArgs g, const Jobs& jobs, int j0, const T* x, const T* F, T* u, T* uT, hipStream_t s) {
     // 32 rows a wave fill the chip from some 16,384 rows on; below, four waves split 16 rows
-    if (g.M >= 16384) k_shrink<T, RT, 1><<<(unsigned)cdiv(g.M, 128), 256, 0, s>>>(g, j0, x, F, u, uT);
-    else k_shrink<T, RT, 4><<<dim3((unsigned)cdiv(g.M, 16), (unsigned)(g.M >= 2048 ? 1 : (g.E < 16 ? g.E : 16))), 256, 0, s>>>(g, j0, x, F, u, uT);
+    const int turns = g.M >= 4096 ? 2 : g.M >= 2048 ? 4 : 16;
+    g.turns = g.E < turns ? g.E : turns;
+    g.tiles = (int)cdiv(g.M, g.M >= 16384 ? 128 : 16);
+    const unsigned grid = (unsigned)(g.tiles * g.turns + jobs.blocks);
+    if (g.M >= 16384) k_shrink<T, RT, 1><<<grid, 256, 0, s>>>(g, jobs, j0, x, F, u, uT);
+    else k_shrink<T, RT, 4><<<grid, 256, 0, s>>>(g, jobs, j0, x, F, u, uT);
 }
 template <typename T>
-void shrink(const ShrinkArgs& g, const T* x, const T* F, T* u, T* uT, hipStream_t s) {
-    for (int j0 = 0; j0 < g.r; j0 += 64) {
-        if (g.r - j0 > 32) shrink_launch<T, 4>(g, j0, x, F, u, uT, s);
-        else if (g.r - j0 > 16) shrink_launch<T, 2>(g, j0, x, F, u, uT, s);
-        else shrink_launch<T, 1>(g, j0, x, F, u, uT, s);
+void shrink(const ShrinkArgs& g, Jobs jobs, const T* x, const T* F, T* u, T* uT, hipStream_t s) {
+    for (int j0 = 0; j0 < g.r; j0 += 64, jobs.n = jobs.blocks = 0) {
+        if (g.r - j0 > 32) shrink_launch<T, 4>(g, jobs, j0, x, F, u, uT, s);
+        else if (g.r - j0 > 16) shrink_launch<T, 2>(g, jobs, j0, x, F, u, uT, s);
+        else shrink_launch<T, 1>(g, jobs, j0, x, F, u, uT, s);
     }
 }
 template <typename T>
@@ -1296,9 +1316,9 @@ extern "C" int mtk_adapter_forward(int64_t M, int din, int dout, int r, int E, i
         const Shape& sh = wk.sh;
         T* u = (T*)((char*)saved + sv.u);
         T* uT = keep && sizeof(T) == 2 ? (T*)((char*)saved + sv.uT) : nullptr;
-        ShrinkArgs sa{M, din, r, sh.rp, E, x_ld, offsets, scales, (float)scale, sv.Mp};
+        ShrinkArgs sa{M, din, r, sh.rp, E, x_ld, offsets, scales, (float)scale, sv.Mp, 1, 1};
         if (sh.few) {
-            shrink<T>(sa, (const T*)x, (const T*)down, u, uT, s);
+            shrink<T>(sa, Jobs(), (const T*)x, (const T*)down, u, uT, s);
             linear_few<T>(FewArgs{M, x_ld, dout, din, r, sh.rp, E, act, offsets}, (const T*)x, (const T*)W, (const T*)bias, u, (const T*)up, (T*)y, s);
             return;
         }
@@ -1313,16 +1333,17 @@ extern "C" int mtk_adapter_forward(int64_t M, int din, int dout, int r, int E, i
                 g.low = (char*)work + wk.pk.Bp;
             }
         }
-        const T *sx = (const T*)x, *sf = (const T*)down;
-        if (g.X != x) {  // x was padded to whole lines: the shrink reads them too
+        // x padded to whole lines: the shrink reads them too (20,011 rows of 517 in fp16: 11 us for the lines and 13 for the shrink; 33 for
+        // both in one launch from rows as they are).  Else its launch takes the jobs along.
+        if (g.X != x) {
             job_pad(jobs, down, din, (char*)work + wk.pk.F, (int64_t)E * r, din, sh.Kp, mtk_piece<T>::n);
-            sx = (const T*)g.X;
-            sf = (const T*)((char*)work + wk.pk.F);
             sa.K = sh.Kp;
             sa.x_ld = sh.Kp;
+            prep<T>(jobs, s);
+            shrink<T>(sa, Jobs(), (const T*)g.X, (const T*)((char*)work + wk.pk.F), u, uT, s);
+        } else {
+            shrink<T>(sa, jobs, (const T*)x, (const T*)down, u, uT, s);
         }
-        prep<T>(jobs, s);
-        shrink<T>(sa, sx, sf, u, uT, s);
         rc = linear<T>(sh, g, (T*)y, s);
     });
     if (rc) return rc;
@@ -1373,7 +1394,7 @@ extern "C" int mtk_adapter_backward(int64_t M, int din, int dout, int r, int E, 
         }
         prep<T>(jobs, s);
         if (dx || ddown)
-            shrink<T>(ShrinkArgs{M, gk, r, sh.rp, E, gk, offsets, scales, (float)scale, sv.Mp}, g, (const T*)(wb + wk.Bt), t, ddown && sizeof(T) == 2 ? tT : nullptr, s);
+            shrink<T>(ShrinkArgs{M, gk, r, sh.rp, E, gk, offsets, scales, (float)scale, sv.Mp, 1, 1}, Jobs(), g, (const T*)(wb + wk.Bt), t, ddown && sizeof(T) == 2 ? tT : nullptr, s);
         if (dx) {
             if (sh.few) linear_few<T>(FewArgs{M, dout, din, dout, r, sh.rp, E, 0, offsets}, g, (const T*)(wb + wk.Wt), nullptr, t, (const T*)(wb + wk.At), (T*)dx, s);
             else rc = linear<T>(sh, lin, (T*)dx, s);
