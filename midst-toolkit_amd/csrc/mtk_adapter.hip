@@ -61,16 +61,6 @@ constexpr int kRankT = 16;  // rows of u^T come in whole 16s
 
 // The models that own rows [at, end): each call yields one (e, first row, behind its last row).  Whatever the offsets hold, every step moves
 // forward and stays inside [at, end), so no other row is named and the walk ends.
-// One lane's search, by bisection:
-__device__ __forceinline__ int owner_of(const int32_t* off, int E, int64_t at) {  // number of offsets <= at, less one
-    int lo = 0, hi = E + 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (off[mid] <= at) lo = mid + 1;
-        else hi = mid;
-    }
-    return lo - 1;
-}
 // A wave's walk: its lanes hold an offset each, so a step is a ballot and not a chain of loads (beyond 64 offsets, one load a 64).
 struct Owners {
     const int32_t* off;
@@ -81,13 +71,17 @@ struct Owners {
         const int lane = __lane_id();
         held = lane <= E ? off[lane] : 0x7fffffff;
     }
+    __device__ int behind(int64_t row) const {  // offsets <= row
+        int lo = __popcll(__ballot(held <= row));
+        for (int i = 64; i <= E && lo == i; i += 64) {
+            const int k = i + (int)__lane_id();
+            lo += __popcll(__ballot((k <= E ? off[k] : 0x7fffffff) <= row));
+        }
+        return lo;
+    }
     __device__ bool next(int& e, int64_t& a, int64_t& b) {
         while (at < end) {
-            int lo = __popcll(__ballot(held <= at));
-            for (int i = 64; i <= E && lo == i; i += 64) {
-                const int k = i + (int)__lane_id();
-                lo += __popcll(__ballot((k <= E ? off[k] : 0x7fffffff) <= at));
-            }
+            const int lo = behind(at);
             if (lo > E) return false;  // behind the last model's rows
             int64_t to = lo < 64 ? __builtin_amdgcn_readlane(held, lo) : __builtin_amdgcn_readfirstlane(off[lo]);
             to = to > at ? to : at + 1;
@@ -103,6 +97,26 @@ struct Owners {
     }
 };
 
+// The models of a row tile: the first, how many (0: none, or too many for a run of k-blocks each), whether some rows are not the first's, whether
+// there are too many.
+constexpr int kTileModels = 8;
+struct TileModels {
+    int e, count, ranged, many;
+    __device__ int packed() const { return e | count << 16 | ranged << 24 | many << 25; }
+    __device__ static TileModels of(int packed) { return TileModels{packed & 0xffff, packed >> 16 & 0xff, packed >> 24 & 1, packed >> 25 & 1}; }
+    // Of rows first .. first + rows - 1 of M.  Whatever the offsets hold, the models named are below E, and all who ask get the same.
+    __device__ static TileModels of_tile(const Owners& own, int64_t first, int rows, int64_t M, int E) {
+        const int64_t last = (first + rows < M ? first + rows : M) - 1;
+        const int e0 = own.behind(first) - 1, e1 = own.behind(last) - 1;  // -1: before the first offset, E: behind the last (no model)
+        TileModels m = {e0 < 0 ? 0 : e0, 0, e0 != e1, 0};
+        m.count = (e1 < E ? e1 : E - 1) - m.e + 1;
+        if (m.count < 0) m.count = 0;
+        if (m.count > kTileModels) m.count = 0, m.many = 1;
+        if (m.count == 0) m.e = m.ranged = 0;
+        return m;
+    }
+};
+
 // ------------------------------------------------------------------------------------------------------------------ shrink
 struct ShrinkArgs {
     int64_t M;
@@ -112,6 +126,8 @@ struct ShrinkArgs {
     const float* scales;
     float scale;
     int64_t Mp;  // row stride of uT
+    void* pairs;  // with BM > 0: the rows of tiles that models share, once a model (see k_linear)
+    int BM;
     int turns, tiles;  // workgroups: turns x tiles
 };
 
@@ -135,6 +151,9 @@ __device__ void shrink_body(const ShrinkArgs& g, unsigned block, int j0, const T
     for (int p = 0; p < RR; ++p) xr[p] = x + (m0 + p * 16 + li < g.M ? m0 + p * 16 + li : g.M - 1) * g.x_ld + q * V;
     f32x4 keep[RR][RT] = {};
     bool mine[RR] = {}, any[RR] = {};  // this lane's rows: computed here / owned by any model
+    int who[RR];
+#pragma unroll
+    for (int p = 0; p < RR; ++p) who[p] = -1;
     Owners own(g.offsets, g.E, m0, end);
     int e, turn = 0;
     int64_t a, b;
@@ -144,6 +163,7 @@ __device__ void shrink_body(const ShrinkArgs& g, unsigned block, int j0, const T
         for (int p = 0; p < RR; ++p) {
             in[p] = m0 + p * 16 + li >= a && m0 + p * 16 + li < b;
             any[p] |= in[p];
+            who[p] = in[p] ? e : who[p];
         }
         if (turn++ % g.turns != my_turn) continue;
 #pragma unroll
@@ -220,6 +240,9 @@ __device__ void shrink_body(const ShrinkArgs& g, unsigned block, int j0, const T
                 for (int i = 0; i < 4; ++i) keep[p][t][i] = in[p] ? s * acc[p][t][i] : keep[p][t][i];
     }
     if (KS > 1 && wave > 0) return;
+    TileModels tm = {};
+    const int tile = g.BM > 0 ? (int)(m0 / g.BM) : 0;  // 64 rows or more: all of this wave's are in it
+    if (g.BM > 0) tm = TileModels::of_tile(own, (int64_t)tile * g.BM, g.BM, g.M, g.E);
 #pragma unroll
     for (int p = 0; p < RR; ++p) {
         if (!(mine[p] || (my_turn == 0 && !any[p]))) continue;  // a row without a model: zeros
@@ -242,6 +265,13 @@ __device__ void shrink_body(const ShrinkArgs& g, unsigned block, int j0, const T
             if (at < g.M && j < half) {
                 *reinterpret_cast<Quad*>(ur + j) = o;
                 if (kSplit) *reinterpret_cast<Quad*>(ur + half + j) = l;
+                if (tm.ranged)
+                    for (int i = 0; i < tm.count; ++i) {
+                        T* pr = (T*)g.pairs + ((int64_t)(tile + tm.e + i) * g.BM + (at - (int64_t)tile * g.BM)) * g.rp + j;
+                        const bool its = tm.e + i == who[p];
+                        *reinterpret_cast<Quad*>(pr) = its ? o : Quad{};
+                        if (kSplit) *reinterpret_cast<Quad*>(pr + half) = its ? l : Quad{};
+                    }
             }
             if (uT && at < g.Mp)  // mtk_up(r, 64) rows of Mp
 #pragma unroll
@@ -254,6 +284,12 @@ __device__ void shrink_body(const ShrinkArgs& g, unsigned block, int j0, const T
             for (int j = j0 + RT * 16 + q * 4; j < half; j += 16) {
                 *reinterpret_cast<Quad*>(ur + j) = Quad{};
                 if (kSplit) *reinterpret_cast<Quad*>(ur + half + j) = Quad{};
+                if (tm.ranged)
+                    for (int i = 0; i < tm.count; ++i) {
+                        T* pr = (T*)g.pairs + ((int64_t)(tile + tm.e + i) * g.BM + (at - (int64_t)tile * g.BM)) * g.rp + j;
+                        *reinterpret_cast<Quad*>(pr) = Quad{};
+                        if (kSplit) *reinterpret_cast<Quad*>(pr + half) = Quad{};
+                    }
             }
     }
 }
@@ -264,18 +300,24 @@ __device__ void shrink_body(const ShrinkArgs& g, unsigned block, int j0, const T
 // k_linear, for more than a few rows: persistent workgroups walk tiles of BM rows x BN features; the k-blocks of ALL their tiles form one
 // stream of LDS-DMA (DX buffers for rows, DW for weights), so a tile's epilogue runs with the next tile's first blocks in flight.
 // The low-rank product is the last k-blocks of a tile: rows of u against rows of B_e (both zero behind the rank), the same
-// instructions through the same buffers.  That needs one model per tile; a tile with several (or none) takes a block of zeros there and a
-// several-model tile adds its products in the epilogue, made per model and selected by row.  With fewer rows a model than a tile
-// has (nkx = 0) all tiles do.
-// The stream wants whole, 16-byte aligned lines: k_prep pads what is not, and lays out B, the bias in fp32 and the tiles' models.
+// instructions through the same buffers.  A tile that several models share, or some rows of which have none, takes these blocks once
+// per model e from the tile's pair (t, e) of rows, in which the other models' are zero.  Walking the tiles, each step to the next pair raises t, e or
+// both, so t + e numbers the pairs.  Zero times B_e is zero while B_e is finite; a shared tile with one that is not is made once more, without
+// the stream.  There, in tiles of more than kTileModels models, and (nkx = 0) with far fewer rows a model than a tile has, the
+// low-rank products are made in the epilogue, per model, and selected by row.
+// The stream wants whole, 16-byte aligned lines: k_prep pads what is not, and lays out B, the bias in fp32, the tiles' models and which B_e
+// hold infinities or NaN.
 struct LinearArgs {
     int64_t M, MT;        // rows, row tiles
     int N, nb_n;          // features, feature tiles
     int nkb, nkx;         // k-blocks of the shared and of the low-rank product
     int64_t x_ld, w_ld;   // row strides, in bytes
-    const void *X, *W, *U, *Bp;  // U [M][nkx lines], Bp [E + 1][N][nkx lines], model E: zeros
+    const void *X, *W, *U, *Bp;  // U [M][nkx lines], Bp [E][N][nkx lines]
+    const void* pairs;    // [MT + E][BM][nkx lines]
+    void* Y;
     const float* bias;    // [nb_n * BN]
-    const int32_t* owner; // [MT] the tile's model; E: none; -1: several
+    const int32_t* owner; // [MT] TileModels
+    const int32_t* odd;   // [E] not 0: B_e holds infinities or NaN
     const int32_t* offsets;
     int E, relu;
     const void* low;      // [E][N][low_ld] B_e for the epilogue, in whole pieces, zeros behind the rank
@@ -294,6 +336,15 @@ template <int WR, int WC_, int MW, int NT, int DX_, int DW_> struct Geo {
 
 extern __shared__ __attribute__((aligned(16))) unsigned char ad_smem[];
 
+// The arguments, read anew where they are used: the work between two tiles needs them all, and kept in scalar registers over the k-blocks (or
+// spilled to lanes of vector registers) they would be paid for in every one.
+typedef const __attribute__((address_space(4))) LinearArgs KernelArgs;
+__device__ __forceinline__ KernelArgs& linear_args() {
+    auto p = __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(KernelArgs*)p;
+}
+
 // a uniform value through the scalar cache: a vector load would wait for all the DMA requested before it
 __device__ __forceinline__ int scalar_load(const int32_t* p) {
     int v;
@@ -302,7 +353,7 @@ __device__ __forceinline__ int scalar_load(const int32_t* p) {
 }
 
 template <typename T, int WR, int WC, int MW, int NT, int DX, int DW>
-__global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)) void k_linear(LinearArgs g, T* __restrict__ y) {
+__global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)) void k_linear(LinearArgs) {  // (linear_args)
     typedef Geo<WR, WC, MW, NT, DX, DW> G;
     constexpr int V = mtk_piece<T>::n, kWBase = DX * G::kTileX;
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
@@ -311,11 +362,10 @@ __global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)
     // workgroups go round-robin over the 8 XCDs: each XCD takes a contiguous eighth of the tiles (features fastest), so a row tile's
     // feature tiles run side by side on one XCD's L2 and every XCD has work
     const int xcd = blockIdx.x & 7, wq = blockIdx.x >> 3, wstride = gridDim.x >> 3;
-    const int tiles = (int)g.MT * g.nb_n, per = (tiles + 7) / 8, first = xcd * per;
+    KernelArgs& first_args = linear_args();
+    const int nb_n = first_args.nb_n, tiles = (int)first_args.MT * nb_n, per = (tiles + 7) / 8, first = xcd * per;
     const int slots = tiles - first < per ? tiles - first : per;
     if (wq >= slots) return;
-    const int nk = g.nkb + g.nkx;
-
     // DMA of one 8-row piece (64 lanes x 16 bytes): lane -> row lane >> 3, piece slot lane & 7.  The LDS image is linear in the lane, so the
     // bank swizzle (slot s of row r holds piece s ^ ((r >> 1) & 7)) is applied to the global address.  Rows behind the last are
     // clamped: they are read again, never stored.  M0 (the LDS address) is written with every piece; the compiler puts nothing there.
@@ -334,15 +384,25 @@ __global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)
     };
     // The common step of a cursor is an addition, a wrap and a countdown: with one or two waves on a SIMD, scalar work between two
     // barriers is time.
-    const unsigned lo_ld = (unsigned)g.nkx * 128, x_ld = (unsigned)g.x_ld, w_ld = (unsigned)g.w_ld;
     const unsigned x_dst0 = (unsigned)(wv * G::XPW * 1024), w_dst0 = (unsigned)(kWBase + wv * G::WPW * 1024);
     unsigned x_dst = x_dst0, w_dst = w_dst0;
     int cx_slot = wq, cw_slot = wq, x_left = 0, w_left = 0;  // blocks left at the source
     int x_low = 1, w_low = 1;  // 1: the source is the low-rank lines (an int: a bool that loops is kept as a lane mask, and its selects in vector registers)
     const unsigned char *xb = nullptr, *wb = nullptr;
     unsigned xoff[G::XPW], woff[G::WPW];
+    int x_more = 0, w_more = 0;  // models of the tile still to come
     auto x_source = [&]() {  // the next source of the row cursor; none: never counts down again
-        x_low = x_low == 0 && g.nkx > 0 ? 1 : 0;
+        KernelArgs& g = linear_args();
+        const unsigned lo_ld = (unsigned)g.nkx * 128;
+        if (x_more > 0) {  // from behind this pair's lines to the next pair's
+            --x_more;
+            x_left = g.nkx;
+            xb += (int64_t)(G::BM - 1) * lo_ld;
+            return;
+        }
+        TileModels m = {0, 0, 0, 0};
+        if (x_low == 0 && g.nkx > 0) m = TileModels::of(scalar_load(g.owner + (first + cx_slot) / nb_n));
+        x_low = m.count > 0 ? 1 : 0;
         if (x_low == 0) {
             if (x_left < 0) cx_slot += wstride;
             if (cx_slot >= slots) {
@@ -350,22 +410,34 @@ __global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)
                 return;
             }
         }
-        const int64_t m0 = (int64_t)((first + cx_slot) / g.nb_n) * G::BM;
+        const int mt = (first + cx_slot) / nb_n;
+        const int64_t m0 = (int64_t)mt * G::BM;
         const int rows = g.M - m0 < G::BM ? (int)(g.M - m0) : G::BM;
         unsigned ld;
         if (x_low) {
             x_left = g.nkx;
-            xb = (const unsigned char*)g.U + m0 * lo_ld;
+            x_more = m.count - 1;
+            xb = m.ranged ? (const unsigned char*)g.pairs + (int64_t)(mt + m.e) * G::BM * lo_ld : (const unsigned char*)g.U + m0 * lo_ld;
             ld = lo_ld;
         } else {
             x_left = g.nkb;
             xb = (const unsigned char*)g.X + m0 * g.x_ld;
-            ld = x_ld;
+            ld = (unsigned)g.x_ld;
         }
         offsets(xoff, G::XPW, wv * G::XPW, rows, ld);
     };
     auto w_source = [&]() {
-        w_low = w_low == 0 && g.nkx > 0 ? 1 : 0;
+        KernelArgs& g = linear_args();
+        const unsigned lo_ld = (unsigned)g.nkx * 128;
+        if (w_more > 0) {  // from behind this model's lines to the next model's
+            --w_more;
+            w_left = g.nkx;
+            wb += (int64_t)(g.N - 1) * lo_ld;
+            return;
+        }
+        TileModels m = {0, 0, 0, 0};
+        if (w_low == 0 && g.nkx > 0) m = TileModels::of(scalar_load(g.owner + (first + cw_slot) / nb_n));
+        w_low = m.count > 0 ? 1 : 0;
         if (w_low == 0) {
             if (w_left < 0) cw_slot += wstride;
             if (cw_slot >= slots) {
@@ -373,19 +445,18 @@ __global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)
                 return;
             }
         }
-        const int id = first + cw_slot, mt = id / g.nb_n, n0 = (id - mt * g.nb_n) * G::BN;
+        const int id = first + cw_slot, mt = id / nb_n, n0 = (id - mt * nb_n) * G::BN;
         const int rows = g.N - n0 < G::BN ? g.N - n0 : G::BN;
         unsigned ld;
         if (w_low) {
-            int e = scalar_load(g.owner + mt);
-            e = e < 0 || e > g.E ? g.E : e;
             w_left = g.nkx;
-            wb = (const unsigned char*)g.Bp + ((int64_t)e * g.N + n0) * lo_ld;
+            w_more = m.count - 1;
+            wb = (const unsigned char*)g.Bp + ((int64_t)m.e * g.N + n0) * lo_ld;
             ld = lo_ld;
         } else {
             w_left = g.nkb;
             wb = (const unsigned char*)g.W + (int64_t)n0 * g.w_ld;
-            ld = w_ld;
+            ld = (unsigned)g.w_ld;
         }
         offsets(woff, G::WPW, wv * G::WPW, rows, ld);
     };
@@ -441,6 +512,25 @@ __global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)
     // and the DMA requests behind it ride under them.  After the barrier of block c a wave requests its pieces of weight block c + DW,
     // THEN of row block c + DX (DX >= DW).  Loads return in order, so at the end of block c all but the kYounger pieces requested after
     // weight block c + 1 (row block c + 1 is older still) done means that block c + 1 has landed.
+    // the accumulators start from the bias, through the SCALAR cache: vector loads here would queue behind the DMA in flight
+    auto start = [&](int n0) {
+        const float* bp = linear_args().bias + n0 + wc * G::WN;
+#pragma unroll
+        for (int h = 0; h < 2 * NT; ++h) {  // 16 features at a time: more would spill scalar registers
+            f32x8 b0, b1;
+            asm volatile("s_load_dwordx8 %0, %2, 0x0\n\ts_load_dwordx8 %1, %2, 0x20\n\ts_waitcnt lgkmcnt(0)" : "=&s"(b0), "=&s"(b1) : "s"(bp + h * 16) : "memory");
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float v0 = hh ? b0[4 + j] : b0[j], v1 = hh ? b1[4 + j] : b1[j];
+#pragma unroll
+                for (int a = 0; a < MW; ++a) {
+                    acc[a][h >> 1][8 * (h & 1) + j] = v0;
+                    acc[a][h >> 1][8 * (h & 1) + 4 + j] = v1;
+                }
+            }
+        }
+    };
+
     Frags F0, F1;
     x_source();
     w_source();
@@ -459,26 +549,12 @@ __global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)
     int xi = 0, wi = 0;   // buffers of the block being consumed
     bool x_tail = false;  // the previous block's tail requested row pieces after its weight pieces
     for (int slot = wq; slot < slots; slot += wstride) {
-        const int id = first + slot, mtile = id / g.nb_n, n0 = (id - mtile * g.nb_n) * G::BN;
+        const int id = first + slot, mtile = id / nb_n, n0 = (id - mtile * nb_n) * G::BN;
         const int64_t m0 = (int64_t)mtile * G::BM;
-        // the accumulators start from the bias, through the SCALAR cache: vector loads here would queue behind the DMA in flight
-        {
-            const float* bp = g.bias + n0 + wc * G::WN;
-#pragma unroll
-            for (int h = 0; h < 2 * NT; ++h) {  // 16 features at a time: more would spill scalar registers
-                f32x8 b0, b1;
-                asm volatile("s_load_dwordx8 %0, %2, 0x0\n\ts_load_dwordx8 %1, %2, 0x20\n\ts_waitcnt lgkmcnt(0)" : "=&s"(b0), "=&s"(b1) : "s"(bp + h * 16) : "memory");
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float v0 = hh ? b0[4 + j] : b0[j], v1 = hh ? b1[4 + j] : b1[j];
-#pragma unroll
-                    for (int a = 0; a < MW; ++a) {
-                        acc[a][h >> 1][8 * (h & 1) + j] = v0;
-                        acc[a][h >> 1][8 * (h & 1) + 4 + j] = v1;
-                    }
-                }
-            }
-        }
+        KernelArgs& ga = linear_args();
+        const int tm = ga.nkx ? scalar_load(ga.owner + mtile) : 0;
+        const int nk = ga.nkb + ga.nkx * TileModels::of(tm).count;
+        start(n0);
         read_frags(F0, xi, wi, 0);
         for (int kb = 0; kb < nk; ++kb) {
             read_frags(F1, xi, wi, 1);
@@ -520,14 +596,40 @@ __global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)
         int lane_e = lane;
         asm volatile("" : "+v"(lane_e));
         const int li_e = lane_e & 31, hh_e = lane_e >> 5;
-        if (g.low && (!g.nkx || scalar_load(g.owner + mtile) < 0)) {  // several models in this tile
+        KernelArgs& g = linear_args();
+        T* const __restrict__ y = (T*)g.Y;
+        int apart = !g.nkx || TileModels::of(tm).many;  // the low-rank products are still to come
+        if (TileModels::of(tm).ranged) {
+            int odd = 0;
+            for (int i = 0; i < TileModels::of(tm).count; ++i) odd |= scalar_load(g.odd + TileModels::of(tm).e + i);
+            if (odd) {  // 0 x inf has been in it: once more, straight from memory, the same products in the same order
+                apart = 1;
+                start(n0);
+#pragma unroll 1
+                for (int kp = hh_e * 16; kp < g.nkb * 128; kp += 32) {
+                    Frags f;
+#pragma unroll
+                    for (int q = 0; q < MW; ++q) {
+                        const int64_t row = m0 + (wr * MW + q) * 32 + li_e;
+                        f.x[q] = mtk_ld((const T*)((const char*)g.X + (row < g.M ? row : g.M - 1) * g.x_ld + kp));
+                    }
+#pragma unroll
+                    for (int q = 0; q < NT; ++q) {
+                        const int n = n0 + wc * G::WN + q * 32 + li_e;
+                        f.w[q] = mtk_ld((const T*)((const char*)g.W + (int64_t)(n < g.N ? n : g.N - 1) * g.w_ld + kp));
+                    }
+                    mma_all(f);
+                }
+            }
+        }
+        if (g.low && apart) {
             const int64_t w0 = m0 + wr * MW * 32, w1 = w0 + MW * 32;
             Owners own(g.offsets, g.E, w0, w1 < g.M ? w1 : g.M);
             int e;
             int64_t a, b;
             const T* u = (const T*)g.U;
-            constexpr int H = sizeof(T) == 2 ? 2 : 1, S = 32 / (2 * V);  // halves of u; steps of 32 values of the rank
-            const int half = g.rp / H, low_n = g.low_ld < half ? g.low_ld : half;  // B_e's values, once
+            constexpr int S = 32 / (2 * V);  // steps of 32 values of the rank
+            const int half = sizeof(T) == 2 ? g.rp / 2 : g.rp, low_n = g.low_ld < half ? g.low_ld : half;  // B_e's values, once
             while (own.next(e, a, b)) {
                 const T* be = (const T*)g.low + (int64_t)e * g.N * g.low_ld + hh_e * V;
 #pragma unroll
@@ -540,30 +642,27 @@ __global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)
                     for (int nt = 0; nt < NT; ++nt) {
                         const int n = n0 + wc * G::WN + nt * 32 + li_e;
                         const T* bn = be + (int64_t)(n < g.N ? n : g.N - 1) * g.low_ld;
-                        f32x16 low = {};
-                        auto steps = [&](int j0, auto count) {  // requested together: one round trip
+                        f32x16 low = acc[mt][nt];
+                        auto steps = [&](int j0, int h, auto count) {  // requested together: one round trip
                             constexpr int C = decltype(count)::value;
-                            mtk_vec<T> uv[C][H], bv[C];
+                            mtk_vec<T> uv[C], bv[C];
 #pragma unroll
                             for (int s = 0; s < C; ++s) {
                                 const int j = j0 + s * 2 * V;
                                 const bool in = j + hh_e * V < low_n;
                                 const uint4 w = __builtin_bit_cast(uint4, mtk_ld(in ? bn + j : be));
                                 bv[s] = __builtin_bit_cast(mtk_vec<T>, make_uint4(in ? w.x : 0u, in ? w.y : 0u, in ? w.z : 0u, in ? w.w : 0u));
-#pragma unroll
-                                for (int h = 0; h < H; ++h) uv[s][h] = mtk_ld(ur + h * half + j);
+                                uv[s] = mtk_ld(ur + h + j);
                             }
 #pragma unroll
-                            for (int s = 0; s < C; ++s)
-#pragma unroll
-                                for (int h = 0; h < H; ++h) low = mma32(bv[s], uv[s][h], low);
+                            for (int s = 0; s < C; ++s) low = mma32(bv[s], uv[s], low);
                         };
-                        for (int j0 = 0; j0 < g.r; j0 += 32) {
-                            if (g.r - j0 <= 16) steps(j0, std::integral_constant<int, S / 2>());
-                            else steps(j0, std::integral_constant<int, S>());
-                        }
+#pragma unroll 1
+                        for (int h = 0; h < g.rp; h += half)
+#pragma unroll 1
+                            for (int j0 = 0; j0 < g.r; j0 += 32) steps(j0, h, std::integral_constant<int, S>());
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) acc[mt][nt][q] += mine ? low[q] : 0.f;
+                        for (int q = 0; q < 16; ++q) acc[mt][nt][q] = mine ? low[q] : acc[mt][nt][q];
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
@@ -951,17 +1050,18 @@ __global__ __launch_bounds__(256) void k_wgrad_join(WgradBoth<T> both) {
 
 // ------------------------------------------------------------------------------------------------------------------ helpers
 // k_prep: everything that has to be laid out before the products, in one launch.  A job owns consecutive workgroups.
-enum { JOB_TURN, JOB_PAD, JOB_BIAS, JOB_OWNER };
+enum { JOB_TURN, JOB_PAD, JOB_BIAS, JOB_OWNER, JOB_ODD };
 struct Job {
     int type, first;      // first workgroup
     const void* src;
     void* dst;
     int64_t rows, ld;     // PAD: rows and source row stride; OWNER: rows of x; BIAS: padded length
-    int R, C, ldo;        // TURN: [batch][R][C] -> [batch][C][ldo]; PAD: [rows][C] -> [rows][ldo]; zeros behind; BIAS: C values; OWNER: C tiles of R rows
+    int R, C, ldo;        // TURN: [batch][R][C] -> [batch][C][ldo]; PAD: [rows][C] -> [rows][ldo]; zeros behind; BIAS: C values; OWNER: C tiles of R rows;
+                          // ODD: four workgroups for each of the runs of `rows` values
     int E;                // OWNER
     int rep;              // TURN, PAD: a row repeats every rep elements (a multiple of 32)
 };
-constexpr int kJobs = 9;
+constexpr int kJobs = 10;
 struct Jobs {
     Job job[kJobs];
     int n = 0, blocks = 0;
@@ -1005,16 +1105,25 @@ __device__ void prep_body(const Jobs& jobs, int block, float* lds) {
     } else if (j.type == JOB_BIAS) {
         const int64_t i = blk * 256 + threadIdx.x;
         if (i < j.rows) ((float*)j.dst)[i] = i < j.C ? (float)((const T*)j.src)[i] : 0.f;
-    } else {
-        const int64_t i = blk * 256 + threadIdx.x;
+    } else if (j.type == JOB_OWNER) {
+        const int64_t i = blk * 4 + (threadIdx.x >> 6);  // a wave a tile
         if (i < j.C) {
-            const int64_t a0 = i * j.R, a1 = a0 + j.R < j.rows ? a0 + j.R : j.rows;
-            const int32_t* off = (const int32_t*)j.src;
-            const int e0 = owner_of(off, j.E, a0), e1 = owner_of(off, j.E, a1 - 1);
-            // rows before the first offset (-1) and behind the last (E) have no model
-            const int who = e0 == e1 ? (e0 < 0 ? j.E : e0) : -1;
-            ((int32_t*)j.dst)[i] = who;
+            const Owners own((const int32_t*)j.src, j.E, 0, 0);
+            const TileModels m = TileModels::of_tile(own, i * j.R, j.R, j.rows, j.E);
+            if ((threadIdx.x & 63) == 0) ((int32_t*)j.dst)[i] = m.packed();
         }
+    } else {  // ODD: a byte each, so nobody clears them first
+        const int64_t run = blk >> 2, share = blk & 3, pieces = (j.rows + V - 1) / V;
+        const T* in = (const T*)j.src + run * j.rows;
+        bool odd = false;
+        for (int64_t p = share * 256 + threadIdx.x; p < pieces; p += 1024) {
+            const int64_t left = j.rows - p * V;
+            const mtk_vec<T> v = left >= V ? mtk_ld(in + p * V) : mtk_ld_n(in + p * V, (int)left);
+#pragma unroll
+            for (int i = 0; i < V; ++i) odd |= !(fabsf((float)v.v[i]) <= 3.4028235e38f);
+        }
+        odd = __syncthreads_or(odd);
+        if (threadIdx.x == 0) ((unsigned char*)j.dst)[blk] = odd;
     }
 }
 
@@ -1143,15 +1252,17 @@ struct Shape {
 };
 // what k_linear reads beside its operands, and their padded copies where they need one
 struct Packed {
-    int64_t X, W, F, Bp, bias, owner;  // F: the factors that the shrink multiplies, in whole lines like X
+    int64_t X, W, F, Bp, bias, owner, odd, pairs;  // F: the factors that the shrink multiplies, in whole lines like X
     Packed(Layout& l, const Shape& sh, int64_t M, int N, int r, int E, int dtype, bool pad_x, bool pad_w, bool pad_low) {
         const int64_t z = mtk_dtype_size(dtype);
         X = l.take(!sh.few && pad_x ? M * sh.Kp * z : 0);
         W = l.take(!sh.few && pad_w ? (int64_t)N * sh.Kp * z : 0);
         F = l.take(!sh.few && pad_x ? (int64_t)E * r * sh.Kp * z : 0);
-        Bp = l.take(sh.blocks ? (int64_t)(E + 1) * N * sh.rp * z : pad_low ? (int64_t)E * N * sh.low_ld * z : 0);
+        Bp = l.take(sh.blocks ? (int64_t)E * N * sh.rp * z : pad_low ? (int64_t)E * N * sh.low_ld * z : 0);
         bias = l.take((int64_t)sh.nb_n * sh.BN * 4);
         owner = l.take(sh.blocks ? sh.MT * 4 : 0);
+        odd = l.take(sh.blocks ? (int64_t)E * 4 : 0);
+        pairs = l.take(sh.blocks ? (sh.MT + E) * sh.BM * sh.rp * z : 0);
     }
 };
 // rows that LDS-DMA can stream as they are: whole lines, 16-byte aligned, offsets inside a tile in 32 bits
@@ -1214,7 +1325,7 @@ DeviceState* device_state() {
 }
 
 template <typename T, int WR, int WC, int MW, int NT, int DX, int DW>
-int launch_linear(LinearArgs& g, T* y, int which, hipStream_t s) {
+int launch_linear(const LinearArgs& g, int which, hipStream_t s) {
     typedef Geo<WR, WC, MW, NT, DX, DW> G;
     DeviceState* st = device_state();
     if (!st) MTK_FAIL(MTK_ERR_HIP, "adapter product: no device properties");
@@ -1223,15 +1334,16 @@ int launch_linear(LinearArgs& g, T* y, int which, hipStream_t s) {
         st->lds[which] = true;
     }
     const int64_t per_xcd = cdiv(g.MT * g.nb_n, 8), room = (int64_t)st->cus / 8 * G::kRoom;
-    k_linear<T, WR, WC, MW, NT, DX, DW><<<(unsigned)(8 * (per_xcd < room ? per_xcd : room)), 64 * G::NW, G::kLds, s>>>(g, y);
+    k_linear<T, WR, WC, MW, NT, DX, DW><<<(unsigned)(8 * (per_xcd < room ? per_xcd : room)), 64 * G::NW, G::kLds, s>>>(g);
     return MTK_OK;
 }
 template <typename T> int linear(const Shape& sh, LinearArgs& g, T* y, hipStream_t s) {
+    g.Y = y;
     constexpr int base = sizeof(T) == 4 ? 0 : std::is_same<T, mtk_bf16>::value ? 3 : 6;
     if constexpr (sizeof(T) == 2)
-        if (sh.kind == 0) return launch_linear<T, 2, 4, 4, 2, 3, 2>(g, y, base, s);
-    if (sh.kind == 1) return launch_linear<T, 4, 2, 1, 2, 3, 2>(g, y, base + 1, s);
-    return launch_linear<T, 2, 2, 1, 1, 3, 2>(g, y, base + 2, s);
+        if (sh.kind == 0) return launch_linear<T, 2, 4, 4, 2, 3, 2>(g, base, s);
+    if (sh.kind == 1) return launch_linear<T, 4, 2, 1, 2, 3, 2>(g, base + 1, s);
+    return launch_linear<T, 2, 2, 1, 1, 3, 2>(g, base + 2, s);
 }
 template <typename T>
 void linear_few(const FewArgs& g, const T* x, const T* W, const T* bias, const T* u, const T* up, T* y, hipStream_t s) {
@@ -1267,9 +1379,11 @@ LinearArgs plan_linear(Jobs& jobs, const Shape& sh, const Packed& pk, char* wb, 
         const int half = sizeof(T) == 2 ? sh.rp / 2 : sh.rp;
         if (turned) job_turn(jobs, L, wb + pk.Bp, r, N, sh.rp, E, half);
         else job_pad(jobs, L, r, wb + pk.Bp, (int64_t)E * N, r, sh.rp, V, half);
-        job_pad(jobs, L, 0, wb + pk.Bp + (int64_t)E * N * sh.rp * sizeof(T), N, 0, sh.rp, V);
-        jobs.add(Job{JOB_OWNER, 0, offsets, wb + pk.owner, M, 0, sh.BM, (int)sh.MT, 0, E, 1}, cdiv(sh.MT, 256));
+        jobs.add(Job{JOB_ODD, 0, L, wb + pk.odd, (int64_t)N * r, 0, 0, 0, 0, E, 1}, (int64_t)E * 4);
+        jobs.add(Job{JOB_OWNER, 0, offsets, wb + pk.owner, M, 0, sh.BM, (int)sh.MT, 0, E, 1}, cdiv(sh.MT, 4));
         g.owner = (const int32_t*)(wb + pk.owner);
+        g.odd = (const int32_t*)(wb + pk.odd);
+        g.pairs = wb + pk.pairs;
         g.Bp = g.low = wb + pk.Bp;
         g.low_ld = sh.rp;
     }
@@ -1316,7 +1430,7 @@ extern "C" int mtk_adapter_forward(int64_t M, int din, int dout, int r, int E, i
         const Shape& sh = wk.sh;
         T* u = (T*)((char*)saved + sv.u);
         T* uT = keep && sizeof(T) == 2 ? (T*)((char*)saved + sv.uT) : nullptr;
-        ShrinkArgs sa{M, din, r, sh.rp, E, x_ld, offsets, scales, (float)scale, sv.Mp, 1, 1};
+        ShrinkArgs sa{M, din, r, sh.rp, E, x_ld, offsets, scales, (float)scale, sv.Mp, (char*)work + wk.pk.pairs, sh.blocks && !sh.few ? sh.BM : 0, 1, 1};
         if (sh.few) {
             shrink<T>(sa, Jobs(), (const T*)x, (const T*)down, u, uT, s);
             linear_few<T>(FewArgs{M, x_ld, dout, din, r, sh.rp, E, act, offsets}, (const T*)x, (const T*)W, (const T*)bias, u, (const T*)up, (T*)y, s);
@@ -1394,7 +1508,8 @@ extern "C" int mtk_adapter_backward(int64_t M, int din, int dout, int r, int E, 
         }
         prep<T>(jobs, s);
         if (dx || ddown)
-            shrink<T>(ShrinkArgs{M, gk, r, sh.rp, E, gk, offsets, scales, (float)scale, sv.Mp, 1, 1}, Jobs(), g, (const T*)(wb + wk.Bt), t, ddown && sizeof(T) == 2 ? tT : nullptr, s);
+            shrink<T>(ShrinkArgs{M, gk, r, sh.rp, E, gk, offsets, scales, (float)scale, sv.Mp, wb + wk.pk.pairs, dx && sh.blocks && !sh.few ? sh.BM : 0, 1, 1},
+                      Jobs(), g, (const T*)(wb + wk.Bt), t, ddown && sizeof(T) == 2 ? tT : nullptr, s);
         if (dx) {
             if (sh.few) linear_few<T>(FewArgs{M, dout, din, dout, r, sh.rp, E, 0, offsets}, g, (const T*)(wb + wk.Wt), nullptr, t, (const T*)(wb + wk.At), (T*)dx, s);
             else rc = linear<T>(sh, lin, (T*)dx, s);

@@ -359,6 +359,79 @@ def test_a_diverged_model_leaves_the_others_alone(M, dt):
                 assert not bool(torch.isfinite(y[rows]).any()), what
 
 
+def shared_offsets(M, E, tile, apart=0):
+    """Offsets whose borders fall inside tiles: no model has the first `apart` rows nor the last, two models have no rows, one has a single
+    row, and the borders of three lie in one tile"""
+    off = [apart + (M - 2 * apart) * e // E for e in range(E + 1)]
+    off[2] = off[1]
+    off[E - 1] = off[E]
+    off[4], off[5] = off[3] + 1, off[3] + tile // 4
+    return torch.tensor(off, dtype=torch.int32, device=DEV)
+
+
+# rows, widths: each tile of the product (64, 128, 256 rows) with whole and with ragged feature tiles, both products of a step alike
+SHARED = [(1500, 72, 80, 7, 64), (33 * 128 + 5, 1030, 1030, 7, 128), (52 * 256 + 77, 1000, 1000, 9, 256)]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("M,din,dout,E,tile", SHARED)
+def test_tiles_that_models_share(M, din, dout, E, tile, dt):
+    g = gen(M)
+    a = adapter_inputs(g, M, din, dout, 12, E, dt)
+    a["offsets"] = shared_offsets(M, E, tile, 37)
+    gy = randn(g, M, dout, dt=dt)
+    for n in ("x", "down", "up"):
+        a[n].requires_grad_()
+    y = call(a)
+    dx, dd, du = torch.autograd.grad(y, (a["x"], a["down"], a["up"]), gy)
+    ref = adapter_reference(**{**a, "relu": False, "gy": gy})
+    within(y, ref["y"], tol(ref["y_terms"], ref["y_low"], din, 12, ref["y"], dt, a["up"]))
+    within(dx, ref["dx"], tol(ref["dx_terms"], ref["dx_low"], dout, 12, ref["dx"], dt, a["down"]))
+    # a row is the same whatever the other models' factors hold: finite ones ..
+    b = {n: t.detach().clone() for n, t in a.items()}
+    off = a["offsets"].tolist()
+    rest = torch.ones(M, dtype=torch.bool)
+    for e in (0, 5):
+        rest[off[e]:off[e + 1]] = False
+    with torch.no_grad():
+        for value in (2.0, float("inf"), float("nan")):
+            for n, t in (("up", b["up"]), ("down", b["down"])):
+                keep = t.clone()
+                t[0, 0, 0], t[5] = value, value
+                again = call(b)
+                assert torch.equal(again.cpu()[rest], y.detach().cpu()[rest]), (n, value)
+                if value != 2.0 and n == "up":
+                    assert not bool(torch.isfinite(again[off[5]:off[6]]).any()) and not bool(torch.isfinite(again[off[0]:off[1], 0]).any())
+                    assert torch.equal(again[off[0]:off[1], 1:], y.detach()[off[0]:off[1], 1:])  # what the value does not reach
+                t.copy_(keep)
+    for value in (float("inf"), float("nan")):  # .. and so its gradient
+        c = {n: t.detach().clone() for n, t in a.items()}
+        c["down"][5] = value
+        c["x"].requires_grad_()
+        again = torch.autograd.grad(call(c), c["x"], gy)[0]
+        mine = torch.zeros(M, dtype=torch.bool)
+        mine[off[5]:off[6]] = True
+        assert torch.equal(again.cpu()[~mine], dx.cpu()[~mine]) and not bool(torch.isfinite(again.cpu()[mine]).any()), value
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_more_models_in_a_tile_than_it_streams(dt):
+    """Twelve models inside one tile of 64 rows beside eight long ones, and two dozen of three rows each"""
+    g = gen(31)
+    M, din, dout, r = 1600, 72, 80, 5
+    for off in ([0, 200, 400, 600, 800] + [801 + 3 * i for i in range(12)] + [1000, 1200, 1400, 1600], [0, 1390] + [1390 + 3 * i for i in range(1, 24)] + [1590]):
+        E = len(off) - 1
+        a = adapter_inputs(g, M, din, dout, r, E, dt)
+        a["offsets"] = torch.tensor(off, dtype=torch.int32, device=DEV)
+        gy = randn(g, M, dout, dt=dt)
+        a["x"].requires_grad_()
+        y = call(a)
+        dx = torch.autograd.grad(y, a["x"], gy)[0]
+        ref = adapter_reference(**{**a, "relu": False, "gy": gy})
+        within(y, ref["y"], tol(ref["y_terms"], ref["y_low"], din, r, ref["y"], dt, a["up"]))
+        within(dx, ref["dx"], tol(ref["dx_terms"], ref["dx_low"], dout, r, ref["dx"], dt, a["down"]))
+
+
 def test_adapter_strides_scales_and_plans():
     g = gen(4)
     M, din, dout, r, E = 60, 40, 24, 4, 3
