@@ -1376,9 +1376,9 @@ void linear_few(const FewArgs& g, const T* x, const T* W, const T* bias, const T
     else k_linear_few<T, 32><<<(unsigned)(cdiv(g.M, 32) * cdiv(g.N, 32)), 512, 0, s>>>(g, x, W, bias, u, up, y);
 }
 // the jobs of a k_linear product: x and W padded where they do not stream, B_e in whole lines and a block of zeros, bias, tiles' models.
-// F: W [N][K], or its transpose [K][N] when `turned`; L: B [E][N][r], or [E][r][N]
+// `early`: what the shrink reads.  F: W [N][K], or its transpose [K][N] when `turned`; L: B [E][N][r], or [E][r][N]
 template <typename T>
-LinearArgs plan_linear(Jobs& jobs, const Shape& sh, const Packed& pk, char* wb, int64_t M, int N, int K, int r, int E, int dtype, const T* x, int64_t x_ld,
+LinearArgs plan_linear(Jobs& early, Jobs& jobs, const Shape& sh, const Packed& pk, char* wb, int64_t M, int N, int K, int r, int E, int dtype, const T* x, int64_t x_ld,
                        const T* F, bool turned, const T* bias, const T* L, const T* u, const int32_t* offsets, int relu) {
     constexpr int V = mtk_piece<T>::n;
     LinearArgs g{};
@@ -1388,7 +1388,7 @@ LinearArgs plan_linear(Jobs& jobs, const Shape& sh, const Packed& pk, char* wb, 
     g.X = x;
     g.x_ld = x_ld * sizeof(T);
     if (!streams(x, x_ld, K, dtype)) {
-        job_pad(jobs, x, x_ld, wb + pk.X, M, K, sh.Kp, V);
+        job_pad(early, x, x_ld, wb + pk.X, M, K, sh.Kp, V);
         g.X = wb + pk.X;
         g.x_ld = sh.Kp * sizeof(T);
     }
@@ -1461,8 +1461,8 @@ extern "C" int mtk_adapter_forward(int64_t M, int din, int dout, int r, int E, i
             linear_few<T>(FewArgs{M, x_ld, dout, din, r, sh.rp, E, act, offsets}, (const T*)x, (const T*)W, (const T*)bias, u, (const T*)up, (T*)y, s);
             return;
         }
-        Jobs jobs;
-        LinearArgs g = plan_linear<T>(jobs, sh, wk.pk, (char*)work, M, dout, din, r, E, dtype, (const T*)x, x_ld, (const T*)W, false, (const T*)bias, (const T*)up, u,
+        Jobs early, jobs;
+        LinearArgs g = plan_linear<T>(early, jobs, sh, wk.pk, (char*)work, M, dout, din, r, E, dtype, (const T*)x, x_ld, (const T*)W, false, (const T*)bias, (const T*)up, u,
                                       offsets, act);
         if (!sh.blocks) {
             g.low = up;
@@ -1473,16 +1473,17 @@ extern "C" int mtk_adapter_forward(int64_t M, int din, int dout, int r, int E, i
             }
         }
         // x padded to whole lines: the shrink reads them too (20,011 rows of 517 in fp16: 11 us for the lines and 13 for the shrink; 33 for
-        // both in one launch from rows as they are).  Else its launch takes the jobs along.
+        // both in one launch from rows as they are).
+        const T *sx = (const T*)x, *sf = (const T*)down;
         if (g.X != x) {
-            job_pad(jobs, down, din, (char*)work + wk.pk.F, (int64_t)E * r, din, sh.Kp, mtk_piece<T>::n);
+            job_pad(early, down, din, (char*)work + wk.pk.F, (int64_t)E * r, din, sh.Kp, mtk_piece<T>::n);
+            sx = (const T*)g.X;
+            sf = (const T*)((char*)work + wk.pk.F);
             sa.K = sh.Kp;
             sa.x_ld = sh.Kp;
-            prep<T>(jobs, s);
-            shrink<T>(sa, Jobs(), (const T*)g.X, (const T*)((char*)work + wk.pk.F), u, uT, s);
-        } else {
-            shrink<T>(sa, jobs, (const T*)x, (const T*)down, u, uT, s);
         }
+        prep<T>(early, s);
+        shrink<T>(sa, jobs, sx, sf, u, uT, s);
         rc = linear<T>(sh, g, (T*)y, s);
     });
     if (rc) return rc;
@@ -1515,26 +1516,26 @@ extern "C" int mtk_adapter_backward(int64_t M, int din, int dout, int r, int E, 
             k_relu_grad<T><<<(unsigned)(nb < 65536 ? nb : 65536), 256, 0, s>>>(n, (const T*)y, g, gz);
             g = gz;
         }
-        Jobs jobs;
+        Jobs early, jobs;
         LinearArgs lin{};
         const bool padded = dx && !sh.few && !streams(g, dout, dout, dtype);  // g in whole lines, for all that reads it from here on
         const int gk = padded ? sh.Kp : dout;
         const T* graw = g;
         if (padded) g = (const T*)(wb + wk.pk.X);
-        if (dx || ddown) job_turn(jobs, up, wb + wk.Bt, dout, r, gk, E);
+        if (dx || ddown) job_turn(early, up, wb + wk.Bt, dout, r, gk, E);
         if (dx) {
             if (sh.few) job_turn(jobs, W, wb + wk.Wt, dout, din, dout, 1);
-            else lin = plan_linear<T>(jobs, sh, wk.pk, wb, M, din, dout, r, E, dtype, graw, dout, (const T*)W, true, nullptr, (const T*)down, t, offsets, 0);
+            else lin = plan_linear<T>(early, jobs, sh, wk.pk, wb, M, din, dout, r, E, dtype, graw, dout, (const T*)W, true, nullptr, (const T*)down, t, offsets, 0);
             if (sh.few || !sh.blocks) {
                 job_turn(jobs, down, wb + wk.At, r, din, sh.few ? r : sh.low_ld, E);
                 lin.low = wb + wk.At;
                 lin.low_ld = sh.low_ld;
             }
         }
-        prep<T>(jobs, s);
+        prep<T>(early, s);
         if (dx || ddown)
             shrink<T>(ShrinkArgs{M, gk, r, sh.rp, E, gk, offsets, scales, (float)scale, sv.Mp, wb + wk.pk.pairs, dx && sh.blocks && !sh.few ? sh.BM : 0, 1, 1},
-                      Jobs(), g, (const T*)(wb + wk.Bt), t, ddown && sizeof(T) == 2 ? tT : nullptr, s);
+                      jobs, g, (const T*)(wb + wk.Bt), t, ddown && sizeof(T) == 2 ? tT : nullptr, s);
         if (dx) {
             if (sh.few) linear_few<T>(FewArgs{M, dout, din, dout, r, sh.rp, E, 0, offsets}, g, (const T*)(wb + wk.Wt), nullptr, t, (const T*)(wb + wk.At), (T*)dx, s);
             else rc = linear<T>(sh, lin, (T*)dx, s);
