@@ -1260,12 +1260,12 @@ struct Shape {
         rp = rank_pad(r, dtype);
         low_ld = (int)mtk_up(r, 16 / mtk_dtype_size(dtype));
         Kp = (int)mtk_up(K, line);
-        // us for K = N = 1024, few rows / 64 x 64 tiles (and some 5 for their k_prep): bf16 256 rows 9.0 / 9.9, 512 rows 13.9 / 9.4, 1,024 rows
-        // 26 / 9.3; fp32 256 rows 14 / 26, 512 rows 24 / 26, 1,024 rows 45 / 27
-        few = M <= 512;
+        // few: up to 64 rows, and while its 32 x 32 tiles fit the 256 CUs once.  us for K = N = 1024 and 16 models, few / 64 x 64 tiles: bf16
+        // 64 rows 7.1 / 17, 256 rows 12 / 13, 384 rows 21 / 13, 1,024 rows 42 / 12; fp32 256 rows 19 / 32, 384 rows 33 / 30, 1,024 rows 69 / 31
+        few = M <= 64 || (M <= 512 && cdiv(M, 32) * cdiv(N, 32) <= 256);
         // 256 x 256 tiles (one workgroup a CU) where they fill their rounds over the CUs to four fifths; 64 x 64 while the chip is not full.  us for
-        // K = N = 1024, 256 / 128 / 64: bf16 65,536 rows 123 / 159 / 232, 20,011 rows 77 / 54 / 71, 8,192 rows 33 / 24 / 31, 2,048 rows
-        // 33 / 16 / 13; fp32 20,011 rows 540 / 338 / 346, 8,192 rows 262 / 144 / 140, 2,048 rows 264 / 79 / 43
+        // K = N = 1024, 256 / 128 / 64: bf16 65,536 rows 145 / 193 / 261, 20,011 rows 67 / 56 / 81, 8,192 rows 36 / 28 / 36, 2,048 rows
+        // 31 / 19 / 15; fp32 20,011 rows - / 355 / 378, 8,192 rows - / 157 / 162, 2,048 rows - / 80 / 48
         const int64_t t256 = cdiv(M, 256) * cdiv(N, 256), t128 = cdiv(M, 128) * cdiv(N, 128);
         if (dtype == MTK_DT_F32) kind = t128 >= 1024 ? 1 : 2;
         else kind = t256 * 5 >= cdiv(t256, 256) * 256 * 4 ? 0 : t128 > 256 ? 1 : 2;
