@@ -16,10 +16,14 @@ template <typename T> struct __attribute__((packed, aligned(alignof(T)), may_ali
 
 template <typename T> __device__ __forceinline__ mtk_vec<T> mtk_ld(const T* p) { return *reinterpret_cast<const mtk_vec<T>*>(p); }
 template <typename T> __device__ __forceinline__ void mtk_st(T* p, const mtk_vec<T>& v) { *reinterpret_cast<mtk_vec<T>*>(p) = v; }
-// past the caches
+// past the caches, both ways
 template <typename T> __device__ __forceinline__ void mtk_st_nt(T* p, const mtk_vec<T>& v) {
     typedef uint32_t words __attribute__((ext_vector_type(4), aligned(2)));  // see mtk_vec
     __builtin_nontemporal_store(__builtin_bit_cast(words, v), reinterpret_cast<words*>(p));
+}
+template <typename T> __device__ __forceinline__ mtk_vec<T> mtk_ld_nt(const T* p) {
+    typedef uint32_t words __attribute__((ext_vector_type(4), aligned(2)));
+    return __builtin_bit_cast(mtk_vec<T>, __builtin_nontemporal_load(reinterpret_cast<const words*>(p)));
 }
 // the first `n` elements of a piece, zeros behind them
 template <typename T> __device__ __forceinline__ mtk_vec<T> mtk_ld_n(const T* p, int n) {

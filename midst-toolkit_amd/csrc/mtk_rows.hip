@@ -39,7 +39,8 @@ __global__ __launch_bounds__(RT) void k_route_count(RouteArgs a) {
 
 // Stable placement.  A wave owns a contiguous part of its workgroup's pairs: counts per (wave, key), a prefix over keys, earlier
 // workgroups and earlier waves, then 64 pairs at a time: the lanes with the same key find each other by one ballot per key bit,
-// a lane's place is the wave's running counter plus the equal lanes below it.
+// a lane's place is the wave's running counter plus the equal lanes below it.  Bound by latency: 48 pairs 2.8 us (one workgroup, one launch),
+// 16,396 pairs 10 us and 200,000 pairs 12 us with the counts.
 __global__ __launch_bounds__(RT) void k_route_place(RouteArgs a) {
     extern __shared__ int32_t sm[];
     const int bins = a.E + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -127,7 +128,7 @@ struct RowsArgs {
     const int32_t* map;  // slot [n][k]
     const float* w;      // [pairs] or null
     int lpr;             // lanes of a row: a power of two up to 64
-    bool nt;             // stores past the caches
+    bool nt;             // past the caches
 };
 
 // A pair whose index was out of range has ~place for a slot: its rows are NaN on both ways, loud, and never an out-of-range access.
@@ -157,7 +158,8 @@ __device__ __forceinline__ int64_t place_of(int32_t s, int64_t pairs, bool& bad)
 
 // xs[slot[n, j]] = x[n] (times w[n, j]) for all copies j: a record's row is read once and written k times.  With y: dw[n, j] =
 // <x[n], y[slot[n, j]]> as well (x is the gradient of the combined rows then).  Bound by bandwidth: a row belongs to lpr lanes, each moving
-// 16-byte pieces, so a wave touches whole lines.
+// 16-byte pieces, so a wave touches whole lines.  4,099 rows of 1,021 fp32 in four copies (84 MB): 20 us, with the weights' gradient
+// (151 MB) 36 us; 24 rows of 120: 2.7 us, a launch.
 template <typename T, bool W, bool DOT, int KC>
 __global__ __launch_bounds__(256) void k_dispatch(RowsArgs a, const T* __restrict__ x, T* __restrict__ xs, const T* __restrict__ y, float* __restrict__ dw) {
     constexpr int V = mtk_piece<T>::n;
@@ -185,13 +187,13 @@ __global__ __launch_bounds__(256) void k_dispatch(RowsArgs a, const T* __restric
 #pragma unroll 2
             for (int64_t c = (int64_t)sub * V; c < a.D; c += (int64_t)a.lpr * V) {
                 const int left = a.D - c < V ? (int)(a.D - c) : V;
-                const mtk_vec<T> v = left == V ? mtk_ld(src + c) : mtk_ld_n(src + c, left);
+                const mtk_vec<T> v = left < V ? mtk_ld_n(src + c, left) : a.nt ? mtk_ld_nt(src + c) : mtk_ld(src + c);
                 if (DOT) {
 #pragma unroll
                     for (int j = 0; j < KC; ++j) {
                         if (j >= nj) break;
                         const T* ys = y + at[j] + c;
-                        const mtk_vec<T> q = left == V ? mtk_ld(ys) : mtk_ld_n(ys, left);
+                        const mtk_vec<T> q = left < V ? mtk_ld_n(ys, left) : a.nt ? mtk_ld_nt(ys) : mtk_ld(ys);
 #pragma unroll
                         for (int i = 0; i < V; ++i) dot[j] += (float)v.v[i] * (float)q.v[i];
                     }
@@ -223,7 +225,8 @@ __global__ __launch_bounds__(256) void k_dispatch(RowsArgs a, const T* __restric
     }
 }
 
-// out[n] = sum_j (w[n, j]) y[slot[n, j]], j ascending, fp32, rounded once; four copies' loads in flight
+// out[n] = sum_j (w[n, j]) y[slot[n, j]], j ascending, fp32, rounded once; four copies' loads in flight.  4,099 rows of 1,021 fp32 from four copies
+// each (84 MB): 15 us weighted, with the rows still in the caches, 25 us when not.
 template <typename T, bool W, int KC>
 __global__ __launch_bounds__(256) void k_combine(RowsArgs a, const T* __restrict__ y, T* __restrict__ out) {
     constexpr int V = mtk_piece<T>::n;
@@ -249,7 +252,7 @@ __global__ __launch_bounds__(256) void k_combine(RowsArgs a, const T* __restrict
                     bool bad;
                     const T* src = y + place_of(cp.s[j], a.other, bad) * a.ld + c;
                     w[j] = bad ? __builtin_nanf("") : cp.w[j];
-                    v[j] = left == V ? mtk_ld(src) : mtk_ld_n(src, left);
+                    v[j] = left < V ? mtk_ld_n(src, left) : a.nt ? mtk_ld_nt(src) : mtk_ld(src);
                 }
 #pragma unroll
                 for (int j = 0; j < KC; ++j) {
@@ -277,8 +280,9 @@ int lanes_per_row(int64_t D, int V) {
     return l;
 }
 
-// Stores go past the caches where what a call reads and writes exceeds what they hold (256 MB): the result's readers would find nothing there.
-// us, past them / through them: 100,000 rows of 1024 bf16, two copies, out 128 / 221.
+// Rows go past the caches, read and written, where what a call moves exceeds what they hold (256 MB): the result's readers would find nothing
+// there.  us, 100,000 rows of 1024 bf16, two copies, past them / reads through them / all through them: dispatch 117 / 115 / 221, weighted combine
+// 131 / 158, dispatch with the weights' gradient 214 / 270 (1.0 GB: 4.8 TB/s, what a large copy reaches).
 constexpr int64_t kCaches = 256ll << 20;
 template <typename F> void by_flags(bool a, bool b, int k, F f) {
     auto third = [&](auto ta, auto tb) {
