@@ -14,8 +14,8 @@
 //
 // Bound by bandwidth: 28 B a value with fp32 and 32-bit moments, 10 B with bf16 and 8-bit ones.  Up to 64 tensors ride in one launch's
 // arguments (nothing to upload, nothing that a captured graph could find changed); a workgroup takes one chunk of one tensor.
-// 55 million fp32 values in 192 tensors, 32-bit moments: 293 us (1.54 GB: 5.3 TB/s); 220 million bf16 values, 8-bit moments: 466 us (2.2 GB: 4.7 TB/s); 2.2 million
-// fp32 values in 12 tensors: 10 us either way, from the caches.
+// 55 million fp32 values in 192 tensors, 32-bit moments: 257 us (1.54 GB: 6.0 TB/s); 220 million bf16 values, 8-bit moments: 426 us (2.2 GB: 5.2 TB/s);
+// 2.2 million fp32 values in 12 tensors: 11 us either way, from the caches.
 #include <math.h>
 
 #include "mtk_lowp.h"
@@ -23,6 +23,9 @@
 namespace {
 
 constexpr int MAXT = 64;       // tensors of a launch: 3.9 KB of kernel arguments
+// Everything goes past the caches, both ways, where a step moves more than they hold: the next step would find nothing there.  us, past / through
+// them: 55 million fp32 values with 32-bit moments 257 / 293, 220 million bf16 values with 8-bit ones 426 / 466.
+constexpr int64_t kCaches = 256ll << 20;
 constexpr int QB = 256;        // values that share a scale
 
 struct AdamwHyper {
@@ -40,6 +43,7 @@ struct AdamwArgs {
     int64_t numel[MAXT];
     int32_t first[MAXT + 1];   // first chunk of a tensor; first[n] = chunks of the launch
     int n;
+    bool nt;                   // past the caches
     AdamwHyper h;
     const AdamwHyper* dyn;     // read instead of h where given (a step whose count lives on the device)
 };
@@ -70,10 +74,16 @@ __device__ __forceinline__ float fast_sqrt(float v) {
 }
 
 template <int N> struct __attribute__((packed, aligned(1), may_alias)) CodeVec { uint32_t w[N / 4]; };
+typedef uint32_t CodeWord __attribute__((aligned(1), may_alias));
 
-template <int N> __device__ __forceinline__ void ld_codes(const uint8_t* p, int left, float* f) {
+template <int N> __device__ __forceinline__ void ld_codes(const uint8_t* p, int left, float* f, bool nt) {
     CodeVec<N> c;
-    if (left >= N) c = *reinterpret_cast<const CodeVec<N>*>(p);
+    if (left >= N) {
+        if (nt)
+#pragma unroll
+            for (int i = 0; i < N / 4; ++i) c.w[i] = __builtin_nontemporal_load(reinterpret_cast<const CodeWord*>(p) + i);
+        else c = *reinterpret_cast<const CodeVec<N>*>(p);
+    }
     else {
 #pragma unroll
         for (int i = 0; i < N / 4; ++i) {
@@ -89,35 +99,41 @@ template <int N> __device__ __forceinline__ void ld_codes(const uint8_t* p, int 
         f[4 * i] = lo[0]; f[4 * i + 1] = lo[1]; f[4 * i + 2] = hi[0]; f[4 * i + 3] = hi[1];
     }
 }
-template <int N> __device__ __forceinline__ void st_codes(uint8_t* p, int left, const float* q) {
+template <int N> __device__ __forceinline__ void st_codes(uint8_t* p, int left, const float* q, bool nt) {
     CodeVec<N> c;
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
         int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i], q[4 * i + 1], 0, false);
         c.w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i + 2], q[4 * i + 3], w, true);
     }
-    if (left >= N) *reinterpret_cast<CodeVec<N>*>(p) = c;
+    if (left >= N) {
+        if (nt)
+#pragma unroll
+            for (int i = 0; i < N / 4; ++i) __builtin_nontemporal_store(c.w[i], reinterpret_cast<CodeWord*>(p) + i);
+        else *reinterpret_cast<CodeVec<N>*>(p) = c;
+    }
     else
 #pragma unroll
         for (int i = 0; i < N; ++i)
             if (i < left) p[i] = (uint8_t)(c.w[i / 4] >> (8 * (i & 3)));
 }
-template <int N> __device__ __forceinline__ void ld_f32(const float* p, int left, float* f) {
+template <int N> __device__ __forceinline__ void ld_f32(const float* p, int left, float* f, bool nt) {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
-        const mtk_vec<float> v = left - i >= 4 ? mtk_ld(p + i) : mtk_ld_n(p + i, left - i);
+        const mtk_vec<float> v = left - i < 4 ? mtk_ld_n(p + i, left - i) : nt ? mtk_ld_nt(p + i) : mtk_ld(p + i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[i + j] = v.v[j];
     }
 }
-template <int N> __device__ __forceinline__ void st_f32(float* p, int left, const float* f) {
+template <int N> __device__ __forceinline__ void st_f32(float* p, int left, const float* f, bool nt) {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
         mtk_vec<float> v;
 #pragma unroll
         for (int j = 0; j < 4; ++j) v.v[j] = f[i + j];
-        if (left - i >= 4) mtk_st(p + i, v);
-        else mtk_st_n(p + i, v, left - i);
+        if (left - i < 4) mtk_st_n(p + i, v, left - i);
+        else if (nt) mtk_st_nt(p + i, v);
+        else mtk_st(p + i, v);
     }
 }
 
@@ -137,12 +153,13 @@ __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
     const int left = n - i0 >= V ? V : (n > i0 ? (int)(n - i0) : 0);
     T* pp = (T*)a.p[lo] + i0;
     const T* gp = (const T*)a.g[lo] + i0;
-    const mtk_vec<T> p0 = left == V ? mtk_ld(pp) : mtk_ld_n(pp, left), g0 = left == V ? mtk_ld(gp) : mtk_ld_n(gp, left);
+    const bool nt = a.nt;
+    const mtk_vec<T> p0 = left < V ? mtk_ld_n(pp, left) : nt ? mtk_ld_nt(pp) : mtk_ld(pp), g0 = left < V ? mtk_ld_n(gp, left) : nt ? mtk_ld_nt(gp) : mtk_ld(gp);
     float m[V], v[V];
     const int64_t blk = i0 / QB;
     if (Q8) {
-        ld_codes<V>((const uint8_t*)a.m[lo] + i0, left, m);
-        ld_codes<V>((const uint8_t*)a.v[lo] + i0, left, v);
+        ld_codes<V>((const uint8_t*)a.m[lo] + i0, left, m, nt);
+        ld_codes<V>((const uint8_t*)a.v[lo] + i0, left, v, nt);
         const float sm = left ? a.ms[lo][blk] : 0.f, sv = left ? a.vs[lo][blk] : 0.f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -151,8 +168,8 @@ __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
             v[i] *= v[i];
         }
     } else {
-        ld_f32<V>((const float*)a.m[lo] + i0, left, m);
-        ld_f32<V>((const float*)a.v[lo] + i0, left, v);
+        ld_f32<V>((const float*)a.m[lo] + i0, left, m, nt);
+        ld_f32<V>((const float*)a.v[lo] + i0, left, v, nt);
     }
     mtk_vec<T> p1;
     float r[V];
@@ -173,11 +190,12 @@ __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
             p1.v[i] = (T)((float)p0.v[i] * h.decay - h.step_size * (m[i] / (r[i] * h.inv_bc2 + h.eps)));
         }
     }
-    if (left == V) mtk_st(pp, p1);
-    else mtk_st_n(pp, p1, left);
+    if (left < V) mtk_st_n(pp, p1, left);
+    else if (nt) mtk_st_nt(pp, p1);
+    else mtk_st(pp, p1);
     if (!Q8) {
-        st_f32<V>((float*)a.m[lo] + i0, left, m);
-        st_f32<V>((float*)a.v[lo] + i0, left, v);
+        st_f32<V>((float*)a.m[lo] + i0, left, m, nt);
+        st_f32<V>((float*)a.v[lo] + i0, left, v, nt);
         return;
     }
     auto block_max = [](uint32_t a) {
@@ -221,8 +239,8 @@ __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
             qr[i] = (__float_as_uint(r[i]) & 0x7fffffffu) < kInf ? qr[i] : __builtin_nanf("");
         }
     }
-    st_codes<V>((uint8_t*)a.m[lo] + i0, left, qm);
-    st_codes<V>((uint8_t*)a.v[lo] + i0, left, qr);
+    st_codes<V>((uint8_t*)a.m[lo] + i0, left, qm, nt);
+    st_codes<V>((uint8_t*)a.v[lo] + i0, left, qr, nt);
     if (left && (threadIdx.x & (QB / V - 1)) == 0) {
         a.ms[lo][blk] = pow2(km);
         a.vs[lo][blk] = pow2(kr);
@@ -278,6 +296,9 @@ extern "C" int mtk_adamw_step(int n_tensors, void* const* p, const void* const* 
         if (numel[i] / chunk >= (1 << 23)) MTK_FAIL(MTK_ERR_UNSUPPORTED, "mtk_adamw_step: tensor %d has %lld values", i, (long long)numel[i]);
     }
     AdamwArgs a;
+    int64_t bytes = 0;
+    for (int i = 0; i < n_tensors; ++i) bytes += numel[i] * (3 * mtk_dtype_size(dtype) + (state_bits == 8 ? 4 : 16));
+    a.nt = bytes > kCaches;
     if (!hyper_dev) a.h = hyper(lr, beta1, beta2, eps, weight_decay, (double)step, (uint32_t)step);
     a.dyn = (const AdamwHyper*)hyper_dev;
     int i = 0;
