@@ -1448,6 +1448,7 @@ extern "C" int mtk_adapter_forward(int64_t M, int din, int dout, int r, int E, i
     if (const int rc = adapter_check("mtk_adapter_forward", M, din, dout, r, E, dtype, x_ld, act)) return rc;
     if (M == 0) return MTK_OK;
     if (!x || !W || !down || !up || !offsets || !y || !saved) MTK_FAIL(MTK_ERR_ARG, "mtk_adapter_forward: null pointer");
+    if (((uintptr_t)saved | (uintptr_t)work) % 256) MTK_FAIL(MTK_ERR_ARG, "mtk_adapter_forward: saved and work have to lie on 256 bytes");
     const Saved sv(M, r, dtype);
     if (saved_bytes < sv.bytes) MTK_FAIL(MTK_ERR_ARG, "mtk_adapter_forward: a buffer of %lld bytes for the low-rank rows, %lld needed", (long long)saved_bytes, (long long)sv.bytes);
     const ForwardWork wk(Layout(), M, din, dout, r, E, dtype, !streams(x, x_ld, din, dtype), !streams(W, din, din, dtype));
@@ -1501,6 +1502,7 @@ extern "C" int mtk_adapter_backward(int64_t M, int din, int dout, int r, int E, 
     if (const int rc = adapter_check("mtk_adapter_backward", M, din, dout, r, E, dtype, x_ld, act)) return rc;
     if (M == 0) return MTK_OK;
     if (!x || !W || !down || !up || !offsets || !dy || !saved || !work || (act && !y)) MTK_FAIL(MTK_ERR_ARG, "mtk_adapter_backward: null pointer");
+    if (((uintptr_t)saved | (uintptr_t)work) % 256) MTK_FAIL(MTK_ERR_ARG, "mtk_adapter_backward: saved and work have to lie on 256 bytes");
     const Saved sv(M, r, dtype);
     // (under an activation the masked gradient is a copy in the workspace, aligned)
     const BackwardWork wk(Layout(), M, din, dout, r, E, dtype, act == 1, act ? !streams(nullptr, dout, dout, dtype) : !streams(dy, dout, dout, dtype));

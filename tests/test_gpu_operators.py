@@ -178,6 +178,34 @@ def test_rows_past_the_caches():
     assert torch.equal(mtk.combine_rows(big, plan), torch.cat([2 * x, 2 * x], 1))
 
 
+@pytest.mark.parametrize("dt,D", [(torch.float32, 509), (torch.bfloat16, 1021), (torch.float16, 8)])
+def test_rows_past_the_caches_are_the_same_rows(dt, D):
+    """Odd rows, weights and gradients of a call that goes past the caches, against the same records in two calls that do not"""
+    size = torch.finfo(dt).bits // 8
+    N, k = (400 << 20) // (3 * D * size), 2  # x and its two copies: 400 MB
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x, y = (torch.randn(n, D, device=DEV, generator=g).to(dt) for n in (N, N * k))
+    w = torch.randn(N, k, device=DEV, generator=g)
+    idx = torch.randint(-1, 5, (N, k), device=DEV, generator=g)
+    plan = mtk.route_rows(idx, 5)
+    ys = y[plan.slot.long().view(-1)]  # a pair's row, in pair order
+    leaves = [t.clone().requires_grad_() for t in (y, w)]
+    out = mtk.combine_rows(leaves[0], plan, leaves[1])
+    dy, dw = torch.autograd.grad(out, leaves, x)
+    xs = mtk.dispatch_rows(x, plan)
+    assert min(t.numel() * size for t in (xs, y)) + x.numel() * size > 256 << 20
+    for part in (slice(0, N // 2), slice(N // 2, N)):
+        p = mtk.route_rows(idx[part], 5)
+        rows = ys.view(N, k, D)[part].reshape(-1, D)[p.order.long()].contiguous()
+        small = [rows.requires_grad_(), w[part].clone().requires_grad_()]
+        o = mtk.combine_rows(small[0], p, small[1])
+        sy, sw = torch.autograd.grad(o, small, x[part])
+        pairs = plan.slot[part].long().view(-1)
+        assert torch.equal(o, out[part]) and torch.equal(sw, dw[part])
+        assert torch.equal(sy[p.slot.long().view(-1)], dy[pairs])
+        assert torch.equal(mtk.dispatch_rows(x[part], p)[p.slot.long().view(-1)], xs[pairs])
+
+
 def test_rows_strides_and_shapes():
     g = gen(3)
     N, k, E, D = 40, 2, 5, 24
@@ -678,6 +706,38 @@ def test_adamw_extremes():
                 opt.step()
             assert bool(torch.isfinite(p).all()), (value, bits)
             assert bool((p <= 1).all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dt", DTYPES)
+def test_a_step_past_the_caches_is_the_same_step(dt, bits):
+    """Tensors that together exceed what the caches hold take another way through memory; one by one they do not"""
+    per = 3 * torch.finfo(dt).bits // 8 + (16 if bits == 32 else 4)
+    n = (300 << 20) // per // 3
+    g = torch.Generator(device=DEV).manual_seed(5)
+    sides = []
+    for odd in (0, 1, 3):  # a start inside a tensor: rows of 16 bytes begin anywhere
+        p, q = (torch.randn(n + odd, device=DEV, generator=g).to(dt)[odd:] for _ in range(2))
+        sides.append((p, q))
+    assert sum(p.numel() for p, _ in sides) * per > 256 << 20
+    blocks = -(-n // 256)
+
+    def state():
+        if bits == 8:
+            return [torch.zeros(n, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn) for _ in range(2)] + [torch.ones(blocks, device=DEV) for _ in range(2)]
+        return [torch.zeros(n, device=DEV) for _ in range(2)]
+
+    def run(ps, qs, states, t):
+        kw = dict(exp_avg_scales=[s[2] for s in states], exp_avg_sq_scales=[s[3] for s in states]) if bits == 8 else {}
+        mtk.adamw_step(ps, qs, [s[0] for s in states], [s[1] for s in states], t, lr=1e-2, **kw)
+
+    whole, single = ([(p.clone(), q, state()) for p, q in sides] for _ in range(2))
+    for t in (1, 2):
+        run(*zip(*whole), t)
+        for one in single:
+            run(*zip(one), t)
+    for (p, _, s), (q, _, z) in zip(whole, single):
+        assert torch.equal(p, q) and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(s, z))
 
 
 def test_adamw_many_tensors_and_empty_ones():

@@ -70,6 +70,9 @@ def test_c_entries_refuse_before_any_launch():
     assert fwd(M=5000, din=64, dout=64) == ARG  # no workspace
     assert l.mtk_adapter_backward(4, 8, 8, 2, 2, 0, one, 8, one, one, one, one, None, 1.0, 0, None, one, one, one, one, one, one, 16, None) == ARG
     assert l.mtk_adapter_backward(4, 8, 8, 2, 2, 0, one, 8, one, one, one, one, None, 1.0, 1, None, one, one, one, one, one, one, 1 << 30, None) == ARG
+    for saved, work in ((264, 256), (256, 272)):  # 256-byte alignment is part of the layout
+        assert l.mtk_adapter_forward(600, 8, 8, 2, 2, 0, one, 8, one, one, one, one, one, None, 1.0, 0, 0, one, saved, 1 << 30, work, 1 << 30, None) == ARG
+        assert l.mtk_adapter_backward(600, 8, 8, 2, 2, 0, one, 8, one, one, one, one, None, 1.0, 0, None, one, saved, one, one, one, work, 1 << 30, None) == ARG
     ptrs, n = (C.c_void_p * 1)(256), (C.c_int64 * 1)(5)
     step = lambda dt=0, bits=32, lr=1e-3, b1=0.9, t=1, sc=ptrs, size=n, p=ptrs: l.mtk_adamw_step(  # noqa: E731
         1, p, ptrs, ptrs, ptrs, sc, sc, size, dt, bits, lr, b1, 0.999, 1e-8, 0.01, t, None, None)
