@@ -442,6 +442,46 @@ def test_tiles_that_models_share(M, din, dout, E, tile, dt):
         assert torch.equal(again.cpu()[~mine], dx.cpu()[~mine]) and not bool(torch.isfinite(again.cpu()[mine]).any()), value
 
 
+@pytest.mark.parametrize("M,din,dout,dt", [(1500, 72, 80, torch.bfloat16), (33 * 128 + 5, 1030, 1030, torch.float16), (700, 64, 96, torch.float32)])
+def test_a_captured_layer_follows_its_offsets(M, din, dout, dt):
+    """The models' borders are on the device: a replay takes those that its offsets hold, and what the last replay left in the workspace (rows of
+    tiles that other models shared, a model that diverged) is not seen"""
+    g = gen(M + 1)
+    E = 7
+    a = adapter_inputs(g, M, din, dout, 12, E, dt)
+    gy = randn(g, M, dout, dt=dt)
+    borders = [shared_offsets(M, E, 64), torch.tensor([0] * E + [M], dtype=torch.int32, device=DEV), shared_offsets(M, E, 128, 19), torch.zeros(E + 1, dtype=torch.int32, device=DEV),
+               shared_offsets(M, E, 32, 5)]
+    for n in ("x", "down", "up"):
+        a[n].requires_grad_()
+    off = borders[0].clone()
+
+    def work():
+        y = call(a, offsets=off)
+        return (y.detach(),) + torch.autograd.grad(y, (a["x"], a["down"], a["up"]), gy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    finite = a["up"].detach().clone()
+    for turn, border in enumerate(borders + borders):
+        off.copy_(border)
+        with torch.no_grad():
+            a["up"].copy_(finite)
+            if turn == 4:
+                a["up"][5] = float("nan")
+        want = work()
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(got, want):
+            assert torch.equal(torch.nan_to_num(p.float(), nan=7e4), torch.nan_to_num(q.float(), nan=7e4)), turn
+
+
 @pytest.mark.parametrize("dt", DTYPES)
 def test_more_models_in_a_tile_than_it_streams(dt):
     """Twelve models inside one tile of 64 rows beside eight long ones, and two dozen of three rows each"""
