@@ -724,23 +724,31 @@ __global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)
 
 // k_linear_few, for few rows: bound by the latency of streaming W once.  TS rows x TS features a workgroup (16 up to 64 rows, else 32), its eight
 // waves split k and take their fragments straight from memory; partial sums meet in LDS.  The low-rank product is plain FMAs there, each row
-// with its own model.  One row of 1,024 bf16 6.0 us, 61 rows of 512 to 1,024 features fp32 5.5 us.
+// with its own model.  61 rows of 512 to 1,024 features fp32 5.5 us.
 // What the end needs (offsets, bias, the low-rank operands) is requested between the first lines' loads and their
 // products: each would be a round trip of its own otherwise.
+// FUSED, for a row or some (M r <= kFusedPairs): every workgroup computes u itself, a wave a value at a time, under W's loads; the first writes it
+// for the backward.  One launch for two, whose own time is, fused / apart, in us: one row of 1,024 at rank 8 in bf16 7.3 / 6.2 + 3.8, at rank
+// 32 10.8 / 6.8 + 5.1, sixteen of 512 at rank 2 in fp32 9.5 / 6.0 + 4.8; four values at a time 15 for the first.
+constexpr int kFusedPairs = 32;
 struct FewArgs {
     int64_t M, x_ld;
     int N, K, r, rp, E, relu;
     const int32_t* offsets;
+    const float* scales;  // FUSED from here on
+    float scale;
+    int64_t Mp;
 };
 
-template <typename T, int TS>
+template <typename T, int TS, bool FUSED>
 __global__ __launch_bounds__(512) void k_linear_few(FewArgs g, const T* __restrict__ x, const T* __restrict__ W, const T* __restrict__ bias, const T* __restrict__ u,
-                                                    const T* __restrict__ up, T* __restrict__ y) {
+                                                    const T* __restrict__ up, T* __restrict__ y, const T* __restrict__ down, T* __restrict__ u_out, T* __restrict__ uT) {
     constexpr int V = mtk_piece<T>::n, KB = kLine<T>, NW = 8;
     constexpr int LANES = 64 / TS, S = 8 / LANES;  // lanes that share a row, steps of a line
     constexpr int OUT = TS * TS > 512 ? 2 : 1;     // outputs of a thread
     typedef typename std::conditional<TS == 32, f32x16, f32x4>::type Acc;
     __shared__ float part[NW][TS][TS + 1];
+    __shared__ float us[FUSED ? kFusedPairs : 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & (TS - 1), hh = lane / TS;
     const int nb = (g.N + TS - 1) / TS;
     const int64_t m0 = (int64_t)(blockIdx.x / nb) * TS;
@@ -794,8 +802,29 @@ __global__ __launch_bounds__(512) void k_linear_few(FewArgs g, const T* __restri
 #pragma unroll
         for (int p = 0; p < LP; ++p) {
 #pragma unroll
-            for (int h = 0; h < H; ++h) ua[i][p][h] = mtk_ld(ur + h * half + p * V);  // whole lines, zeros behind the rank
+            for (int h = 0; h < H; ++h)
+                if (!FUSED) ua[i][p][h] = mtk_ld(ur + h * half + p * V);  // whole lines, zeros behind the rank
             ba[i][p] = p * V + V <= g.r ? mtk_ld(br + p * V) : mtk_ld_n(br + p * V, g.r - p * V);
+        }
+    }
+    if constexpr (FUSED) {
+        for (int q = wave; q < (int)g.M * g.r; q += NW) {
+            const int row = q / g.r, j = q - row * g.r;
+            int c = __popcll(__ballot(held <= row));
+            for (int e0 = 64; e0 <= g.E; e0 += 64) c += __popcll(__ballot((e0 + lane <= g.E ? g.offsets[e0 + lane] : 0x7fffffff) <= row));
+            const int e = c - 1;
+            float v = 0.f;
+            if (e >= 0 && e < g.E) {
+                const T *xp = x + row * g.x_ld, *ap = down + ((int64_t)e * g.r + j) * g.K;
+                for (int k = lane * V; k < g.K; k += 64 * V) {
+                    const mtk_vec<T> a = k + V <= g.K ? mtk_ld(ap + k) : mtk_ld_n(ap + k, g.K - k), b = k + V <= g.K ? mtk_ld(xp + k) : mtk_ld_n(xp + k, g.K - k);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) v += (float)a.v[i] * (float)b.v[i];
+                }
+                for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+                v *= g.scales ? g.scales[e] : g.scale;
+            }
+            if (lane == 0) us[q] = v;
         }
     }
     Acc acc = {};
@@ -840,7 +869,18 @@ __global__ __launch_bounds__(512) void k_linear_few(FewArgs g, const T* __restri
         float v = bv;
 #pragma unroll
         for (int w = 0; w < NW; ++w) v += part[w][rr + 16 * i][tid & (TS - 1)];
-        if (who[i] >= 0) {
+        if (FUSED && who[i] >= 0) {
+            const float* ui = us + row * g.r;
+            const T* br = up + ((int64_t)who[i] * g.N + n) * g.r;
+            float low = 0.f;
+#pragma unroll
+            for (int p = 0; p < LP; ++p)
+#pragma unroll
+                for (int c = 0; c < V; ++c)
+                    if (p * V + c < g.r) low += ui[p * V + c] * (float)ba[i][p].v[c];
+            for (int j = LP * V; j < g.r; ++j) low += ui[j] * (float)br[j];
+            v += low;
+        } else if (who[i] >= 0) {
             float low = 0.f;
 #pragma unroll
             for (int p = 0; p < LP; ++p)
@@ -856,6 +896,23 @@ __global__ __launch_bounds__(512) void k_linear_few(FewArgs g, const T* __restri
         }
         if (g.relu) v = v < 0.f ? 0.f : v;
         y[row * g.N + n] = (T)v;
+    }
+    if (FUSED && n0 == 0) {  // u for the backward, laid out as k_shrink does
+        for (int i = tid; i < (int)g.M * half; i += 512) {
+            const int row = i / half, j = i - row * half;
+            const float v = j < g.r ? us[row * g.r + j] : 0.f;
+            u_out[row * g.rp + j] = (T)v;
+            if (H == 2) u_out[row * g.rp + half + j] = low_half(v, (T)v);
+        }
+        if (uT) {
+            const int64_t plane = mtk_up(g.r, 64) * g.Mp;
+            for (int i = tid; i < (int)(mtk_up(g.r, 16) * g.Mp); i += 512) {
+                const int j = i / (int)g.Mp, row = i - j * (int)g.Mp;
+                const float v = j < g.r && row < g.M ? us[row * g.r + j] : 0.f;
+                uT[i] = (T)v;
+                uT[plane + i] = low_half(v, (T)v);
+            }
+        }
     }
 }
 
@@ -1376,8 +1433,13 @@ template <typename T> int linear(const Shape& sh, LinearArgs& g, T* y, hipStream
 }
 template <typename T>
 void linear_few(const FewArgs& g, const T* x, const T* W, const T* bias, const T* u, const T* up, T* y, hipStream_t s) {
-    if (g.M <= 64) k_linear_few<T, 16><<<(unsigned)(cdiv(g.M, 16) * cdiv(g.N, 16)), 512, 0, s>>>(g, x, W, bias, u, up, y);
-    else k_linear_few<T, 32><<<(unsigned)(cdiv(g.M, 32) * cdiv(g.N, 32)), 512, 0, s>>>(g, x, W, bias, u, up, y);
+    if (g.M <= 64) k_linear_few<T, 16, false><<<(unsigned)(cdiv(g.M, 16) * cdiv(g.N, 16)), 512, 0, s>>>(g, x, W, bias, u, up, y, nullptr, nullptr, nullptr);
+    else k_linear_few<T, 32, false><<<(unsigned)(cdiv(g.M, 32) * cdiv(g.N, 32)), 512, 0, s>>>(g, x, W, bias, u, up, y, nullptr, nullptr, nullptr);
+}
+// the shrink and the product of a row or some
+template <typename T>
+void linear_fused(const FewArgs& g, const T* x, const T* W, const T* bias, const T* down, const T* up, T* u, T* uT, T* y, hipStream_t s) {
+    k_linear_few<T, 16, true><<<(unsigned)cdiv(g.N, 16), 512, 0, s>>>(g, x, W, bias, u, up, y, down, u, uT);
 }
 // the jobs of a k_linear product: x and W padded where they do not stream, B_e in whole lines and a block of zeros, bias, tiles' models.
 // `early`: what the shrink reads.  F: W [N][K], or its transpose [K][N] when `turned`; L: B [E][N][r], or [E][r][N]
@@ -1462,8 +1524,13 @@ extern "C" int mtk_adapter_forward(int64_t M, int din, int dout, int r, int E, i
         T* uT = keep && sizeof(T) == 2 ? (T*)((char*)saved + sv.uT) : nullptr;
         ShrinkArgs sa{M, din, r, sh.rp, E, x_ld, offsets, scales, (float)scale, sv.Mp, (char*)work + wk.pk.pairs, sh.blocks && !sh.few ? sh.BM : 0, 1, 1};
         if (sh.few) {
+            const FewArgs fa{M, x_ld, dout, din, r, sh.rp, E, act, offsets, scales, (float)scale, sv.Mp};
+            if (M * r <= kFusedPairs && M <= 16) {
+                linear_fused<T>(fa, (const T*)x, (const T*)W, (const T*)bias, (const T*)down, (const T*)up, u, uT, (T*)y, s);
+                return;
+            }
             shrink<T>(sa, Jobs(), (const T*)x, (const T*)down, u, uT, s);
-            linear_few<T>(FewArgs{M, x_ld, dout, din, r, sh.rp, E, act, offsets}, (const T*)x, (const T*)W, (const T*)bias, u, (const T*)up, (T*)y, s);
+            linear_few<T>(fa, (const T*)x, (const T*)W, (const T*)bias, u, (const T*)up, (T*)y, s);
             return;
         }
         Jobs early, jobs;
@@ -1543,7 +1610,7 @@ extern "C" int mtk_adapter_backward(int64_t M, int din, int dout, int r, int E, 
             shrink<T>(ShrinkArgs{M, gk, r, sh.rp, E, gk, offsets, scales, (float)scale, sv.Mp, wb + wk.pk.pairs, dx && sh.blocks && !sh.few ? sh.BM : 0, 1, 1},
                       jobs, g, (const T*)(wb + wk.Bt), t, ddown && sizeof(T) == 2 ? tT : nullptr, s);
         if (dx) {
-            if (sh.few) linear_few<T>(FewArgs{M, dout, din, dout, r, sh.rp, E, 0, offsets}, g, (const T*)(wb + wk.Wt), nullptr, t, (const T*)(wb + wk.At), (T*)dx, s);
+            if (sh.few) linear_few<T>(FewArgs{M, dout, din, dout, r, sh.rp, E, 0, offsets, scales, (float)scale, sv.Mp}, g, (const T*)(wb + wk.Wt), nullptr, t, (const T*)(wb + wk.At), (T*)dx, s);
             else rc = linear<T>(sh, lin, (T*)dx, s);
         }
         if (ddown || dup)

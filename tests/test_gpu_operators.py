@@ -272,7 +272,7 @@ def tol_factor(mag, K, rows, want, dt, other):
 SHAPES = [(1, 1, 1, 1, 1, "any"), (1, 64, 64, 8, 4, "any"), (2, 7, 5, 3, 2, "any"), (31, 130, 67, 12, 5, "any"), (33, 64, 128, 16, 3, "last"), (64, 33, 130, 17, 64, "any"),
           (127, 257, 129, 33, 7, "few"), (130, 96, 200, 64, 4, "any"), (300, 70, 66, 100, 2, "any"), (700, 128, 192, 40, 2, "last"), (1100, 100, 130, 70, 3, "any"), (129, 40, 24, 256, 3, "any"), (513, 128, 256, 8, 1, "any"),
           (200, 120, 128, 4, 1024, "few"), (1000, 512, 48, 16, 16, "any"), (77, 64, 64, 8, 3, "base"), (2049, 64, 72, 16, 9, "few"), (16, 2050, 40, 8, 4, "any"),
-          (700, 256, 1024, 16, 5, "any"), (9, 300, 1000, 9, 3, "any"), (300, 1030, 1030, 5, 9, "any"), (65, 40, 4100, 6, 7, "any")]
+          (700, 256, 1024, 16, 5, "any"), (9, 300, 1000, 9, 3, "any"), (300, 1030, 1030, 5, 9, "any"), (65, 40, 4100, 6, 7, "any"), (1, 1030, 40, 32, 3, "any"), (4, 513, 33, 8, 70, "any"), (16, 40, 50, 2, 3, "any"), (3, 20, 9, 10, 2, "base")]
 
 
 @pytest.mark.parametrize("dt", DTYPES)
