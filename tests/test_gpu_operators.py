@@ -567,6 +567,35 @@ def test_offsets_that_make_no_sense_stay_inside_the_tensors(M, off):
         within(y, ref["y"], tol(ref["y_terms"], ref["y_low"], din, r, ref["y"], torch.float32, a["up"]))
 
 
+@pytest.mark.parametrize("off", [[0, 3000, 10, 40], [3, 2, 1, 0], [-5, 20, 5000, 9000], [4229, 60, 30, 0], [2**31 - 1] * 4])
+@pytest.mark.parametrize("M,r,dt", [(4, 4, torch.bfloat16), (13, 2, torch.float32), (4229, 12, torch.float16)])
+def test_such_offsets_in_the_fused_call_and_the_larger_tiles(M, r, dt, off):
+    g = gen(M)
+    wide = 1030 if M > 512 else 40
+    a = adapter_inputs(g, M, wide, wide, r, 3, dt)
+    a["offsets"] = torch.tensor(off, dtype=torch.int32, device=DEV)
+    a["x"].requires_grad_()
+    y = call(a)
+    dx = torch.autograd.grad(y, a["x"], torch.ones_like(y))[0]
+    assert bool(torch.isfinite(y).all()) and bool(torch.isfinite(dx).all())
+
+
+def test_operators_in_inference_mode():
+    g = gen(2)
+    a = adapter_inputs(g, 33, 40, 24, 4, 3, torch.float32)
+    idx = torch.randint(-1, 3, (33, 2), generator=g).to(DEV)
+    want = mtk.route_rows(idx, 3)
+    w = torch.rand(33, 2, generator=g).to(DEV)
+    base = mtk.combine_rows(mtk.adapter_linear(mtk.dispatch_rows(a["x"], want), a["weight"], a["bias"], a["down"], a["up"], want), want, w)
+    with torch.inference_mode():
+        plan = mtk.route_rows(idx, 3)
+        got = mtk.combine_rows(mtk.adapter_linear(mtk.dispatch_rows(a["x"], plan), a["weight"], a["bias"], a["down"], a["up"], plan), plan, w)
+        assert torch.equal(got, base) and got.is_inference()
+        p, q, m, v = (torch.ones(300, device=DEV) for _ in range(4))
+        mtk.adamw_step([p], [q], [m], [v], 1, lr=0.1)
+        assert not bool((p == 1).any())
+
+
 # one shape for each tile of the products: 256 x 256 and 128 x 128 with 16 bits, 128 x 128 with fp32, both directions; 32 rows a wave in the shrink
 BIG = [(16384, 64, 1024, 8, 3), (16384, 1024, 64, 20, 2), (20011, 131, 1000, 12, 33), (16500, 1000, 131, 33, 40), (16384, 96, 1024, 40, 70)]
 
