@@ -156,10 +156,14 @@ __device__ __forceinline__ int64_t place_of(int32_t s, int64_t pairs, bool& bad)
     return s < pairs ? s : pairs - 1;
 }
 
+// A row's last piece, where it is not whole, starts earlier and brings some elements a second time: the same values are written twice, and a dot product
+// skips what the lane before has.  (Loads and stores of single elements instead cost every row a second pass through the loop's
+// body; only rows narrower than a piece have them.)
+//
 // xs[slot[n, j]] = x[n] (times w[n, j]) for all copies j: a record's row is read once and written k times.  With y: dw[n, j] =
 // <x[n], y[slot[n, j]]> as well (x is the gradient of the combined rows then).  Bound by bandwidth: a row belongs to lpr lanes, each moving
 // 16-byte pieces, so a wave touches whole lines.  4,099 rows of 1,021 fp32 in four copies (84 MB): 20 us, with the weights' gradient
-// (151 MB) 36 us; 24 rows of 120: 2.7 us, a launch.
+// (151 MB) 30 us; 24 rows of 120: 2.7 us, a launch.
 template <typename T, bool W, bool DOT, int KC>
 __global__ __launch_bounds__(256) void k_dispatch(RowsArgs a, const T* __restrict__ x, T* __restrict__ xs, const T* __restrict__ y, float* __restrict__ dw) {
     constexpr int V = mtk_piece<T>::n;
@@ -185,8 +189,9 @@ __global__ __launch_bounds__(256) void k_dispatch(RowsArgs a, const T* __restric
                 dot[j] = 0.f;
             }
 #pragma unroll 2
-            for (int64_t c = (int64_t)sub * V; c < a.D; c += (int64_t)a.lpr * V) {
-                const int left = a.D - c < V ? (int)(a.D - c) : V;
+            for (int64_t c0 = (int64_t)sub * V; c0 < a.D; c0 += (int64_t)a.lpr * V) {
+                const int64_t c = c0 + V <= a.D || a.D < V ? c0 : a.D - V;
+                const int left = a.D < V ? (int)a.D : V, first = (int)(c0 - c);
                 const mtk_vec<T> v = left < V ? mtk_ld_n(src + c, left) : a.nt ? mtk_ld_nt(src + c) : mtk_ld(src + c);
                 if (DOT) {
 #pragma unroll
@@ -195,7 +200,7 @@ __global__ __launch_bounds__(256) void k_dispatch(RowsArgs a, const T* __restric
                         const T* ys = y + at[j] + c;
                         const mtk_vec<T> q = left < V ? mtk_ld_n(ys, left) : a.nt ? mtk_ld_nt(ys) : mtk_ld(ys);
 #pragma unroll
-                        for (int i = 0; i < V; ++i) dot[j] += (float)v.v[i] * (float)q.v[i];
+                        for (int i = 0; i < V; ++i) dot[j] += i >= first ? (float)v.v[i] * (float)q.v[i] : 0.f;
                     }
                 }
                 if (!DOT || xs) {
@@ -238,8 +243,9 @@ __global__ __launch_bounds__(256) void k_combine(RowsArgs a, const T* __restrict
         const Copies<KC> first = next;
         next = copies_of<W, KC>(a, n + stride, 0);
 #pragma unroll 2
-        for (int64_t c = (int64_t)sub * V; c < a.D; c += (int64_t)a.lpr * V) {
-            const int left = a.D - c < V ? (int)(a.D - c) : V;
+        for (int64_t c0 = (int64_t)sub * V; c0 < a.D; c0 += (int64_t)a.lpr * V) {
+            const int64_t c = c0 + V <= a.D || a.D < V ? c0 : a.D - V;
+            const int left = a.D < V ? (int)a.D : V;
             float acc[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] = 0.f;
@@ -282,7 +288,7 @@ int lanes_per_row(int64_t D, int V) {
 
 // Rows go past the caches, read and written, where what a call moves exceeds what they hold (256 MB): the result's readers would find nothing
 // there.  us, 100,000 rows of 1024 bf16, two copies, past them / reads through them / all through them: dispatch 117 / 115 / 221, weighted combine
-// 131 / 158, dispatch with the weights' gradient 214 / 270 (1.0 GB: 4.8 TB/s, what a large copy reaches).
+// 131 / 158, dispatch with the weights' gradient 204 / 270 (1.0 GB: 5.0 TB/s, past what a large copy reaches).
 constexpr int64_t kCaches = 256ll << 20;
 template <typename F> void by_flags(bool a, bool b, int k, F f) {
     auto third = [&](auto ta, auto tb) {
