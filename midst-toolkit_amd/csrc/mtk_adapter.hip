@@ -17,6 +17,7 @@
 // a row of u holds both halves side by side, against B_e twice: for ranks up to 32 that costs nothing.
 #include <type_traits>
 
+#include "mtk_low_piece.h"
 #include "mtk_lowp.h"
 
 namespace {
@@ -634,26 +635,25 @@ __global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)
             constexpr int S = 32 / (2 * V);  // steps of 32 values of the rank
             const int half = sizeof(T) == 2 ? g.rp / 2 : g.rp, low_n = g.low_ld < half ? g.low_ld : half;  // B_e's values, once
             while (own.next(e, a, b)) {
-                const T* be = (const T*)g.low + (int64_t)e * g.N * g.low_ld + hh_e * V;
+                const T* be = (const T*)g.low + (int64_t)e * g.N * g.low_ld;
 #pragma unroll
                 for (int mt = 0; mt < MW; ++mt) {
                     const int64_t row = w0 + mt * 32 + li_e, rc = row < g.M ? row : g.M - 1;
                     const bool mine = row >= a && row < b;
                     if (a >= w0 + mt * 32 + 32 || b <= w0 + mt * 32) continue;
-                    const T* ur = u + rc * g.rp + hh_e * V;
+                    const T* ur = u + rc * g.rp;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         const int n = n0 + wc * G::WN + nt * 32 + li_e;
-                        const T* bn = be + (int64_t)(n < g.N ? n : g.N - 1) * g.low_ld;
                         f32x16 low = acc[mt][nt];
                         auto steps = [&](int j0, int h, auto count) {  // requested together: one round trip
                             constexpr int C = decltype(count)::value;
                             mtk_vec<T> uv[C], bv[C];
 #pragma unroll
                             for (int s = 0; s < C; ++s) {
-                                const int j = j0 + s * 2 * V;
-                                const bool in = j + hh_e * V < low_n;
-                                const uint4 w = __builtin_bit_cast(uint4, mtk_ld(in ? bn + j : be));
+                                const int j = j0 + s * 2 * V + hh_e * V;
+                                const bool in = j < low_n;
+                                const uint4 w = __builtin_bit_cast(uint4, mtk_ld(be + mtk_low_piece(n, g.N, g.low_ld, low_n, j)));
                                 bv[s] = __builtin_bit_cast(mtk_vec<T>, make_uint4(in ? w.x : 0u, in ? w.y : 0u, in ? w.z : 0u, in ? w.w : 0u));
                                 uv[s] = mtk_ld(ur + h + j);
                             }

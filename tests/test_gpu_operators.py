@@ -500,6 +500,26 @@ def test_more_models_in_a_tile_than_it_streams(dt):
         within(dx, ref["dx"], tol(ref["dx_terms"], ref["dx_low"], dout, r, ref["dx"], dt, a["down"]))
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("r", [4, 8, 5])
+def test_a_layer_of_one_feature_with_many_models(r, dt):
+    """Fewer rows a model than a tile has, and factors of one piece: the last model's is the end of its tensor"""
+    g = gen(r)
+    M, din, E = 1000, 40, 32
+    a = adapter_inputs(g, M, din, 1, r, E, dt)
+    gy = randn(g, M, 1, dt=dt)
+    for n in ("x", "down", "up"):
+        a[n].requires_grad_()
+    y = call(a)
+    ref = adapter_reference(**{**a, "relu": False, "gy": gy})
+    dx, ddown, dup = torch.autograd.grad(y, (a["x"], a["down"], a["up"]), gy)
+    within(y, ref["y"], tol(ref["y_terms"], ref["y_low"], din, r, ref["y"], dt, a["up"]))
+    within(dx, ref["dx"], tol(ref["dx_terms"], ref["dx_low"], 1, r, ref["dx"], dt, a["down"]))
+    rows = int((a["offsets"][1:] - a["offsets"][:-1]).max())
+    within(ddown, ref["ddown"], tol_factor(ref["ddown_terms"], 1, rows, ref["ddown"], dt, a["x"]))
+    within(dup, ref["dup"], tol_factor(ref["dup_terms"], din, rows, ref["dup"], dt, gy))
+
+
 def test_adapter_strides_scales_and_plans():
     g = gen(4)
     M, din, dout, r, E = 60, 40, 24, 4, 3

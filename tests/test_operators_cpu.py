@@ -1,5 +1,7 @@
 """CPU: refusals of the row routing, low-rank adapter and AdamW entry points, and the arithmetic of the 8-bit moments' rounding."""
 import ctypes as C
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -123,3 +125,34 @@ def test_eight_bit_moments_follow_a_change_of_scale():
         ms, rs = float(ms[0]), float(rs[0])
     want = np.sqrt(0.01 + 0.99 * 0.999**3000)
     assert np.all(np.abs(r * rs / want - 1) < 0.25), (r * rs).min()
+
+
+def test_pieces_of_a_factor_lie_inside_it(tmp_path):
+    """The adapter kernels' lanes without a piece of their own load one all the same (and clear it): for every width from one feature on and
+    every rank, each lane's piece has to lie inside its model's factor, the last model's with nothing behind it."""
+    main = tmp_path / "pieces.cpp"
+    main.write_text(r'''
+#include <cstdio>
+#include <initializer_list>
+#include "mtk_low_piece.h"
+int main() {
+    for (int V : {4, 8})                                     // values of a 16-byte piece
+        for (int N : {1, 2, 31, 33})
+            for (int r = 1; r <= 256; ++r) {
+                const int ld = (r + V - 1) / V * V;
+                for (int n = 0; n < 64; ++n)                     // features of a tile, behind the last too
+                    for (int j = 0; j < (r + 31) / 32 * 32; j += V) {  // the pieces of 32 values of the rank at a time
+                        const int64_t at = mtk_low_piece(n, N, ld, ld, j);
+                        if (at < 0 || at + V > (int64_t)N * ld || (j < r && at != (int64_t)(n < N ? n : N - 1) * ld + j)) {
+                            std::printf("V %d N %d r %d feature %d value %d: offset %lld\n", V, N, r, n, j, (long long)at);
+                            return 1;
+                        }
+                    }
+            }
+}
+''')
+    exe = tmp_path / "pieces"
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "midst-toolkit_amd", "csrc")
+    subprocess.run(["g++", "-std=c++17", "-I", csrc, str(main), "-o", str(exe)], check=True)
+    got = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert got.returncode == 0, got.stdout
