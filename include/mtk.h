@@ -544,7 +544,9 @@ int mtk_adapter_backward(int64_t M, int din, int dout, int r, int n_models, int 
  * (mtk_adamw_scales(numel) of them); a non-finite value is NaN.  step: the count of this step, from 1.
  * mtk_adamw_count: for a step count on the device (*step is raised by one when the call RUNS, so a captured step counts its replays);
  * it writes what the step needs to hyper_dev (mtk_adamw_hyper_bytes), which mtk_adamw_step then reads instead of lr ... step.
- * lr_dev: fp32 scalar read instead of lr, or NULL. */
+ * lr_dev: fp32 scalar read instead of lr, or NULL.
+ * The _each forms: a count for every tensor.  step_host: n_steps HOST-side entries of DEVICE pointers, no counter twice; hyper_dev: n_steps
+ * times mtk_adamw_hyper_bytes, in the order of the tensors of the step that reads them. */
 int64_t mtk_adamw_scales(int64_t numel);
 int64_t mtk_adamw_hyper_bytes(void);
 int mtk_adamw_count(int64_t* step, const float* lr_dev, double lr, double beta1, double beta2, double eps, double weight_decay, void* hyper_dev,
@@ -552,6 +554,10 @@ int mtk_adamw_count(int64_t* step, const float* lr_dev, double lr, double beta1,
 int mtk_adamw_step(int n_tensors, void* const* p_host, const void* const* g_host, void* const* m_host, void* const* v_host, float* const* m_scale_host,
                    float* const* v_scale_host, const int64_t* numel_host, int dtype, int state_bits, double lr, double beta1, double beta2, double eps,
                    double weight_decay, int64_t step, const void* hyper_dev, mtk_stream stream);
+int mtk_adamw_count_each(int n_steps, int64_t* const* step_host, const float* lr_dev, double lr, double beta1, double beta2, double eps, double weight_decay,
+                         void* hyper_dev, mtk_stream stream);
+int mtk_adamw_step_each(int n_tensors, void* const* p_host, const void* const* g_host, void* const* m_host, void* const* v_host, float* const* m_scale_host,
+                        float* const* v_scale_host, const int64_t* numel_host, int dtype, int state_bits, const void* hyper_dev, mtk_stream stream);
 
 #ifdef __cplusplus
 }

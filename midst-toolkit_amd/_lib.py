@@ -29,7 +29,7 @@ _lib = None
 _native = None
 # the library functions that _mtk_torch calls, in the order of its table
 _NATIVE = ["mtk_last_error", "mtk_route_rows_work", "mtk_route_rows", "mtk_rows_dispatch", "mtk_rows_combine", "mtk_adapter_saved_bytes", "mtk_adapter_streams", "mtk_adapter_work_bytes",
-           "mtk_adapter_forward", "mtk_adapter_backward", "mtk_adamw_step"]
+           "mtk_adapter_forward", "mtk_adapter_backward", "mtk_adamw_step", "mtk_adamw_step_each"]
 
 _p, _i64, _i32, _u64 = C.c_void_p, C.c_int64, C.c_int, C.c_uint64
 _SIGS = {
@@ -113,6 +113,8 @@ _SIGS = {
     "mtk_adamw_hyper_bytes": (_i64, []),
     "mtk_adamw_count": (C.c_int, [_p, _p, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, _p, _p]),
     "mtk_adamw_step": (C.c_int, [_i32, _p, _p, _p, _p, _p, _p, _p, _i32, _i32, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, _i64, _p, _p]),
+    "mtk_adamw_count_each": (C.c_int, [_i32, _p, _p, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, _p, _p]),
+    "mtk_adamw_step_each": (C.c_int, [_i32, _p, _p, _p, _p, _p, _p, _p, _i32, _i32, _p, _p]),
     "mtk_train_export": (C.c_int, [_p, _i32, _p, _p, _p]),
     "mtk_train_import": (C.c_int, [_p, _i32, _p, _p, _p]),
 }

@@ -45,7 +45,8 @@ struct AdamwArgs {
     int n;
     bool nt;                   // past the caches
     AdamwHyper h;
-    const AdamwHyper* dyn;     // read instead of h where given (a step whose count lives on the device)
+    const AdamwHyper* dyn;     // read instead of h where given (a step whose count lives on the device): dyn[each * tensor]
+    int each;                  // 1: every tensor has its own count, 0: one for all
 };
 
 constexpr uint32_t kPhi = 0x9E3779B1u, kPlaceM = 0x6A09E667u, kPlaceR = 0xBB67AE85u;
@@ -148,7 +149,7 @@ __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
         if (a.first[mid] <= b) lo = mid;
         else hi = mid - 1;
     }
-    const AdamwHyper h = a.dyn ? *a.dyn : a.h;
+    const AdamwHyper h = a.dyn ? a.dyn[lo * a.each] : a.h;
     const int64_t n = a.numel[lo], i0 = (int64_t)(b - a.first[lo]) * CH + (int64_t)threadIdx.x * V;
     const int left = n - i0 >= V ? V : (n > i0 ? (int)(n - i0) : 0);
     T* pp = (T*)a.p[lo] + i0;
@@ -258,11 +259,19 @@ __host__ __device__ inline AdamwHyper hyper(double lr, double b1, double b2, dou
     return h;
 }
 
-// the step count on the device: counted up here, so a replayed graph's steps are its own
-__global__ void k_adamw_count(int64_t* step, const float* lr_dev, double lr, double b1, double b2, double eps, double wd, AdamwHyper* out) {
-    const int64_t t = *step + 1;
-    *step = t;
-    *out = hyper(lr_dev ? (double)*lr_dev : lr, b1, b2, eps, wd, (double)t, (uint32_t)t);
+// Step counts on the device: counted up here, so a replayed graph's steps are its own.  A count belongs to a tensor (one may go without a gradient
+// where its neighbours have theirs); a thread takes one.
+constexpr int MAXC = 256;      // counts of a launch
+struct CountArgs {
+    int64_t* step[MAXC];
+    int n;
+};
+__global__ __launch_bounds__(MAXC) void k_adamw_count(CountArgs a, const float* lr_dev, double lr, double b1, double b2, double eps, double wd, AdamwHyper* out) {
+    const int i = threadIdx.x;
+    if (i >= a.n) return;
+    const int64_t t = *a.step[i] + 1;
+    *a.step[i] = t;
+    out[i] = hyper(lr_dev ? (double)*lr_dev : lr, b1, b2, eps, wd, (double)t, (uint32_t)t);
 }
 
 }  // namespace
@@ -270,17 +279,28 @@ __global__ void k_adamw_count(int64_t* step, const float* lr_dev, double lr, dou
 extern "C" int64_t mtk_adamw_scales(int64_t numel) { return numel > 0 ? (numel + QB - 1) / QB : 0; }
 extern "C" int64_t mtk_adamw_hyper_bytes(void) { return (int64_t)sizeof(AdamwHyper); }
 
-extern "C" int mtk_adamw_count(int64_t* step, const float* lr_dev, double lr, double beta1, double beta2, double eps, double weight_decay,
-                               void* hyper_dev, mtk_stream stream) {
-    if (!step || !hyper_dev) MTK_FAIL(MTK_ERR_ARG, "mtk_adamw_count: null pointer");
-    k_adamw_count<<<1, 1, 0, (hipStream_t)stream>>>(step, lr_dev, lr, beta1, beta2, eps, weight_decay, (AdamwHyper*)hyper_dev);
+extern "C" int mtk_adamw_count_each(int n_steps, int64_t* const* step, const float* lr_dev, double lr, double beta1, double beta2, double eps, double weight_decay,
+                                    void* hyper_dev, mtk_stream stream) {
+    if (n_steps < 0 || (n_steps > 0 && (!step || !hyper_dev))) MTK_FAIL(MTK_ERR_ARG, "mtk_adamw_count: null pointer or negative count");
+    for (int i = 0; i < n_steps; ++i)
+        if (!step[i]) MTK_FAIL(MTK_ERR_ARG, "mtk_adamw_count: step %d: null pointer", i);
+    for (int i = 0; i < n_steps; i += MAXC) {
+        CountArgs a;
+        a.n = n_steps - i < MAXC ? n_steps - i : MAXC;
+        for (int j = 0; j < a.n; ++j) a.step[j] = step[i + j];
+        k_adamw_count<<<1, MAXC, 0, (hipStream_t)stream>>>(a, lr_dev, lr, beta1, beta2, eps, weight_decay, (AdamwHyper*)hyper_dev + i);
+    }
     MTK_HIP(hipGetLastError());
     return MTK_OK;
 }
+extern "C" int mtk_adamw_count(int64_t* step, const float* lr_dev, double lr, double beta1, double beta2, double eps, double weight_decay,
+                               void* hyper_dev, mtk_stream stream) {
+    return mtk_adamw_count_each(1, &step, lr_dev, lr, beta1, beta2, eps, weight_decay, hyper_dev, stream);
+}
 
-extern "C" int mtk_adamw_step(int n_tensors, void* const* p, const void* const* g, void* const* m, void* const* v, float* const* m_scale,
-                              float* const* v_scale, const int64_t* numel, int dtype, int state_bits, double lr, double beta1, double beta2,
-                              double eps, double weight_decay, int64_t step, const void* hyper_dev, mtk_stream stream) {
+static int adamw_step(int n_tensors, void* const* p, const void* const* g, void* const* m, void* const* v, float* const* m_scale, float* const* v_scale,
+                      const int64_t* numel, int dtype, int state_bits, double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step,
+                      const void* hyper_dev, int each, mtk_stream stream) {
     if (n_tensors < 0 || (n_tensors > 0 && (!p || !g || !m || !v || !numel))) MTK_FAIL(MTK_ERR_ARG, "mtk_adamw_step: null pointer or negative count");
     if (!mtk_dtype_ok(dtype)) MTK_FAIL(MTK_ERR_UNSUPPORTED, "mtk_adamw_step: dtype %d", dtype);
     if (state_bits != 32 && state_bits != 8) MTK_FAIL(MTK_ERR_UNSUPPORTED, "mtk_adamw_step: moments in %d bits (8 or 32)", state_bits);
@@ -300,13 +320,13 @@ extern "C" int mtk_adamw_step(int n_tensors, void* const* p, const void* const* 
     for (int i = 0; i < n_tensors; ++i) bytes += numel[i] * (3 * mtk_dtype_size(dtype) + (state_bits == 8 ? 4 : 16));
     a.nt = bytes > kCaches;
     if (!hyper_dev) a.h = hyper(lr, beta1, beta2, eps, weight_decay, (double)step, (uint32_t)step);
-    a.dyn = (const AdamwHyper*)hyper_dev;
+    a.each = each;
     int i = 0;
     while (i < n_tensors) {
         a.n = 0;
+        a.dyn = hyper_dev ? (const AdamwHyper*)hyper_dev + (each ? i : 0) : nullptr;
         int64_t chunks = 0;
-        for (; i < n_tensors && a.n < MAXT; ++i) {
-            if (numel[i] == 0) continue;
+        for (; i < n_tensors && a.n < MAXT; ++i) {  // an empty tensor has no chunk, but its place among the counts
             const int64_t c = (numel[i] + chunk - 1) / chunk;
             if (chunks + c >= (1 << 24)) break;  // a launch holds fewer than 2^32 threads
             a.p[a.n] = p[i]; a.g[a.n] = g[i]; a.m[a.n] = m[i]; a.v[a.n] = v[i];
@@ -316,7 +336,7 @@ extern "C" int mtk_adamw_step(int n_tensors, void* const* p, const void* const* 
             a.first[a.n++] = (int32_t)chunks;
             chunks += c;
         }
-        if (a.n == 0) break;
+        if (chunks == 0) continue;
         a.first[a.n] = (int32_t)chunks;
         mtk_by_type(dtype, [&](auto t) {
             typedef decltype(t) T;
@@ -326,4 +346,15 @@ extern "C" int mtk_adamw_step(int n_tensors, void* const* p, const void* const* 
     }
     MTK_HIP(hipGetLastError());
     return MTK_OK;
+}
+
+extern "C" int mtk_adamw_step(int n_tensors, void* const* p, const void* const* g, void* const* m, void* const* v, float* const* m_scale,
+                              float* const* v_scale, const int64_t* numel, int dtype, int state_bits, double lr, double beta1, double beta2,
+                              double eps, double weight_decay, int64_t step, const void* hyper_dev, mtk_stream stream) {
+    return adamw_step(n_tensors, p, g, m, v, m_scale, v_scale, numel, dtype, state_bits, lr, beta1, beta2, eps, weight_decay, step, hyper_dev, 0, stream);
+}
+extern "C" int mtk_adamw_step_each(int n_tensors, void* const* p, const void* const* g, void* const* m, void* const* v, float* const* m_scale, float* const* v_scale,
+                                   const int64_t* numel, int dtype, int state_bits, const void* hyper_dev, mtk_stream stream) {
+    if (n_tensors > 0 && !hyper_dev) MTK_FAIL(MTK_ERR_ARG, "mtk_adamw_step: null pointer or negative count");
+    return adamw_step(n_tensors, p, g, m, v, m_scale, v_scale, numel, dtype, state_bits, 0.0, 0.0, 0.0, 0.0, 0.0, 1, hyper_dev, 1, stream);
 }

@@ -40,6 +40,7 @@ struct Table {
     decltype(&mtk_adapter_forward) adapter_forward;
     decltype(&mtk_adapter_backward) adapter_backward;
     decltype(&mtk_adamw_step) adamw_step;
+    decltype(&mtk_adamw_step_each) adamw_step_each;
 };
 constexpr int kEntries = sizeof(Table) / sizeof(void*);
 union {
@@ -439,9 +440,11 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int64_t step = integer(a[6]);
         const double lr = real(a[7]), b1 = real(a[8]), b2 = real(a[9]), eps = real(a[10]), wd = real(a[11]);
         const at::Tensor hyper = maybe(a[12]);
+        float *const *ms = q8 ? (float* const*)at[4].data() : nullptr, *const *vs = q8 ? (float* const*)at[5].data() : nullptr;
         call([&] {
-            return lib.fn.adamw_step((int)count, at[0].data(), at[1].data(), at[2].data(), at[3].data(), q8 ? (float* const*)at[4].data() : nullptr,
-                                     q8 ? (float* const*)at[5].data() : nullptr, numel.data(), dt, q8 ? 8 : 32, lr, b1, b2, eps, wd, step, ptr(hyper), stream_of(d));
+            return hyper.defined() ? lib.fn.adamw_step_each((int)count, at[0].data(), at[1].data(), at[2].data(), at[3].data(), ms, vs, numel.data(), dt, q8 ? 8 : 32, ptr(hyper), stream_of(d))
+                                   : lib.fn.adamw_step((int)count, at[0].data(), at[1].data(), at[2].data(), at[3].data(), ms, vs, numel.data(), dt, q8 ? 8 : 32, lr, b1, b2, eps, wd, step,
+                                                       nullptr, stream_of(d));
         });
         // written through raw pointers: autograd and the modules' caches have to see it
         for (Py_ssize_t j = 0; j < count; ++j) {

@@ -80,16 +80,19 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     keep = [_addresses(ts) for ts in lists]
     addr = [a for _, a in keep] + ([] if q8 else [None, None])
     numel = array("q", sizes)
-    launch(p0.device, _lib.lib().mtk_adamw_step, len(params), *addr, numel.buffer_info()[0], DTYPES[p0.dtype], 8 if q8 else 32, lr, betas[0], betas[1], eps,
-           weight_decay, step, None if _hyper is None else _hyper.data_ptr())
+    args = [len(params), *addr, numel.buffer_info()[0], DTYPES[p0.dtype], 8 if q8 else 32]
+    if _hyper is not None:
+        launch(p0.device, _lib.lib().mtk_adamw_step_each, *args, _hyper.data_ptr())
+    else:
+        launch(p0.device, _lib.lib().mtk_adamw_step, *args, lr, betas[0], betas[1], eps, weight_decay, step, None)
     torch.autograd.graph.increment_version(params)  # written through raw pointers: autograd and the modules' caches have to see it
 
 
 class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW``'s update and arguments, plus ``state_bits`` (32 or 8: the moments' width).
 
-    ``capturable=True`` keeps the step count (and, given as a float32 device tensor, the learning rate) on the device, so a step captured into a
-    HIP graph counts its own replays; take one step before the capture, which creates the state.  Without it a step under capture is
+    ``capturable=True`` keeps every parameter's step count (and, given as a float32 device tensor, the learning rate) on the device, so a step
+    captured into a HIP graph counts its own replays; take one step before the capture, which creates the state.  Without it a step under capture is
     refused.  Parameters have to be contiguous, dense tensors of float32, bfloat16 or float16.  ``amsgrad`` and ``maximize`` are not offered."""
 
     def __init__(self, params, lr: float | Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
@@ -105,15 +108,9 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: betas {betas}, eps {eps}, weight_decay {weight_decay}")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, capturable=capturable))
 
-    def _init_state(self, p: Tensor, group: dict, counts: dict) -> dict:
-        """``counts``: the step counters created by this call, one per device - parameters that start together share theirs, and with it a launch."""
+    def _init_state(self, p: Tensor, group: dict) -> dict:
         st = self.state[p]
-        if group["capturable"]:
-            if p.device not in counts:
-                counts[p.device] = torch.zeros((), dtype=torch.int64, device=p.device)
-            st["step"] = counts[p.device]
-        else:
-            st["step"] = 0
+        st["step"] = torch.zeros((), dtype=torch.int64, device=p.device) if group["capturable"] else 0
         if group["state_bits"] == 8:
             n = -(-p.numel() // SCALE_BLOCK)
             for name in ("exp_avg", "exp_avg_sq"):
@@ -125,23 +122,13 @@ class AdamW(torch.optim.Optimizer):
         return st
 
     def load_state_dict(self, state_dict) -> None:
-        """torch casts a loaded state to its parameter's type and copies shared tensors apart; here the moments keep their own type and
-        parameters that shared a step counter share one again."""
+        """torch casts a loaded state to its parameter's type; here the moments and step counts keep their own."""
         super().load_state_dict(state_dict)
         by_id = {i: p for g, q in zip(self.param_groups, state_dict["param_groups"]) for i, p in zip(q["params"], g["params"])}
-        counts: dict = {}
         for i, saved in state_dict["state"].items():
             p = by_id[i]
             for name, v in saved.items():
-                if not isinstance(v, Tensor):
-                    self.state[p][name] = v
-                elif name == "step":
-                    key = (v.data_ptr(), p.device)
-                    if key not in counts:
-                        counts[key] = v.detach().to(device=p.device, copy=True)
-                    self.state[p][name] = counts[key]
-                else:
-                    self.state[p][name] = v.detach().to(device=p.device, copy=True)
+                self.state[p][name] = v.detach().to(device=p.device, copy=True) if isinstance(v, Tensor) else v
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -150,8 +137,7 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for group in self.param_groups:
-            counts: dict = {}
-            sets: dict = {}  # one call per (device, type, step count)
+            sets: dict = {}  # one call per (device, type, step count); counts on the device are each parameter's own
             for p in group["params"]:
                 if p.grad is None:
                     continue
@@ -164,11 +150,11 @@ class AdamW(torch.optim.Optimizer):
                 capturing = torch.cuda.is_current_stream_capturing()
                 if capturing and (not group["capturable"] or p not in self.state):
                     raise RuntimeError("AdamW: a captured step needs capturable=True and one step before the capture")
-                st = self.state[p] if p in self.state and self.state[p] else self._init_state(p, group, counts)
+                st = self.state[p] if p in self.state and self.state[p] else self._init_state(p, group)
                 g = p.grad if p.grad.dtype == p.dtype else p.grad.to(p.dtype)
                 if not group["capturable"]:
                     st["step"] += 1
-                key = (p.device, p.dtype, st["step"].data_ptr() if group["capturable"] else st["step"])
+                key = (p.device, p.dtype, 1 if group["capturable"] else st["step"])
                 sets.setdefault(key, []).append((p, g if g.is_contiguous() else g.contiguous(), st))
             for (dev, _, step), items in sets.items():
                 self._run(group, dev, step, items)
@@ -181,12 +167,13 @@ class AdamW(torch.optim.Optimizer):
         b1, b2 = group["betas"]
         if group["capturable"]:
             l = _lib.lib()
-            hyper = torch.empty(l.mtk_adamw_hyper_bytes(), dtype=torch.uint8, device=dev)
+            hyper = torch.empty(len(items) * l.mtk_adamw_hyper_bytes(), dtype=torch.uint8, device=dev)
             lr_dev = lr if isinstance(lr, Tensor) else None
             if lr_dev is not None and lr_dev.device != dev:
                 raise ValueError(f"AdamW: lr on {lr_dev.device}, parameters on {dev}")
-            launch(dev, l.mtk_adamw_count, step, None if lr_dev is None else lr_dev.data_ptr(), 0.0 if lr_dev is not None else lr, b1, b2, group["eps"],
+            steps, at = _addresses(col("step"))
+            launch(dev, l.mtk_adamw_count_each, len(steps), at, None if lr_dev is None else lr_dev.data_ptr(), 0.0 if lr_dev is not None else lr, b1, b2, group["eps"],
                    group["weight_decay"], hyper.data_ptr())
-            lr, step = 0.0, 1
+            lr = 0.0
         adamw_step([p for p, _, _ in items], [g for _, g, _ in items], col("exp_avg"), col("exp_avg_sq"), step, lr=lr, betas=(b1, b2), eps=group["eps"],
                    weight_decay=group["weight_decay"], _hyper=hyper, **scales)

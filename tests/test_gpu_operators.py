@@ -876,6 +876,81 @@ def test_adamw_state_round_trip(bits, dt):
         assert int(second.state[q]["step"]) == 6
 
 
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_counts_every_parameters_own_steps(bits):
+    """Counts on the device are those on the host: parameters of two types, an empty one, some that go without a gradient now and then, from the
+    first step on or later, more than a launch holds, and through a saved state.  The same bits."""
+    g = gen(33)
+    kinds = [(3 + i % 300, (torch.float32, torch.bfloat16, torch.float16)[i % 3]) for i in range(600)] + [(0, torch.float32), (40, torch.bfloat16)]
+    start = [randn(g, n).to(dt) for n, dt in kinds]
+    sides = []
+    for capturable in (False, True):
+        ps = [torch.nn.Parameter(t.clone()) for t in start]
+        groups = [{"params": ps[:250]}, {"params": ps[250:], "weight_decay": 0.1}]
+        sides.append([ps, mtk.AdamW(groups, lr=1e-2, state_bits=bits, capturable=capturable)])
+    taken = [0] * len(kinds)
+    for t in range(5):
+        for i, (n, dt) in enumerate(kinds):
+            grad = None if (i % 5 == 1 and t in (1, 2)) or (i % 7 == 3 and t == 0) or (i == 4 and t > 0) else randn(g, n).to(dt)
+            taken[i] += grad is not None
+            for ps, _ in sides:
+                ps[i].grad = None if grad is None else grad.clone()
+        for _, opt in sides:
+            opt.step()
+        if t == 2:  # go on from a saved state
+            for side in sides:
+                state = side[1].state_dict()
+                side[1] = mtk.AdamW([{"params": side[0][:250]}, {"params": side[0][250:]}], capturable=side[1].defaults["capturable"])
+                side[1].load_state_dict(state)
+        for (p, q) in zip(*(ps for ps, _ in sides)):
+            assert torch.equal(p, q), t
+    for i, (p, q) in enumerate(zip(*(ps for ps, _ in sides))):
+        a, b = (opt.state[w] for (_, opt), w in zip(sides, (p, q)))
+        assert int(a["step"]) == int(b["step"]) == taken[i], i
+        assert all(torch.equal(a[k].view(torch.uint8) if bits == 8 else a[k], b[k].view(torch.uint8) if bits == 8 else b[k]) for k in ("exp_avg", "exp_avg_sq"))
+
+
+def test_a_captured_step_counts_what_it_steps():
+    """A graph that steps two of three parameters, of two types, with eager steps of all three in between"""
+    g = gen(34)
+    start = [randn(g, 300), randn(g, 300).bfloat16(), randn(g, 300)]
+    sides = []
+    for capturable in (False, True):
+        ps = [torch.nn.Parameter(t.clone()) for t in start]
+        sides.append((ps, mtk.AdamW(ps, lr=1e-2, capturable=capturable)))
+    grads = [torch.zeros_like(t) for t in start]
+
+    def step(ps, opt, which):
+        for i, p in enumerate(ps):
+            p.grad = grads[i] if i in which else None
+        opt.step()
+
+    def fill():
+        for t in grads:
+            t.copy_(randn(g, *t.shape))
+
+    fill()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*sides[1], (0, 1, 2))
+    torch.cuda.current_stream().wait_stream(side)
+    step(*sides[0], (0, 1, 2))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(*sides[1], (0, 1))
+    for t in range(5):
+        fill()
+        if t in (1, 2):
+            for s in sides:
+                step(*s, (1, 2))
+        step(*sides[0], (0, 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(sides[0][0], sides[1][0])), t
+    assert [int(sides[1][1].state[p]["step"]) for p in sides[1][0]] == [6, 8, 3]
+
+
 def test_adamw_groups_closures_and_refusals():
     g = gen(32)
     a, b, c = (torch.nn.Parameter(randn(g, 4, 5)) for _ in range(3))

@@ -82,6 +82,11 @@ def test_c_entries_refuse_before_any_launch():
     assert step(bits=8, sc=None) == ARG and step(size=(C.c_int64 * 1)(-1)) == ARG and step(p=(C.c_void_p * 1)(None)) == ARG
     assert step(size=(C.c_int64 * 1)(1 << 40)) == UNS
     assert l.mtk_adamw_count(None, None, 1e-3, 0.9, 0.999, 1e-8, 0.0, one, None) == ARG
+    assert l.mtk_adamw_count_each(2, None, None, 1e-3, 0.9, 0.999, 1e-8, 0.0, one, None) == ARG
+    assert l.mtk_adamw_count_each(-1, ptrs, None, 1e-3, 0.9, 0.999, 1e-8, 0.0, one, None) == ARG
+    assert l.mtk_adamw_count_each(1, (C.c_void_p * 1)(None), None, 1e-3, 0.9, 0.999, 1e-8, 0.0, one, None) == ARG
+    assert l.mtk_adamw_step_each(1, ptrs, ptrs, ptrs, ptrs, None, None, n, 0, 32, None, None) == ARG
+    assert l.mtk_adamw_step_each(1, ptrs, ptrs, ptrs, ptrs, None, None, n, 7, 32, one, None) == UNS
     assert l.mtk_adamw_scales(0) == 0 and l.mtk_adamw_scales(256) == 1 and l.mtk_adamw_scales(257) == 2
 
 
