@@ -10,6 +10,7 @@ import ctypes as C
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("MTK_LIB_PATH") or os.path.join(_HERE, "libmtk_hip.so")  # override: A/B builds of the same ABI
@@ -202,6 +203,12 @@ def ordinary(what: str, device: torch.device, fn, *args):
     if got is None:
         raise RuntimeError(f"{what}: libmtk_hip: {lib().mtk_last_error().decode()}")
     return got
+
+
+def no_tangents(what: str, *tensors) -> None:
+    """Refuses forward-mode differentiation: the operators' nodes go backward, and their results would lose the tangent."""
+    if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: forward-mode differentiation is not offered; detach the tangent (torch.autograd.forward_ad.unpack_dual)")
 
 
 def require_cuda(t: torch.Tensor, what: str) -> None:

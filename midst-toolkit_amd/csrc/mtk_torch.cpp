@@ -146,6 +146,10 @@ bool tracked(std::initializer_list<at::Tensor> ts) {
         if (t.defined() && t.requires_grad()) return true;
     return false;
 }
+// The nodes go backward only: a tangent that the result would lose is left to the Python layer, which refuses it.
+void no_tangents(std::initializer_list<at::Tensor> ts) {
+    for (const at::Tensor& t : ts) need(!t.defined() || !t._fw_grad(0).defined());
+}
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 // The nodes differentiate once: a second time raises where it is tried.
@@ -284,6 +288,7 @@ PyObject* dispatch(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 4, [&]() -> PyObject* {
         const at::Tensor& x = tensor(a[0]);
         const Pairs p{tensor(a[1]), integer(a[2]), integer(a[3])};
+        no_tangents({x});
         return THPVariable_Wrap(tracked({x}) ? DispatchNode::apply(x, p.slot, p.N, p.k) : rows_out(x, p, {}, {}, true).first);
     });
 }
@@ -293,6 +298,7 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor& y = tensor(a[0]);
         const Pairs p{tensor(a[1]), integer(a[2]), integer(a[3])};
         const at::Tensor w = maybe(a[4]);
+        no_tangents({y, w});
         return THPVariable_Wrap(tracked({y, w}) ? CombineNode::apply(y, p.slot, given(w), p.N, p.k) : rows_back(y, p, w));
     });
 }
@@ -390,6 +396,7 @@ PyObject* adapter(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (THPVariable_Check(a[6])) l.scales = tensor(a[6]);
         else l.scale = real(a[6]);
         need(!tracked({l.weight, l.bias}));
+        no_tangents({l.x, l.weight, l.bias, l.down, l.up, l.scales});
         at::Tensor saved;
         if (!tracked({l.x, l.down, l.up})) return THPVariable_Wrap(l.forward(false, saved));
         return THPVariable_Wrap(AdapterNode::apply(l.x, l.down, l.up, l.weight, l.offsets, given(l.bias), given(l.scales.defined() ? l.scales.detach() : l.scales), l.scale, (int64_t)l.act));

@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from ._lib import native, ordinary
+from ._lib import native, no_tangents, ordinary
 
 MAX_GROUPS = 1024  # MTK_ROUTE_MAX_GROUPS of include/mtk.h
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # enum mtk_dtype
@@ -80,6 +80,7 @@ def dispatch_rows(x: Tensor, plan: RowPlan) -> Tensor:
         if got is not None:
             return got
     _check_rows("dispatch_rows", x, plan.n_rows, plan)
+    no_tangents("dispatch_rows", x)
     return ordinary("dispatch_rows", x.device, native().dispatch, rows_of(x), plan.slot, plan.n_rows, plan.copies)
 
 
@@ -91,6 +92,7 @@ def combine_rows(y: Tensor, plan: RowPlan, weights: Tensor | None = None) -> Ten
         if got is not None:
             return got
     _check_rows("combine_rows", y, plan.n_rows * plan.copies, plan)
+    no_tangents("combine_rows", y, weights)
     if weights is not None:
         if weights.device != y.device:
             raise ValueError(f"combine_rows: weights on {weights.device}, rows on {y.device}")

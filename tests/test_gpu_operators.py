@@ -687,6 +687,27 @@ def test_nodes_differentiate_once():
         assert torch.equal(plain, first.detach())
 
 
+def test_forward_mode_is_refused():
+    """A result without the tangent would be a wrong derivative: with and without requires_grad, for every differentiable argument and the frozen
+    ones; in a dual level without tangents all is as ever."""
+    g = gen(91)
+    a = adapter_inputs(g, 20, 8, 6, 2, 3, torch.float32)
+    plan = mtk.route_rows(torch.randint(0, 3, (10, 2), generator=g).to(DEV), 3)
+    x, y, w = randn(g, 10, 5), randn(g, 20, 5), randn(g, 10, 2)
+    want = (call(a), mtk.dispatch_rows(x, plan), mtk.combine_rows(y, plan, w))
+    fw = torch.autograd.forward_ad
+    with fw.dual_level():
+        dual = lambda t, grad: fw.make_dual(t.clone().requires_grad_(grad), torch.ones_like(t))  # noqa: E731
+        for grad in (False, True):
+            calls = [lambda n=n: call(a, **{n: dual(a[n], grad)}) for n in ("x", "weight", "bias", "down", "up", "scale")]
+            calls += [lambda: mtk.dispatch_rows(dual(x, grad), plan), lambda: mtk.combine_rows(dual(y, grad), plan, w), lambda: mtk.combine_rows(y, plan, dual(w, grad))]
+            calls += [lambda: call(a, x=dual(a["x"], grad)[:, :8].t().contiguous().t())]  # strides to copy
+            for f in calls:
+                with pytest.raises(NotImplementedError):
+                    f()
+        assert all(torch.equal(p, q) for p, q in zip((call(a), mtk.dispatch_rows(x, plan), mtk.combine_rows(y, plan, w)), want))
+
+
 # ------------------------------------------------------------------------------------------------------------------- AdamW
 SIZES = [1, 2, 3, 5, 255, 256, 257, 1000, 1024, 4099]
 
