@@ -31,7 +31,7 @@ def adapter_linear(x: Tensor, weight: Tensor, bias: Tensor | None, down: Tensor,
     ``x`` [M, din]; ``weight`` [dout, din] and ``bias`` [dout] (or None): the shared layer, frozen; ``down`` [E, r, din], ``up`` [E, dout, r]: one
     update per model; all of one type (float32, bfloat16, float16).  ``offsets``: int32 [E + 1], model e owns rows ``offsets[e]`` to
     ``offsets[e + 1] - 1`` (a ``RowPlan`` stands for its offsets); rows behind the last model's have the shared layer alone.  ``scale``: one
-    number, or float32 [E] on the device.  ``activation``: "none" or "relu".  Differentiable in ``x``, ``down`` and ``up``, backward and once."""
+    number, or float32 [E] on the device, a constant.  ``activation``: "none" or "relu".  Differentiable in ``x``, ``down`` and ``up``, backward and once."""
     if isinstance(offsets, RowPlan):
         offsets = offsets.offsets
     if not x.is_cuda:
@@ -65,6 +65,8 @@ def adapter_linear(x: Tensor, weight: Tensor, bias: Tensor | None, down: Tensor,
         raise ValueError(f"adapter_linear: x on {x.device}, offsets on {offsets.device}" + ("" if scales is None else f", scale on {scales.device}"))
     if torch.is_grad_enabled() and (weight.requires_grad or (bias is not None and bias.requires_grad)):
         raise NotImplementedError("adapter_linear: the shared layer is frozen; detach weight and bias")
+    if torch.is_grad_enabled() and scales is not None and scales.requires_grad:
+        raise NotImplementedError("adapter_linear: scale gets no gradient; detach it")
     no_tangents("adapter_linear", x, weight, bias, down, up, scale)
     c = lambda t: t if t is None else t.contiguous()  # noqa: E731
     return ordinary("adapter_linear", x.device, native().adapter, rows_of(x), c(weight), c(bias), c(down), c(up), c(offsets),

@@ -389,17 +389,17 @@ struct AdapterNode : torch::autograd::Function<AdapterNode> {
     }
 };
 
-// adapter(x, weight, bias | None, down, up, offsets, scale, act) -> y.  A shared layer that autograd tracks is declined.
+// adapter(x, weight, bias | None, down, up, offsets, scale, act) -> y.  A shared layer or scale that autograd tracks is declined.
 PyObject* adapter(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 8, [&]() -> PyObject* {
         Layer l{tensor(a[0]), tensor(a[1]), tensor(a[3]), tensor(a[4]), tensor(a[5]), maybe(a[2]), {}, 1.0, (int)integer(a[7])};
         if (THPVariable_Check(a[6])) l.scales = tensor(a[6]);
         else l.scale = real(a[6]);
-        need(!tracked({l.weight, l.bias}));
+        need(!tracked({l.weight, l.bias, l.scales}));
         no_tangents({l.x, l.weight, l.bias, l.down, l.up, l.scales});
         at::Tensor saved;
         if (!tracked({l.x, l.down, l.up})) return THPVariable_Wrap(l.forward(false, saved));
-        return THPVariable_Wrap(AdapterNode::apply(l.x, l.down, l.up, l.weight, l.offsets, given(l.bias), given(l.scales.defined() ? l.scales.detach() : l.scales), l.scale, (int64_t)l.act));
+        return THPVariable_Wrap(AdapterNode::apply(l.x, l.down, l.up, l.weight, l.offsets, given(l.bias), given(l.scales), l.scale, (int64_t)l.act));
     });
 }
 

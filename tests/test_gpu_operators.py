@@ -567,6 +567,22 @@ def test_adapter_refusals():
         call(a, weight=a["weight"].clone().requires_grad_())
 
 
+def test_a_scale_that_requires_grad_is_refused():
+    """It would get none: refused whether or not anything else of the layer is trained"""
+    g = gen(93)
+    a = adapter_inputs(g, 30, 8, 6, 2, 3, torch.float32)
+    want = call(a)
+    scale = a["scale"].clone().requires_grad_()
+    for kw in ({}, {n: a[n].clone().requires_grad_() for n in ("x", "down", "up")}, {"x": a["x"].t().contiguous().t()}):
+        with pytest.raises(NotImplementedError, match="scale"):
+            call(a, scale=scale, **kw)
+    with torch.no_grad():
+        assert torch.equal(call(a, scale=scale), want)
+    x = a["x"].clone().requires_grad_()
+    y = call(a, scale=scale.detach(), x=x)
+    assert torch.equal(y, want) and torch.equal(torch.autograd.grad(y.sum(), x)[0], torch.autograd.grad(call(a, x=x).sum(), x)[0])
+
+
 @pytest.mark.parametrize("off", [[0, 90, 10, 40], [50, 60, 70, 80], [-5, 20, 1000, 2000], [100, 60, 30, 0], [-9, -8, -7, -6], [2**31 - 1] * 4])
 @pytest.mark.parametrize("M", [64, 700])
 def test_offsets_that_make_no_sense_stay_inside_the_tensors(M, off):
