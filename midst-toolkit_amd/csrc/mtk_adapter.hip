@@ -12,9 +12,12 @@
 // The backward of x is the same two kernels on g with W, A_e, B_e transposed first (W is small beside the rows).
 // One diverged model leaves the others' rows alone, to the bit: what is not finite never meets another model's rows in an accumulator
 // (0 x inf is NaN), their products are made per model and SELECTED by row.
-// Every sum is in fp32.  u and t = s_e g B_e are MFMA operands, so with 16-bit rows they are 16-bit numbers: two each, u = hi + lo, which keeps
-// 16 bits of u or more (one rounded number would add as much error as the result's own rounding, and all of a row's at once).  The line of
-// a row of u holds both halves side by side, against B_e twice: for ranks up to 32 that costs nothing.
+// Every sum is in fp32.  u and t = s_e g B_e are MFMA operands, so with 16-bit rows they are 16-bit numbers, and more than one each: a single rounded
+// number would add as much error as the result's own rounding, and all of a row's at once.  A row of u holds them in sections side by side:
+//   bf16  two, u = hi + lo (2^-17 of u), against B_e twice; for ranks up to 32 the line of 64 numbers holds both
+//   fp16  three bf16 numbers, u = h + m + l (2^-25), against B_e = b + c, two bf16 numbers (exact): h b + m b + l b + h c + m c.  Not fp16 numbers:
+//         t is small (the factors start at zero, gradients are small), and below 2^-14 fp16 has fewer bits with every binade, 6e-8 of
+//         absolute error; at the other end u passes 65,504 where y does not.  bf16 has fp32's exponents.  One line up to rank 12.
 #include <type_traits>
 
 #include "mtk_low_piece.h"
@@ -54,10 +57,50 @@ __device__ __forceinline__ f32x4 mma16(const mtk_vec<float>& a, const mtk_vec<fl
     return c;
 }
 
-// A k-block is one 128-byte line of a row.  A row of u is rank_pad elements, whole k-blocks: fp32 [u, zeros], 16 bits [hi, zeros | lo, zeros]
+// A k-block is one 128-byte line of a row.  A row of u is rank_pad elements, whole lines: kSections sections of `section` values, zeros behind the rank
+// and behind the last.
 template <typename T> constexpr int kLine = 128 / (int)sizeof(T);
-inline int rank_pad(int r, int dtype) { return (int)mtk_up(r, 32) * (dtype == MTK_DT_F32 ? 1 : 2); }
-template <typename T> __device__ __forceinline__ T low_half(float v, T hi) { return fabsf((float)hi) <= 3.0e38f ? (T)(v - (float)hi) : T(0); }
+template <typename T> constexpr bool kF16 = std::is_same<T, mtk_f16>::value;
+template <typename T> using Low = typename std::conditional<kF16<T>, mtk_bf16, T>::type;  // what u is made of
+template <typename T> constexpr int kParts = sizeof(T) == 4 ? 1 : kF16<T> ? 3 : 2;        // numbers of a value of u
+template <typename T> constexpr int kSections = kF16<T> ? 5 : kParts<T>;
+template <typename T> __host__ __device__ constexpr int section(int r) { return kF16<T> ? (r + 3) / 4 * 4 : (r + 31) / 32 * 32; }
+constexpr int section_part(int s) { return s < 3 ? s : s - 3; }  // the number that section s holds
+constexpr bool section_second(int s) { return s >= 3; }          // whether it meets the second number of B_e
+// eight fp16 values as two bf16 numbers each, exactly (an infinity: inf and NaN)
+__device__ __forceinline__ void two_numbers(const mtk_vec<mtk_f16>& v, mtk_vec<mtk_bf16>& b, mtk_vec<mtk_bf16>& c) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float f = (float)v.v[i];
+        b.v[i] = (mtk_bf16)f;
+        c.v[i] = (mtk_bf16)(f - (float)b.v[i]);
+    }
+}
+// the first of them, or the second
+__device__ __forceinline__ mtk_vec<mtk_bf16> number_of(const mtk_vec<mtk_f16>& v, bool second) {
+    mtk_vec<mtk_bf16> o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float f = (float)v.v[i];
+        o.v[i] = (mtk_bf16)(f - (second ? (float)(mtk_bf16)f : 0.f));
+    }
+    return o;
+}
+inline int rank_pad(int r, int dtype) {
+    return dtype == MTK_DT_F32 ? section<float>(r) : dtype == MTK_DT_BF16 ? 2 * section<mtk_bf16>(r) : (int)mtk_up(5 * section<mtk_f16>(r), kLine<mtk_f16>);
+}
+// the numbers of v, largest first; what follows an infinity is 0
+template <typename L, int N> __device__ __forceinline__ void parts_of(float v, L (&p)[N]) {
+    p[0] = (L)v;
+    if constexpr (N > 1) {
+        float rest = fabsf((float)p[0]) <= 3.0e38f ? v - (float)p[0] : 0.f;
+#pragma unroll
+        for (int i = 1; i < N; ++i) {
+            p[i] = (L)rest;
+            rest -= (float)p[i];
+        }
+    }
+}
 constexpr int kRankT = 16;  // rows of u^T come in whole 16s
 
 // The models that own rows [at, end): each call yields one (e, first row, behind its last row).  Whatever the offsets hold, every step moves
@@ -140,7 +183,7 @@ struct ShrinkArgs {
 // 65,536 rows of 1,024 bf16: 29 us (4.6 TB/s; 33 with 16 models), 2,048 rows fp32 7 us (8 with 16 models), 61 rows of 512 fp32 6 us.
 template <int RT, int KS> constexpr int kShrinkLds = KS > 1 ? KS * RT * 4 * 64 : 1;  // floats
 template <typename T, int RT, int KS>
-__device__ void shrink_body(const ShrinkArgs& g, unsigned block, int j0, const T* __restrict__ x, const T* __restrict__ F, T* __restrict__ u, T* __restrict__ uT, float* lds) {
+__device__ void shrink_body(const ShrinkArgs& g, unsigned block, int j0, const T* __restrict__ x, const T* __restrict__ F, Low<T>* __restrict__ u, Low<T>* __restrict__ uT, float* lds) {
     constexpr int V = mtk_piece<T>::n, KB = kLine<T>, RR = KS > 1 ? 1 : 2;
     float (*part)[KS > 1 ? RT * 4 : 1][64] = reinterpret_cast<float (*)[KS > 1 ? RT * 4 : 1][64]>(lds);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, q = lane >> 4;
@@ -249,50 +292,53 @@ __device__ void shrink_body(const ShrinkArgs& g, unsigned block, int j0, const T
     for (int p = 0; p < RR; ++p) {
         if (!(mine[p] || (my_turn == 0 && !any[p]))) continue;  // a row without a model: zeros
         const int64_t at = m0 + p * 16 + li;  // D[j][record]: lane & 15 -> record, j = 4 (lane >> 4) + register
-        struct __attribute__((aligned(4 * sizeof(T)), may_alias)) Quad { T v[4]; };
-        constexpr bool kSplit = sizeof(T) == 2;
-        const int half = kSplit ? g.rp / 2 : g.rp;
-        const int64_t plane = mtk_up(g.r, 64) * g.Mp;  // of u^T: hi, then lo
-        T* ur = u + at * g.rp;
+        typedef Low<T> L;
+        constexpr int P = kParts<T>, S = kSections<T>;
+        struct __attribute__((aligned(4 * sizeof(L)), may_alias)) Quad { L v[4]; };
+        const int sec = section<T>(g.r);
+        const int64_t plane = mtk_up(g.r, 64) * g.Mp;  // of u^T: a number each
+        L* ur = u + at * g.rp;
+        auto put = [&](L* row, const Quad (&o)[P], bool its) {
+#pragma unroll
+            for (int c = 0; c < S; ++c) *reinterpret_cast<Quad*>(row + c * sec) = its ? o[section_part(c)] : Quad{};
+        };
+        auto pair_row = [&](int i) { return (L*)g.pairs + ((int64_t)(tile + tm.e + i) * g.BM + (at - (int64_t)tile * g.BM)) * g.rp; };
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            Quad o, l;
+            Quad o[P];
             const int j = j0 + t * 16 + q * 4;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float v = j + i < g.r ? keep[p][t][i] : 0.f;
-                o.v[i] = (T)v;
-                l.v[i] = low_half(v, o.v[i]);
+                L n[P];
+                parts_of(j + i < g.r ? keep[p][t][i] : 0.f, n);
+#pragma unroll
+                for (int c = 0; c < P; ++c) o[c].v[i] = n[c];
             }
-            if (at < g.M && j < half) {
-                *reinterpret_cast<Quad*>(ur + j) = o;
-                if (kSplit) *reinterpret_cast<Quad*>(ur + half + j) = l;
+            if (at < g.M && j < sec) {
+                put(ur + j, o, true);
                 if (tm.ranged)
-                    for (int i = 0; i < tm.count; ++i) {
-                        T* pr = (T*)g.pairs + ((int64_t)(tile + tm.e + i) * g.BM + (at - (int64_t)tile * g.BM)) * g.rp + j;
-                        const bool its = tm.e + i == who[p];
-                        *reinterpret_cast<Quad*>(pr) = its ? o : Quad{};
-                        if (kSplit) *reinterpret_cast<Quad*>(pr + half) = its ? l : Quad{};
-                    }
+                    for (int i = 0; i < tm.count; ++i) put(pair_row(i) + j, o, tm.e + i == who[p]);
             }
             if (uT && at < g.Mp)  // mtk_up(r, 64) rows of Mp
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uT[(int64_t)(j + i) * g.Mp + at] = o.v[i];
-                    uT[plane + (int64_t)(j + i) * g.Mp + at] = l.v[i];
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < P; ++c) uT[c * plane + (int64_t)(j + i) * g.Mp + at] = o[c].v[i];
+        }
+        if (j0 + RT * 16 >= g.r && at < g.M) {  // zeros up to the end of the sections, and of the row
+            const Quad zero[P] = {};
+            for (int j = j0 + RT * 16 + q * 4; j < sec; j += 16) {
+                put(ur + j, zero, true);
+                if (tm.ranged)
+                    for (int i = 0; i < tm.count; ++i) put(pair_row(i) + j, zero, true);
+            }
+            if constexpr (kF16<T>)
+                for (int j = S * sec + q * 4; j < g.rp; j += 16) {
+                    *reinterpret_cast<Quad*>(ur + j) = Quad{};
+                    if (tm.ranged)
+                        for (int i = 0; i < tm.count; ++i) *reinterpret_cast<Quad*>(pair_row(i) + j) = Quad{};
                 }
         }
-        if (j0 + RT * 16 >= g.r && at < g.M)  // zeros up to the end of the half
-            for (int j = j0 + RT * 16 + q * 4; j < half; j += 16) {
-                *reinterpret_cast<Quad*>(ur + j) = Quad{};
-                if (kSplit) *reinterpret_cast<Quad*>(ur + half + j) = Quad{};
-                if (tm.ranged)
-                    for (int i = 0; i < tm.count; ++i) {
-                        T* pr = (T*)g.pairs + ((int64_t)(tile + tm.e + i) * g.BM + (at - (int64_t)tile * g.BM)) * g.rp + j;
-                        *reinterpret_cast<Quad*>(pr) = Quad{};
-                        if (kSplit) *reinterpret_cast<Quad*>(pr + half) = Quad{};
-                    }
-            }
     }
 }
 
@@ -309,6 +355,8 @@ __device__ void shrink_body(const ShrinkArgs& g, unsigned block, int j0, const T
 // low-rank products are made in the epilogue, per model, and selected by row.
 // 65,536 x 1,024 x 1,024 in bf16 144 us, 17 lines of k for the 16 of the shared product alone, which the library's plain product does in 133; 2,048 rows
 // in fp32 47 us (33 lines for 32; 35): there the matrix pipes are busy 81 % of the time at some 2.0 GHz, the rest is start and end.
+// RAW, fp16 without such blocks: B_e as it lies, split into its two numbers where it is read (a kernel of its own: with the lines' loop beside
+// it the accumulators spill; lines for all would be laid out at length: 2,048 rows of 128 models 58 us for 20).
 // The stream wants whole, 16-byte aligned lines: k_prep pads what is not, and lays out B, the bias in fp32, the tiles' models and which B_e
 // hold infinities or NaN.
 struct LinearArgs {
@@ -356,7 +404,7 @@ __device__ __forceinline__ int scalar_load(const int32_t* p) {
     return v;
 }
 
-template <typename T, int WR, int WC, int MW, int NT, int DX, int DW>
+template <typename T, int WR, int WC, int MW, int NT, int DX, int DW, bool RAW>
 __global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)) void k_linear(LinearArgs) {  // (linear_args)
     typedef Geo<WR, WC, MW, NT, DX, DW> G;
     constexpr int V = mtk_piece<T>::n, kWBase = DX * G::kTileX;
@@ -501,14 +549,15 @@ __global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)
         }
     };
     f32x16 acc[MW][NT];
-    auto mma_row = [&](const Frags& f, int mt) {
+    auto mma_row = [&](auto type, const Frags& f, int mt) {  // type: of the numbers in the fragments
+        typedef mtk_vec<decltype(type)> F;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = mma32(f.w[nt], f.x[mt], acc[mt][nt]);
+        for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = mma32(__builtin_bit_cast(F, f.w[nt]), __builtin_bit_cast(F, f.x[mt]), acc[mt][nt]);
     };
-    auto mma_all = [&](const Frags& f) {
+    auto mma_all = [&](auto type, const Frags& f) {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int mt = 0; mt < MW; ++mt) mma_row(f, mt);
+        for (int mt = 0; mt < MW; ++mt) mma_row(type, f, mt);
         __builtin_amdgcn_sched_barrier(0);
     };
 
@@ -560,41 +609,51 @@ __global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)
         const int nk = ga.nkb + ga.nkx * TileModels::of(tm).count;
         start(n0);
         read_frags(F0, xi, wi, 0);
-        for (int kb = 0; kb < nk; ++kb) {
-            read_frags(F1, xi, wi, 1);
-            mma_all(F0);
-            read_frags(F0, xi, wi, 2);
-            mma_all(F1);
-            read_frags(F1, xi, wi, 3);
-            mma_all(F0);
-            // Stores of the previous tile may be outstanding too and do not return in order with the loads, but the count still holds: with S stores,
-            // N needed and kYounger younger pieces in flight, "at most kYounger outstanding" needs S + N completions, and fewer than
-            // N loads done (the needed ones come first) would leave at most S + N - 1.
-            if (x_tail) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(G::kYounger) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __syncthreads();  // everyone's share has landed, and this block's buffers have no readers left
-            __builtin_amdgcn_sched_barrier(0);
-            const int xn = xi == DX - 1 ? 0 : xi + 1, wn = wi == DW - 1 ? 0 : wi + 1;
-            if (kb + 1 < nk) read_frags(F0, xn, wn, 0);
-            constexpr int OPW = G::XPW + G::WPW;
-#pragma unroll
-            for (int mt = 0; mt < MW; ++mt) {
-                __builtin_amdgcn_sched_barrier(0);
-                mma_row(F1, mt);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int j = mt * OPW / MW; j < (mt + 1) * OPW / MW; ++j) {
-                    if (j < G::WPW) w_op(j);
-                    else x_op(j - G::WPW);
-                }
-            }
-            w_advance();
-            x_tail = cx_slot < slots;
-            x_advance();
-            xi = xn;
-            wi = wn;
-            __builtin_amdgcn_sched_barrier(0);
+        // Stores of the previous tile may be outstanding too and do not return in order with the loads, but the count still holds: with S stores,
+        // N needed and kYounger younger pieces in flight, "at most kYounger outstanding" needs S + N completions, and fewer than
+        // N loads done (the needed ones come first) would leave at most S + N - 1.
+        // (The barrier: everyone's share has landed, and this block's buffers have no readers left.)  A macro: as a lambda, whose captures are kept
+        // differently, the same lines cost fp32 3 % (2,048 rows 52.1 -> 54.3 us).
+#define MTK_BLOCKS(TYPE, FROM, TO) \
+        for (int kb = FROM; kb < TO; ++kb) { \
+            read_frags(F1, xi, wi, 1); \
+            mma_all(TYPE, F0); \
+            read_frags(F0, xi, wi, 2); \
+            mma_all(TYPE, F1); \
+            read_frags(F1, xi, wi, 3); \
+            mma_all(TYPE, F0); \
+            if (x_tail) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(G::kYounger) : "memory"); \
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); \
+            __syncthreads(); \
+            __builtin_amdgcn_sched_barrier(0); \
+            const int xn = xi == DX - 1 ? 0 : xi + 1, wn = wi == DW - 1 ? 0 : wi + 1; \
+            if (kb + 1 < nk) read_frags(F0, xn, wn, 0); \
+            constexpr int OPW = G::XPW + G::WPW; \
+_Pragma("unroll") \
+            for (int mt = 0; mt < MW; ++mt) { \
+                __builtin_amdgcn_sched_barrier(0); \
+                mma_row(TYPE, F1, mt); \
+                __builtin_amdgcn_sched_barrier(0); \
+_Pragma("unroll") \
+                for (int j = mt * OPW / MW; j < (mt + 1) * OPW / MW; ++j) { \
+                    if (j < G::WPW) w_op(j); \
+                    else x_op(j - G::WPW); \
+                } \
+            } \
+            w_advance(); \
+            x_tail = cx_slot < slots; \
+            x_advance(); \
+            xi = xn; \
+            wi = wn; \
+            __builtin_amdgcn_sched_barrier(0); \
         }
+        if constexpr (kF16<T> && !RAW) {  // the low-rank blocks hold other numbers
+            MTK_BLOCKS(T(0), 0, ga.nkb)
+            MTK_BLOCKS(Low<T>(0), ga.nkb, nk)
+        } else {
+            MTK_BLOCKS(T(0), 0, nk)
+        }
+#undef MTK_BLOCKS
 
         // opaque copy of the lane id: what the epilogue derives from it is recomputed per tile instead of being kept alive across the k-loop
         int lane_e = lane;
@@ -622,7 +681,7 @@ __global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)
                         const int n = n0 + wc * G::WN + q * 32 + li_e;
                         f.w[q] = mtk_ld((const T*)((const char*)g.W + (int64_t)(n < g.N ? n : g.N - 1) * g.w_ld + kp));
                     }
-                    mma_all(f);
+                    mma_all(T(0), f);
                 }
             }
         }
@@ -631,9 +690,10 @@ __global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)
             Owners own(g.offsets, g.E, w0, w1 < g.M ? w1 : g.M);
             int e;
             int64_t a, b;
-            const T* u = (const T*)g.U;
+            typedef Low<T> L;
+            const L* u = (const L*)g.U;
             constexpr int S = 32 / (2 * V);  // steps of 32 values of the rank
-            const int half = sizeof(T) == 2 ? g.rp / 2 : g.rp, low_n = g.low_ld < half ? g.low_ld : half;  // B_e's values, once
+            const int sec = section<T>(g.r), low_n = kF16<T> || g.low_ld < sec ? g.low_ld : sec;  // B_e's values, once
             while (own.next(e, a, b)) {
                 const T* be = (const T*)g.low + (int64_t)e * g.N * g.low_ld;
 #pragma unroll
@@ -641,29 +701,62 @@ __global__ __launch_bounds__(64 * WR * WC, (Geo<WR, WC, MW, NT, DX, DW>::kWaves)
                     const int64_t row = w0 + mt * 32 + li_e, rc = row < g.M ? row : g.M - 1;
                     const bool mine = row >= a && row < b;
                     if (a >= w0 + mt * 32 + 32 || b <= w0 + mt * 32) continue;
-                    const T* ur = u + rc * g.rp;
+                    const L* ur = u + rc * g.rp;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         const int n = n0 + wc * G::WN + nt * 32 + li_e;
                         f32x16 low = acc[mt][nt];
-                        auto steps = [&](int j0, int h, auto count) {  // requested together: one round trip
-                            constexpr int C = decltype(count)::value;
-                            mtk_vec<T> uv[C], bv[C];
+                        if constexpr (kF16<T> && !RAW) {  // whole lines against whole lines, in the stream's order: a row that is made once more keeps its bits
+                            const L* bn = (const L*)be + (int64_t)(n < g.N ? n : g.N - 1) * g.low_ld;
+#pragma unroll 1
+                            for (int k = hh_e * V; k < g.rp; k += 2 * V * S) {
+                                mtk_vec<L> uv[S], bv[S];  // requested together: one round trip
 #pragma unroll
-                            for (int s = 0; s < C; ++s) {
-                                const int j = j0 + s * 2 * V + hh_e * V;
+                                for (int s = 0; s < S; ++s) {
+                                    uv[s] = mtk_ld(ur + k + s * 2 * V);
+                                    bv[s] = mtk_ld(bn + k + s * 2 * V);
+                                }
+#pragma unroll
+                                for (int s = 0; s < S; ++s) low = mma32(bv[s], uv[s], low);
+                            }
+                        } else {
+                            auto piece = [&](int j) {  // of B_e, zeros behind the rank
                                 const bool in = j < low_n;
                                 const uint4 w = __builtin_bit_cast(uint4, mtk_ld(be + mtk_low_piece(n, g.N, g.low_ld, low_n, j)));
-                                bv[s] = __builtin_bit_cast(mtk_vec<T>, make_uint4(in ? w.x : 0u, in ? w.y : 0u, in ? w.z : 0u, in ? w.w : 0u));
-                                uv[s] = mtk_ld(ur + h + j);
-                            }
+                                return __builtin_bit_cast(mtk_vec<T>, make_uint4(in ? w.x : 0u, in ? w.y : 0u, in ? w.z : 0u, in ? w.w : 0u));
+                            };
+                            if constexpr (kF16<T>) {
+#pragma unroll 1
+                                for (int j = hh_e * V; j < g.r + hh_e * V; j += 2 * V) {  // (what is behind a section of u meets zeros)
+                                    const mtk_vec<T> bt = piece(j);
+                                    const mtk_vec<L> u0 = mtk_ld(ur + j), u1 = mtk_ld(ur + sec + j), u2 = mtk_ld(ur + 2 * sec + j);
+                                    mtk_vec<L> bv = number_of(bt, false);
+                                    low = mma32(bv, u2, low);
+                                    low = mma32(bv, u1, low);
+                                    low = mma32(bv, u0, low);
+                                    bv = number_of(bt, true);
+                                    low = mma32(bv, u1, low);
+                                    low = mma32(bv, u0, low);
+                                }
+                            } else {
+                                auto steps = [&](int j0, int h, auto count) {  // requested together: one round trip
+                                    constexpr int C = decltype(count)::value;
+                                    mtk_vec<T> uv[C], bv[C];
 #pragma unroll
-                            for (int s = 0; s < C; ++s) low = mma32(bv[s], uv[s], low);
-                        };
+                                    for (int s = 0; s < C; ++s) {
+                                        const int j = j0 + s * 2 * V;
+                                        bv[s] = piece(j + hh_e * V);
+                                        uv[s] = mtk_ld(ur + h + j + hh_e * V);
+                                    }
+#pragma unroll
+                                    for (int s = 0; s < C; ++s) low = mma32(bv[s], uv[s], low);
+                                };
 #pragma unroll 1
-                        for (int h = 0; h < g.rp; h += half)
+                                for (int h = 0; h < g.rp; h += sec)
 #pragma unroll 1
-                            for (int j0 = 0; j0 < g.r; j0 += 32) steps(j0, h, std::integral_constant<int, S>());
+                                    for (int j0 = 0; j0 < g.r; j0 += 32) steps(j0, h, std::integral_constant<int, S>());
+                            }
+                        }
 #pragma unroll
                         for (int q = 0; q < 16; ++q) acc[mt][nt][q] = mine ? low[q] : acc[mt][nt][q];
                         __builtin_amdgcn_sched_barrier(0);
@@ -741,8 +834,9 @@ struct FewArgs {
 };
 
 template <typename T, int TS, bool FUSED>
-__global__ __launch_bounds__(512) void k_linear_few(FewArgs g, const T* __restrict__ x, const T* __restrict__ W, const T* __restrict__ bias, const T* __restrict__ u,
-                                                    const T* __restrict__ up, T* __restrict__ y, const T* __restrict__ down, T* __restrict__ u_out, T* __restrict__ uT) {
+__global__ __launch_bounds__(512) void k_linear_few(FewArgs g, const T* __restrict__ x, const T* __restrict__ W, const T* __restrict__ bias, const Low<T>* __restrict__ u,
+                                                    const T* __restrict__ up, T* __restrict__ y, const T* __restrict__ down, Low<T>* __restrict__ u_out, Low<T>* __restrict__ uT) {
+    typedef Low<T> L;
     constexpr int V = mtk_piece<T>::n, KB = kLine<T>, NW = 8;
     constexpr int LANES = 64 / TS, S = 8 / LANES;  // lanes that share a row, steps of a line
     constexpr int OUT = TS * TS > 512 ? 2 : 1;     // outputs of a thread
@@ -780,11 +874,18 @@ __global__ __launch_bounds__(512) void k_linear_few(FewArgs g, const T* __restri
     // this thread's outputs: row rr + 16 i, feature n; models by ballots over the offsets
     const int rr = tid / TS, n = n0 + (tid & (TS - 1)), nc = n < g.N ? n : g.N - 1;
     constexpr int LP = 16 / V;  // pieces of the rank requested ahead: 16 values
-    constexpr int H = sizeof(T) == 2 ? 2 : 1;  // halves of u
-    const int half = g.rp / H;
+    constexpr int H = kParts<T>;  // numbers of a value of u, in the first sections
+    const int sec = section<T>(g.r);
+    auto value = [](const mtk_vec<L> (&v)[H], int c) {
+        float f = (float)v[0].v[c];
+#pragma unroll
+        for (int h = 1; h < H; ++h) f += (float)v[h].v[c];
+        return f;
+    };
     const float bv = bias ? (float)bias[nc] : 0.f;
     int who[OUT];
-    mtk_vec<T> ua[OUT][LP][H], ba[OUT][LP];
+    mtk_vec<L> ua[OUT][LP][H];
+    mtk_vec<T> ba[OUT][LP];
 #pragma unroll
     for (int i = 0; i < OUT; ++i) {
         const int64_t row = m0 + rr + 16 * i, rc = row < g.M ? row : g.M - 1;
@@ -798,12 +899,13 @@ __global__ __launch_bounds__(512) void k_linear_few(FewArgs g, const T* __restri
         }
         who[i] = c - 1;
         if (who[i] < 0 || who[i] >= g.E || row >= g.M || rr + 16 * i >= TS) who[i] = -1;
-        const T *ur = u + rc * g.rp, *br = up + ((int64_t)(who[i] < 0 ? 0 : who[i]) * g.N + nc) * g.r;
+        const L* ur = u + rc * g.rp;
+        const T* br = up + ((int64_t)(who[i] < 0 ? 0 : who[i]) * g.N + nc) * g.r;
 #pragma unroll
         for (int p = 0; p < LP; ++p) {
 #pragma unroll
             for (int h = 0; h < H; ++h)
-                if (!FUSED) ua[i][p][h] = mtk_ld(ur + h * half + p * V);  // whole lines, zeros behind the rank
+                if (!FUSED) ua[i][p][h] = mtk_ld(ur + h * sec + p * V);  // inside the row, which is whole lines; up's zeros behind the rank
             ba[i][p] = p * V + V <= g.r ? mtk_ld(br + p * V) : mtk_ld_n(br + p * V, g.r - p * V);
         }
     }
@@ -885,12 +987,16 @@ __global__ __launch_bounds__(512) void k_linear_few(FewArgs g, const T* __restri
 #pragma unroll
             for (int p = 0; p < LP; ++p)
 #pragma unroll
-                for (int c = 0; c < V; ++c) low += (H == 2 ? (float)ua[i][p][0].v[c] + (float)ua[i][p][H - 1].v[c] : (float)ua[i][p][0].v[c]) * (float)ba[i][p].v[c];
-            const T *ur = u + row * g.rp, *br = up + ((int64_t)who[i] * g.N + n) * g.r;
+                for (int c = 0; c < V; ++c) low += value(ua[i][p], c) * (float)ba[i][p].v[c];
+            const L* ur = u + row * g.rp;
+            const T* br = up + ((int64_t)who[i] * g.N + n) * g.r;
             for (int j = LP * V; j < g.r; j += V) {
-                const mtk_vec<T> uv = mtk_ld(ur + j), ul = mtk_ld(ur + (H - 1) * half + j), bq = j + V <= g.r ? mtk_ld(br + j) : mtk_ld_n(br + j, g.r - j);
+                mtk_vec<L> uv[H];
 #pragma unroll
-                for (int c = 0; c < V; ++c) low += (H == 2 ? (float)uv.v[c] + (float)ul.v[c] : (float)uv.v[c]) * (float)bq.v[c];
+                for (int h = 0; h < H; ++h) uv[h] = mtk_ld(ur + h * sec + j);
+                const mtk_vec<T> bq = j + V <= g.r ? mtk_ld(br + j) : mtk_ld_n(br + j, g.r - j);
+#pragma unroll
+                for (int c = 0; c < V; ++c) low += value(uv, c) * (float)bq.v[c];
             }
             v += low;
         }
@@ -898,19 +1004,23 @@ __global__ __launch_bounds__(512) void k_linear_few(FewArgs g, const T* __restri
         y[row * g.N + n] = (T)v;
     }
     if (FUSED && n0 == 0) {  // u for the backward, laid out as k_shrink does
-        for (int i = tid; i < (int)g.M * half; i += 512) {
-            const int row = i / half, j = i - row * half;
-            const float v = j < g.r ? us[row * g.r + j] : 0.f;
-            u_out[row * g.rp + j] = (T)v;
-            if (H == 2) u_out[row * g.rp + half + j] = low_half(v, (T)v);
+        for (int i = tid; i < (int)g.M * g.rp; i += 512) {
+            const int row = i / g.rp, at = i - row * g.rp, c = at / sec, j = at - c * sec;
+            L n[H];
+            parts_of(c < kSections<T> && j < g.r ? us[row * g.r + j] : 0.f, n);
+            L o = n[0];
+#pragma unroll
+            for (int h = 1; h < H; ++h) o = section_part(c) == h ? n[h] : o;
+            u_out[i] = o;
         }
         if (uT) {
             const int64_t plane = mtk_up(g.r, 64) * g.Mp;
             for (int i = tid; i < (int)(mtk_up(g.r, 16) * g.Mp); i += 512) {
                 const int j = i / (int)g.Mp, row = i - j * (int)g.Mp;
-                const float v = j < g.r && row < g.M ? us[row * g.r + j] : 0.f;
-                uT[i] = (T)v;
-                uT[plane + i] = low_half(v, (T)v);
+                L n[H];
+                parts_of(j < g.r && row < g.M ? us[row * g.r + j] : 0.f, n);
+#pragma unroll
+                for (int h = 0; h < H; ++h) uT[h * plane + i] = n[h];
             }
         }
     }
@@ -929,11 +1039,11 @@ struct WgradArgs {
 // of columns and take the chunk's row groups in turn, the next group's loads in flight under the current one's products; their sums
 // meet in LDS.  Two such products (down's and up's gradient) share a launch.
 // 16-bit types: MFMA 16 x 16 x 32, the rows are its k.  u^T gives a lane's eight rows of one j as one piece; x's eight rows of eight
-// columns come as eight pieces and are turned in registers.  fp32: 16 x 16 x 4, a lane holds one row's four columns and one j.
+// columns come as eight pieces and are turned in registers, with fp16 into two bf16 numbers (exact) as B_e is.  fp32: 16 x 16 x 4, a lane holds one row's four columns and one j.
 // Rows of other models are zeroed in BOTH operands (0 x inf).  65,536 rows of 1,024 bf16, both factors: 59 us (268 MB: 4.6 TB/s); the join 7 us.
 template <typename T> constexpr int kStrip = sizeof(T) == 4 ? 64 : 128;  // columns of a workgroup
 template <typename T, int JT>
-__device__ void wgrad_body(const WgradArgs& g, int strip, int c, int j0, const T* __restrict__ u, const T* __restrict__ uT, const T* __restrict__ x, float* __restrict__ part,
+__device__ void wgrad_body(const WgradArgs& g, int strip, int c, int j0, const Low<T>* __restrict__ u, const Low<T>* __restrict__ uT, const T* __restrict__ x, float* __restrict__ part,
                            float (*sum)[64 * 4]) {
     constexpr int V = mtk_piece<T>::n, NV = V;  // columns per lane
     constexpr int GR = sizeof(T) == 4 ? 16 : 32, PL = sizeof(T) == 4 ? 4 : 8;  // rows of a group, pieces of x per lane
@@ -949,7 +1059,8 @@ __device__ void wgrad_body(const WgradArgs& g, int strip, int c, int j0, const T
         f32x4 acc[JT][NV] = {};
         mtk_vec<T> xv[PL];
         T us[sizeof(T) == 4 ? PL : 1][JT];
-        mtk_vec<T> ut[2][JT];  // hi, lo
+        constexpr int P = kParts<T>;
+        mtk_vec<Low<T>> ut[P][JT];  // the numbers of u
         // A scalar base and one 32-bit offset per lane.  A group with rows of other models clamps its rows to this one's and clears what it read
         // for them: a load that is made under a condition costs a branch (2,048 rows of 16 models in bf16: 26 us with such loads, _NOW_ without)
         const int64_t plane = mtk_up(g.r, 64) * g.Mp;
@@ -990,12 +1101,12 @@ __device__ void wgrad_body(const WgradArgs& g, int strip, int c, int j0, const T
 #pragma unroll
                 for (int t = 0; t < JT; ++t)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) ut[h][t] = mtk_ld(uT + h * plane + (int64_t)(j0 + t * 16 + li) * g.Mp + r0 + q * 8);
+                    for (int h = 0; h < P; ++h) ut[h][t] = mtk_ld(uT + h * plane + (int64_t)(j0 + t * 16 + li) * g.Mp + r0 + q * 8);
             }
             if (!inside) {
-                auto clear = [](mtk_vec<T>& v, uint4 m) {
+                auto clear = [](auto& v, uint4 m) {
                     const uint4 w = __builtin_bit_cast(uint4, v);
-                    v = __builtin_bit_cast(mtk_vec<T>, make_uint4(w.x & m.x, w.y & m.y, w.z & m.z, w.w & m.w));
+                    v = __builtin_bit_cast(typename std::remove_reference<decltype(v)>::type, make_uint4(w.x & m.x, w.y & m.y, w.z & m.z, w.w & m.w));
                 };
                 auto keeps = [&](int row) { return row >= lo_r && row < hi_r ? 0xffffffffu : 0u; };
 #pragma unroll
@@ -1013,26 +1124,44 @@ __device__ void wgrad_body(const WgradArgs& g, int strip, int c, int j0, const T
 #pragma unroll
                     for (int t = 0; t < JT; ++t)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) clear(ut[h][t], make_uint4(m[0], m[1], m[2], m[3]));
+                        for (int h = 0; h < P; ++h) clear(ut[h][t], make_uint4(m[0], m[1], m[2], m[3]));
                 }
             }
         };
         const int64_t start = a / GR * GR + wave * GR;
         if (start < b) load(start);
         for (int64_t r0 = start; r0 < b; r0 += 4 * GR) {
-            mtk_vec<T> xc[PL], uc[2][JT];
+            mtk_vec<T> xc[PL];
+            mtk_vec<Low<T>> uc[P][JT];
             T uu[sizeof(T) == 4 ? PL : 1][JT];
 #pragma unroll
             for (int i = 0; i < PL; ++i) xc[i] = xv[i];
 #pragma unroll
             for (int t = 0; t < JT; ++t) {
-                if constexpr (sizeof(T) == 2) uc[0][t] = ut[0][t], uc[1][t] = ut[1][t];
-                else
+                if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                    for (int h = 0; h < P; ++h) uc[h][t] = ut[h][t];
+                } else
 #pragma unroll
                     for (int i = 0; i < PL; ++i) uu[i][t] = us[i][t];
             }
             if (r0 + 4 * GR < b) load(r0 + 4 * GR);
-            if constexpr (sizeof(T) == 2) {
+            if constexpr (kF16<T>) {
+#pragma unroll
+                for (int cc = 0; cc < NV; ++cc) {
+                    mtk_vec<T> col;
+                    mtk_vec<Low<T>> b, d;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) col.v[i] = xc[i].v[cc];
+                    two_numbers(col, b, d);
+#pragma unroll
+                    for (int t = 0; t < JT; ++t) {  // small ones first
+                        f32x4 a = mma16(uc[1][t], d, acc[t][cc]);
+                        a = mma16(uc[0][t], d, mma16(uc[2][t], b, a));
+                        acc[t][cc] = mma16(uc[0][t], b, mma16(uc[1][t], b, a));
+                    }
+                }
+            } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
                 for (int cc = 0; cc < NV; ++cc) {
                     mtk_vec<T> col;
@@ -1084,7 +1213,8 @@ __device__ void wgrad_body(const WgradArgs& g, int strip, int c, int j0, const T
 template <typename T> struct WgradOne {
     WgradArgs g;
     int strips, chunks;
-    const T *u, *uT, *x;
+    const Low<T> *u, *uT;
+    const T* x;
     float* part;
     T* out;
     int turn;
@@ -1133,14 +1263,15 @@ __global__ __launch_bounds__(256) void k_wgrad_join(WgradBoth<T> both) {
 
 // ------------------------------------------------------------------------------------------------------------------ helpers
 // k_prep: everything that has to be laid out before the products, in one launch.  A job owns consecutive workgroups.
-enum { JOB_TURN, JOB_PAD, JOB_BIAS, JOB_OWNER, JOB_ODD };
+enum { JOB_TURN, JOB_PAD, JOB_BIAS, JOB_OWNER, JOB_ODD, JOB_TURN_TWO, JOB_TWO };
 struct Job {
     int type, first;      // first workgroup
     const void* src;
     void* dst;
     int64_t rows, ld;     // PAD: rows and source row stride; OWNER: rows of x; BIAS: padded length
     int R, C, ldo;        // TURN: [batch][R][C] -> [batch][C][ldo]; PAD: [rows][C] -> [rows][ldo]; zeros behind; BIAS: C values; OWNER: C tiles of R rows;
-                          // ODD: four workgroups for each of the runs of `rows` values
+                          // ODD: four workgroups for each of the runs of `rows` values; TURN_TWO, TWO: as TURN and PAD, from fp16 to
+                          // rows of sections of two bf16 numbers
     int E;                // OWNER
     int rep;              // TURN, PAD: a row repeats every rep elements (a multiple of 32)
 };
@@ -1175,6 +1306,49 @@ __device__ void prep_body(const Jobs& jobs, int block, float* lds) {
         __syncthreads();
         for (int i = ty; i < 32; i += 8)
             if (c0 + i < j.C && r0 + tx < j.ldo) out[(int64_t)(c0 + i) * j.ldo + r0 + tx] = tile[tx][i];
+    } else if (kF16<T> && j.type == JOB_TURN_TWO) {
+        if constexpr (kF16<T>) {
+            const int nc = (j.C + 31) / 32, nr = (j.R + 31) / 32, sec = section<T>(j.R);
+            const int64_t bat = blk / (nc * nr);
+            const int rest = (int)(blk - bat * nc * nr), c0 = rest % nc * 32, r0 = rest / nc * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+            const T* in = (const T*)j.src + bat * j.R * j.C;
+            Low<T>* out = (Low<T>*)j.dst + bat * j.C * j.ldo;
+            for (int i = ty; i < 32; i += 8) tile[i][tx] = r0 + i < j.R && c0 + tx < j.C ? in[(int64_t)(r0 + i) * j.C + c0 + tx] : T(0);
+            __syncthreads();
+            for (int i = ty; i < 32; i += 8) {
+                if (c0 + i >= j.C) break;
+                Low<T>* row = out + (int64_t)(c0 + i) * j.ldo;
+                Low<T> n[2];
+                parts_of((float)tile[tx][i], n);
+                if (r0 + tx < sec)
+#pragma unroll
+                    for (int c = 0; c < kSections<T>; ++c) row[c * sec + r0 + tx] = n[section_second(c)];
+                if (r0 == 0)
+                    for (int k = kSections<T> * sec + tx; k < j.ldo; k += 32) row[k] = Low<T>(0.f);
+            }
+        }
+    } else if (kF16<T> && j.type == JOB_TWO) {  // four values a thread
+        if constexpr (kF16<T>) {
+            struct __attribute__((aligned(8), may_alias)) Quad { Low<T> v[4]; };
+            const int sec = section<T>(j.C), quads = sec / 4;
+            const int64_t p = blk * 256 + threadIdx.x, at = p / quads;
+            if (at < j.rows) {
+                const int k0 = (int)(p - at * quads) * 4;
+                const T* in = (const T*)j.src + at * j.ld + k0;
+                Low<T>* row = (Low<T>*)j.dst + at * j.ldo;
+                Quad o[2];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    Low<T> n[2];
+                    parts_of(k0 + i < j.C ? (float)in[i] : 0.f, n);
+                    o[0].v[i] = n[0];
+                    o[1].v[i] = n[1];
+                }
+#pragma unroll
+                for (int c = 0; c < kSections<T>; ++c) *reinterpret_cast<Quad*>(row + c * sec + k0) = o[section_second(c)];
+                for (int k = kSections<T> * sec + k0; k < j.ldo; k += sec) *reinterpret_cast<Quad*>(row + k) = Quad{};
+            }
+        }
     } else if (j.type == JOB_PAD) {  // ldo is a multiple of a piece, dst 16-byte aligned
         const int ppr = j.ldo / V;
         const int64_t n = j.rows * ppr;
@@ -1218,7 +1392,7 @@ __global__ __launch_bounds__(256) void k_prep(Jobs jobs) {
 // the shrink and what neither waits for the other: the jobs' workgroups run under its own (behind them: in front they leave the CUs' free
 // places uneven: 65,536 rows of 64 models in bf16 56 us for 39)
 template <typename T, int RT, int KS>
-__global__ __launch_bounds__(256) void k_shrink(ShrinkArgs g, Jobs jobs, int j0, const T* __restrict__ x, const T* __restrict__ F, T* __restrict__ u, T* __restrict__ uT) {
+__global__ __launch_bounds__(256) void k_shrink(ShrinkArgs g, Jobs jobs, int j0, const T* __restrict__ x, const T* __restrict__ F, Low<T>* __restrict__ u, Low<T>* __restrict__ uT) {
     __shared__ float lds[kShrinkLds<RT, KS> > 32 * 33 ? kShrinkLds<RT, KS> : 32 * 33];
     const int own = g.tiles * g.turns;
     if ((int)blockIdx.x < own) shrink_body<T, RT, KS>(g, blockIdx.x, j0, x, F, u, uT, lds);
@@ -1252,7 +1426,7 @@ int wgrad_chunk(int64_t M, int D, int dtype) {
 int64_t wgrad_part(int64_t M, int D, int r, int E, int dtype) { return (cdiv(M, wgrad_chunk(M, D, dtype)) + E) * mtk_up(r, kRankT) * D; }
 
 template <typename T, int RT>
-void shrink_launch(ShrinkArgs g, const Jobs& jobs, int j0, const T* x, const T* F, T* u, T* uT, hipStream_t s) {
+void shrink_launch(ShrinkArgs g, const Jobs& jobs, int j0, const T* x, const T* F, Low<T>* u, Low<T>* uT, hipStream_t s) {
     // 32 rows a wave fill the chip from some 16,384 rows on; below, four waves split 16 rows
     const int turns = g.M >= 4096 ? 2 : g.M >= 2048 ? 4 : 16;
     g.turns = g.E < turns ? g.E : turns;
@@ -1262,7 +1436,7 @@ void shrink_launch(ShrinkArgs g, const Jobs& jobs, int j0, const T* x, const T* 
     else k_shrink<T, RT, 4><<<grid, 256, 0, s>>>(g, jobs, j0, x, F, u, uT);
 }
 template <typename T>
-void shrink(const ShrinkArgs& g, Jobs jobs, const T* x, const T* F, T* u, T* uT, hipStream_t s) {
+void shrink(const ShrinkArgs& g, Jobs jobs, const T* x, const T* F, Low<T>* u, Low<T>* uT, hipStream_t s) {
     for (int j0 = 0; j0 < g.r; j0 += 64, jobs.n = jobs.blocks = 0) {
         if (g.r - j0 > 32) shrink_launch<T, 4>(g, jobs, j0, x, F, u, uT, s);
         else if (g.r - j0 > 16) shrink_launch<T, 2>(g, jobs, j0, x, F, u, uT, s);
@@ -1270,7 +1444,7 @@ void shrink(const ShrinkArgs& g, Jobs jobs, const T* x, const T* F, T* u, T* uT,
     }
 }
 template <typename T>
-WgradOne<T> wgrad_one(int64_t M, int64_t x_ld, int64_t Mp, int D, int r, int rp, int E, const int32_t* offsets, int dtype, int turn, const T* u, const T* uT, const T* x,
+WgradOne<T> wgrad_one(int64_t M, int64_t x_ld, int64_t Mp, int D, int r, int rp, int E, const int32_t* offsets, int dtype, int turn, const Low<T>* u, const Low<T>* uT, const T* x,
                       float* part, T* out) {
     const int chunk = wgrad_chunk(M, D, dtype);
     return WgradOne<T>{WgradArgs{M, x_ld, Mp, D, r, rp, E, chunk, offsets}, (int)cdiv(D, kStrip<T>), out ? (int)cdiv(M, chunk) : 0, u, uT, x, part, out, turn};
@@ -1304,7 +1478,7 @@ struct Saved {
         Layout l;
         Mp = mtk_up(M, 32);
         u = l.take(M * rank_pad(r, dtype) * mtk_dtype_size(dtype));
-        uT = dtype == MTK_DT_F32 ? l.at : l.take(2 * Mp * mtk_up(r, 64) * mtk_dtype_size(dtype));
+        uT = dtype == MTK_DT_F32 ? l.at : l.take((dtype == MTK_DT_F16 ? kParts<mtk_f16> : kParts<mtk_bf16>) * Mp * mtk_up(r, 64) * mtk_dtype_size(dtype));
         bytes = l.at;
     }
 };
@@ -1332,6 +1506,8 @@ struct Shape {
         else kind = t256 * 5 >= cdiv(t256, 256) * 256 * 4 ? 0 : t128 > 256 ? 1 : 2;
         BM = BN = kind == 0 ? 256 : kind == 1 ? 128 : 64;
         blocks = M >= (int64_t)E * BM;
+        // k_linear with RAW: in 256 x 256 tiles its accumulators spill.  us, 128 / 256: 65,536 rows of 512 models 241 / 291, of 1,000 296 / 413
+        if (dtype == MTK_DT_F16 && !blocks && kind == 0) kind = 1, BM = BN = 128;
         MT = cdiv(M, BM);
         nb_n = (int)cdiv(N, BN);
     }
@@ -1389,6 +1565,13 @@ void job_turn(Jobs& jobs, const void* src, void* dst, int R, int C, int ldo, int
 void job_pad(Jobs& jobs, const void* src, int64_t ld, void* dst, int64_t rows, int C, int ldo, int V, int rep = 1 << 30) {
     jobs.add(Job{JOB_PAD, 0, src, dst, rows, ld, 0, C, ldo, 0, rep}, cdiv(rows * (ldo / V), kPadPieces));
 }
+// the same for rows of sections
+void job_turn_two(Jobs& jobs, const void* src, void* dst, int R, int C, int ldo, int batch) {
+    jobs.add(Job{JOB_TURN_TWO, 0, src, dst, 0, 0, R, C, ldo, 0, 1}, cdiv(C, 32) * cdiv(R, 32) * batch);
+}
+void job_two(Jobs& jobs, const void* src, void* dst, int64_t rows, int C, int ldo) {
+    jobs.add(Job{JOB_TWO, 0, src, dst, rows, C, 0, C, ldo, 0, 1}, cdiv(rows * (section<mtk_f16>(C) / 4), 256));
+}
 template <typename T> void prep(const Jobs& jobs, hipStream_t s) {
     if (jobs.blocks) k_prep<T><<<(unsigned)jobs.blocks, 256, 0, s>>>(jobs);
 }
@@ -1396,7 +1579,7 @@ template <typename T> void prep(const Jobs& jobs, hipStream_t s) {
 // CUs of the current device, and whether a kernel's LDS limit has been raised there
 struct DeviceState {
     int cus = 0;
-    bool lds[9] = {};
+    bool lds[11] = {};
 };
 DeviceState* device_state() {
     static DeviceState st[64];
@@ -1410,42 +1593,47 @@ DeviceState* device_state() {
     return &st[d];
 }
 
-template <typename T, int WR, int WC, int MW, int NT, int DX, int DW>
+template <typename T, bool RAW, int WR, int WC, int MW, int NT, int DX, int DW>
 int launch_linear(const LinearArgs& g, int which, hipStream_t s) {
     typedef Geo<WR, WC, MW, NT, DX, DW> G;
     DeviceState* st = device_state();
     if (!st) MTK_FAIL(MTK_ERR_HIP, "adapter product: no device properties");
     if (!st->lds[which]) {
-        MTK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear<T, WR, WC, MW, NT, DX, DW>), hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds));
+        MTK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(k_linear<T, WR, WC, MW, NT, DX, DW, RAW>), hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds));
         st->lds[which] = true;
     }
     const int64_t per_xcd = cdiv(g.MT * g.nb_n, 8), room = (int64_t)st->cus / 8 * G::kRoom;
-    k_linear<T, WR, WC, MW, NT, DX, DW><<<(unsigned)(8 * (per_xcd < room ? per_xcd : room)), 64 * G::NW, G::kLds, s>>>(g);
+    k_linear<T, WR, WC, MW, NT, DX, DW, RAW><<<(unsigned)(8 * (per_xcd < room ? per_xcd : room)), 64 * G::NW, G::kLds, s>>>(g);
     return MTK_OK;
+}
+template <typename T, bool RAW> int linear_tile(const Shape& sh, LinearArgs& g, hipStream_t s) {
+    constexpr int base = RAW ? 8 : sizeof(T) == 4 ? 0 : std::is_same<T, mtk_bf16>::value ? 3 : 6;
+    if constexpr (sizeof(T) == 2 && !RAW)
+        if (sh.kind == 0) return launch_linear<T, RAW, 2, 4, 4, 2, 3, 2>(g, base, s);
+    if (sh.kind == 1) return launch_linear<T, RAW, 4, 2, 1, 2, 3, 2>(g, base + 1, s);
+    return launch_linear<T, RAW, 2, 2, 1, 1, 3, 2>(g, base + 2, s);
 }
 template <typename T> int linear(const Shape& sh, LinearArgs& g, T* y, hipStream_t s) {
     g.Y = y;
-    constexpr int base = sizeof(T) == 4 ? 0 : std::is_same<T, mtk_bf16>::value ? 3 : 6;
-    if constexpr (sizeof(T) == 2)
-        if (sh.kind == 0) return launch_linear<T, 2, 4, 4, 2, 3, 2>(g, base, s);
-    if (sh.kind == 1) return launch_linear<T, 4, 2, 1, 2, 3, 2>(g, base + 1, s);
-    return launch_linear<T, 2, 2, 1, 1, 3, 2>(g, base + 2, s);
+    if constexpr (kF16<T>)
+        if (!sh.blocks) return linear_tile<T, true>(sh, g, s);
+    return linear_tile<T, false>(sh, g, s);
 }
 template <typename T>
-void linear_few(const FewArgs& g, const T* x, const T* W, const T* bias, const T* u, const T* up, T* y, hipStream_t s) {
+void linear_few(const FewArgs& g, const T* x, const T* W, const T* bias, const Low<T>* u, const T* up, T* y, hipStream_t s) {
     if (g.M <= 64) k_linear_few<T, 16, false><<<(unsigned)(cdiv(g.M, 16) * cdiv(g.N, 16)), 512, 0, s>>>(g, x, W, bias, u, up, y, nullptr, nullptr, nullptr);
     else k_linear_few<T, 32, false><<<(unsigned)(cdiv(g.M, 32) * cdiv(g.N, 32)), 512, 0, s>>>(g, x, W, bias, u, up, y, nullptr, nullptr, nullptr);
 }
 // the shrink and the product of a row or some
 template <typename T>
-void linear_fused(const FewArgs& g, const T* x, const T* W, const T* bias, const T* down, const T* up, T* u, T* uT, T* y, hipStream_t s) {
+void linear_fused(const FewArgs& g, const T* x, const T* W, const T* bias, const T* down, const T* up, Low<T>* u, Low<T>* uT, T* y, hipStream_t s) {
     k_linear_few<T, 16, true><<<(unsigned)cdiv(g.N, 16), 512, 0, s>>>(g, x, W, bias, u, up, y, down, u, uT);
 }
 // the jobs of a k_linear product: x and W padded where they do not stream, B_e in whole lines and a block of zeros, bias, tiles' models.
 // `early`: what the shrink reads.  F: W [N][K], or its transpose [K][N] when `turned`; L: B [E][N][r], or [E][r][N]
 template <typename T>
 LinearArgs plan_linear(Jobs& early, Jobs& jobs, const Shape& sh, const Packed& pk, char* wb, int64_t M, int N, int K, int r, int E, int dtype, const T* x, int64_t x_ld,
-                       const T* F, bool turned, const T* bias, const T* L, const T* u, const int32_t* offsets, int relu) {
+                       const T* F, bool turned, const T* bias, const T* L, const Low<T>* u, const int32_t* offsets, int relu) {
     constexpr int V = mtk_piece<T>::n;
     LinearArgs g{};
     g.M = M; g.MT = sh.MT; g.N = N; g.nb_n = sh.nb_n;
@@ -1467,9 +1655,10 @@ LinearArgs plan_linear(Jobs& early, Jobs& jobs, const Shape& sh, const Packed& p
     const int64_t nbias = (int64_t)sh.nb_n * sh.BN;
     jobs.add(Job{JOB_BIAS, 0, bias, wb + pk.bias, nbias, 0, 0, bias ? N : 0, 0, 0, 1}, cdiv(nbias, 256));
     if (sh.blocks) {
-        const int half = sizeof(T) == 2 ? sh.rp / 2 : sh.rp;
-        if (turned) job_turn(jobs, L, wb + pk.Bp, r, N, sh.rp, E, half);
-        else job_pad(jobs, L, r, wb + pk.Bp, (int64_t)E * N, r, sh.rp, V, half);
+        if (kF16<T> && turned) job_turn_two(jobs, L, wb + pk.Bp, r, N, sh.rp, E);
+        else if (kF16<T>) job_two(jobs, L, wb + pk.Bp, (int64_t)E * N, r, sh.rp);
+        else if (turned) job_turn(jobs, L, wb + pk.Bp, r, N, sh.rp, E, section<T>(r));
+        else job_pad(jobs, L, r, wb + pk.Bp, (int64_t)E * N, r, sh.rp, V, section<T>(r));
         jobs.add(Job{JOB_ODD, 0, L, wb + pk.odd, (int64_t)N * r, 0, 0, 0, 0, E, 1}, (int64_t)E * 4);
         jobs.add(Job{JOB_OWNER, 0, offsets, wb + pk.owner, M, 0, sh.BM, (int)sh.MT, 0, E, 1}, cdiv(sh.MT, 4));
         g.owner = (const int32_t*)(wb + pk.owner);
@@ -1520,8 +1709,8 @@ extern "C" int mtk_adapter_forward(int64_t M, int din, int dout, int r, int E, i
         typedef decltype(tag) T;
         const hipStream_t s = (hipStream_t)stream;
         const Shape& sh = wk.sh;
-        T* u = (T*)((char*)saved + sv.u);
-        T* uT = keep && sizeof(T) == 2 ? (T*)((char*)saved + sv.uT) : nullptr;
+        Low<T>* u = (Low<T>*)((char*)saved + sv.u);
+        Low<T>* uT = keep && sizeof(T) == 2 ? (Low<T>*)((char*)saved + sv.uT) : nullptr;
         ShrinkArgs sa{M, din, r, sh.rp, E, x_ld, offsets, scales, (float)scale, sv.Mp, (char*)work + wk.pk.pairs, sh.blocks && !sh.few ? sh.BM : 0, 1, 1};
         if (sh.few) {
             const FewArgs fa{M, x_ld, dout, din, r, sh.rp, E, act, offsets, scales, (float)scale, sv.Mp};
@@ -1580,8 +1769,8 @@ extern "C" int mtk_adapter_backward(int64_t M, int din, int dout, int r, int E, 
         const hipStream_t s = (hipStream_t)stream;
         const Shape& sh = wk.sh;
         char* wb = (char*)work;
-        const T *u = (const T*)((const char*)saved + sv.u), *uT = (const T*)((const char*)saved + sv.uT);
-        T *t = (T*)(wb + wk.t + sv.u), *tT = (T*)(wb + wk.t + sv.uT);
+        const Low<T> *u = (const Low<T>*)((const char*)saved + sv.u), *uT = (const Low<T>*)((const char*)saved + sv.uT);
+        Low<T> *t = (Low<T>*)(wb + wk.t + sv.u), *tT = (Low<T>*)(wb + wk.t + sv.uT);
         const T* g = (const T*)dy;
         if (act) {
             T* gz = (T*)(wb + wk.g);

@@ -567,6 +567,72 @@ def test_adapter_refusals():
         call(a, weight=a["weight"].clone().requires_grad_())
 
 
+# a row, few rows in both tiles, each tile of the product as one run of lines and (many models) apart from it; ranks of a line and of several
+HALVES = [(1, 72, 40, 8, 1), (2, 40, 72, 20, 2), (61, 130, 67, 12, 5), (300, 40, 72, 33, 4), (700, 72, 80, 12, 3), (700, 80, 72, 20, 40), (4229, 1030, 1030, 16, 7), (2048, 130, 1030, 64, 3),
+          (16500, 1000, 131, 8, 40), (16384, 64, 1024, 100, 2)]
+
+
+def strictly(mag, K, want):
+    """Sums of K terms of magnitude `mag`, the low-rank rows off by 2^-22 of their own magnitude whatever that is, and the result's own rounding: of
+    its magnitude, or half the smallest step."""
+    return (TWICE * (K + 8) * U32 + 2.0**-22) * mag + half(torch.float16) * want.abs() * 1.01 + 2.0**-25 * 1.01
+
+
+@pytest.mark.parametrize("M,din,dout,r,E", HALVES)
+def test_half_precision_keeps_small_low_rank_values(M, din, dout, r, E):
+    """Gradients of 1e-3 against factors that have just left zero: t = s g B_e is far below fp16's normal numbers (and u in the forward direction),
+    the results are not.  The shared weights are zero, or they would drown the low-rank part."""
+    g = gen(M + r)
+    dt = torch.float16
+    a = adapter_inputs(g, M, din, dout, r, E, dt)
+    a["weight"].zero_(), a["bias"].zero_()
+    rows = int((a["offsets"][1:] - a["offsets"][:-1]).max())
+
+    def run(gy):
+        leaves = {n: a[n].detach().clone().requires_grad_() for n in ("x", "down", "up")}
+        y = call(a, **leaves)
+        grads = torch.autograd.grad(y, list(leaves.values()), gy)
+        return y, grads, adapter_reference(**{**a, "relu": False, "gy": gy})
+
+    a["up"] = randn(g, E, dout, r, dt=dt) * 2e-4
+    a["down"] = randn(g, E, r, din, dt=dt) * 16
+    gy = randn(g, M, dout, dt=dt) * 1e-3
+    _, (dx, ddown, _), ref = run(gy)
+    assert float((a["scale"].max() * (gy.double() @ a["up"][0].double())).abs().max()) < 2.0**-12
+    within(dx, ref["dx"], strictly(ref["dx_low"], dout + r, ref["dx"]))
+    within(ddown, ref["ddown"], strictly(ref["ddown_terms"], dout + rows, ref["ddown"]))
+    a["x"] = randn(g, M, din, dt=dt) * 1e-3
+    a["down"] = randn(g, E, r, din, dt=dt) * 2e-4
+    a["up"] = randn(g, E, dout, r, dt=dt) * 64
+    y, (_, _, dup), ref = run(randn(g, M, dout, dt=dt) * 64)
+    within(y, ref["y"], strictly(ref["y_low"], din + r, ref["y"]))
+    within(dup, ref["dup"], strictly(ref["dup_terms"], din + rows, ref["dup"]))
+
+
+@pytest.mark.parametrize("M,din,dout,r,E", HALVES)
+def test_half_precision_keeps_large_low_rank_values(M, din, dout, r, E):
+    """u beyond fp16's largest number where y, dx and the factors' gradients are well inside"""
+    g = gen(M + r + 1)
+    dt = torch.float16
+    a = adapter_inputs(g, M, din, dout, r, E, dt)
+    a["x"], a["down"] = randn(g, M, din, dt=dt) * 2048, randn(g, E, r, din, dt=dt) * 128
+    a["up"], gy = randn(g, E, dout, r, dt=dt) * 2.0**-20, randn(g, M, dout, dt=dt) * 2.0**-12
+    for n in ("x", "down", "up"):
+        a[n].requires_grad_()
+    a["weight"] *= 2.0**-9
+    y = call(a)
+    dx, ddown, dup = torch.autograd.grad(y, (a["x"], a["down"], a["up"]), gy)
+    ref = adapter_reference(**{**a, "relu": False, "gy": gy})
+    rows = int((a["offsets"][1:] - a["offsets"][:-1]).max())
+    assert rows == 0 or float((a["x"].detach().double() @ a["down"][0].detach().double().t()).abs().max()) > 65504
+    within(y, ref["y"], strictly(ref["y_terms"] + ref["y_low"], din + r, ref["y"]))
+    within(dx, ref["dx"], strictly(ref["dx_terms"] + ref["dx_low"], dout + r, ref["dx"]))
+    within(ddown, ref["ddown"], strictly(ref["ddown_terms"], dout + rows, ref["ddown"]))
+    inside = ref["dup"].abs() < 65000
+    assert bool(inside.any())
+    within(torch.where(inside.to(DEV), dup, 0), torch.where(inside, ref["dup"], 0), strictly(ref["dup_terms"], din + rows, torch.where(inside, ref["dup"], 0)))
+
+
 def test_a_scale_that_requires_grad_is_refused():
     """It would get none: refused whether or not anything else of the layer is trained"""
     g = gen(93)
