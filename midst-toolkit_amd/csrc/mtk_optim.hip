@@ -67,10 +67,11 @@ __device__ __forceinline__ float dither(float x, float inv_scale, uint32_t w, fl
     const float q = __uint_as_float((__float_as_uint(y + lift) + (w >> 12)) & 0xfff00000u) - lift;
     return __builtin_amdgcn_fmed3f(q, lowest, 448.f);
 }
-// sqrt(v), correctly rounded but for rare ties, in six instructions: the hardware's reciprocal root and one correction.  Roots of zero (the cap)
-// and of numbers below 2^-126 (counted as 0 by the instruction) stay small.
+// sqrt(v), correctly rounded but for rare ties, in six instructions: the hardware's reciprocal root and one correction.  The cap is the reciprocal
+// root of the smallest normal number: it serves 0 and numbers below 2^-126 (counted as 0 by the instruction), whose roots stay small.  Of an
+// infinity it makes NaN, which the rare path of the kernel looks after (220 million bf16 values 417 -> 420 us; by a select here 435).
 __device__ __forceinline__ float fast_sqrt(float v) {
-    const float y = fminf(__builtin_amdgcn_rsqf(v), 0x1p60f), r = v * y;
+    const float y = fminf(__builtin_amdgcn_rsqf(v), 0x1p63f), r = v * y;
     return __builtin_fmaf(__builtin_fmaf(-r, r, v) * 0.5f, y, r);
 }
 
@@ -191,10 +192,13 @@ __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
             p1.v[i] = (T)((float)p0.v[i] * h.decay - h.step_size * (m[i] / (r[i] * h.inv_bc2 + h.eps)));
         }
     }
-    if (left < V) mtk_st_n(pp, p1, left);
-    else if (nt) mtk_st_nt(pp, p1);
-    else mtk_st(pp, p1);
+    auto store_p = [&]() {
+        if (left < V) mtk_st_n(pp, p1, left);
+        else if (nt) mtk_st_nt(pp, p1);
+        else mtk_st(pp, p1);
+    };
     if (!Q8) {
+        store_p();
         st_f32<V>((float*)a.m[lo] + i0, left, m, nt);
         st_f32<V>((float*)a.v[lo] + i0, left, v, nt);
         return;
@@ -212,6 +216,14 @@ __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
     constexpr uint32_t kInf = 0x7f800000u;
     const bool bad = am >= kInf || ar >= kInf;  // the same in all lanes of a block
     if (__any(bad)) {  // rare: the scales go by the finite values (blocks without others keep theirs)
+        // A mean square that overflowed (its root came out as NaN, though neither the gradient, which m would show, nor the old root is one): the
+        // quotient is m / inf.  What was read is read again: kept for this, it would cost a quarter of the waves of a CU.
+        float old[V];
+        ld_codes<V>((const uint8_t*)a.v[lo] + i0, left, old, false);
+        const mtk_vec<T> q0 = mtk_ld_n(pp, left);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (r[i] != r[i] && m[i] == m[i] && old[i] == old[i]) p1.v[i] = (T)((float)q0.v[i] * h.decay - h.step_size * (m[i] * 0.f));
         uint32_t fm = 0, fr = 0;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -222,6 +234,7 @@ __global__ __launch_bounds__(256) void k_adamw(AdamwArgs a) {
         am = block_max(fm);
         ar = block_max(fr);
     }
+    store_p();
     const int km = am ? scale_exp(am) : 0, kr = ar ? scale_exp(ar) : 0;
     const float im = pow2(-km), ir = pow2(-kr);
     uint32_t wm = (uint32_t)i0 * kPlaceM + h.phase, wr = (uint32_t)i0 * kPlaceR + h.phase;

@@ -900,6 +900,43 @@ def test_adamw_extremes():
             assert bool((p <= 1).all())
 
 
+def test_adamw_where_a_squared_gradient_overflows():
+    """The mean square is infinite, the quotient 0: parameters decay and no more, in both forms alike.  Gradients beside them go on as ever."""
+    g = gen(35)
+    n = 600
+    grad = randn(g, n)
+    far = torch.zeros(n, dtype=torch.bool)
+    far[[0, 7, 300, 599]] = True
+    grad[[0, 7, 300, 599]] = torch.tensor([1e20, -3e19, 2e38, 6e21], device=DEV)
+    start, sides = randn(g, n), []
+    for bits in (32, 8):
+        p = torch.nn.Parameter(start.clone())
+        opt = mtk.AdamW([p], lr=1e-2, weight_decay=0.5, state_bits=bits)
+        p.grad = grad.clone()
+        opt.step()
+        sides.append(p.detach().cpu())
+    decayed = start.cpu() * float(np.float32(1 - 1e-2 * 0.5))
+    assert torch.equal(sides[0][far], decayed[far]) and torch.equal(sides[1][far], decayed[far])
+    # elsewhere: the quotient by a reciprocal of one unit in its last place and a product, a root that may round the other way
+    assert bool(((sides[0] - sides[1]).abs()[~far] <= 1e-2 * 8 * U32 + 2 * U32 * sides[0].abs()[~far]).all())
+
+
+def test_adamw_roots_of_the_smallest_normal_numbers():
+    """v = (1 - b2) g^2 from 2^-126 to 2^-118: the codes and scales of its root are those of the exact one"""
+    b2 = 0.75  # (1 - b2) g^2 is exact for these g
+    grad = torch.cat([torch.full((256,), 2.0 ** (k / 2) if k % 2 == 0 else 1.5 * 2.0 ** ((k - 1) // 2)) for k in range(-124, -115)]).to(DEV)
+    n = grad.numel()
+    code = lambda: torch.zeros(n, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)  # noqa: E731
+    m, v = code(), code()
+    ms, vs = (torch.ones(n // 256, device=DEV) for _ in range(2))
+    p = torch.ones(n, device=DEV)
+    z = np.zeros(n, np.float32)
+    mtk.adamw_step([p], [grad], [m], [v], 1, lr=1e-3, betas=(0.9, b2), exp_avg_scales=[ms], exp_avg_sq_scales=[vs])
+    _, wm, wms, wv, wvs = adamw8_reference(np.ones(n, np.float32), grad.cpu().numpy(), z, np.ones(n // 256), z, np.ones(n // 256), 1, b2=b2)
+    assert np.array_equal(vs.cpu().numpy(), wvs.astype(np.float32)) and np.array_equal(v.cpu().float().numpy(), wv.astype(np.float32))
+    assert np.array_equal(ms.cpu().numpy(), wms.astype(np.float32)) and np.array_equal(m.cpu().float().numpy(), wm.astype(np.float32))
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("dt", DTYPES)
 def test_a_step_past_the_caches_is_the_same_step(dt, bits):
