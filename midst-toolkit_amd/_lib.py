@@ -201,7 +201,10 @@ def ordinary(what: str, device: torch.device, fn, *args):
     with torch.cuda.device(device):
         got = fn(*args)
     if got is None:
-        raise RuntimeError(f"{what}: libmtk_hip: {lib().mtk_last_error().decode()}")
+        why = native().declined()
+        if why:
+            raise RuntimeError(f"{what}: libmtk_hip: {why}")
+        raise NotImplementedError(f"{what}: takes plain tensors that hold their own memory (not those inside torch.func transforms, vmap, or torch.compile's tracing)")
     return got
 
 

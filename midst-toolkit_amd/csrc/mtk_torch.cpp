@@ -49,6 +49,7 @@ union {
 } lib = {};
 
 struct Decline {};  // thrown to leave a call to the Python layer
+thread_local std::string refusal;  // what the library said, where the last decline was its own
 
 void need(bool ok) {
     if (!ok) throw Decline();
@@ -113,7 +114,10 @@ template <typename F> void call(F f) {  // a library call without the interprete
         } unlocked;
         rc = f();
     }
-    need(rc != MTK_ERR_ARG && rc != MTK_ERR_UNSUPPORTED);
+    if (rc == MTK_ERR_ARG || rc == MTK_ERR_UNSUPPORTED) {
+        refusal = lib.fn.last_error();
+        throw Decline();
+    }
     if (rc != MTK_OK) throw std::runtime_error(std::string("libmtk_hip: ") + lib.fn.last_error());
 }
 PyObject* pack(std::initializer_list<at::Tensor> ts) {
@@ -129,6 +133,7 @@ template <typename F> PyObject* guarded(Py_ssize_t n, Py_ssize_t want, F f) {
         return nullptr;
     }
     try {
+        refusal.clear();
         return f();
     } catch (const Decline&) {
         Py_RETURN_NONE;
@@ -146,9 +151,10 @@ bool tracked(std::initializer_list<at::Tensor> ts) {
         if (t.defined() && t.requires_grad()) return true;
     return false;
 }
-// The nodes go backward only: a tangent that the result would lose is left to the Python layer, which refuses it.
-void no_tangents(std::initializer_list<at::Tensor> ts) {
-    for (const at::Tensor& t : ts) need(!t.defined() || !t._fw_grad(0).defined());
+// The nodes go backward only, on tensors with memory: a tangent that the result would lose, or a functional transform's tensor, is left to the
+// Python layer, which refuses it.
+void plain(std::initializer_list<at::Tensor> ts) {
+    for (const at::Tensor& t : ts) need(!t.defined() || (t.has_storage() && !t._fw_grad(0).defined()));
 }
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
@@ -177,6 +183,9 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Py_RETURN_TRUE;
     });
 }
+
+// declined() -> what the library said to this thread's last call that returned None; empty where its tensors were the reason
+PyObject* declined(PyObject*, PyObject*) { return PyUnicode_FromString(refusal.c_str()); }
 
 // route(index, n_groups) -> (order, slot, offsets)
 PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -288,7 +297,7 @@ PyObject* dispatch(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 4, [&]() -> PyObject* {
         const at::Tensor& x = tensor(a[0]);
         const Pairs p{tensor(a[1]), integer(a[2]), integer(a[3])};
-        no_tangents({x});
+        plain({x});
         return THPVariable_Wrap(tracked({x}) ? DispatchNode::apply(x, p.slot, p.N, p.k) : rows_out(x, p, {}, {}, true).first);
     });
 }
@@ -298,7 +307,7 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor& y = tensor(a[0]);
         const Pairs p{tensor(a[1]), integer(a[2]), integer(a[3])};
         const at::Tensor w = maybe(a[4]);
-        no_tangents({y, w});
+        plain({y, w});
         return THPVariable_Wrap(tracked({y, w}) ? CombineNode::apply(y, p.slot, given(w), p.N, p.k) : rows_back(y, p, w));
     });
 }
@@ -396,7 +405,7 @@ PyObject* adapter(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (THPVariable_Check(a[6])) l.scales = tensor(a[6]);
         else l.scale = real(a[6]);
         need(!tracked({l.weight, l.bias, l.scales}));
-        no_tangents({l.x, l.weight, l.bias, l.down, l.up, l.scales});
+        plain({l.x, l.weight, l.bias, l.down, l.up, l.scales});
         at::Tensor saved;
         if (!tracked({l.x, l.down, l.up})) return THPVariable_Wrap(l.forward(false, saved));
         return THPVariable_Wrap(AdapterNode::apply(l.x, l.down, l.up, l.weight, l.offsets, given(l.bias), given(l.scales), l.scale, (int64_t)l.act));
@@ -463,7 +472,7 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 #define ENTRY(name) {#name, (PyCFunction)(void (*)())name, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {ENTRY(bind), ENTRY(route), ENTRY(dispatch), ENTRY(combine), ENTRY(adapter), ENTRY(adamw), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {ENTRY(bind), ENTRY(route), ENTRY(dispatch), ENTRY(combine), ENTRY(adapter), ENTRY(adamw), {"declined", declined, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mtk_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

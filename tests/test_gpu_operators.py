@@ -790,6 +790,21 @@ def test_forward_mode_is_refused():
         assert all(torch.equal(p, q) for p, q in zip((call(a), mtk.dispatch_rows(x, plan), mtk.combine_rows(y, plan, w)), want))
 
 
+def test_functional_transforms_are_refused_by_name():
+    """Whatever the library said last: the message is about this call"""
+    g = gen(92)
+    a = adapter_inputs(g, 20, 8, 6, 2, 3, torch.float32)
+    plan = mtk.route_rows(torch.randint(0, 3, (10, 2), generator=g).to(DEV), 3)
+    x, y = randn(g, 2, 10, 5), randn(g, 20, 5)
+    with pytest.raises(AssertionError):  # the library refuses something else
+        mtk.adamw_step([y], [y], [y.clone()], [y.clone()], 0, lr=1e-3)
+    for f in (lambda: torch.vmap(lambda t: mtk.dispatch_rows(t, plan))(x), lambda: torch.vmap(lambda t: mtk.combine_rows(y, plan, t))(randn(g, 3, 10, 2)),
+              lambda: torch.vmap(lambda t: call(a, scale=t))(torch.ones(4, 3, device=DEV)), lambda: torch.func.grad(lambda t: call(a, up=t).sum())(a["up"]),
+              lambda: torch.func.jvp(lambda t: call(a, x=t), (a["x"],), (a["x"],)), lambda: torch.vmap(lambda t: mtk.route_rows(t, 3).slot)(torch.zeros(2, 4, dtype=torch.int64, device=DEV))):
+        with pytest.raises(NotImplementedError, match="torch.func|forward-mode"):
+            f()
+
+
 # ------------------------------------------------------------------------------------------------------------------- AdamW
 SIZES = [1, 2, 3, 5, 255, 256, 257, 1000, 1024, 4099]
 
