@@ -93,20 +93,33 @@ class AdamW(torch.optim.Optimizer):
 
     ``capturable=True`` keeps every parameter's step count (and, given as a float32 device tensor, the learning rate) on the device, so a step
     captured into a HIP graph counts its own replays; take one step before the capture, which creates the state.  Without it a step under capture is
-    refused.  Parameters have to be contiguous, dense tensors of float32, bfloat16 or float16.  ``amsgrad`` and ``maximize`` are not offered."""
+    refused.  Parameters have to be contiguous, dense tensors of float32, bfloat16 or float16.  ``amsgrad``, ``maximize`` and ``differentiable``
+    are refused unless False; ``foreach`` and ``fused`` choose between torch's own ways and say nothing here."""
 
-    def __init__(self, params, lr: float | Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
-                 state_bits: int = 32, capturable: bool = False):
-        if state_bits not in (8, 32):
-            raise ValueError(f"AdamW: state_bits {state_bits} (8 or 32)")
+    def __init__(self, params, lr: float | Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, amsgrad: bool = False, *,
+                 maximize: bool = False, foreach: bool | None = None, capturable: bool = False, differentiable: bool = False, fused: bool | None = None, state_bits: int = 32):
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=amsgrad, maximize=maximize, foreach=foreach, capturable=capturable,
+                                      differentiable=differentiable, fused=fused, state_bits=state_bits))
+
+    @staticmethod
+    def _check_group(group: dict) -> None:
+        if group["state_bits"] not in (8, 32):
+            raise ValueError(f"AdamW: state_bits {group['state_bits']} (8 or 32)")
+        lr = group["lr"]
         if isinstance(lr, Tensor):
-            if not capturable or lr.numel() != 1 or lr.dtype != torch.float32 or not lr.is_cuda:
+            if not group["capturable"] or lr.numel() != 1 or lr.dtype != torch.float32 or not lr.is_cuda:
                 raise ValueError("AdamW: a tensor lr is one float32 number on the device, with capturable=True")
         elif not lr >= 0:
             raise ValueError(f"AdamW: lr {lr}")
-        if not eps >= 0 or not weight_decay >= 0 or not all(0 <= b < 1 for b in betas):
-            raise ValueError(f"AdamW: betas {betas}, eps {eps}, weight_decay {weight_decay}")
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, capturable=capturable))
+        if not group["eps"] >= 0 or not group["weight_decay"] >= 0 or not all(0 <= b < 1 for b in group["betas"]):
+            raise ValueError(f"AdamW: betas {group['betas']}, eps {group['eps']}, weight_decay {group['weight_decay']}")
+        for name in ("amsgrad", "maximize", "differentiable"):
+            if group.get(name):
+                raise NotImplementedError(f"AdamW: {name} is not offered")
+
+    def add_param_group(self, param_group: dict) -> None:
+        self._check_group({**self.defaults, **param_group})
+        super().add_param_group(param_group)
 
     def _init_state(self, p: Tensor, group: dict) -> dict:
         st = self.state[p]

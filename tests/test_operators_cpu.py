@@ -38,6 +38,26 @@ def test_adamw_arguments(bad):
         mtk.AdamW([torch.nn.Parameter(torch.zeros(2))], **bad)
 
 
+def test_adamw_takes_torchs_arguments():
+    """The constructor calls that torch.optim.AdamW's users make, and what is refused: for all parameters, a group, one that is added"""
+    p = lambda: torch.nn.Parameter(torch.zeros(2))  # noqa: E731
+    kw = dict(amsgrad=False, maximize=False, foreach=None, capturable=False, differentiable=False, fused=None)
+    torch.optim.AdamW([p()], 1e-3, (0.9, 0.99), 1e-8, 0.1, False, **{k: v for k, v in kw.items() if k != "amsgrad"})
+    mtk.AdamW([p()], 1e-3, (0.9, 0.99), 1e-8, 0.1, False, **{k: v for k, v in kw.items() if k != "amsgrad"})
+    opt = mtk.AdamW([{"params": [p()], "lr": 1e-2}], **{**kw, "foreach": True, "fused": True}, state_bits=8)
+    assert opt.defaults["weight_decay"] == 1e-2 and opt.param_groups[0]["state_bits"] == 8
+    for name in ("amsgrad", "maximize", "differentiable"):
+        for make in (lambda n: mtk.AdamW([p()], **{n: True}), lambda n: mtk.AdamW([{"params": [p()], n: True}]), lambda n: opt.add_param_group({"params": [p()], n: True})):
+            with pytest.raises(NotImplementedError, match=name):
+                make(name)
+    for bad in (dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=float("nan")), dict(state_bits=4), dict(lr=torch.tensor(1e-3))):
+        with pytest.raises(ValueError):
+            mtk.AdamW([{"params": [p()], **bad}], capturable=True)
+        with pytest.raises(ValueError):
+            opt.add_param_group({"params": [p()], **bad})
+    assert len(opt.param_groups) == 1
+
+
 def test_adamw_lists_are_optional():
     mtk.adamw_step([], [], [], [], 1, lr=1e-3)
 
