@@ -134,14 +134,26 @@ class AdamW(torch.optim.Optimizer):
                 st[name] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
         return st
 
+    def __setstate__(self, state: dict) -> None:
+        super().__setstate__(state)
+        for group in self.param_groups:  # torch.optim.AdamW's groups have no width of the moments
+            group.setdefault("state_bits", 32)
+            group.setdefault("capturable", False)
+
     def load_state_dict(self, state_dict) -> None:
-        """torch casts a loaded state to its parameter's type; here the moments and step counts keep their own."""
+        """Of an ``AdamW`` or a ``torch.optim.AdamW``.  torch casts a loaded state to its parameter's type; here the moments are float32, or the codes
+        they were, and every parameter has its step count: a number, or with ``capturable`` int64 on the device."""
+        for saved in state_dict["param_groups"]:
+            self._check_group({"state_bits": 32, "capturable": False, **saved})
         super().load_state_dict(state_dict)
-        by_id = {i: p for g, q in zip(self.param_groups, state_dict["param_groups"]) for i, p in zip(q["params"], g["params"])}
-        for i, saved in state_dict["state"].items():
-            p = by_id[i]
-            for name, v in saved.items():
-                self.state[p][name] = v.detach().to(device=p.device, copy=True) if isinstance(v, Tensor) else v
+        for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+            for i, p in zip(saved["params"], group["params"]):
+                for name, v in state_dict["state"].get(i, {}).items():
+                    if name == "step":
+                        v = torch.tensor(int(v), dtype=torch.int64, device=p.device) if group["capturable"] else int(v)
+                    elif isinstance(v, Tensor):
+                        v = v.detach().to(device=p.device, dtype=torch.float32 if group["state_bits"] == 32 else v.dtype, copy=True).contiguous()
+                    self.state[p][name] = v
 
     @torch.no_grad()
     def step(self, closure=None):

@@ -1031,6 +1031,45 @@ def test_adamw_state_round_trip(bits, dt):
         assert int(second.state[q]["step"]) == 6
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("theirs", [dict(foreach=False), dict(capturable=True)])
+def test_adamw_goes_on_from_torchs_state(theirs, dt):
+    """A state that torch.optim.AdamW saved (its steps are float tensors, its moments of the parameters' type): the next step is that of the formula from
+    those moments and that count, with a gradient for every parameter and for some."""
+    g = gen(36)
+    ps = [torch.nn.Parameter(randn(g, *shape).to(dt)) for shape in ((40, 3), (257,), (0,))]
+    first = torch.optim.AdamW(ps, lr=1e-2, weight_decay=0.1, **theirs)
+    for t in range(3):
+        for i, p in enumerate(ps):
+            p.grad = randn(g, *p.shape).to(dt) if i == 0 or t != 1 else None
+        first.step()
+    opt = mtk.AdamW(ps, lr=5.0)
+    opt.load_state_dict(first.state_dict())
+    assert opt.param_groups[0]["lr"] == 1e-2 and opt.param_groups[0]["state_bits"] == 32
+    before = [p.detach().clone() for p in ps]
+    moments = [[first.state[p][k].detach().double() for k in ("exp_avg", "exp_avg_sq")] for p in ps]
+    grads = [randn(g, *p.shape).to(dt) for p in ps]
+    for p, q in zip(ps, grads):
+        p.grad = q.clone()
+    opt.step()
+    for p, p0, (m, v), q, t in zip(ps, before, moments, grads, (4, 3, 3)):
+        st = opt.state[p]
+        assert int(st["step"]) == t and st["exp_avg"].dtype == st["exp_avg_sq"].dtype == torch.float32
+        q, p0 = q.double(), p0.double()
+        wm, wv = 0.9 * m + 0.1 * q, 0.999 * v + 0.001 * q * q
+        within(st["exp_avg"], wm.cpu(), (6 * U32 * (m.abs() + q.abs())).cpu())
+        within(st["exp_avg_sq"], wv.cpu(), (6 * U32 * (v + q * q)).cpu() + 2.0**-140)
+        den = torch.sqrt(wv) / math.sqrt(1 - 0.999**t) + 1e-8
+        want = p0 * (1 - 1e-3) - 1e-2 / (1 - 0.9**t) * wm / den
+        mag = 1e-2 / (1 - 0.9**t) * (m.abs() + q.abs()) / den
+        within(p, want.cpu(), (4 * U32 * p0.abs() + 16 * U32 * mag + half(dt) * (want.abs() + 1e-6) * 1.01).cpu() + tiny(dt))
+    assert (first.state[ps[0]]["exp_avg"].dtype == dt) and int(first.state[ps[0]]["step"]) == 3  # the other's state is its own
+    bad = torch.optim.AdamW(ps, amsgrad=True)
+    with pytest.raises(NotImplementedError, match="amsgrad"):
+        opt.load_state_dict(bad.state_dict())
+    assert opt.param_groups[0]["lr"] == 1e-2 and int(opt.state[ps[0]]["step"]) == 4  # as it was
+
+
 @pytest.mark.parametrize("bits", [8, 32])
 def test_adamw_counts_every_parameters_own_steps(bits):
     """Counts on the device are those on the host: parameters of two types, an empty one, some that go without a gradient now and then, from the
