@@ -11,6 +11,7 @@ memory of 32-bit ones; rounded up or down by a dither that depends on a value's 
 from __future__ import annotations
 
 from array import array
+from bisect import bisect_left
 from operator import attrgetter
 from typing import Sequence
 
@@ -44,13 +45,27 @@ def _check_list(what: str, ts: Sequence[Tensor], dtype: torch.dtype, device: int
                              f"{t.device}" + ("" if t.is_contiguous() else ", not contiguous"))
 
 
+def _check_apart(params: Sequence[Tensor], grads: Sequence[Tensor], written: Sequence[Tensor]) -> None:
+    span = lambda t: (t.data_ptr(), t.data_ptr() + t.nbytes)  # noqa: E731
+    spans = sorted(span(t) for t in written if t.numel())
+    if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+        raise ValueError("adamw_step: the same tensor twice, or tensors that share memory, among params and moments")
+    starts = [a for a, _ in spans]
+    for p, g in zip(params, grads):
+        at, end = span(g)
+        i = bisect_left(starts, end)
+        if g.numel() and span(p) != (at, end) and i and spans[i - 1][1] > at:
+            raise ValueError("adamw_step: a gradient shares memory with what the step writes")
+
+
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor], exp_avg_sqs: Sequence[Tensor], step: int, *, lr: float,
                betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, exp_avg_scales: Sequence[Tensor] | None = None,
                exp_avg_sq_scales: Sequence[Tensor] | None = None, _hyper: Tensor | None = None) -> None:
     """One step, in place, over tensors of one type (float32, bfloat16, float16) on one device; ``step`` counts from 1.
 
     32-bit moments: ``exp_avgs`` / ``exp_avg_sqs`` are float32.  8-bit moments: they are float8_e4m3fn codes of the mean and of the ROOT mean
-    square, and ``exp_avg_scales`` / ``exp_avg_sq_scales`` hold float32 [ceil(numel / 256)] scales.  A moment that is not finite becomes NaN."""
+    square, and ``exp_avg_scales`` / ``exp_avg_sq_scales`` hold float32 [ceil(numel / 256)] scales.  A moment that is not finite becomes NaN.
+    What is written (params, moments, scales) may not share memory, nor may a gradient with any of it (its own whole parameter excepted)."""
     if len(params) == 0:
         return
     q8 = exp_avg_scales is not None
@@ -75,8 +90,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
         _check_list("exp_avg_scales", exp_avg_scales, torch.float32, at, blocks)
         _check_list("exp_avg_sq_scales", exp_avg_sq_scales, torch.float32, at, blocks)
         lists += [exp_avg_scales, exp_avg_sq_scales]
-    if len({p.data_ptr() for p in params if p.numel()}) < sum(n > 0 for n in sizes):
-        raise ValueError("adamw_step: the same tensor twice among params")
+    _check_apart(params, grads, [t for i, ts in enumerate(lists) if i != 1 for t in ts])
     keep = [_addresses(ts) for ts in lists]
     addr = [a for _, a in keep] + ([] if q8 else [None, None])
     numel = array("q", sizes)

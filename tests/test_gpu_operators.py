@@ -915,6 +915,33 @@ def test_adamw_extremes():
             assert bool((p <= 1).all())
 
 
+def test_adamw_refuses_tensors_that_share_memory():
+    """Two of a launch's tensors in one place would be a race: the same one twice, or views that overlap, among all that is written; a gradient may be
+    shared between parameters, or be its whole parameter."""
+    z = lambda n=300: torch.ones(n, device=DEV)  # noqa: E731
+    flat, m, g = z(1000), z(600), z()
+    f8 = lambda: torch.zeros(300, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)  # noqa: E731
+    ok = dict(params=[flat[:300], flat[300:600]], grads=[g, g], exp_avgs=[m[:300], m[300:]], exp_avg_sqs=[z(), z()])
+    bad = [dict(exp_avgs=[m[:300]] * 2), dict(exp_avg_sqs=[m[100:400], z()]), dict(params=[flat[:300], flat[299:599]]), dict(exp_avgs=[flat[600:900], flat[700:]]),
+           dict(grads=[flat[1:301], g]), dict(grads=[g, flat[:300]]), dict(grads=[g, m[:300]])]
+    e8 = dict(params=ok["params"], grads=ok["grads"], exp_avgs=[f8(), f8()], exp_avg_sqs=[f8(), f8()], exp_avg_scales=[m[:2], m[2:4]], exp_avg_sq_scales=[m[4:6], m[6:8]])
+    same = f8()
+    bad8 = [dict(exp_avg_sq_scales=[m[1:3], m[6:8]]), dict(exp_avgs=[same, f8()], exp_avg_sqs=[f8(), same]), dict(exp_avg_scales=[flat[:2], m[2:4]])]
+    for base, cases in ((ok, bad), (e8, bad8)):
+        for kw in cases:
+            before = [t.clone() for t in (flat, m)]
+            with pytest.raises(ValueError, match="memory"):
+                mtk.adamw_step(**{**base, **kw}, step=1, lr=1e-2)
+            assert torch.equal(flat, before[0]) and torch.equal(m, before[1])
+        mtk.adamw_step(**base, step=1, lr=1e-2)
+        mtk.adamw_step(**{**base, "grads": [base["params"][0], g]}, step=2, lr=1e-2)
+    p = torch.nn.Parameter(z())
+    q = torch.nn.Parameter(z())
+    p.grad = q.grad = torch.ones(300, device=DEV)
+    mtk.AdamW([p, q]).step()
+    assert torch.equal(p, q) and not bool((p == 1).any())
+
+
 def test_adamw_where_a_squared_gradient_overflows():
     """The mean square is infinite, the quotient 0: parameters decay and no more, in both forms alike.  Gradients beside them go on as ever."""
     g = gen(35)
