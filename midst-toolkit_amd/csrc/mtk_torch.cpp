@@ -14,6 +14,7 @@
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -126,7 +127,7 @@ PyObject* pack(std::initializer_list<at::Tensor> ts) {
     for (const at::Tensor& t : ts) PyTuple_SET_ITEM(out, i++, t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None));
     return out;
 }
-// the body of a module function: a decline is None, an error of torch's (out of memory) a RuntimeError
+// the body of a module function: a decline is None; an error of torch's, or of a hook in Python, is the exception that torch's own functions raise
 template <typename F> PyObject* guarded(Py_ssize_t n, Py_ssize_t want, F f) {
     if (n != want) {
         PyErr_Format(PyExc_TypeError, "%zd arguments, %zd expected", n, want);
@@ -137,8 +138,8 @@ template <typename F> PyObject* guarded(Py_ssize_t n, Py_ssize_t want, F f) {
         return f();
     } catch (const Decline&) {
         Py_RETURN_NONE;
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (const std::exception&) {
+        torch::translate_exception_to_python(std::current_exception());
         return nullptr;
     } catch (...) {
         PyErr_SetString(PyExc_RuntimeError, "midst_toolkit_amd: unknown C++ exception");

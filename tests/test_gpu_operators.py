@@ -790,6 +790,34 @@ def test_forward_mode_is_refused():
         assert all(torch.equal(p, q) for p, q in zip((call(a), mtk.dispatch_rows(x, plan), mtk.combine_rows(y, plan, w)), want))
 
 
+def test_torchs_errors_keep_their_type():
+    """Out of memory is torch's exception, and so is what a saved-tensor hook raises"""
+    g = gen(94)
+    a = adapter_inputs(g, 4, 8, 8192, 2, 1, torch.float32)
+    free, total = torch.cuda.mem_get_info()
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (64 << 20)) / total)
+    try:
+        with pytest.raises(torch.cuda.OutOfMemoryError):
+            call(a, x=a["x"][:1].expand(1 << 20, 8))  # 32 GiB of results
+        plan = mtk.route_rows(torch.zeros(1 << 21, dtype=torch.int64, device=DEV), 1)
+        with pytest.raises(torch.cuda.OutOfMemoryError):
+            mtk.dispatch_rows(a["up"].view(-1)[:4096].view(1, 4096).expand(1 << 21, 4096), plan)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+
+    class Stop(Exception):
+        pass
+
+    def pack(t):
+        raise Stop
+
+    a["x"].requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        with pytest.raises(Stop):
+            call(a)
+    assert torch.isfinite(call(a)).all()
+
+
 def test_functional_transforms_are_refused_by_name():
     """Whatever the library said last: the message is about this call"""
     g = gen(92)

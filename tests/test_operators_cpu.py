@@ -58,6 +58,11 @@ def test_adamw_takes_torchs_arguments():
     assert len(opt.param_groups) == 1
 
 
+def test_the_module_on_torchs_side_loads():
+    """Its symbols resolve and it takes the library's functions, GPU or not"""
+    assert _lib.native().declined() == ""
+
+
 def test_adamw_lists_are_optional():
     mtk.adamw_step([], [], [], [], 1, lr=1e-3)
 
