@@ -7,6 +7,8 @@ to its pairs' places, the layers work on rows sorted by model (``adapters.adapte
 """
 from __future__ import annotations
 
+import operator
+
 import torch
 from torch import Tensor
 
@@ -51,6 +53,10 @@ def route_rows(index: Tensor, n_groups: int) -> RowPlan:
         return RowPlan(*got, n_groups, index.shape[0], 1 if index.dim() == 1 else index.shape[1])
     if index.dim() not in (1, 2) or index.dtype.is_floating_point or index.dtype.is_complex or index.dtype == torch.bool:
         raise ValueError(f"route_rows: index is [N] or [N, k] whole numbers, got {tuple(index.shape)} {index.dtype}")
+    try:
+        n_groups = operator.index(n_groups)
+    except TypeError:
+        raise ValueError(f"route_rows: n_groups is a whole number, got {n_groups!r}") from None
     if not 1 <= n_groups <= MAX_GROUPS:
         raise ValueError(f"route_rows: {n_groups} groups (1 to {MAX_GROUPS})")
     copies = 1 if index.dim() == 1 else index.shape[1]
@@ -58,8 +64,8 @@ def route_rows(index: Tensor, n_groups: int) -> RowPlan:
         raise ValueError("route_rows: index has no copies")
     if index.numel() > 0x7FFFFFFF:
         raise ValueError(f"route_rows: {index.numel()} pairs exceed 2^31 - 1")
-    got = ordinary("route_rows", index.device, native().route, index.to(torch.int64).contiguous(), int(n_groups))
-    return RowPlan(*got, int(n_groups), index.shape[0], copies)
+    got = ordinary("route_rows", index.device, native().route, index.to(torch.int64).contiguous(), n_groups)
+    return RowPlan(*got, n_groups, index.shape[0], copies)
 
 
 def _check_rows(what: str, t: Tensor, rows: int, plan: RowPlan) -> None:
@@ -96,7 +102,7 @@ def combine_rows(y: Tensor, plan: RowPlan, weights: Tensor | None = None) -> Ten
     if weights is not None:
         if weights.device != y.device:
             raise ValueError(f"combine_rows: weights on {weights.device}, rows on {y.device}")
-        if weights.dtype != torch.float32 or weights.numel() != plan.n_rows * plan.copies or weights.shape[0] != plan.n_rows:
+        if weights.dtype != torch.float32 or weights.numel() != plan.n_rows * plan.copies or weights.shape[:1] != (plan.n_rows,):
             raise ValueError(f"combine_rows: weights are float32 [{plan.n_rows}, {plan.copies}], got {weights.dtype} {tuple(weights.shape)}")
         weights = weights.reshape(plan.n_rows, plan.copies).contiguous()
     return ordinary("combine_rows", y.device, native().combine, rows_of(y), plan.slot, plan.n_rows, plan.copies, weights)

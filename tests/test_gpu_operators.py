@@ -80,6 +80,18 @@ def test_plan_shapes_and_types():
             mtk.route_rows(torch.zeros(3, dtype=torch.int64, device=DEV), e)
 
 
+def test_plans_and_weights_that_are_not_what_they_say():
+    """A number of models that is not whole is not cut, weights without dimensions are not a record's"""
+    idx = torch.zeros(1, dtype=torch.int64, device=DEV)
+    for bad in (2.5, 2.0, "2", None):
+        with pytest.raises(ValueError, match="whole number"):
+            mtk.route_rows(idx, bad)
+    assert mtk.route_rows(idx, np.int64(2)).n_groups == 2
+    plan = mtk.route_rows(idx, 2)
+    with pytest.raises(ValueError, match="weights"):
+        mtk.combine_rows(torch.ones(1, 3, device=DEV), plan, torch.tensor(1.0, device=DEV))
+
+
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("N,k,E,D", [(0, 2, 3, 5), (1, 1, 1, 1), (3, 8, 2, 2), (33, 2, 5, 7), (100, 4, 9, 33), (257, 3, 16, 120), (1000, 2, 7, 257), (70, 5, 1000, 1021), (50, 2, 4, 2050)])
 def test_rows_forth_and_back(N, k, E, D, dt):
