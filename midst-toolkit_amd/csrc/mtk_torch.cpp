@@ -13,11 +13,14 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <algorithm>
 #include <optional>
@@ -168,8 +171,32 @@ variable_list once(const variable_list& grads, variable_list out, const char* wh
         if (t.defined()) t = t.detach().requires_grad_(true);
     return (*std::make_shared<torch::autograd::DelayedError>(std::string(what) + " differentiates once only", (int64_t)out.size()))(std::move(out));
 }
+// A node runs on the stream that was current when it was made, a leaf's accumulator on that of the first graph that needed it and still lives.  Where
+// that is the default stream, a captured backward pass would make the default stream wait for the capture, which no stream outside of one
+// may; the process did not survive it.
+bool on_default_stream(torch::autograd::Node* node) {
+    if (!node) return false;
+    const auto s = node->stream();
+    return s && s->id() == 0;
+}
+void may_capture(const char* what) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return;
+    const auto* only = torch::autograd::get_current_graph_task_exec_info();  // torch.autograd.grad: what it asks for is not accumulated
+    for (const torch::autograd::Edge& e : node->next_edges()) {
+        if (!on_default_stream(e.function.get())) continue;
+        if (only && !only->empty()) {
+            const auto it = only->find(e.function.get());
+            if (it == only->end() || !it->second.needed_) continue;
+        }
+        throw std::runtime_error(std::string(what) + ": a captured backward pass, whose gradient an eager graph's node would take on the default stream: let go of the eager graphs of the same "
+                                                     "parameters (their losses and outputs) before the capture");
+    }
+}
 template <typename F> variable_list backward_of(const char* what, const at::Tensor& like_, F f) {
     const c10::DeviceGuard guard(like_.device());
+    may_capture(what);
     try {
         return f();
     } catch (const Decline&) {
@@ -187,6 +214,15 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // declined() -> what the library said to this thread's last call that returned None; empty where its tensors were the reason
 PyObject* declined(PyObject*, PyObject*) { return PyUnicode_FromString(refusal.c_str()); }
+
+// accumulates_on_default(tensor) -> whether the tensor's gradient goes to a node of the default stream: what may_capture refuses
+PyObject* accumulates_on_default(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 1, [&]() -> PyObject* {
+        const at::Tensor& t = tensor(a[0]);
+        const auto node = t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t);
+        return PyBool_FromLong(on_default_stream(node.get()));
+    });
+}
 
 // route(index, n_groups) -> (order, slot, offsets)
 PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -506,7 +542,7 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 #define ENTRY(name) {#name, (PyCFunction)(void (*)())name, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {ENTRY(bind), ENTRY(route), ENTRY(dispatch), ENTRY(combine), ENTRY(adapter), ENTRY(adamw), {"declined", declined, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {ENTRY(bind), ENTRY(route), ENTRY(dispatch), ENTRY(combine), ENTRY(adapter), ENTRY(adamw), ENTRY(accumulates_on_default), {"declined", declined, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mtk_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

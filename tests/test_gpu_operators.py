@@ -1436,6 +1436,73 @@ def test_a_captured_training_step_replays_like_the_eager_one(bits):
             plain.step()
 
 
+def test_gradients_that_a_captured_backward_may_not_take():
+    """What a captured backward pass refuses, seen without a capture: a leaf whose accumulator an eager graph of the default stream keeps alive, and an
+    eager graph's own nodes.  (The refused pass itself is not run: before, it ended the process.)"""
+    from midst_toolkit_amd import _lib
+
+    g = gen(95)
+    a = adapter_inputs(g, 20, 8, 6, 2, 3, torch.float32)
+    down = a["down"].requires_grad_()
+    held = _lib.native().accumulates_on_default
+    assert not held(down)  # no graph
+    y = call(a)
+    assert held(down) and held(y)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        z = call(a)
+    assert held(down)  # still the first graph's
+    del y, z
+    assert not held(down)
+    with torch.cuda.stream(side):
+        z = call(a)
+        assert not held(down) and not held(z)
+        z.sum().backward()
+    torch.cuda.current_stream().wait_stream(side)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_captured_backward_accumulates(bits):
+    """backward() itself inside the capture, with no eager graph of the parameters alive: gradients and step are the eager ones at every replay"""
+    g = gen(96)
+    N, D, E = 80, 24, 3
+    x, noise = randn(g, N, D), randn(g, N, D)
+    t, idx = torch.randint(0, 50, (N,), generator=g).to(DEV), torch.randint(0, E, (N,), generator=g).to(DEV)
+
+    def one(ens, opt):
+        opt.zero_grad(set_to_none=True)
+        ((ens(x, t, idx) - noise) ** 2).sum().backward()
+        opt.step()
+
+    _, eager = ensemble(gen(1))
+    _, graph = ensemble(gen(1))
+    with torch.no_grad():
+        for p, q in zip(eager.parameters(), graph.parameters()):
+            q.copy_(p)
+    oe, og = (mtk.AdamW(m.parameters(), lr=1e-3, state_bits=bits, capturable=True) for m in (eager, graph))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        one(graph, og)
+    torch.cuda.current_stream().wait_stream(side)
+    one(eager, oe)
+    og.zero_grad(set_to_none=True)
+    from midst_toolkit_amd import _lib
+
+    assert not any(_lib.native().accumulates_on_default(p) for p in graph.parameters())
+    cg = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(cg):
+        one(graph, og)
+    for i in range(4):
+        x.copy_(randn(gen(60 + i), N, D))
+        one(eager, oe)
+        cg.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(eager.parameters(), graph.parameters()):
+            assert torch.equal(p, q) and torch.equal(p.grad, q.grad), i
+
+
 def test_our_step_refreshes_the_modules_that_cache_their_weights():
     """TabSyn's denoiser keeps a packed copy keyed by its parameters' versions: after our step its loss is that of the new weights."""
     torch.manual_seed(0)
