@@ -295,6 +295,8 @@ extern "C" int64_t mtk_adamw_hyper_bytes(void) { return (int64_t)sizeof(AdamwHyp
 extern "C" int mtk_adamw_count_each(int n_steps, int64_t* const* step, const float* lr_dev, double lr, double beta1, double beta2, double eps, double weight_decay,
                                     void* hyper_dev, mtk_stream stream) {
     if (n_steps < 0 || (n_steps > 0 && (!step || !hyper_dev))) MTK_FAIL(MTK_ERR_ARG, "mtk_adamw_count: null pointer or negative count");
+    if (!(lr_dev || lr >= 0) || !(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !(eps >= 0) || !(weight_decay >= 0))
+        MTK_FAIL(MTK_ERR_ARG, "mtk_adamw_count: lr %g, betas %g %g, eps %g, weight_decay %g", lr, beta1, beta2, eps, weight_decay);
     for (int i = 0; i < n_steps; ++i)
         if (!step[i]) MTK_FAIL(MTK_ERR_ARG, "mtk_adamw_count: step %d: null pointer", i);
     for (int i = 0; i < n_steps; i += MAXC) {

@@ -110,6 +110,9 @@ def test_c_entries_refuse_before_any_launch():
     assert l.mtk_adamw_count_each(2, None, None, 1e-3, 0.9, 0.999, 1e-8, 0.0, one, None) == ARG
     assert l.mtk_adamw_count_each(-1, ptrs, None, 1e-3, 0.9, 0.999, 1e-8, 0.0, one, None) == ARG
     assert l.mtk_adamw_count_each(1, (C.c_void_p * 1)(None), None, 1e-3, 0.9, 0.999, 1e-8, 0.0, one, None) == ARG
+    for bad in ((-1e-3, 0.9, 0.999, 1e-8, 0.0), (float("nan"), 0.9, 0.999, 1e-8, 0.0), (1e-3, 1.0, 0.999, 1e-8, 0.0), (1e-3, 0.9, -0.1, 1e-8, 0.0), (1e-3, 0.9, 0.999, -1.0, 0.0),
+                (1e-3, 0.9, 0.999, 1e-8, -0.1)):  # what the step refuses, whose numbers these become
+        assert l.mtk_adamw_count_each(1, ptrs, None, *bad, one, None) == ARG and l.mtk_adamw_count(one, None, *bad, one, None) == ARG, bad
     assert l.mtk_adamw_step_each(1, ptrs, ptrs, ptrs, ptrs, None, None, n, 0, 32, None, None) == ARG
     assert l.mtk_adamw_step_each(1, ptrs, ptrs, ptrs, ptrs, None, None, n, 7, 32, one, None) == UNS
     assert l.mtk_adamw_scales(0) == 0 and l.mtk_adamw_scales(256) == 1 and l.mtk_adamw_scales(257) == 2
