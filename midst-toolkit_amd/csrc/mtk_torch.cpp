@@ -200,7 +200,7 @@ template <typename F> variable_list backward_of(const char* what, const at::Tens
     try {
         return f();
     } catch (const Decline&) {
-        throw std::runtime_error(std::string(what) + ": a gradient or saved tensor does not fit the layer");
+        throw std::runtime_error(std::string(what) + ": a gradient or saved tensor does not fit, or is no plain tensor (batched gradients are not offered)");
     }
 }
 
@@ -395,7 +395,8 @@ struct Layer {  // an adapted layer's arguments, checked
     }
     variable_list backward(const at::Tensor& y, const at::Tensor& dy, const at::Tensor& saved, bool want_x, bool want_down, bool want_up) {
         check();
-        need(dy.scalar_type() == x.scalar_type() && dy.dim() == 2 && dy.size(0) == M && dy.size(1) == dout && dy.is_contiguous() && dy.device() == x.device());
+        dense(dy, device);
+        need(dy.scalar_type() == x.scalar_type() && dy.dim() == 2 && dy.size(0) == M && dy.size(1) == dout);
         need(act == MTK_ACT_NONE || (y.defined() && y.is_contiguous() && y.sizes() == dy.sizes() && y.scalar_type() == x.scalar_type()));
         at::Tensor dx, ddown, dup;
         if (want_x) dx = like(x, {M, din}, x.scalar_type());

@@ -802,6 +802,20 @@ def test_forward_mode_is_refused():
         assert all(torch.equal(p, q) for p, q in zip((call(a), mtk.dispatch_rows(x, plan), mtk.combine_rows(y, plan, w)), want))
 
 
+def test_batched_gradients_are_refused():
+    g = gen(97)
+    a = adapter_inputs(g, 20, 8, 6, 2, 3, torch.float32)
+    plan = mtk.route_rows(torch.randint(0, 3, (10, 2), generator=g).to(DEV), 3)
+    w = randn(g, 10, 2)
+    for f, leaf in ((lambda t: call(a, x=t), randn(g, 20, 8)), (lambda t: mtk.dispatch_rows(t, plan), randn(g, 10, 5)), (lambda t: mtk.combine_rows(t, plan, w), randn(g, 20, 5))):
+        leaf.requires_grad_()
+        y = f(leaf)
+        with pytest.raises(RuntimeError, match="batched|vmap"):
+            torch.autograd.grad(y, leaf, torch.ones(3, *y.shape, device=DEV), is_grads_batched=True)
+        y = f(leaf)
+        assert torch.isfinite(torch.autograd.grad(y, leaf, torch.ones_like(y))[0]).all()
+
+
 def test_torchs_errors_keep_their_type():
     """Out of memory is torch's exception, and so is what a saved-tensor hook raises"""
     g = gen(94)
