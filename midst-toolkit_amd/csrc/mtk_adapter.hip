@@ -180,7 +180,8 @@ struct ShrinkArgs {
 // straight into fragments, two lines at a time.  KS = 1: a wave has 32 rows to itself, which halves what it reads of F.  KS = 4, for few
 // rows: four waves split the lines of 16 rows, their sums meet in LDS.  g.turns workgroups share a tile's models in turn (one model's product is
 // a chain of loads of some microseconds); the first of them clears what no model owns.
-// 65,536 rows of 1,024 bf16: 29 us (4.6 TB/s; 33 with 16 models), 2,048 rows fp32 7 us (8 with 16 models), 61 rows of 512 fp32 6 us.
+// In a pass, with the layout that rides along: 65,536 rows of 1,024 bf16 of 16 models 43 us (35 the fastest, 134 MB: 3.8 TB/s), 2,048 rows fp32
+// 10 us (8.7), 61 rows of 512 fp32 6.6 us.
 template <int RT, int KS> constexpr int kShrinkLds = KS > 1 ? KS * RT * 4 * 64 : 1;  // floats
 template <typename T, int RT, int KS>
 __device__ void shrink_body(const ShrinkArgs& g, unsigned block, int j0, const T* __restrict__ x, const T* __restrict__ F, Low<T>* __restrict__ u, Low<T>* __restrict__ uT, float* lds) {
@@ -353,8 +354,9 @@ __device__ void shrink_body(const ShrinkArgs& g, unsigned block, int j0, const T
 // both, so t + e numbers the pairs.  Zero times B_e is zero while B_e is finite; a shared tile with one that is not is made once more, without
 // the stream.  There, in tiles of more than kTileModels models, and (nkx = 0) with far fewer rows a model than a tile has, the
 // low-rank products are made in the epilogue, per model, and selected by row.
-// 65,536 x 1,024 x 1,024 in bf16 144 us, 17 lines of k for the 16 of the shared product alone, which the library's plain product does in 133; 2,048 rows
-// in fp32 47 us (33 lines for 32; 35): there the matrix pipes are busy 81 % of the time at some 2.0 GHz, the rest is start and end.
+// 65,536 x 1,024 x 1,024 in bf16, in a pass, 161 us (146 the fastest), 17 lines of k for the 16 of the shared product alone, which the library's plain
+// product does in 133; 2,048 rows in fp32 51 us (48.5; 33 lines for 32; 35): there the matrix pipes are busy 69 % of the kernel's cycles, the
+// rest is start, end and a barrier a line.
 // RAW, fp16 without such blocks: B_e as it lies, split into its two numbers where it is read (a kernel of its own: with the lines' loop beside
 // it the accumulators spill; lines for all would be laid out at length: 2,048 rows of 128 models 58 us for 20).
 // The stream wants whole, 16-byte aligned lines: k_prep pads what is not, and lays out B, the bias in fp32, the tiles' models and which B_e
@@ -1062,7 +1064,7 @@ __device__ void wgrad_body(const WgradArgs& g, int strip, int c, int j0, const L
         constexpr int P = kParts<T>;
         mtk_vec<Low<T>> ut[P][JT];  // the numbers of u
         // A scalar base and one 32-bit offset per lane.  A group with rows of other models clamps its rows to this one's and clears what it read
-        // for them: a load that is made under a condition costs a branch (2,048 rows of 16 models in bf16: 26 us with such loads, _NOW_ without)
+        // for them: a load that is made under a condition costs a branch (2,048 rows of 16 models in bf16: 21 us with such loads, 12 without)
         const int64_t plane = mtk_up(g.r, 64) * g.Mp;
         const unsigned ld = (unsigned)g.x_ld * (unsigned)sizeof(T);
         const unsigned first_row = sizeof(T) == 4 ? q : q * 8;

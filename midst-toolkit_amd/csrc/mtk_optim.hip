@@ -14,7 +14,7 @@
 //
 // Bound by bandwidth: 28 B a value with fp32 and 32-bit moments, 10 B with bf16 and 8-bit ones.  Up to 64 tensors ride in one launch's
 // arguments (nothing to upload, nothing that a captured graph could find changed); a workgroup takes one chunk of one tensor.
-// 55 million fp32 values in 192 tensors, 32-bit moments: 257 us (1.54 GB: 6.0 TB/s); 220 million bf16 values, 8-bit moments: 426 us (2.2 GB: 5.2 TB/s);
+// 55 million fp32 values in 192 tensors, 32-bit moments: 257 us (1.54 GB: 6.0 TB/s); 220 million bf16 values, 8-bit moments: 417 us (2.2 GB: 5.3 TB/s);
 // 2.2 million fp32 values in 12 tensors: 11 us either way, from the caches.
 #include <math.h>
 
