@@ -14,8 +14,8 @@
 // (0 x inf is NaN), their products are made per model and SELECTED by row.
 // Every sum is in fp32.  u and t = s_e g B_e are MFMA operands, so with 16-bit rows they are 16-bit numbers, and more than one each: a single rounded
 // number would add as much error as the result's own rounding, and all of a row's at once.  A row of u holds them in sections side by side:
-//   bf16  two, u = hi + lo (2^-17 of u), against B_e twice; for ranks up to 32 the line of 64 numbers holds both
-//   fp16  three bf16 numbers, u = h + m + l (2^-25), against B_e = b + c, two bf16 numbers (exact): h b + m b + l b + h c + m c.  Not fp16 numbers:
+//   bf16  two, u = hi + lo (2^-18 of u), against B_e twice; for ranks up to 32 the line of 64 numbers holds both
+//   fp16  three bf16 numbers, u = h + m + l (2^-27), against B_e = b + c, two bf16 numbers (exact): h b + m b + l b + h c + m c.  Not fp16 numbers:
 //         t is small (the factors start at zero, gradients are small), and below 2^-14 fp16 has fewer bits with every binade, 6e-8 of
 //         absolute error; at the other end u passes 65,504 where y does not.  bf16 has fp32's exponents.  One line up to rank 12.
 #include <type_traits>
