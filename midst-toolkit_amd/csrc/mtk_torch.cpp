@@ -183,12 +183,12 @@ void may_capture(const char* what) {
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
     const auto node = torch::autograd::get_current_node();
     if (!node) return;
-    const auto* only = torch::autograd::get_current_graph_task_exec_info();  // torch.autograd.grad: what it asks for is not accumulated
+    const auto* only = torch::autograd::get_current_graph_task_exec_info();  // torch.autograd.grad: the nodes on the way to what it asks for, and those
     for (const torch::autograd::Edge& e : node->next_edges()) {
         if (!on_default_stream(e.function.get())) continue;
         if (only && !only->empty()) {
             const auto it = only->find(e.function.get());
-            if (it == only->end() || !it->second.needed_) continue;
+            if (it == only->end() || !it->second.should_execute()) continue;
         }
         throw std::runtime_error(std::string(what) + ": a captured backward pass, whose gradient an eager graph's node would take on the default stream: let go of the eager graphs of the same "
                                                      "parameters (their losses and outputs) before the capture");
