@@ -1185,6 +1185,31 @@ def test_adamw_counts_every_parameters_own_steps(bits):
         assert all(torch.equal(a[k].view(torch.uint8) if bits == 8 else a[k], b[k].view(torch.uint8) if bits == 8 else b[k]) for k in ("exp_avg", "exp_avg_sq"))
 
 
+def test_one_count_on_the_device_for_all_tensors():
+    """The C entries with a single count (mtk_adamw_count, then mtk_adamw_step with its numbers), over more tensors than a launch takes"""
+    import ctypes as C
+
+    from midst_toolkit_amd import _lib
+
+    l, g = _lib.lib(), gen(37)
+    sizes = [1 + 37 * i % 500 for i in range(70)]
+    sizes[3] = sizes[69] = 0
+    lists = [[randn(g, n) for n in sizes], None, [torch.zeros(n, device=DEV) for n in sizes], [torch.zeros(n, device=DEV) for n in sizes]]
+    want = [[t.clone() for t in lists[i]] for i in (0, 2, 3)]
+    step = torch.zeros((), dtype=torch.int64, device=DEV)
+    hyper = torch.empty(l.mtk_adamw_hyper_bytes(), dtype=torch.uint8, device=DEV)
+    numel = (C.c_int64 * len(sizes))(*sizes)
+    stream = torch.cuda.current_stream().cuda_stream
+    at = lambda ts: (C.c_void_p * len(ts))(*[t.data_ptr() for t in ts])  # noqa: E731
+    for t in (1, 2, 3):
+        lists[1] = [randn(g, n) for n in sizes]
+        assert l.mtk_adamw_count(step.data_ptr(), None, 1e-2, 0.9, 0.99, 1e-8, 0.1, hyper.data_ptr(), stream) == 0
+        assert l.mtk_adamw_step(len(sizes), *[at(ts) for ts in lists], None, None, numel, 0, 32, 0.0, 0.0, 0.0, 0.0, 0.0, 1, hyper.data_ptr(), stream) == 0
+        mtk.adamw_step(want[0], lists[1], want[1], want[2], t, lr=1e-2, betas=(0.9, 0.99), weight_decay=0.1)
+    assert int(step) == 3
+    assert all(torch.equal(a, b) for got, ref in zip((lists[0], lists[2], lists[3]), want) for a, b in zip(got, ref))
+
+
 def test_a_captured_step_counts_what_it_steps():
     """A graph that steps two of three parameters, of two types, with eager steps of all three in between"""
     g = gen(34)
